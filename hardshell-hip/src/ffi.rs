@@ -292,6 +292,95 @@ unsafe extern "C" {
         out: *mut i8,
         stream: *mut c_void,
     ) -> c_int;
+    /// No counterpart in the reference: attention of trees of drafted tokens.
+    pub fn hs_op_attend_tree_dev(
+        dev: *mut hs_device,
+        q: *const i8,
+        k_cache: *const i8,
+        v_cache: *const i8,
+        ctx: *const u32,
+        nodes: *const u32,
+        mask: *const u64,
+        b: usize,
+        t: usize,
+        h: usize,
+        hd: usize,
+        ctx_cap: usize,
+        score_m: i32,
+        score_s: u8,
+        out_m: i32,
+        out_s: u8,
+        attn_exp: *const i32,
+        len: usize,
+        softmax_p: u8,
+        out: *mut i8,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+        stream: *mut c_void,
+    ) -> c_int;
+    /// No counterpart in the reference: causal attention that adds up each key's weights.
+    pub fn hs_op_attend_mass_dev(
+        dev: *mut hs_device,
+        q: *const i8,
+        k_cache: *const i8,
+        v_cache: *const i8,
+        ctx: *const u32,
+        rows: *const u32,
+        mass: *mut u64,
+        b: usize,
+        t: usize,
+        h: usize,
+        hd: usize,
+        ctx_cap: usize,
+        score_m: i32,
+        score_s: u8,
+        out_m: i32,
+        out_s: u8,
+        attn_exp: *const i32,
+        len: usize,
+        softmax_p: u8,
+        out: *mut i8,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn hs_op_attend_rows_workspace(b: usize, t: usize, h: usize, hd: usize, ctx_cap: usize) -> usize;
+    /// No counterpart in the reference: caches cut to a budget by accumulated weight.
+    pub fn hs_op_cache_evict_dev(
+        dev: *mut hs_device,
+        k_caches: *const *mut i8,
+        v_caches: *const *mut i8,
+        layers: usize,
+        mass: *const u64,
+        ctx: *const u32,
+        b: usize,
+        h: usize,
+        hd: usize,
+        ctx_cap: usize,
+        budget: usize,
+        recent: usize,
+        mass_out: *mut u64,
+        ctx_out: *mut u32,
+        kept: *mut u32,
+        stream: *mut c_void,
+    ) -> c_int;
+    /// No counterpart in the reference: the accepted path of a tree of drafts.
+    pub fn hs_op_cache_commit_dev(
+        dev: *mut hs_device,
+        k_caches: *const *mut i8,
+        v_caches: *const *mut i8,
+        layers: usize,
+        ctx: *const u32,
+        path: *const u32,
+        accepted: *const u32,
+        b: usize,
+        t: usize,
+        h: usize,
+        hd: usize,
+        ctx_cap: usize,
+        ctx_out: *mut u32,
+        stream: *mut c_void,
+    ) -> c_int;
     pub fn hs_op_coder(
         dev: *mut hs_device,
         logits: *const i64,

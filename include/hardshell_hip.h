@@ -290,6 +290,68 @@ hs_status hs_op_attend_decode_dev_noalloc(hs_device *dev, const int8_t *q, const
                                           const int32_t *attn_exp, size_t len, uint8_t softmax_p,
                                           int8_t *out, void *stream);
 
+/* ---- Trees of drafts and bounded caches. No counterparts in the reference: it drafts chains (a
+ * tree of one branch) and keeps every key until a context restarts. Device pointers throughout but
+ * for the arrays of layer pointers; `stream` a hipStream_t or NULL (the device's own); nothing waits for
+ * the GPU. Rules, tables and caches as in hs_op_attend_decode_dev; rows, caches, tables and counts
+ * 4-byte aligned, masks and accumulators 8-byte. At most 2^22 keys a cache. Safe under graph capture
+ * (with a workspace of the caller's where one is needed). ---------------------------------------- */
+/* Attention of a tree of drafted tokens for each stream. q and out [b, t, h, hd] i8; row i < nodes[s]
+ * (NULL: t for every stream) is node i of the tree of stream s, whose key and value the caller has
+ * stored at cache position ctx[s] + i. mask [b, t, ceil(t / 64)] u64: bit n % 64 of word n / 64 of row i
+ * is set where node i sees node n (its ancestors and itself); bits n >= nodes[s] count for nothing.
+ * Every node sees the ctx[s] keys of the context (ctx[s] = 0 is allowed). A row that sees no key, or whose
+ * table entries sum to 0, is 0; rows i >= nodes[s] of out are left as they were. t <= 256; keys past the
+ * cache are not read. */
+hs_status hs_op_attend_tree_dev(hs_device *dev, const int8_t *q, const int8_t *k_cache,
+                                const int8_t *v_cache, const uint32_t *ctx, const uint32_t *nodes,
+                                const uint64_t *mask, size_t b, size_t t, size_t h, size_t hd,
+                                size_t ctx_cap, int32_t score_m, uint8_t score_s, int32_t out_m,
+                                uint8_t out_s, const int32_t *attn_exp, size_t len,
+                                uint8_t softmax_p, int8_t *out, void *workspace,
+                                size_t workspace_bytes, void *stream);
+/* Causal attention of the last rows[s] <= t tokens of each stream (NULL: t for every stream; t = 1
+ * is the decode step), which also adds up how much weight each key receives: row i sees the first
+ * ctx[s] - rows[s] + 1 + i of the stream's ctx[s] keys, and mass [b, h, ctx_cap] u64 gains
+ * mass[s][h][j] += sum over the rows of p_j (p_j <= 2^softmax_p: 2^34 rows fit). Sums of integers: the
+ * result depends on no order. A row that sees no key, or whose entries sum to 0, is 0 and adds nothing;
+ * rows i >= rows[s] of out are left as they were. */
+hs_status hs_op_attend_mass_dev(hs_device *dev, const int8_t *q, const int8_t *k_cache,
+                                const int8_t *v_cache, const uint32_t *ctx, const uint32_t *rows,
+                                uint64_t *mass, size_t b, size_t t, size_t h, size_t hd,
+                                size_t ctx_cap, int32_t score_m, uint8_t score_s, int32_t out_m,
+                                uint8_t out_s, const int32_t *attn_exp, size_t len,
+                                uint8_t softmax_p, int8_t *out, void *workspace,
+                                size_t workspace_bytes, void *stream);
+/* The bytes of workspace (256-byte aligned) that a call of these shapes of either needs, 0 where
+ * none. A call that gets NULL allocates them on the stream. Calls that can overlap, captured graphs
+ * among them, need workspaces of their own; nothing is kept in it between calls. */
+size_t hs_op_attend_rows_workspace(size_t b, size_t t, size_t h, size_t hd, size_t ctx_cap);
+/* Cuts the caches of each stream with n = ctx[s] > budget keys to budget keys, in place, in every
+ * layer (k_caches, v_caches: host arrays of `layers` device caches [b, h, ctx_cap, hd]) and head by
+ * itself: the budget - recent keys of the largest accumulated weights among the first n - recent (ties: the
+ * lowest index) and the last `recent` keys stay. mass, mass_out [layers, b, h, ctx_cap] u64 (the same array,
+ * or two that do not overlap); kept [layers, b, h, budget] u32 (or NULL) receives the place each kept
+ * row came from. The result at place i < budget - recent: row i itself if it stays, and the a-th free place
+ * takes the a-th kept row from behind (attention does not depend on the order of its keys, so
+ * only those rows move); then the recent rows in order. mass_out moves along and is 0 at places budget ..
+ * n - 1. A stream with n <= budget keeps its rows (kept and mass_out: its n keys as they are). Rows of
+ * the caches from the budget on, and entries past those named, are left as they were.
+ * ctx_out[b] (or NULL; not overlapping ctx) receives min(n, budget). 1 <= budget <= ctx_cap, recent <= budget. */
+hs_status hs_op_cache_evict_dev(hs_device *dev, int8_t *const *k_caches, int8_t *const *v_caches,
+                                size_t layers, const uint64_t *mass, const uint32_t *ctx, size_t b,
+                                size_t h, size_t hd, size_t ctx_cap, size_t budget, size_t recent,
+                                uint64_t *mass_out, uint32_t *ctx_out, uint32_t *kept, void *stream);
+/* Commits the accepted path of each stream's tree in every layer's caches (as above): row ctx[s] +
+ * path[s][i] moves to row ctx[s] + i for i < accepted[s] <= t, as if all were read before any is
+ * written. path [b, t] u32 with path[s][i] >= i (any path from a root down is ascending, so it has that);
+ * a row that lies past the cache is left out. ctx_out[b] (or NULL; not overlapping ctx) receives ctx[s] +
+ * accepted[s]. */
+hs_status hs_op_cache_commit_dev(hs_device *dev, int8_t *const *k_caches, int8_t *const *v_caches,
+                                 size_t layers, const uint32_t *ctx, const uint32_t *path,
+                                 const uint32_t *accepted, size_t b, size_t t, size_t h, size_t hd,
+                                 size_t ctx_cap, uint32_t *ctx_out, void *stream);
+
 /* The coder op alone (the logits_weights + coder_interval kernels of
  * crates/hardshell-cuda/kernels/hardshell.cu:1393-1611, no public counterpart; for tests): for
  * each of `rows` rows of i64 logits [rows, vocab] (host pointers, each within +-2^40), the

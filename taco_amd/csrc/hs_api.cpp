@@ -10,6 +10,7 @@
 #include <cmath>
 #include <cstddef>
 #include <cstring>
+#include <initializer_list>
 #include <memory>
 #include <mutex>
 #include <new>
@@ -1685,6 +1686,187 @@ extern "C" hs_status hs_op_attend_decode_dev_noalloc(hs_device *dev, const int8_
                                                std::to_string(HS_FIXED_SCRATCH_BYTES));
     HIP_TRY(hipSetDevice(dev->ordinal));
     HIP_TRY(hs::launch_attend_split(at, (int)b, plan, bytes ? dev->fixed_scratch : nullptr, st));
+    return HS_OK;
+}
+
+// ---- Trees of drafts and bounded caches -------------------------------------------------------------
+
+namespace {
+
+bool overlap(const void *x, size_t nx, const void *y, size_t ny) {
+    const uintptr_t a = (uintptr_t)x, b = (uintptr_t)y;
+    return x && y && a < b + ny && b < a + nx;
+}
+
+bool aligned(size_t n, std::initializer_list<const void *> ps) {
+    for (const void *p : ps)
+        if ((uintptr_t)p % n) return false;
+    return true;
+}
+
+constexpr size_t HS_MAX_NODES = 256;  // drafted nodes of a stream (four mask words a row)
+
+// The arguments that the entries of several rows share; on HS_OK `g` is filled but for the counts, the mask
+// and the accumulators.
+hs_status rows_args(hs_device *dev, const int8_t *q, const int8_t *k_cache, const int8_t *v_cache, const uint32_t *ctx,
+                    size_t b, size_t t, size_t h, size_t hd, size_t ctx_cap, int32_t score_m, uint8_t score_s,
+                    int32_t out_m, uint8_t out_s, const int32_t *attn_exp, size_t len, uint8_t softmax_p, int8_t *out,
+                    hs::RowsArgs &g) {
+    if (!dev || !q || !k_cache || !v_cache || !ctx || !attn_exp || !out)
+        return hs::fail(HS_INVALID_ARGUMENT, 0, "NULL argument");
+    if (hd == 0 || hd % 4 != 0 || hd > 256 || h == 0 || len == 0 || softmax_p > 30 || ctx_cap == 0)
+        return hs::fail(HS_UNSUPPORTED, 0, "head_dim must be a multiple of 4 in 4..=256; h, len and ctx_cap >= 1; P <= 30");
+    if (!aligned(4, {q, k_cache, v_cache, ctx, attn_exp, out}))
+        return hs::fail(HS_INVALID_ARGUMENT, 0, "rows, caches, counts and the table must be 4-byte aligned");
+    if (t > (size_t)INT32_MAX || h > (size_t)INT32_MAX || b > (size_t)INT32_MAX || len > (size_t)INT32_MAX ||
+        ctx_cap > (size_t)1 << 22 || h * hd > (size_t)INT32_MAX || b * t > (size_t)INT32_MAX / h)
+        return hs::fail(HS_UNSUPPORTED, 0, "too many rows, heads or keys (at most 2^22 keys)");
+    hs::AttnArgs &at = g.a;
+    at.q = q; at.ldq = (int)(h * hd); at.kc = k_cache; at.vc = v_cache;
+    at.n_head = (int)h; at.hd = (int)hd; at.ctx_cap = (int)ctx_cap; at.score_m = score_m;
+    at.score_s = score_s; at.out_m = out_m; at.out_s = out_s; at.exp_table = attn_exp;
+    at.exp_len = (int)len; at.softmax_p = softmax_p; at.out = out; at.ldo = (int)(h * hd);
+    g.streams = (int)b; g.t = (int)t; g.ctx = ctx;
+    return HS_OK;
+}
+
+hs_status run_rows(hs_device *dev, const hs::RowsArgs &g, void *workspace, size_t workspace_bytes, void *stream) {
+    const size_t need = hs::rows_workspace(g);
+    if (workspace && (workspace_bytes < need || !aligned(256, {workspace})))
+        return hs::fail(HS_INVALID_ARGUMENT, 0, "the workspace needs " + std::to_string(need) + " bytes, 256-byte aligned");
+    hipStream_t st = stream ? (hipStream_t)stream : dev->stream;
+    HIP_TRY(hipSetDevice(dev->ordinal));
+    if (need == 0 || workspace) {
+        HIP_TRY(hs::launch_rows(g, workspace, st));
+        return HS_OK;
+    }
+    void *scratch = nullptr;
+    HIP_TRY(hipMallocAsync(&scratch, need, st));
+    const hipError_t e = hs::launch_rows(g, scratch, st);
+    const hipError_t f = hipFreeAsync(scratch, st);
+    HIP_TRY(e);
+    HIP_TRY(f);
+    return HS_OK;
+}
+
+// The layer pointers of a launch, and the checks that the cache operators share.
+hs_status cache_args(hs_device *dev, int8_t *const *k_caches, int8_t *const *v_caches, size_t layers, size_t b, size_t h,
+                     size_t hd, size_t ctx_cap) {
+    if (!dev || (layers && (!k_caches || !v_caches))) return hs::fail(HS_INVALID_ARGUMENT, 0, "NULL argument");
+    if (hd == 0 || hd % 4 != 0 || hd > 256 || h == 0 || ctx_cap == 0)
+        return hs::fail(HS_UNSUPPORTED, 0, "head_dim must be a multiple of 4 in 4..=256; h and ctx_cap >= 1");
+    if (ctx_cap > (size_t)INT32_MAX || b > (size_t)INT32_MAX || h > (size_t)INT32_MAX / 128 ||
+        (b && h > (size_t)INT32_MAX / 128 / b))  // 64 layers of K and V in a launch
+        return hs::fail(HS_UNSUPPORTED, 0, "too many panels or keys");
+    for (size_t l = 0; l < layers; l++) {
+        if (!k_caches[l] || !v_caches[l]) return hs::fail(HS_INVALID_ARGUMENT, 0, "NULL cache");
+        if (!aligned(4, {k_caches[l], v_caches[l]}))
+            return hs::fail(HS_INVALID_ARGUMENT, 0, "the caches must be 4-byte aligned");
+    }
+    return HS_OK;
+}
+
+}  // namespace
+
+extern "C" size_t hs_op_attend_rows_workspace(size_t b, size_t t, size_t h, size_t hd, size_t ctx_cap) {
+    hs::RowsArgs g;
+    if (b * t * h == 0 || hd == 0 || b * t > (size_t)INT32_MAX / h || ctx_cap > (size_t)1 << 22) return 0;
+    g.streams = (int)b; g.t = (int)t; g.a.n_head = (int)h; g.a.hd = (int)hd; g.a.ctx_cap = (int)ctx_cap;
+    return hs::rows_workspace(g);
+}
+
+extern "C" hs_status hs_op_attend_tree_dev(hs_device *dev, const int8_t *q, const int8_t *k_cache, const int8_t *v_cache,
+                                           const uint32_t *ctx, const uint32_t *nodes, const uint64_t *mask, size_t b,
+                                           size_t t, size_t h, size_t hd, size_t ctx_cap, int32_t score_m,
+                                           uint8_t score_s, int32_t out_m, uint8_t out_s, const int32_t *attn_exp,
+                                           size_t len, uint8_t softmax_p, int8_t *out, void *workspace,
+                                           size_t workspace_bytes, void *stream) {
+    hs::clear_error();
+    hs::RowsArgs g;
+    HS_TRY(rows_args(dev, q, k_cache, v_cache, ctx, b, t, h, hd, ctx_cap, score_m, score_s, out_m, out_s, attn_exp, len,
+                     softmax_p, out, g));
+    if (!mask) return hs::fail(HS_INVALID_ARGUMENT, 0, "mask is NULL");
+    if (t > HS_MAX_NODES) return hs::fail(HS_UNSUPPORTED, 0, "a tree holds at most 256 nodes");
+    if (!aligned(8, {mask}) || !aligned(4, {nodes}))
+        return hs::fail(HS_INVALID_ARGUMENT, 0, "the mask must be 8-byte aligned, the counts 4-byte");
+    if (b == 0 || t == 0) return HS_OK;
+    g.count = nodes; g.mask = mask; g.words = (int)((t + 63) / 64);
+    return run_rows(dev, g, workspace, workspace_bytes, stream);
+}
+
+extern "C" hs_status hs_op_attend_mass_dev(hs_device *dev, const int8_t *q, const int8_t *k_cache, const int8_t *v_cache,
+                                           const uint32_t *ctx, const uint32_t *rows, uint64_t *mass, size_t b, size_t t,
+                                           size_t h, size_t hd, size_t ctx_cap, int32_t score_m, uint8_t score_s,
+                                           int32_t out_m, uint8_t out_s, const int32_t *attn_exp, size_t len,
+                                           uint8_t softmax_p, int8_t *out, void *workspace, size_t workspace_bytes,
+                                           void *stream) {
+    hs::clear_error();
+    hs::RowsArgs g;
+    HS_TRY(rows_args(dev, q, k_cache, v_cache, ctx, b, t, h, hd, ctx_cap, score_m, score_s, out_m, out_s, attn_exp, len,
+                     softmax_p, out, g));
+    if (!mass) return hs::fail(HS_INVALID_ARGUMENT, 0, "mass is NULL");
+    if (!aligned(8, {mass}) || !aligned(4, {rows}))
+        return hs::fail(HS_INVALID_ARGUMENT, 0, "the accumulators must be 8-byte aligned, the counts 4-byte");
+    if (b == 0 || t == 0) return HS_OK;
+    g.count = rows; g.mass = mass;
+    return run_rows(dev, g, workspace, workspace_bytes, stream);
+}
+
+extern "C" hs_status hs_op_cache_evict_dev(hs_device *dev, int8_t *const *k_caches, int8_t *const *v_caches,
+                                           size_t layers, const uint64_t *mass, const uint32_t *ctx, size_t b, size_t h,
+                                           size_t hd, size_t ctx_cap, size_t budget, size_t recent, uint64_t *mass_out,
+                                           uint32_t *ctx_out, uint32_t *kept, void *stream) {
+    hs::clear_error();
+    HS_TRY(cache_args(dev, k_caches, v_caches, layers, b, h, hd, ctx_cap));
+    if (!mass || !ctx || !mass_out) return hs::fail(HS_INVALID_ARGUMENT, 0, "NULL argument");
+    if (budget == 0 || budget > ctx_cap || recent > budget)
+        return hs::fail(HS_UNSUPPORTED, 0, "1 <= budget <= ctx_cap and recent <= budget");
+    if (!aligned(8, {mass, mass_out}) || !aligned(4, {ctx, ctx_out, kept}))
+        return hs::fail(HS_INVALID_ARGUMENT, 0, "the accumulators must be 8-byte aligned, the counts 4-byte");
+    const size_t masses = 8 * layers * b * h * ctx_cap;
+    if (overlap(ctx, 4 * b, ctx_out, 4 * b) || (mass != mass_out && overlap(mass, masses, mass_out, masses)))
+        return hs::fail(HS_INVALID_ARGUMENT, 0, "ctx_out must not overlap ctx, nor mass_out overlap mass in part");
+    if (b == 0 || layers == 0) return HS_OK;
+    HIP_TRY(hipSetDevice(dev->ordinal));
+    hipStream_t st = stream ? (hipStream_t)stream : dev->stream;
+    hs::EvictArgs a{mass, ctx, (int)b, (int)h, (int)hd, (int)ctx_cap, (int)budget, (int)recent, 0, mass_out, ctx_out, kept};
+    for (size_t l0 = 0; l0 < layers; l0 += hs::CACHE_LAYERS) {
+        const int n = (int)std::min<size_t>(hs::CACHE_LAYERS, layers - l0);
+        hs::CachePtrs c{};
+        for (int l = 0; l < n; l++) {
+            c.k[l] = k_caches[l0 + l];
+            c.v[l] = v_caches[l0 + l];
+        }
+        a.layer0 = (int)l0;
+        HIP_TRY(hs::launch_evict(c, n, a, st));
+    }
+    return HS_OK;
+}
+
+extern "C" hs_status hs_op_cache_commit_dev(hs_device *dev, int8_t *const *k_caches, int8_t *const *v_caches,
+                                            size_t layers, const uint32_t *ctx, const uint32_t *path,
+                                            const uint32_t *accepted, size_t b, size_t t, size_t h, size_t hd,
+                                            size_t ctx_cap, uint32_t *ctx_out, void *stream) {
+    hs::clear_error();
+    HS_TRY(cache_args(dev, k_caches, v_caches, layers, b, h, hd, ctx_cap));
+    if (!ctx || !accepted || (t && !path)) return hs::fail(HS_INVALID_ARGUMENT, 0, "NULL argument");
+    if (t > (size_t)INT32_MAX) return hs::fail(HS_UNSUPPORTED, 0, "a path is too long");
+    if (!aligned(4, {ctx, path, accepted, ctx_out})) return hs::fail(HS_INVALID_ARGUMENT, 0, "the counts must be 4-byte aligned");
+    if (overlap(ctx, 4 * b, ctx_out, 4 * b)) return hs::fail(HS_INVALID_ARGUMENT, 0, "ctx_out must not overlap ctx");
+    if (b == 0 || layers == 0) return HS_OK;
+    HIP_TRY(hipSetDevice(dev->ordinal));
+    hipStream_t st = stream ? (hipStream_t)stream : dev->stream;
+    hs::CommitArgs a{ctx, path, accepted, (int)b, (int)t, (int)h, (int)hd, (int)ctx_cap, 0, ctx_out};
+    for (size_t l0 = 0; l0 < layers; l0 += hs::CACHE_LAYERS) {
+        const int n = (int)std::min<size_t>(hs::CACHE_LAYERS, layers - l0);
+        hs::CachePtrs c{};
+        for (int l = 0; l < n; l++) {
+            c.k[l] = k_caches[l0 + l];
+            c.v[l] = v_caches[l0 + l];
+        }
+        a.first = l0 == 0;
+        HIP_TRY(hs::launch_commit(c, n, a, st));
+    }
     return HS_OK;
 }
 

@@ -221,6 +221,45 @@ struct AttnGroup {
 hipError_t launch_attend_groups(const AttnArgs &a, const AttnGroup *groups, int n_groups, int max_keys,
                                 hipStream_t stream);
 
+// Attention of several rows a stream (attend_rows.hip): the rows of a tree of drafted tokens, or causal
+// chunks. `a` holds the caches, the rules and the layouts of q and out (its rows and keys are unused).
+struct RowsArgs {
+    AttnArgs a;
+    int streams = 0, t = 0;  // rows of a stream: at most t
+    // the rows, slot and context length of each stream; without it stream s has rows s t .. of slot s,
+    const AttnGroup *groups = nullptr;
+    const uint32_t *ctx = nullptr;    // ctx[s] keys (with a mask: before the rows' own)
+    const uint32_t *count = nullptr;  // and count[s] rows (t where it is null)
+    // tree: row r sees the keys before its stream's rows, and row n of the stream where bit n of its
+    // `words` words is set (bits from the row count on are 0). Null: causal rows.
+    const uint64_t *mask = nullptr;
+    int words = 0;
+    uint64_t *mass = nullptr;  // [slots][H][ctx_cap]: the weights p of each key are added
+};
+size_t rows_workspace(const RowsArgs &g);
+hipError_t launch_rows(const RowsArgs &g, void *workspace, hipStream_t stream);
+
+// The caches of up to CACHE_LAYERS layers in one launch, each [b][h][cap][hd].
+constexpr int CACHE_LAYERS = 64;
+struct CachePtrs {
+    int8_t *k[CACHE_LAYERS], *v[CACHE_LAYERS];
+};
+struct CommitArgs {
+    const uint32_t *ctx, *path, *accepted;  // [b], [b][t], [b]
+    int b, t, h, hd, cap, first;            // first: this launch writes ctx_out
+    uint32_t *ctx_out;                      // [b] or null
+};
+hipError_t launch_commit(const CachePtrs &c, int layers, const CommitArgs &a, hipStream_t stream);
+struct EvictArgs {
+    const uint64_t *mass;  // [layers][b][h][cap]
+    const uint32_t *ctx;   // [b]
+    int b, h, hd, cap, budget, recent, layer0;  // layer0: the first layer of this launch
+    uint64_t *mass_out;    // mass, or an array of its own
+    uint32_t *ctx_out;     // [b] or null
+    uint32_t *kept;        // [layers][b][h][budget] or null
+};
+hipError_t launch_evict(const CachePtrs &c, int layers, const EvictArgs &a, hipStream_t stream);
+
 // The mix record of a row for the mixed coder op of the logs profile (8 u32 words, the layout of
 // crates/hardshell-cuda/src/mixed.rs:54-90): the predicted token p (MIX_NONE: no prediction,
 // weights max(1, w); MIX_PLAIN: the weights of GPT-2 alone), k and m of rule 5 (w'[i] = max(1,

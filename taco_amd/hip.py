@@ -10,7 +10,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 from dataclasses import dataclass
-from typing import Iterable, List, Optional, Sequence, Tuple
+from typing import Iterable, List, NamedTuple, Optional, Sequence, Tuple
 
 import numpy as np
 
@@ -159,6 +159,14 @@ def lib() -> C.CDLL:
         L.hs_op_attend_decode_dev.argtypes = [P, P, P, P, P, S, S, S, S, C.c_int32, C.c_uint8,
                                               C.c_int32, C.c_uint8, P, S, C.c_uint8, P, P]
         L.hs_op_attend_decode_dev_noalloc.argtypes = L.hs_op_attend_decode_dev.argtypes
+        rows = [P, P, P, P, P, P, P, S, S, S, S, S, C.c_int32, C.c_uint8, C.c_int32, C.c_uint8, P, S,
+                C.c_uint8, P, P, S, P]
+        L.hs_op_attend_tree_dev.argtypes = rows
+        L.hs_op_attend_mass_dev.argtypes = rows
+        L.hs_op_attend_rows_workspace.argtypes = [S] * 5
+        L.hs_op_attend_rows_workspace.restype = S
+        L.hs_op_cache_evict_dev.argtypes = [P, P, P, S, P, P, S, S, S, S, S, S, P, P, P, P]
+        L.hs_op_cache_commit_dev.argtypes = [P, P, P, S, P, P, P, S, S, S, S, S, P, P]
         L.hs_read_bw.argtypes = [P, S, S, C.POINTER(C.c_uint64)]
         L.hs_probe_issue.argtypes = [P, C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(C.c_uint64)]
         L.hs_model_load_with.argtypes = [P, P, S, P, C.POINTER(P)]
@@ -485,6 +493,96 @@ def gemm_requant_i8(dev: HipDevice, w, a, bias, mult, shift: int) -> np.ndarray:
     _check(lib().hs_op_gemm_requant_i8(dev.h, _ptr(w), _ptr(a), _ptr(bias), _ptr(mult), shift,
                                        m, n, k, _ptr(out)))
     return out
+
+
+def _dptr(x):
+    """The device address of x: a tensor (data_ptr()), an address or a ctypes pointer, or None."""
+    return x.data_ptr() if hasattr(x, "data_ptr") else x
+
+
+def _dptrs(xs):
+    """The layers' device addresses as a host array, from a list of them or from one contiguous tensor
+    whose first axis is the layers."""
+    if hasattr(xs, "data_ptr"):
+        if not xs.is_contiguous():
+            raise ValueError("a tensor of all layers' caches must be contiguous")
+        n, at = xs.shape[0], xs.data_ptr()
+        step = xs.stride(0) * xs.element_size()
+        return (C.c_void_p * n)(*range(at, at + n * step, step)) if step else (C.c_void_p * 0)()
+    return (C.c_void_p * len(xs))(*[_dptr(x) for x in xs])
+
+
+class AttentionRule(NamedTuple):
+    """The integer rule of an attention layer: score = clamp(rescale(q . k, score_m, score_s), +-2^40),
+    weights of softmax_p bits over the device table attn_exp of `length` i32 entries, outputs rescaled
+    by (out_m, out_s)."""
+    score_m: int
+    score_s: int
+    out_m: int
+    out_s: int
+    attn_exp: object
+    length: int
+    softmax_p: int
+
+
+def attend_tree(dev: HipDevice, q, k_cache, v_cache, ctx, nodes, mask, dims, rule: AttentionRule, out,
+                workspace=None, workspace_bytes: int = 0, stream=None) -> None:
+    """Attention of each stream's tree of drafted tokens over its cache (hs_op_attend_tree_dev): dims =
+    (streams, t, heads, head_dim, ctx_cap); nodes may be None (t each); `tree_mask` builds the mask."""
+    m, s, om, os_, table, length, p = rule
+    _check(lib().hs_op_attend_tree_dev(dev.h, _dptr(q), _dptr(k_cache), _dptr(v_cache), _dptr(ctx), _dptr(nodes),
+                                       _dptr(mask), *dims, m, s, om, os_, _dptr(table), length, p, _dptr(out),
+                                       _dptr(workspace), workspace_bytes, stream))
+
+
+def attend_mass(dev: HipDevice, q, k_cache, v_cache, ctx, rows, mass, dims, rule: AttentionRule, out,
+                workspace=None, workspace_bytes: int = 0, stream=None) -> None:
+    """Causal attention of the last rows of each stream that adds every key's weights to the u64
+    accumulators `mass` (hs_op_attend_mass_dev); dims as in attend_tree, rows may be None (t each)."""
+    m, s, om, os_, table, length, p = rule
+    _check(lib().hs_op_attend_mass_dev(dev.h, _dptr(q), _dptr(k_cache), _dptr(v_cache), _dptr(ctx), _dptr(rows),
+                                       _dptr(mass), *dims, m, s, om, os_, _dptr(table), length, p, _dptr(out),
+                                       _dptr(workspace), workspace_bytes, stream))
+
+
+def attend_rows_workspace(streams: int, t: int, heads: int, head_dim: int, ctx_cap: int) -> int:
+    """The bytes of workspace of attend_tree and attend_mass (hs_op_attend_rows_workspace)."""
+    return lib().hs_op_attend_rows_workspace(streams, t, heads, head_dim, ctx_cap)
+
+
+def tree_mask(parents) -> np.ndarray:
+    """The ancestor mask [t, ceil(t / 64)] u64 of a tree given as each node's parent (-1: the context's
+    end), parents before children."""
+    t = len(parents)
+    sees = np.zeros((t, (t + 63) // 64 * 64), bool)
+    for i, p in enumerate(parents):
+        if not -1 <= p < i:
+            raise ValueError(f"the parent of node {i} is {p}: parents come before their children")
+        if p >= 0:
+            sees[i] = sees[p]
+        sees[i, i] = True
+    return np.packbits(sees, axis=1, bitorder="little").view(np.uint64)
+
+
+def cache_evict(dev: HipDevice, k_caches, v_caches, mass, ctx, dims, budget: int, recent: int, mass_out, ctx_out,
+                kept=None, stream=None) -> None:
+    """Cuts the caches (a list of one a layer, or one tensor of all) to `budget` keys by accumulated weight, in
+    place (hs_op_cache_evict_dev): dims = (streams, heads, head_dim, ctx_cap)."""
+    k, v = _dptrs(k_caches), _dptrs(v_caches)
+    if len(k) != len(v):
+        raise LengthMismatch(HS_LENGTH_MISMATCH, 0, f"length mismatch: expected {len(k)}, found {len(v)}")
+    _check(lib().hs_op_cache_evict_dev(dev.h, k, v, len(k), _dptr(mass), _dptr(ctx), *dims, budget, recent,
+                                       _dptr(mass_out), _dptr(ctx_out), _dptr(kept), stream))
+
+
+def cache_commit(dev: HipDevice, k_caches, v_caches, ctx, path, accepted, dims, ctx_out, stream=None) -> None:
+    """Moves the rows of each stream's accepted path behind its context in every layer's cache
+    (hs_op_cache_commit_dev): dims = (streams, t, heads, head_dim, ctx_cap)."""
+    k, v = _dptrs(k_caches), _dptrs(v_caches)
+    if len(k) != len(v):
+        raise LengthMismatch(HS_LENGTH_MISMATCH, 0, f"length mismatch: expected {len(k)}, found {len(v)}")
+    _check(lib().hs_op_cache_commit_dev(dev.h, k, v, len(k), _dptr(ctx), _dptr(path), _dptr(accepted), *dims,
+                                        _dptr(ctx_out), stream))
 
 
 def kernel_resources(dev: HipDevice):
