@@ -213,7 +213,7 @@ def _run_own(s):
         hip.attend_mass(dev, s["q"], s["k"], s["v"], s["ctx"], s["rows"], s["mass"], (b, c["rows"], h, hd, cap), rule,
                         s["out"])
         return {"out": s["out"], "mass": s["mass"]}
-    k, v = list(s["k"]), list(s["v"])
+    k, v = s["k"], s["v"]  # one tensor of all layers
     if c["kind"] == "evict":
         hip.cache_evict(dev, k, v, s["mass"], s["ctx"], (b, h, hd, cap), c["budget"], c["recent"], s["mass_out"],
                         s["ctx_out"], s["kept"])
