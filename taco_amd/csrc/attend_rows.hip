@@ -108,11 +108,369 @@ __global__ __launch_bounds__(256) void k_rows(RowsArgs g, int n_tasks) {
                 (int8_t)clamp128(rescale_full(acc[u], a.out_m, a.out_s), -127, 127);
 }
 
+// ---- Tiles of 16 rows on MFMA ------------------------------------------------------------------------
+// One workgroup of NW waves takes 16 rows of one (stream, head); wave w the key blocks (64 keys) w, w + NW, ..,
+// at most NB of them, so every dot of the tile stays in registers (NB x 16 a lane) from the one product with K to
+// the product with V: K and V are read once. K is the first operand of v_mfma_i32_16x16x64_i8, so lane l holds
+// the dots of row l % 16 with keys 16 t + 4 (l / 16) + e of a block. The steps are those of k_attend_short: the
+// extreme dots (the score is monotone in the dot), the table entries and their sum, p as four balanced i8
+// digits, four products with V^T by transposing LDS reads; here the waves share the keys of the same rows, so the
+// extremes and the sums meet in LDS, and the output sums in 64-bit LDS atomics (integers: any order).
+// QC: 64-byte chunks of a head (the last one may be part empty: its lanes hold zeros).
+constexpr int RT_ROWS = 16;
+constexpr int RT_TABLE = 16384;  // entries of the table copied to LDS at most
+constexpr int RT_ACC = 66;       // 64 channels' sums of a row and two of padding (bank spread)
+
+// Sums over the 16 rows (lanes l % 16) of p of a block's 64 keys: lane l receives the sum of key
+// 16 (l % 16 / 4) + 4 (l / 16) + l % 4. A reduce-scatter in four steps: each lane hands half of what it holds to
+// its partner and keeps the other half.
+__device__ __forceinline__ uint64_t row_sums(const uint32_t (&p)[16], int lane) {
+    const bool b3 = lane & 8, b2 = lane & 4, b1 = lane & 2, b0 = lane & 1;
+    uint32_t x[8];  // two rows: at most 2^31
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        x[i] = (b3 ? p[i + 8] : p[i]) + (uint32_t)dpp_mov<0x140>((int32_t)(b3 ? p[i] : p[i + 8]));
+    uint64_t y[4], z[2];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        y[i] = (uint64_t)(b2 ? x[i + 4] : x[i]) + (uint32_t)dpp_mov<0x141>((int32_t)(b2 ? x[i] : x[i + 4]));
+#pragma unroll
+    for (int i = 0; i < 2; i++) z[i] = (b1 ? y[i + 2] : y[i]) + (uint64_t)lane_move64<1>((int64_t)(b1 ? y[i] : y[i + 2]));
+    return (b0 ? z[1] : z[0]) + (uint64_t)lane_move64<0>((int64_t)(b0 ? z[0] : z[1]));
+}
+
+// What a lane needs to know of its row: which keys it sees.
+struct RowSight {
+    int base, lim;  // a key below base + (tree: 0, causal: row + 1) is seen: key <= lim
+    const uint64_t *bits;  // the row's mask words (tree)
+    int count;             // nodes of the stream
+};
+
+__device__ __forceinline__ RowSight row_sight(const RowsArgs &g, const StreamRows &R, int row, int keys) {
+    RowSight v;
+    v.base = R.base;
+    v.count = R.count;
+    v.bits = nullptr;
+    const bool live = row < R.count;
+    if (g.mask) {
+        v.lim = live ? (R.base < keys ? R.base : keys) - 1 : -1;
+        v.bits = live ? R.mask + (size_t)row * g.words : nullptr;
+    } else {
+        v.lim = live ? (R.base + row < keys - 1 ? R.base + row : keys - 1) : -1;
+    }
+    return v;
+}
+
+// The keys 16 t + 4 qg + e of block kb that the row sees, bit 4 t + e.
+__device__ __forceinline__ uint32_t sight_bits(const RowSight &v, int kb, int qg, int keys) {
+    uint32_t ok = 0;
+    const int L = v.lim - 64 * kb - 4 * qg;
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) ok |= (16 * t + e <= L ? 1u : 0u) << (4 * t + e);
+    const int n0 = 64 * kb - v.base;  // the node of the block's first key
+    if (v.bits && n0 + 63 >= 0) {
+        // the 64 mask bits from node n0 on, those of nodes count .. and of keys past the cache cleared
+        const int words = (v.count + 63) >> 6, w = n0 >> 6, o = n0 & 63;
+        uint64_t m = w >= 0 && w < words ? v.bits[w] >> o : 0;
+        if (o && w + 1 >= 0 && w + 1 < words) m |= v.bits[w + 1] << (64 - o);
+        const int most = (v.count < keys - v.base ? v.count : keys - v.base) - n0;  // nodes of the block
+        m = most <= 0 ? 0 : (most < 64 ? m & (((uint64_t)1 << most) - 1) : m);
+        if (n0 < 0) m &= ~(uint64_t)0 << -n0;
+        m >>= 4 * qg;
+#pragma unroll
+        for (int t = 0; t < 4; t++) ok |= ((uint32_t)(m >> (16 * t)) & 15u) << (4 * t);
+    }
+    return ok;
+}
+
+template <bool S32>
+struct ScoreType {
+    typedef int64_t type;
+};
+template <>
+struct ScoreType<true> {
+    typedef int32_t type;
+};
+
+template <int QC, int NB, int NW, bool S32>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void k_rows_tile(RowsArgs g, int tiles, int panels) {
+    typedef typename ScoreType<S32>::type ST;
+    extern __shared__ __attribute__((aligned(1024))) int8_t s_mem[];
+    const AttnArgs &a = g.a;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ql = lane & 15, qg = lane >> 4;
+    // workgroup L runs on XCD L % 8: the tiles of a panel stay on one XCD and share K and V in its L2
+    const int L = blockIdx.x, panel = L / (8 * tiles) * 8 + (L & 7), tile = (L >> 3) % tiles;
+    if (panel >= panels) return;
+    const int s = panel / a.n_head, h = panel - s * a.n_head, hd = a.hd;
+    const StreamRows R = stream_rows(g, s);
+    const int row0 = RT_ROWS * tile, row = row0 + ql;
+    if (row0 >= R.count) return;
+    const int last = a.exp_len - 1, table_chunks = (a.exp_len + 255) / 256;
+    int32_t *s_exp = (int32_t *)s_mem;
+    int8_t *s_v = s_mem + 1024 * table_chunks + 4096 * w;
+    int64_t *s_acc = (int64_t *)(s_mem + 1024 * table_chunks + 4096 * NW);  // [QC][16][RT_ACC]
+    uint64_t *s_sum = (uint64_t *)(s_acc + QC * RT_ROWS * RT_ACC);          // [NW][16]
+    int32_t *s_mm = (int32_t *)(s_sum + NW * RT_ROWS);                      // [2][NW][16]
+
+    int keys = stream_keys(g, R);
+    if (!g.mask) keys = R.base + row0 + RT_ROWS < keys ? R.base + row0 + RT_ROWS : keys;  // causal: the tile's last row
+    keys = keys < 64 * NB * NW ? keys : 64 * NB * NW;  // (the launch's bound holds every count)
+    const int kmost = keys > 0 ? keys - 1 : 0;
+    const size_t base = ((size_t)R.slot * a.n_head + h) * a.ctx_cap * hd;
+    const int8_t *K = a.kc + base, *V = a.vc + base;
+    auto mine = [&](int j) { return 64 * (NW * j + w) < keys; };  // uniform
+
+    const v4i zero = v4i{0, 0, 0, 0};
+    v4i qf[QC];
+#pragma unroll
+    for (int c = 0; c < QC; c++) {
+        const int at = 64 * c + 16 * qg;
+        qf[c] = row < R.count && at < hd ? *(const v4i *)(a.q + (size_t)(R.first + row) * a.ldq + h * hd + at) : zero;
+    }
+    for (int ch = w; ch < table_chunks; ch += NW) {  // the table; a lane past its end reads the last entry
+        const int i = 256 * ch + 4 * lane;
+#pragma unroll
+        for (int e = 0; e < 4; e++) s_exp[i + e] = a.exp_table[i + e < last ? i + e : last];
+    }
+    for (int i = tid; i < QC * RT_ROWS * RT_ACC; i += 64 * NW) s_acc[i] = 0;
+
+    // the dots: D[j][t][e] of key 64 (NW j + w) + 16 t + 4 qg + e (keys past the last reload it)
+    v4i D[NB][4];
+    auto k_row = [&](int j, int t) {
+        const int k = 64 * (NW * j + w) + 16 * t + ql;
+        return K + (size_t)(k < keys ? k : kmost) * hd + 16 * qg;
+    };
+#pragma unroll
+    for (int j = 0; j < NB; j++) {
+        if (!mine(j)) continue;
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const int8_t *k = k_row(j, t);
+            v4i d = zero;
+#pragma unroll
+            for (int c = 0; c < QC; c++)
+                d = __builtin_amdgcn_mfma_i32_16x16x64_i8(64 * c + 16 * qg < hd ? *(const v4i *)(k + 64 * c) : zero, qf[c], d, 0, 0, 0);
+            D[j][t] = d;
+        }
+    }
+    // V of chunk group c, block j: lane l the 16 bytes (l % 4) ^ vsw of rows 16 u + l / 4
+    v4i vr[NB][4];
+    auto v_load = [&](int j, int c) {
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int r = 16 * u + (lane >> 2), k = 64 * (NW * j + w) + r, at = 64 * c + 16 * ((lane & 3) ^ vsw<4>(r & 15));
+            vr[j][u] = at < hd ? *(const v4i *)(V + (size_t)(k < keys ? k : kmost) * hd + at) : zero;
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < NB; j++)
+        if (mine(j)) v_load(j, 0);
+
+    const RowSight sight = row_sight(g, R, row, keys);
+    // a block whose keys every live row sees whole
+    const int whole = g.mask ? R.base : R.base + row0 + 1;
+    auto sees_all = [&](int j) { return 64 * (NW * j + w) + 64 <= whole && 64 * (NW * j + w) + 64 <= keys; };
+    uint32_t ok[NB];
+    int32_t dmax = INT32_MIN, dmin = INT32_MAX;
+#pragma unroll
+    for (int j = 0; j < NB; j++) {
+        ok[j] = 0;
+        if (!mine(j)) continue;
+        ok[j] = sees_all(j) ? 0xffffu : sight_bits(sight, NW * j + w, qg, keys);
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const bool in = (ok[j] >> (4 * t + e)) & 1;
+                const int32_t hi = in ? D[j][t][e] : INT32_MIN, lo = in ? D[j][t][e] : INT32_MAX;
+                dmax = hi > dmax ? hi : dmax;
+                dmin = lo < dmin ? lo : dmin;
+            }
+    }
+#pragma unroll
+    for (int o = 16; o < 64; o <<= 1) {  // the four lanes of the row
+        const int32_t x = __shfl_xor(dmax, o, 64), y = __shfl_xor(dmin, o, 64);
+        dmax = x > dmax ? x : dmax;
+        dmin = y < dmin ? y : dmin;
+    }
+    if (qg == 0) {
+        s_mm[w * RT_ROWS + ql] = dmax;
+        s_mm[(NW + w) * RT_ROWS + ql] = dmin;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NW; i++) {
+        const int32_t x = s_mm[i * RT_ROWS + ql], y = s_mm[(NW + i) * RT_ROWS + ql];
+        dmax = x > dmax ? x : dmax;
+        dmin = y < dmin ? y : dmin;
+    }
+    if (dmax < dmin) dmax = dmin = 0;  // a row that sees nothing: every entry below is masked
+    // the score: an i32 whose differences are i32 too where S32 (the launcher's condition)
+    const int s_eff = a.score_s < 63 ? a.score_s : 63;
+    const int64_t s_half = s_eff ? (int64_t)1 << (s_eff - 1) : 0;
+    auto score = [&](int32_t dot) -> ST {
+        if constexpr (S32) return (int32_t)(((int64_t)dot * a.score_m + s_half) >> s_eff);
+        else return attn_score<false>(a, dot);
+    };
+    const ST m0 = score(dmax), m1 = score(dmin), M = m0 > m1 ? m0 : m1;
+    uint64_t sum = 0;
+#pragma unroll
+    for (int j = 0; j < NB; j++) {
+        if (!mine(j)) continue;
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                // a masked key's score may lie above M: its index is clamped at 0 too
+                if constexpr (S32) {
+                    D[j][t][e] = clamp0_uniform((int32_t)((uint32_t)M - (uint32_t)score(D[j][t][e])), last);
+                } else {
+                    const int64_t dd = M - score(D[j][t][e]);
+                    D[j][t][e] = (int32_t)clamp64(dd, 0, last);
+                }
+            }
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) D[j][t][e] = s_exp[D[j][t][e]];
+        if (!sees_all(j)) {
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) D[j][t][e] = (ok[j] >> (4 * t + e)) & 1 ? D[j][t][e] : 0;
+        }
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) sum += (uint32_t)D[j][t][e] + (uint32_t)D[j][t][e + 1];  // entries below 2^31
+    }
+#pragma unroll
+    for (int o = 16; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+    if (qg == 0) s_sum[w * RT_ROWS + ql] = sum;
+    __syncthreads();
+    sum = 0;
+#pragma unroll
+    for (int i = 0; i < NW; i++) sum += s_sum[i * RT_ROWS + ql];
+    // rows that are not there and rows without weight: p = 0 (R = 0)
+    const double Rs = sum > 0 && row < R.count ? ldexp(1.0 / (double)sum, a.softmax_p) : 0.0;
+    const double sp = softmax_sp(sum, a.softmax_p);
+    v4i (*pf)[4] = D;  // in place: pf[j][k] word t holds digit k of keys 16 t + 4 qg + e
+#pragma unroll
+    for (int j = 0; j < NB; j++) {
+        if (!mine(j)) continue;
+        uint32_t p[16], o[4][4];
+#pragma unroll
+        for (int i = 0; i < 16; i++) p[i] = softmax_p_of((uint32_t)D[j][i >> 2][i & 3], Rs, sp);
+        if (g.mass) {  // uniform
+            const uint64_t x = row_sums(p, lane);
+            const int key = 64 * (NW * j + w) + 16 * (ql >> 2) + 4 * qg + (ql & 3);
+            if (x && key < keys)
+                atomicAdd((unsigned long long *)g.mass + ((size_t)R.slot * a.n_head + h) * a.ctx_cap + key, (unsigned long long)x);
+        }
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+            byte_transpose(p[4 * t] + 0x80808080u, p[4 * t + 1] + 0x80808080u, p[4 * t + 2] + 0x80808080u,
+                           p[4 * t + 3] + 0x80808080u, o[t]);
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) pf[j][k][t] = (int32_t)(o[t][k] ^ 0x80808080u);
+    }
+    const int tr_k = ql >> 1, tr_h = ql & 1, key0 = 16 * (tr_k >> 2) + 4 * qg + (tr_k & 3);
+#pragma unroll
+    for (int c = 0; c < QC; c++) {
+        v4i acc[4][4];  // [digit plane][channel tile]: channel 16 i + 4 qg + e of row ql
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[k][i] = zero;
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+            if (!mine(j)) continue;
+#pragma unroll
+            for (int u = 0; u < 4; u++) *(v4i *)(s_v + 1024 * u + 16 * lane) = vr[j][u];
+            if (c + 1 < QC) v_load(j, c + 1);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int8_t *p0 = s_v + (4 * key0 + (i ^ vsw<4>(key0 & 15))) * 16 + 8 * tr_h;
+                const v2i r0 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)p0);
+                const v2i r1 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)(p0 + 32 * 64));
+                const v4i vf = v4i{r0[0], r0[1], r1[0], r1[1]};
+#pragma unroll
+                for (int k = 0; k < 4; k++) acc[k][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf, pf[j][k], acc[k][i], 0, 0, 0);
+            }
+        }
+        if (mine(0)) {
+            unsigned long long *to = (unsigned long long *)s_acc + (c * RT_ROWS + ql) * RT_ACC + 4 * qg;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    atomicAdd(to + 16 * i + e, (unsigned long long)((int64_t)acc[0][i][e] + (int64_t)acc[1][i][e] * 256 +
+                                                                    (int64_t)acc[2][i][e] * 65536 + (int64_t)acc[3][i][e] * 16777216));
+        }
+    }
+    __syncthreads();
+    const double mo = a.out_s > 95 ? 0.0 : ldexp((double)a.out_m, -a.out_s);
+    for (int i = tid; i < RT_ROWS * hd / 4; i += 64 * NW) {
+        const int r = i / (hd / 4), ch = 4 * (i - r * (hd / 4));
+        if (row0 + r >= R.count) break;
+        const int64_t *x = s_acc + ((ch >> 6) * RT_ROWS + r) * RT_ACC + (ch & 63);
+        uint32_t packed = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) packed |= (uint32_t)(uint8_t)(int8_t)attn_out_byte(x[e], mo, a.out_m, a.out_s) << (8 * e);
+        *(uint32_t *)attn_out(a, R.first + row0 + r, h * hd + ch) = packed;
+    }
+}
+
+template <int QC, int NB, int NW, bool S32>
+static hipError_t launch_tile_t(const RowsArgs &g, hipStream_t stream) {
+    const int tiles = (g.t + RT_ROWS - 1) / RT_ROWS, panels = g.streams * g.a.n_head;
+    const size_t lds = (size_t)1024 * ((g.a.exp_len + 255) / 256) + 4096 * NW + 8 * QC * RT_ROWS * RT_ACC + 16 * NW * RT_ROWS;
+    const hipError_t e = allow_dynamic_lds((const void *)k_rows_tile<QC, NB, NW, S32>, lds);
+    if (e != hipSuccess) return e;
+    launch_k((k_rows_tile<QC, NB, NW, S32>), dim3((unsigned)((panels + 7) / 8 * 8) * tiles), dim3(64 * NW), lds, stream, g, tiles, panels);
+    return hipGetLastError();
+}
+
+template <int QC, bool S32>
+static hipError_t launch_tile(const RowsArgs &g, int keys, hipStream_t stream) {
+    if (keys <= 256) return launch_tile_t<QC, 1, 4, S32>(g, stream);
+    if (keys <= 512) return launch_tile_t<QC, 2, 4, S32>(g, stream);
+    if (keys <= 1024) return launch_tile_t<QC, 4, 4, S32>(g, stream);
+    return launch_tile_t<QC, 4, 8, S32>(g, stream);
+}
+
+constexpr int RT_KEYS = 2048;  // the most keys of a tile in one launch
+
+// Scores and their differences are i32: |dot| <= hd 2^14, |score_m| <= 2^31, so |score| <= hd 2^(45 - s) <= 2^29.
+static bool rows_s32(const AttnArgs &a) {
+    int bits = 0;
+    while ((1 << bits) < a.hd) bits++;
+    return a.score_s >= 16 + bits;
+}
+
+static bool rows_tile_ok(const RowsArgs &g, int keys) {
+    const AttnArgs &a = g.a;
+    const bool aligned = (((uintptr_t)a.q | (uintptr_t)a.kc | (uintptr_t)a.vc | (uintptr_t)a.ldq | (uintptr_t)a.hd) & 15) == 0;
+    const long long tiles = (g.t + RT_ROWS - 1) / RT_ROWS;
+    return aligned && a.exp_len <= RT_TABLE && keys <= RT_KEYS && ((long long)g.streams * a.n_head + 7) * tiles < (1ll << 31);
+}
+
 size_t rows_workspace(const RowsArgs &) { return 0; }
 
 hipError_t launch_rows(const RowsArgs &g, void *, hipStream_t stream) {
-    const int tasks = g.streams * g.t * g.a.n_head;
+    const int tasks = g.streams * g.t * g.a.n_head, keys = g.a.ctx_cap;
     if (tasks <= 0) return hipSuccess;
+    if (rows_tile_ok(g, keys)) {
+        const bool s32 = rows_s32(g.a);
+        if (g.a.hd <= 64) return s32 ? launch_tile<1, true>(g, keys, stream) : launch_tile<1, false>(g, keys, stream);
+        if (g.a.hd <= 128) return s32 ? launch_tile<2, true>(g, keys, stream) : launch_tile<2, false>(g, keys, stream);
+        return s32 ? launch_tile<4, true>(g, keys, stream) : launch_tile<4, false>(g, keys, stream);
+    }
     launch_k(k_rows, dim3((tasks + 3) / 4), dim3(256), 0, stream, g, tasks);
     return hipGetLastError();
 }
