@@ -185,18 +185,156 @@ __device__ __forceinline__ uint32_t sight_bits(const RowSight &v, int kb, int qg
     return ok;
 }
 
-template <bool S32>
-struct ScoreType {
-    typedef int64_t type;
-};
-template <>
-struct ScoreType<true> {
-    typedef int32_t type;
+// ---- The steps on a block: 64 keys x 16 rows, D[t][e] of lane l belongs to row l % 16 and key 16 t + 4 (l / 16) + e
+
+// The largest and smallest dot among the keys the row sees.
+__device__ __forceinline__ void block_extremes(const v4i (&D)[4], bool all, uint32_t ok, int32_t &dmax, int32_t &dmin) {
+    if (all) {  // uniform
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                dmax = D[t][e] > dmax ? D[t][e] : dmax;
+                dmin = D[t][e] < dmin ? D[t][e] : dmin;
+            }
+    } else {
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const bool in = (ok >> (4 * t + e)) & 1;
+                const int32_t hi = in ? D[t][e] : INT32_MIN, lo = in ? D[t][e] : INT32_MAX;
+                dmax = hi > dmax ? hi : dmax;
+                dmin = lo < dmin ? lo : dmin;
+            }
+    }
+}
+
+// The table index min(M - score(dot), last) of a row whose extreme dots are dmax and dmin (the score is monotone
+// in the dot, so M is the score of one of them). Shifts from 32 to 60 (HI; m > -2^31): with x = the high word of
+// dot m + 2^(s-1) and h = s - 32 the score is x >> h, |x| <= 2^21 + 2^27, and
+//   M - (x >> h) = (M 2^h + 2^h - 1 - x) >> h,  -x = the high word of -dot m + 2^32 - 1 - 2^(s-1),
+// so one multiply-add with the row's constant, a shift and a minimum give the index (a masked key's may be
+// negative: as an unsigned number it is past the table, and its entry is not used).
+template <bool HI>
+struct RowIndex {
+    int64_t c;  // HI: the row's addend; else M
+    __device__ __forceinline__ RowIndex(const AttnArgs &a, int32_t dmax, int32_t dmin) {
+        if (dmax < dmin) dmax = dmin = 0;  // a row that sees nothing
+        const int64_t s0 = attn_score<HI>(a, dmax), s1 = attn_score<HI>(a, dmin);
+        const int64_t M = s0 > s1 ? s0 : s1;
+        const int h = a.score_s - 32;
+        if constexpr (HI) c = (((M + 1) << h) - 1) * ((int64_t)1 << 32) + 0xffffffffll - ((int64_t)1 << (a.score_s - 1));
+        else c = M;
+    }
+    __device__ __forceinline__ int32_t at(const AttnArgs &a, int32_t dot, int32_t last) const {
+        if constexpr (HI) {
+            const int64_t y = (int64_t)dot * (-a.score_m) + c;
+            const uint32_t i = (uint32_t)((int32_t)(y >> 32) >> (a.score_s - 32));
+            return (int32_t)(i < (uint32_t)last ? i : (uint32_t)last);
+        } else {
+            return (int32_t)clamp64(c - attn_score<false>(a, dot), 0, last);
+        }
+    }
 };
 
-template <int QC, int NB, int NW, bool S32>
+// The dots of a block to its table entries, in place (0 where the row does not see the key).
+template <bool HI>
+__device__ __forceinline__ void block_entries(const AttnArgs &a, v4i (&D)[4], const RowIndex<HI> &ix, const int32_t *s_exp,
+                                              int32_t last, bool all, uint32_t ok) {
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) D[t][e] = ix.at(a, D[t][e], last);
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) D[t][e] = s_exp[D[t][e]];
+    if (!all) {
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) D[t][e] = (ok >> (4 * t + e)) & 1 ? D[t][e] : 0;
+    }
+}
+
+// Their sum (entries are below 2^31: a pair sums in 32 bits).
+__device__ __forceinline__ uint64_t block_sum(const v4i (&D)[4]) {
+    uint64_t s = 0;
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) s += (uint32_t)D[t][e] + (uint32_t)D[t][e + 1];
+    return s;
+}
+
+// The entries of a block to the digit planes of p = floor(e 2^P / S), in place: D[k] word t holds digit k of keys
+// 16 t + 4 (l / 16) + e. The rule of softmax_p_of with 0x80808080 inside the rounding constant: the low word of the sum
+// is p + 0x80808080 at once, whose bytes xor 0x80 are the balanced digits. Where `mass` is set, each key's weights
+// summed over the 16 rows are added to it.
+__device__ __forceinline__ void block_digits(v4i (&D)[4], double R, double sp, uint64_t *mass, int keys, int lane) {
+    constexpr double magic = 6755399441055744.0 + 2155905152.0;  // 1.5 2^52 + 0x80808080
+    uint32_t o[4][4], dg[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        const double ed = (double)(uint32_t)D[i >> 2][i & 3], w = fma(ed, R, magic), r = fma(w - magic, sp, ed);
+        dg[i] = (uint32_t)__double2loint(w) + (uint32_t)(__double2hiint(r) >> 31);
+    }
+    if (mass) {  // uniform
+        uint32_t p[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) p[i] = dg[i] - 0x80808080u;
+        const uint64_t x = row_sums(p, lane);
+        const int key = 16 * ((lane & 15) >> 2) + 4 * (lane >> 4) + (lane & 3);
+        if (x && key < keys) atomicAdd((unsigned long long *)mass + key, (unsigned long long)x);
+    }
+#pragma unroll
+    for (int t = 0; t < 4; t++) byte_transpose(dg[4 * t], dg[4 * t + 1], dg[4 * t + 2], dg[4 * t + 3], o[t]);
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+#pragma unroll
+        for (int t = 0; t < 4; t++) D[k][t] = (int32_t)(o[t][k] ^ 0x80808080u);
+}
+
+// The factors of p of a row (softmax_p_of); rows that are not there and rows without weight: p = 0 (R = 0).
+struct RowWeight {
+    double R, sp;
+    __device__ __forceinline__ RowWeight(uint64_t sum, int P, bool live)
+        : R(sum > 0 && live ? ldexp(1.0 / (double)sum, P) : 0.0), sp(softmax_sp(sum, P)) {}
+};
+
+// acc[k][i] += V^T digits over a block whose V rows lie in s_v (16-byte chunk c of row r at slot 4 r + (c ^ vsw(r))):
+// channel 16 i + 4 (l / 16) + e of row l % 16.
+__device__ __forceinline__ void block_pv(const int8_t *s_v, const v4i (&pf)[4], int lane, v4i (&acc)[4][4]) {
+    const int ql = lane & 15, qg = lane >> 4, tr_k = ql >> 1, key0 = 16 * (tr_k >> 2) + 4 * qg + (tr_k & 3);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int8_t *p0 = s_v + (4 * key0 + (i ^ vsw<4>(key0 & 15))) * 16 + 8 * (ql & 1);
+        const v2i r0 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)p0);
+        const v2i r1 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)(p0 + 32 * 64));
+        const v4i vf = v4i{r0[0], r0[1], r1[0], r1[1]};
+#pragma unroll
+        for (int k = 0; k < 4; k++) acc[k][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf, pf[k], acc[k][i], 0, 0, 0);
+    }
+}
+
+__device__ __forceinline__ int64_t plane_sum(const v4i (&acc)[4][4], int i, int e) {
+    return (int64_t)acc[0][i][e] + (int64_t)acc[1][i][e] * 256 + (int64_t)acc[2][i][e] * 65536 +
+           (int64_t)acc[3][i][e] * 16777216;
+}
+
+// The table to LDS: whole KiB straight, the end entry by entry (places past it repeat the last one). The caller waits.
+__device__ __forceinline__ void load_table(const AttnArgs &a, int32_t *s_exp, int w, int waves, int lane) {
+    const int whole = a.exp_len / 256;
+    for (int ch = w; ch < whole; ch += waves)
+        __builtin_amdgcn_global_load_lds((const void *)(a.exp_table + ch * 256 + 4 * lane), (lds_void *)(s_exp + ch * 256), 16, 0, 0);
+    if (w == 0)
+        for (int i = 256 * whole + lane; i < (a.exp_len + 255) / 256 * 256; i += 64)
+            s_exp[i] = a.exp_table[i < a.exp_len ? i : a.exp_len - 1];
+}
+
+template <int QC, int NB, int NW, bool HI>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void k_rows_tile(RowsArgs g, int tiles, int panels) {
-    typedef typename ScoreType<S32>::type ST;
     extern __shared__ __attribute__((aligned(1024))) int8_t s_mem[];
     const AttnArgs &a = g.a;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -219,40 +357,36 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     if (!g.mask) keys = R.base + row0 + RT_ROWS < keys ? R.base + row0 + RT_ROWS : keys;  // causal: the tile's last row
     keys = keys < 64 * NB * NW ? keys : 64 * NB * NW;  // (the launch's bound holds every count)
     const int kmost = keys > 0 ? keys - 1 : 0;
-    const size_t base = ((size_t)R.slot * a.n_head + h) * a.ctx_cap * hd;
+    const size_t at = (size_t)R.slot * a.n_head + h, base = at * a.ctx_cap * hd;
     const int8_t *K = a.kc + base, *V = a.vc + base;
-    auto mine = [&](int j) { return 64 * (NW * j + w) < keys; };  // uniform
+    auto block = [&](int j) { return NW * j + w; };
+    auto mine = [&](int j) { return 64 * block(j) < keys; };  // uniform
 
     const v4i zero = v4i{0, 0, 0, 0};
+    load_table(a, s_exp, w, NW, lane);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);  // the table's loads before those of K: who has K has the table
     v4i qf[QC];
 #pragma unroll
     for (int c = 0; c < QC; c++) {
-        const int at = 64 * c + 16 * qg;
-        qf[c] = row < R.count && at < hd ? *(const v4i *)(a.q + (size_t)(R.first + row) * a.ldq + h * hd + at) : zero;
-    }
-    for (int ch = w; ch < table_chunks; ch += NW) {  // the table; a lane past its end reads the last entry
-        const int i = 256 * ch + 4 * lane;
-#pragma unroll
-        for (int e = 0; e < 4; e++) s_exp[i + e] = a.exp_table[i + e < last ? i + e : last];
+        const int o = 64 * c + 16 * qg;
+        qf[c] = row < R.count && o < hd ? *(const v4i *)(a.q + (size_t)(R.first + row) * a.ldq + h * hd + o) : zero;
     }
     for (int i = tid; i < QC * RT_ROWS * RT_ACC; i += 64 * NW) s_acc[i] = 0;
 
-    // the dots: D[j][t][e] of key 64 (NW j + w) + 16 t + 4 qg + e (keys past the last reload it)
+    // the dots (keys past the last reload it)
     v4i D[NB][4];
-    auto k_row = [&](int j, int t) {
-        const int k = 64 * (NW * j + w) + 16 * t + ql;
-        return K + (size_t)(k < keys ? k : kmost) * hd + 16 * qg;
-    };
 #pragma unroll
     for (int j = 0; j < NB; j++) {
         if (!mine(j)) continue;
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            const int8_t *k = k_row(j, t);
+            const int k = 64 * block(j) + 16 * t + ql;
+            const int8_t *kr = K + (size_t)(k < keys ? k : kmost) * hd + 16 * qg;
             v4i d = zero;
 #pragma unroll
             for (int c = 0; c < QC; c++)
-                d = __builtin_amdgcn_mfma_i32_16x16x64_i8(64 * c + 16 * qg < hd ? *(const v4i *)(k + 64 * c) : zero, qf[c], d, 0, 0, 0);
+                d = __builtin_amdgcn_mfma_i32_16x16x64_i8(64 * c + 16 * qg < hd ? *(const v4i *)(kr + 64 * c) : zero, qf[c], d, 0, 0, 0);
             D[j][t] = d;
         }
     }
@@ -261,8 +395,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     auto v_load = [&](int j, int c) {
 #pragma unroll
         for (int u = 0; u < 4; u++) {
-            const int r = 16 * u + (lane >> 2), k = 64 * (NW * j + w) + r, at = 64 * c + 16 * ((lane & 3) ^ vsw<4>(r & 15));
-            vr[j][u] = at < hd ? *(const v4i *)(V + (size_t)(k < keys ? k : kmost) * hd + at) : zero;
+            const int r = 16 * u + (lane >> 2), k = 64 * block(j) + r, o = 64 * c + 16 * ((lane & 3) ^ vsw<4>(r & 15));
+            vr[j][u] = o < hd ? *(const v4i *)(V + (size_t)(k < keys ? k : kmost) * hd + o) : zero;
         }
     };
 #pragma unroll
@@ -270,25 +404,17 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         if (mine(j)) v_load(j, 0);
 
     const RowSight sight = row_sight(g, R, row, keys);
-    // a block whose keys every live row sees whole
+    // a block whose keys every row of the tile sees
     const int whole = g.mask ? R.base : R.base + row0 + 1;
-    auto sees_all = [&](int j) { return 64 * (NW * j + w) + 64 <= whole && 64 * (NW * j + w) + 64 <= keys; };
+    auto all = [&](int j) { return 64 * block(j) + 64 <= (whole < keys ? whole : keys); };
     uint32_t ok[NB];
     int32_t dmax = INT32_MIN, dmin = INT32_MAX;
 #pragma unroll
     for (int j = 0; j < NB; j++) {
         ok[j] = 0;
         if (!mine(j)) continue;
-        ok[j] = sees_all(j) ? 0xffffu : sight_bits(sight, NW * j + w, qg, keys);
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const bool in = (ok[j] >> (4 * t + e)) & 1;
-                const int32_t hi = in ? D[j][t][e] : INT32_MIN, lo = in ? D[j][t][e] : INT32_MAX;
-                dmax = hi > dmax ? hi : dmax;
-                dmin = lo < dmin ? lo : dmin;
-            }
+        if (!all(j)) ok[j] = sight_bits(sight, block(j), qg, keys);
+        block_extremes(D[j], all(j), ok[j], dmax, dmin);
     }
 #pragma unroll
     for (int o = 16; o < 64; o <<= 1) {  // the four lanes of the row
@@ -300,89 +426,37 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         s_mm[w * RT_ROWS + ql] = dmax;
         s_mm[(NW + w) * RT_ROWS + ql] = dmin;
     }
-    __syncthreads();
+    if (!mine(0)) wait_vmcnt<0>();  // (no K to wait for)
+    lds_barrier();                  // not the fence of __syncthreads, which would wait for V too
 #pragma unroll
     for (int i = 0; i < NW; i++) {
         const int32_t x = s_mm[i * RT_ROWS + ql], y = s_mm[(NW + i) * RT_ROWS + ql];
         dmax = x > dmax ? x : dmax;
         dmin = y < dmin ? y : dmin;
     }
-    if (dmax < dmin) dmax = dmin = 0;  // a row that sees nothing: every entry below is masked
-    // the score: an i32 whose differences are i32 too where S32 (the launcher's condition)
-    const int s_eff = a.score_s < 63 ? a.score_s : 63;
-    const int64_t s_half = s_eff ? (int64_t)1 << (s_eff - 1) : 0;
-    auto score = [&](int32_t dot) -> ST {
-        if constexpr (S32) return (int32_t)(((int64_t)dot * a.score_m + s_half) >> s_eff);
-        else return attn_score<false>(a, dot);
-    };
-    const ST m0 = score(dmax), m1 = score(dmin), M = m0 > m1 ? m0 : m1;
+    const RowIndex<HI> ix(a, dmax, dmin);
     uint64_t sum = 0;
 #pragma unroll
     for (int j = 0; j < NB; j++) {
         if (!mine(j)) continue;
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                // a masked key's score may lie above M: its index is clamped at 0 too
-                if constexpr (S32) {
-                    D[j][t][e] = clamp0_uniform((int32_t)((uint32_t)M - (uint32_t)score(D[j][t][e])), last);
-                } else {
-                    const int64_t dd = M - score(D[j][t][e]);
-                    D[j][t][e] = (int32_t)clamp64(dd, 0, last);
-                }
-            }
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) D[j][t][e] = s_exp[D[j][t][e]];
-        if (!sees_all(j)) {
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) D[j][t][e] = (ok[j] >> (4 * t + e)) & 1 ? D[j][t][e] : 0;
-        }
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e += 2) sum += (uint32_t)D[j][t][e] + (uint32_t)D[j][t][e + 1];  // entries below 2^31
+        block_entries<HI>(a, D[j], ix, s_exp, last, all(j), ok[j]);
+        sum += block_sum(D[j]);
     }
 #pragma unroll
     for (int o = 16; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
     if (qg == 0) s_sum[w * RT_ROWS + ql] = sum;
-    __syncthreads();
+    lds_barrier();
     sum = 0;
 #pragma unroll
     for (int i = 0; i < NW; i++) sum += s_sum[i * RT_ROWS + ql];
-    // rows that are not there and rows without weight: p = 0 (R = 0)
-    const double Rs = sum > 0 && row < R.count ? ldexp(1.0 / (double)sum, a.softmax_p) : 0.0;
-    const double sp = softmax_sp(sum, a.softmax_p);
-    v4i (*pf)[4] = D;  // in place: pf[j][k] word t holds digit k of keys 16 t + 4 qg + e
+    const RowWeight wt(sum, a.softmax_p, row < R.count);
 #pragma unroll
-    for (int j = 0; j < NB; j++) {
-        if (!mine(j)) continue;
-        uint32_t p[16], o[4][4];
-#pragma unroll
-        for (int i = 0; i < 16; i++) p[i] = softmax_p_of((uint32_t)D[j][i >> 2][i & 3], Rs, sp);
-        if (g.mass) {  // uniform
-            const uint64_t x = row_sums(p, lane);
-            const int key = 64 * (NW * j + w) + 16 * (ql >> 2) + 4 * qg + (ql & 3);
-            if (x && key < keys)
-                atomicAdd((unsigned long long *)g.mass + ((size_t)R.slot * a.n_head + h) * a.ctx_cap + key, (unsigned long long)x);
-        }
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-            byte_transpose(p[4 * t] + 0x80808080u, p[4 * t + 1] + 0x80808080u, p[4 * t + 2] + 0x80808080u,
-                           p[4 * t + 3] + 0x80808080u, o[t]);
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-#pragma unroll
-            for (int t = 0; t < 4; t++) pf[j][k][t] = (int32_t)(o[t][k] ^ 0x80808080u);
-    }
-    const int tr_k = ql >> 1, tr_h = ql & 1, key0 = 16 * (tr_k >> 2) + 4 * qg + (tr_k & 3);
+    for (int j = 0; j < NB; j++)
+        if (mine(j))
+            block_digits(D[j], wt.R, wt.sp, g.mass ? g.mass + at * a.ctx_cap + 64 * block(j) : nullptr, keys - 64 * block(j), lane);
 #pragma unroll
     for (int c = 0; c < QC; c++) {
-        v4i acc[4][4];  // [digit plane][channel tile]: channel 16 i + 4 qg + e of row ql
+        v4i acc[4][4];
 #pragma unroll
         for (int k = 0; k < 4; k++)
 #pragma unroll
@@ -393,27 +467,17 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
 #pragma unroll
             for (int u = 0; u < 4; u++) *(v4i *)(s_v + 1024 * u + 16 * lane) = vr[j][u];
             if (c + 1 < QC) v_load(j, c + 1);
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int8_t *p0 = s_v + (4 * key0 + (i ^ vsw<4>(key0 & 15))) * 16 + 8 * tr_h;
-                const v2i r0 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)p0);
-                const v2i r1 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)(p0 + 32 * 64));
-                const v4i vf = v4i{r0[0], r0[1], r1[0], r1[1]};
-#pragma unroll
-                for (int k = 0; k < 4; k++) acc[k][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf, pf[j][k], acc[k][i], 0, 0, 0);
-            }
+            block_pv(s_v, D[j], lane, acc);
         }
         if (mine(0)) {
             unsigned long long *to = (unsigned long long *)s_acc + (c * RT_ROWS + ql) * RT_ACC + 4 * qg;
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    atomicAdd(to + 16 * i + e, (unsigned long long)((int64_t)acc[0][i][e] + (int64_t)acc[1][i][e] * 256 +
-                                                                    (int64_t)acc[2][i][e] * 65536 + (int64_t)acc[3][i][e] * 16777216));
+                for (int e = 0; e < 4; e++) atomicAdd(to + 16 * i + e, (unsigned long long)plane_sum(acc, i, e));
         }
     }
-    __syncthreads();
+    lds_barrier();
     const double mo = a.out_s > 95 ? 0.0 : ldexp((double)a.out_m, -a.out_s);
     for (int i = tid; i < RT_ROWS * hd / 4; i += 64 * NW) {
         const int r = i / (hd / 4), ch = 4 * (i - r * (hd / 4));
@@ -426,38 +490,33 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     }
 }
 
-template <int QC, int NB, int NW, bool S32>
+template <int QC, int NB, int NW, bool HI>
 static hipError_t launch_tile_t(const RowsArgs &g, hipStream_t stream) {
     const int tiles = (g.t + RT_ROWS - 1) / RT_ROWS, panels = g.streams * g.a.n_head;
     const size_t lds = (size_t)1024 * ((g.a.exp_len + 255) / 256) + 4096 * NW + 8 * QC * RT_ROWS * RT_ACC + 16 * NW * RT_ROWS;
-    const hipError_t e = allow_dynamic_lds((const void *)k_rows_tile<QC, NB, NW, S32>, lds);
+    const hipError_t e = allow_dynamic_lds((const void *)k_rows_tile<QC, NB, NW, HI>, lds);
     if (e != hipSuccess) return e;
-    launch_k((k_rows_tile<QC, NB, NW, S32>), dim3((unsigned)((panels + 7) / 8 * 8) * tiles), dim3(64 * NW), lds, stream, g, tiles, panels);
+    launch_k((k_rows_tile<QC, NB, NW, HI>), dim3((unsigned)((panels + 7) / 8 * 8) * tiles), dim3(64 * NW), lds, stream, g, tiles, panels);
     return hipGetLastError();
 }
 
-template <int QC, bool S32>
+template <int QC, bool HI>
 static hipError_t launch_tile(const RowsArgs &g, int keys, hipStream_t stream) {
-    if (keys <= 256) return launch_tile_t<QC, 1, 4, S32>(g, stream);
-    if (keys <= 512) return launch_tile_t<QC, 2, 4, S32>(g, stream);
-    if (keys <= 1024) return launch_tile_t<QC, 4, 4, S32>(g, stream);
-    return launch_tile_t<QC, 4, 8, S32>(g, stream);
+    if (keys <= 256) return launch_tile_t<QC, 1, 4, HI>(g, stream);
+    if (keys <= 512) return launch_tile_t<QC, 2, 4, HI>(g, stream);
+    if (keys <= 1024) return launch_tile_t<QC, 4, 4, HI>(g, stream);
+    return launch_tile_t<QC, 4, 8, HI>(g, stream);
 }
 
 constexpr int RT_KEYS = 2048;  // the most keys of a tile in one launch
 
-// Scores and their differences are i32: |dot| <= hd 2^14, |score_m| <= 2^31, so |score| <= hd 2^(45 - s) <= 2^29.
-static bool rows_s32(const AttnArgs &a) {
-    int bits = 0;
-    while ((1 << bits) < a.hd) bits++;
-    return a.score_s >= 16 + bits;
-}
+static bool rows_hi(const AttnArgs &a) { return a.score_s >= 32 && a.score_s <= 60 && a.score_m != INT32_MIN; }
 
 static bool rows_tile_ok(const RowsArgs &g, int keys) {
     const AttnArgs &a = g.a;
-    const bool aligned = (((uintptr_t)a.q | (uintptr_t)a.kc | (uintptr_t)a.vc | (uintptr_t)a.ldq | (uintptr_t)a.hd) & 15) == 0;
+    const uintptr_t bits = (uintptr_t)a.q | (uintptr_t)a.kc | (uintptr_t)a.vc | (uintptr_t)a.exp_table | (uintptr_t)a.ldq | (uintptr_t)a.hd;
     const long long tiles = (g.t + RT_ROWS - 1) / RT_ROWS;
-    return aligned && a.exp_len <= RT_TABLE && keys <= RT_KEYS && ((long long)g.streams * a.n_head + 7) * tiles < (1ll << 31);
+    return bits % 16 == 0 && a.exp_len <= RT_TABLE && keys <= RT_KEYS && ((long long)g.streams * a.n_head + 7) * tiles < (1ll << 31);
 }
 
 size_t rows_workspace(const RowsArgs &) { return 0; }
@@ -466,10 +525,10 @@ hipError_t launch_rows(const RowsArgs &g, void *, hipStream_t stream) {
     const int tasks = g.streams * g.t * g.a.n_head, keys = g.a.ctx_cap;
     if (tasks <= 0) return hipSuccess;
     if (rows_tile_ok(g, keys)) {
-        const bool s32 = rows_s32(g.a);
-        if (g.a.hd <= 64) return s32 ? launch_tile<1, true>(g, keys, stream) : launch_tile<1, false>(g, keys, stream);
-        if (g.a.hd <= 128) return s32 ? launch_tile<2, true>(g, keys, stream) : launch_tile<2, false>(g, keys, stream);
-        return s32 ? launch_tile<4, true>(g, keys, stream) : launch_tile<4, false>(g, keys, stream);
+        const bool hi = rows_hi(g.a);
+        if (g.a.hd <= 64) return hi ? launch_tile<1, true>(g, keys, stream) : launch_tile<1, false>(g, keys, stream);
+        if (g.a.hd <= 128) return hi ? launch_tile<2, true>(g, keys, stream) : launch_tile<2, false>(g, keys, stream);
+        return hi ? launch_tile<4, true>(g, keys, stream) : launch_tile<4, false>(g, keys, stream);
     }
     launch_k(k_rows, dim3((tasks + 3) / 4), dim3(256), 0, stream, g, tasks);
     return hipGetLastError();
