@@ -508,27 +508,378 @@ static hipError_t launch_tile(const RowsArgs &g, int keys, hipStream_t stream) {
     return launch_tile_t<QC, 4, 8, HI>(g, stream);
 }
 
+// ---- Caches longer than a tile's registers ------------------------------------------------------------
+// Key ranges of `span` keys over workgroups of four waves: WT row tiles side by side (each wave walks the blocks
+// of its tile; the others' loads of the same rows hit the L1) and 4 / WT waves to a tile. The integer softmax
+// needs the row maximum before the entries and their sum before p, so there are three walks over the keys, each
+// forming the dots again (4 MFMAs a block, less than keeping them would cost): PHASE 1 the extreme dots, 2 the
+// sums, 3 the products with V, one launch each over all ranges, with the ranges' results in the workspace
+// and a last launch that adds the ranges' outputs. PHASE 0: all three walks in one launch, where the rows alone
+// give enough workgroups. GC: groups of 64 channels of a workgroup (a head dim above 128 takes a workgroup for each).
+struct LongPlan {
+    int tiles = 0, wt = 1, groups = 1, ng = 1, span = 0, cg = 1;
+};
+struct LongScratch {
+    int32_t *mm;    // [panels][rows][ng][2]: the largest and smallest dot of a range
+    uint64_t *ps;   // [panels][rows][ng]: the sum of its entries
+    int64_t *part;  // [panels][ng][rows][hd]: its sum p v
+};
+
+__host__ __device__ inline size_t al256(size_t x) { return (x + 255) / 256 * 256; }
+
+__host__ __device__ inline LongScratch long_scratch(void *base, const LongPlan &p, size_t panels) {
+    const size_t rows = panels * p.tiles * RT_ROWS;
+    LongScratch s;
+    s.mm = (int32_t *)base;
+    s.ps = (uint64_t *)((char *)base + al256(rows * p.ng * 8));
+    s.part = (int64_t *)((char *)s.ps + al256(rows * p.ng * 8));
+    return s;
+}
+
+// One past the last key that the rows of tile group tg see.
+__device__ __forceinline__ int group_keys(const RowsArgs &g, const StreamRows &R, const LongPlan &p, int tg) {
+    const int keys = stream_keys(g, R), most = R.base + (tg + 1) * p.wt * RT_ROWS;
+    return g.mask || keys < most ? keys : most;
+}
+
+template <int QC, int WT, bool HI, int PHASE>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k_rows_long(RowsArgs g, LongPlan pl, int panels, void *scratch) {
+    constexpr int WK = 4 / WT, GC = QC > 2 ? 1 : QC;
+    constexpr bool SUMS = PHASE == 0 || PHASE == 2, PV = PHASE == 0 || PHASE == 3;
+    extern __shared__ __attribute__((aligned(1024))) int8_t s_mem[];
+    __shared__ uint64_t s_sum[4][RT_ROWS];
+    __shared__ int32_t s_mm[2][4][RT_ROWS];
+    const AttnArgs &a = g.a;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ql = lane & 15, qg = lane >> 4, wt = w % WT, ks = w / WT;
+    const int cgs = PV ? pl.cg : 1, inner = pl.groups * pl.ng * cgs;
+    const int L = blockIdx.x, panel = L / (8 * inner) * 8 + (L & 7);  // a panel's workgroups on one XCD
+    int in = (L >> 3) % inner;
+    if (panel >= panels) return;
+    const int cg = in % cgs;
+    in /= cgs;
+    const int tg = in % pl.groups, range = in / pl.groups;
+    const int s = panel / a.n_head, h = panel - s * a.n_head, hd = a.hd;
+    const StreamRows R = stream_rows(g, s);
+    if (tg * WT * RT_ROWS >= R.count) return;
+    const int gkeys = group_keys(g, R, pl, tg), k0 = range * pl.span;
+    if (PHASE != 0 && k0 >= gkeys) return;  // the ranges behind read no result of this one
+    const int tile = tg * WT + wt, row = tile * RT_ROWS + ql, rows = pl.tiles * RT_ROWS;
+    int keys = gkeys;
+    if (!g.mask) keys = R.base + (tile + 1) * RT_ROWS < keys ? R.base + (tile + 1) * RT_ROWS : keys;
+    if (tile * RT_ROWS >= R.count) keys = 0;  // a tile without rows walks nothing
+    const int k1 = k0 + pl.span < keys ? k0 + pl.span : keys, kmost = k1 - 1;
+    const int last = a.exp_len - 1;
+    int32_t *s_exp = (int32_t *)s_mem;
+    int8_t *s_v = s_mem + 4096 * w;  // (its dynamic LDS: V, then the table, which the sums of the outputs take over)
+    if constexpr (SUMS || PV) s_exp = (int32_t *)(s_mem + 16384);
+    if constexpr (SUMS || PV) load_table(a, s_exp, w, 4, lane);
+
+    const size_t at = (size_t)R.slot * a.n_head + h, base = at * a.ctx_cap * hd;
+    const int8_t *K = a.kc + base, *V = a.vc + base;
+    const v4i zero = v4i{0, 0, 0, 0};
+    v4i qf[QC];
+#pragma unroll
+    for (int c = 0; c < QC; c++) {
+        const int o = 64 * c + 16 * qg;
+        qf[c] = row < R.count && o < hd ? *(const v4i *)(a.q + (size_t)(R.first + row) * a.ldq + h * hd + o) : zero;
+    }
+    const RowSight sight = row_sight(g, R, row, keys);
+    const int whole0 = g.mask ? R.base : R.base + tile * RT_ROWS + 1, whole = whole0 < keys ? whole0 : keys;
+    struct Loads {
+        v4i k[4][QC], v[PV ? GC : 1][4];
+    };
+    auto load = [&](int kb, Loads &x, bool v_too) {
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const int k = 64 * kb + 16 * t + ql;
+            const int8_t *kr = K + (size_t)(k < k1 ? k : kmost) * hd + 16 * qg;
+#pragma unroll
+            for (int c = 0; c < QC; c++) x.k[t][c] = 64 * c + 16 * qg < hd ? *(const v4i *)(kr + 64 * c) : zero;
+        }
+        if (!PV || !v_too) return;
+#pragma unroll
+        for (int c = 0; c < (PV ? GC : 1); c++)
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int r = 16 * u + (lane >> 2), k = 64 * kb + r, o = 64 * (GC * cg + c) + 16 * ((lane & 3) ^ vsw<4>(r & 15));
+                x.v[c][u] = o < hd ? *(const v4i *)(V + (size_t)(k < k1 ? k : kmost) * hd + o) : zero;
+            }
+    };
+    // fn(block, its dots, its loads, whether every row sees all of it, what the row sees), the next loads in flight
+    auto walk = [&](bool v_too, auto fn) {
+        int kb = k0 / 64 + ks;
+        if (64 * kb >= k1) return;
+        const bool ahead = QC == 1 || !v_too;  // (K and V of two blocks beside the sums: registers for 64 channels only)
+        Loads x;
+        load(kb, x, v_too);
+        while (true) {
+            const int next = kb + WK;
+            const bool more = 64 * next < k1;
+            Loads y;
+            if (more && ahead) load(next, y, v_too);
+            v4i D[4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                D[t] = zero;
+#pragma unroll
+                for (int c = 0; c < QC; c++) D[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.k[t][c], qf[c], D[t], 0, 0, 0);
+            }
+            const bool all = 64 * kb + 64 <= whole;
+            fn(kb, D, x, all, all ? 0u : sight_bits(sight, kb, qg, keys));
+            if (!more) break;
+            if (ahead) x = y;
+            else load(next, x, v_too);
+            kb = next;
+        }
+    };
+    const LongScratch S = long_scratch(scratch, pl, panels);
+    const size_t slot = ((size_t)panel * rows + row) * pl.ng;  // of the row's ranges
+    const int ranges = (gkeys + pl.span - 1) / pl.span;
+
+    int32_t dmax = INT32_MIN, dmin = INT32_MAX;
+    if constexpr (PHASE <= 1) {
+        walk(false, [&](int, v4i (&D)[4], const Loads &, bool all, uint32_t ok) { block_extremes(D, all, ok, dmax, dmin); });
+#pragma unroll
+        for (int o = 16; o < 64; o <<= 1) {
+            const int32_t x = __shfl_xor(dmax, o, 64), y = __shfl_xor(dmin, o, 64);
+            dmax = x > dmax ? x : dmax;
+            dmin = y < dmin ? y : dmin;
+        }
+        if (WK > 1) {
+            if (qg == 0) {
+                s_mm[0][w][ql] = dmax;
+                s_mm[1][w][ql] = dmin;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < WK; i++) {
+                const int32_t x = s_mm[0][wt + WT * i][ql], y = s_mm[1][wt + WT * i][ql];
+                dmax = x > dmax ? x : dmax;
+                dmin = y < dmin ? y : dmin;
+            }
+        }
+        if constexpr (PHASE == 1) {
+            if (ks == 0 && qg == 0 && row < R.count) {
+                S.mm[2 * (slot + range)] = dmax;
+                S.mm[2 * (slot + range) + 1] = dmin;
+            }
+            return;
+        }
+    } else if (row < R.count) {
+        for (int c = 0; c < ranges; c++) {
+            const int32_t x = S.mm[2 * (slot + c)], y = S.mm[2 * (slot + c) + 1];
+            dmax = x > dmax ? x : dmax;
+            dmin = y < dmin ? y : dmin;
+        }
+    }
+    const RowIndex<HI> ix(a, dmax, dmin);
+    __syncthreads();  // the table
+    uint64_t sum = 0;
+    if constexpr (SUMS) {
+        walk(false, [&](int, v4i (&D)[4], const Loads &, bool all, uint32_t ok) {
+            block_entries<HI>(a, D, ix, s_exp, last, all, ok);
+            sum += block_sum(D);
+        });
+#pragma unroll
+        for (int o = 16; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+        if (WK > 1) {
+            if (qg == 0) s_sum[w][ql] = sum;
+            __syncthreads();
+            sum = 0;
+#pragma unroll
+            for (int i = 0; i < WK; i++) sum += s_sum[wt + WT * i][ql];
+        }
+        if constexpr (PHASE == 2) {
+            if (ks == 0 && qg == 0 && row < R.count) S.ps[slot + range] = sum;
+            return;
+        }
+    } else if (row < R.count) {
+        for (int c = 0; c < ranges; c++) sum += S.ps[slot + c];
+    }
+    if constexpr (PV) {
+        const RowWeight weight(sum, a.softmax_p, row < R.count);
+        v4i acc[GC][4][4];
+#pragma unroll
+        for (int c = 0; c < GC; c++)
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[c][k][i] = zero;
+        uint64_t *mass = g.mass && cg == 0 ? g.mass + at * a.ctx_cap : nullptr;
+        walk(true, [&](int kb, v4i (&D)[4], const Loads &x, bool all, uint32_t ok) {
+            block_entries<HI>(a, D, ix, s_exp, last, all, ok);
+            block_digits(D, weight.R, weight.sp, mass ? mass + 64 * kb : nullptr, k1 - 64 * kb, lane);
+#pragma unroll
+            for (int c = 0; c < GC; c++) {
+#pragma unroll
+                for (int u = 0; u < 4; u++) *(v4i *)(s_v + 1024 * u + 16 * lane) = x.v[c][u];
+                block_pv(s_v, D, lane, acc[c]);
+            }
+        });
+        // A row's sums of one range, or the outputs themselves
+        const double mo = a.out_s > 95 ? 0.0 : ldexp((double)a.out_m, -a.out_s);
+        auto put = [&](int r, int ch, const int64_t (&x)[4]) {  // channels ch .. ch + 3 of row r
+            if (PHASE == 0) {
+                uint32_t packed = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++) packed |= (uint32_t)(uint8_t)(int8_t)attn_out_byte(x[e], mo, a.out_m, a.out_s) << (8 * e);
+                *(uint32_t *)attn_out(a, R.first + r, h * hd + ch) = packed;
+            } else {
+                int64_t *o = S.part + (((size_t)panel * pl.ng + range) * rows + r) * hd + ch;
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[e] = x[e];
+            }
+        };
+        if constexpr (WK == 1) {
+            if (row < R.count) {
+#pragma unroll
+                for (int c = 0; c < GC; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int ch = 64 * (GC * cg + c) + 16 * i + 4 * qg;
+                        int64_t x[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) x[e] = plane_sum(acc[c], i, e);
+                        if (ch < hd) put(row, ch, x);
+                    }
+            }
+        } else {
+            int64_t *s_acc = (int64_t *)s_exp;  // [WT][GC][16][RT_ACC], over the table
+            __syncthreads();
+            for (int i = tid; i < WT * GC * RT_ROWS * RT_ACC; i += 256) s_acc[i] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int c = 0; c < GC; c++) {
+                unsigned long long *to = (unsigned long long *)s_acc + ((wt * GC + c) * RT_ROWS + ql) * RT_ACC + 4 * qg;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) atomicAdd(to + 16 * i + e, (unsigned long long)plane_sum(acc[c], i, e));
+            }
+            __syncthreads();
+            for (int i = tid; i < WT * GC * RT_ROWS * 16; i += 256) {
+                const int q4 = i & 15, r = (i >> 4) & 15, c = (i >> 8) % GC, u = (i >> 8) / GC;
+                const int ch = 64 * (GC * cg + c) + 4 * q4, out_row = (tg * WT + u) * RT_ROWS + r;
+                if (ch >= hd || out_row >= R.count) continue;
+                const int64_t *from = s_acc + ((u * GC + c) * RT_ROWS + r) * RT_ACC + 4 * q4;
+                const int64_t x[4] = {from[0], from[1], from[2], from[3]};
+                put(out_row, ch, x);
+            }
+        }
+    }
+}
+
+// The outputs from the ranges' sums: a thread per four channels.
+__global__ __launch_bounds__(256) void k_rows_out(RowsArgs g, LongPlan pl, int panels, void *scratch) {
+    const AttnArgs &a = g.a;
+    const int rows = pl.tiles * RT_ROWS, quads = a.hd / 4;
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    const size_t pr = i / quads;
+    const int ch = 4 * (int)(i - pr * quads), panel = (int)(pr / rows), r = (int)(pr - (size_t)panel * rows);
+    if (panel >= panels) return;
+    const int s = panel / a.n_head, h = panel - s * a.n_head;
+    const StreamRows R = stream_rows(g, s);
+    if (r >= R.count) return;
+    const int ranges = (group_keys(g, R, pl, r / (pl.wt * RT_ROWS)) + pl.span - 1) / pl.span;
+    const LongScratch S = long_scratch(scratch, pl, panels);
+    int64_t x[4] = {0, 0, 0, 0};
+    for (int c = 0; c < ranges; c++) {
+        const int64_t *p = S.part + (((size_t)panel * pl.ng + c) * rows + r) * a.hd + ch;
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] += p[e];
+    }
+    const double mo = a.out_s > 95 ? 0.0 : ldexp((double)a.out_m, -a.out_s);
+    uint32_t packed = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) packed |= (uint32_t)(uint8_t)(int8_t)attn_out_byte(x[e], mo, a.out_m, a.out_s) << (8 * e);
+    *(uint32_t *)attn_out(a, R.first + r, h * a.hd + ch) = packed;
+}
+
+static LongPlan long_plan(const RowsArgs &g, int keys) {
+    LongPlan p;
+    p.tiles = (g.t + RT_ROWS - 1) / RT_ROWS;
+    p.wt = p.tiles >= 3 ? 4 : p.tiles;
+    p.groups = (p.tiles + p.wt - 1) / p.wt;
+    p.cg = g.a.hd > 128 ? (g.a.hd + 63) / 64 : 1;
+    // about LONG_WGS workgroups, at least four blocks a wave
+    constexpr long long LONG_WGS = 1536;
+    const long long wgs = (long long)g.streams * g.a.n_head * p.groups;
+    const int unit = 64 * (4 / p.wt), most = (keys + 4 * unit - 1) / (4 * unit);
+    long long ng = (LONG_WGS + wgs - 1) / wgs;
+    ng = ng < 1 ? 1 : (ng > most ? most : ng);
+    p.span = (int)(((keys + ng - 1) / ng + unit - 1) / unit) * unit;
+    p.ng = (keys + p.span - 1) / p.span;
+    return p;
+}
+
+template <int QC, int WT, bool HI>
+static hipError_t launch_long_t(const RowsArgs &g, const LongPlan &p, void *scratch, hipStream_t stream) {
+    constexpr int GC = QC > 2 ? 1 : QC;
+    const int panels = g.streams * g.a.n_head;
+    const unsigned grid = (unsigned)((panels + 7) / 8 * 8) * p.groups * p.ng;
+    const size_t table = (size_t)1024 * ((g.a.exp_len + 255) / 256), acc = WT < 4 ? (size_t)8 * WT * GC * RT_ROWS * RT_ACC : 0;
+    auto run = [&](auto kernel, unsigned n, size_t lds) {
+        const hipError_t e = allow_dynamic_lds((const void *)kernel, lds);
+        if (e != hipSuccess) return e;
+        launch_k(kernel, dim3(n), dim3(256), lds, stream, g, p, panels, scratch);
+        return hipGetLastError();
+    };
+    const size_t lds = 16384 + (table > acc ? table : acc);
+    hipError_t e;
+    if (p.ng == 1) return run(k_rows_long<QC, WT, HI, 0>, grid * p.cg, lds);
+    if ((e = run(k_rows_long<QC, WT, HI, 1>, grid, 0)) != hipSuccess) return e;
+    if ((e = run(k_rows_long<QC, WT, HI, 2>, grid, 16384 + table)) != hipSuccess) return e;
+    if ((e = run(k_rows_long<QC, WT, HI, 3>, grid * p.cg, lds)) != hipSuccess) return e;
+    const size_t quads = (size_t)panels * p.tiles * RT_ROWS * (g.a.hd / 4);
+    launch_k(k_rows_out, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, g, p, panels, scratch);
+    return hipGetLastError();
+}
+
+template <int QC, bool HI>
+static hipError_t launch_long(const RowsArgs &g, const LongPlan &p, void *scratch, hipStream_t stream) {
+    if (p.wt == 1) return launch_long_t<QC, 1, HI>(g, p, scratch, stream);
+    if (p.wt == 2) return launch_long_t<QC, 2, HI>(g, p, scratch, stream);
+    return launch_long_t<QC, 4, HI>(g, p, scratch, stream);
+}
+
 constexpr int RT_KEYS = 2048;  // the most keys of a tile in one launch
 
 static bool rows_hi(const AttnArgs &a) { return a.score_s >= 32 && a.score_s <= 60 && a.score_m != INT32_MIN; }
 
-static bool rows_tile_ok(const RowsArgs &g, int keys) {
+// Whether the MFMA forms take the shapes (the grids below 2^31 workgroups), the alignments and the table.
+static bool rows_mfma_ok(const RowsArgs &g) {
     const AttnArgs &a = g.a;
     const uintptr_t bits = (uintptr_t)a.q | (uintptr_t)a.kc | (uintptr_t)a.vc | (uintptr_t)a.exp_table | (uintptr_t)a.ldq | (uintptr_t)a.hd;
-    const long long tiles = (g.t + RT_ROWS - 1) / RT_ROWS;
-    return bits % 16 == 0 && a.exp_len <= RT_TABLE && keys <= RT_KEYS && ((long long)g.streams * a.n_head + 7) * tiles < (1ll << 31);
+    const long long tiles = (g.t + RT_ROWS - 1) / RT_ROWS, panels = (long long)g.streams * a.n_head + 7;
+    if (bits % 16 != 0 || a.exp_len > RT_TABLE) return false;
+    if (a.ctx_cap <= RT_KEYS) return panels * tiles < (1ll << 31);
+    const LongPlan p = long_plan(g, a.ctx_cap);
+    return panels * p.groups * p.ng * p.cg < (1ll << 31) && panels * tiles * RT_ROWS * (a.hd / 4) < (1ll << 38);
 }
 
-size_t rows_workspace(const RowsArgs &) { return 0; }
+size_t rows_workspace(const RowsArgs &g) {
+    if (g.a.ctx_cap <= RT_KEYS || !rows_mfma_ok(g)) return 0;
+    const LongPlan p = long_plan(g, g.a.ctx_cap);
+    if (p.ng == 1) return 0;
+    const size_t panels = (size_t)g.streams * g.a.n_head;
+    return (size_t)long_scratch(nullptr, p, panels).part + panels * p.ng * p.tiles * RT_ROWS * g.a.hd * 8;
+}
 
-hipError_t launch_rows(const RowsArgs &g, void *, hipStream_t stream) {
-    const int tasks = g.streams * g.t * g.a.n_head, keys = g.a.ctx_cap;
+template <int QC, bool HI>
+static hipError_t launch_mfma(const RowsArgs &g, void *workspace, hipStream_t stream) {
+    if (g.a.ctx_cap <= RT_KEYS) return launch_tile<QC, HI>(g, g.a.ctx_cap, stream);
+    return launch_long<QC, HI>(g, long_plan(g, g.a.ctx_cap), workspace, stream);
+}
+
+hipError_t launch_rows(const RowsArgs &g, void *workspace, hipStream_t stream) {
+    const int tasks = g.streams * g.t * g.a.n_head;
     if (tasks <= 0) return hipSuccess;
-    if (rows_tile_ok(g, keys)) {
+    if (rows_mfma_ok(g)) {
         const bool hi = rows_hi(g.a);
-        if (g.a.hd <= 64) return hi ? launch_tile<1, true>(g, keys, stream) : launch_tile<1, false>(g, keys, stream);
-        if (g.a.hd <= 128) return hi ? launch_tile<2, true>(g, keys, stream) : launch_tile<2, false>(g, keys, stream);
-        return hi ? launch_tile<4, true>(g, keys, stream) : launch_tile<4, false>(g, keys, stream);
+        if (g.a.hd <= 64) return hi ? launch_mfma<1, true>(g, workspace, stream) : launch_mfma<1, false>(g, workspace, stream);
+        if (g.a.hd <= 128) return hi ? launch_mfma<2, true>(g, workspace, stream) : launch_mfma<2, false>(g, workspace, stream);
+        return hi ? launch_mfma<4, true>(g, workspace, stream) : launch_mfma<4, false>(g, workspace, stream);
     }
     launch_k(k_rows, dim3((tasks + 3) / 4), dim3(256), 0, stream, g, tasks);
     return hipGetLastError();

@@ -126,6 +126,18 @@ def test_tree_long_contexts_of_other_head_dims(gpu, hd, cap):
     check_tree(gpu, 2, 18, 2, hd, cap, [cap - 18, cap // 2])
 
 
+@pytest.mark.parametrize("t", [1, 16, 17, 33, 64, 90, 256])
+def test_tree_sizes_over_long_contexts(gpu, t):
+    check_tree(gpu, 3, t, 2, 64, 2600, [2600 - t, 300, 0], [t, (t + 1) // 2, t], empty=0.1)
+
+
+@pytest.mark.parametrize("hd", [16, 80, 256])
+def test_many_long_contexts(gpu, hd):
+    """So many streams that a workgroup walks a whole cache by itself."""
+    check_tree(gpu, 400 if hd == 16 else 128, 3, 4 if hd == 16 else 13, hd, 2052, [2049, 5, 2000, 0])
+    check_mass(gpu, 128, 3, 13, hd, 2052, [2049, 5, 2000, 3], seed=hd)
+
+
 @pytest.mark.parametrize("hd", [20, 64, 128])
 def test_tree_rows_that_see_nothing(gpu, hd):
     """No context and empty masks: rows of zeros; every bit set: only the stream's own nodes count."""
