@@ -858,7 +858,15 @@ static bool rows_mfma_ok(const RowsArgs &g) {
     return panels * p.groups * p.ng * p.cg < (1ll << 31) && panels * tiles * RT_ROWS * (a.hd / 4) < (1ll << 38);
 }
 
+// One causal row a stream: the decode kernels, which add up the weights too.
+static bool rows_decode_ok(const RowsArgs &g) {
+    const AttnArgs &a = g.a;
+    const uintptr_t bits = (uintptr_t)a.q | (uintptr_t)a.kc | (uintptr_t)a.vc;
+    return g.t == 1 && !g.mask && !g.groups && attend_split_ok(a.hd) && bits % 16 == 0;
+}
+
 size_t rows_workspace(const RowsArgs &g) {
+    if (rows_decode_ok(g)) return attend_split_bytes(g.a, g.streams, attend_split_plan(g.streams, g.a.n_head, g.a.ctx_cap));
     if (g.a.ctx_cap <= RT_KEYS || !rows_mfma_ok(g)) return 0;
     const LongPlan p = long_plan(g, g.a.ctx_cap);
     if (p.ng == 1) return 0;
@@ -875,6 +883,13 @@ static hipError_t launch_mfma(const RowsArgs &g, void *workspace, hipStream_t st
 hipError_t launch_rows(const RowsArgs &g, void *workspace, hipStream_t stream) {
     const int tasks = g.streams * g.t * g.a.n_head;
     if (tasks <= 0) return hipSuccess;
+    if (rows_decode_ok(g)) {
+        AttnArgs a = g.a;
+        a.keys = g.ctx;
+        a.count = g.count;
+        a.mass = g.mass;
+        return launch_attend_split(a, g.streams, attend_split_plan(g.streams, a.n_head, a.ctx_cap), workspace, stream);
+    }
     if (rows_mfma_ok(g)) {
         const bool hi = rows_hi(g.a);
         if (g.a.hd <= 64) return hi ? launch_mfma<1, true>(g, workspace, stream) : launch_mfma<1, false>(g, workspace, stream);

@@ -1880,6 +1880,11 @@ __device__ __forceinline__ int split_keys(const AttnArgs &a, int r) {
     return keys < 1 ? 1 : (keys > a.ctx_cap ? a.ctx_cap : keys);
 }
 
+// Of a row that keeps accumulators: 0 if it is not there, 1 if it has no key (a row of zeros), else 2.
+__device__ __forceinline__ int mass_row(const AttnArgs &a, int r) {
+    return a.count && a.count[r] == 0 ? 0 : (a.keys[r] == 0 ? 1 : 2);
+}
+
 __device__ __forceinline__ int split_slot(const AttnArgs &a, int r) { return a.rows ? a.rows[r].slot : r; }
 
 // The row maximum of the scores, from every chunk's extreme dots (the score is monotone in the dot).
@@ -1972,6 +1977,11 @@ __global__ void k_split_out(AttnArgs a, int n_rows, SplitPlan pl, void *scratch)
     const int rh = blockIdx.x, t = threadIdx.x;
     const int r = rh / a.n_head, h = rh - r * a.n_head, hd = a.hd;
     if (t >= hd) return;
+    if (a.mass) {
+        const int kind = mass_row(a, r);
+        if (kind == 1) *attn_out(a, r, h * hd + t) = 0;
+        if (kind != 2) return;
+    }
     const SplitScratch S = split_scratch(scratch, n_rows, a.n_head, a.ctx_cap, pl.chunks, hd);
     const int keys = split_keys(a, r), nch = (keys + pl.chunk_keys - 1) / pl.chunk_keys;
     int64_t o = 0;
@@ -1983,7 +1993,7 @@ __global__ void k_split_out(AttnArgs a, int n_rows, SplitPlan pl, void *scratch)
 // next block's V rows in flight. (One i64 multiply-add a channel and key and a butterfly at the end
 // took 29.1 us at head_dim 64, 2,000 keys, 512 row-heads; this 13.0.) At most 4,096 keys: below 2^26
 // a plane.
-template <bool NOCLAMP, int HD>
+template <bool NOCLAMP, int HD, bool MASS>
 __global__ __launch_bounds__(64) void k_split_pv(AttnArgs a, int n_rows, SplitPlan pl, void *scratch) {
     constexpr int QT = HD / 16, NC = HD < 64 ? QT : 4, NG = QT / NC, RB = 16 * NC, RL = 64 / NC, SH = NC / 2;
     __shared__ __attribute__((aligned(16))) int8_t s_v[64 * HD], s_mem[1024];
@@ -2032,6 +2042,7 @@ __global__ __launch_bounds__(64) void k_split_pv(AttnArgs a, int n_rows, SplitPl
                 q = __umul64hi(num, frac);  // q <= floor(num / S) <= q + 1
                 if (num - q * sum >= sum) q++;
             }
+            if (MASS && mass_row(a, r) == 2) a.mass[(size_t)rh * a.ctx_cap + kb + lane] += q;
         }
 #pragma unroll
         for (int g = 0; g < NG; g++)
@@ -2061,7 +2072,7 @@ __global__ __launch_bounds__(64) void k_split_pv(AttnArgs a, int n_rows, SplitPl
 // at 768 row-heads over cold caches: 1,024 keys 20.2 us (100.8 MB: 5.0 TB/s), 512 keys 12.4. What the layout
 // rests on, at 1,024 keys with the sums p v still on 24-bit multiplies: 34.2 us with all of V in LDS
 // (two workgroups per CU), 31.0 with half, 29.8 with none.
-template <bool NOCLAMP>
+template <bool NOCLAMP, bool MASS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k_attend_decode64(AttnArgs a,
                                                                                                   int kmax) {
     __shared__ __attribute__((aligned(16))) int8_t s_v[4][4096];    // a wave's block of V rows
@@ -2070,6 +2081,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     __shared__ uint64_t s_sum[4];
     const int rh = blockIdx.x, tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
     const int r = rh / a.n_head, h = rh - r * a.n_head;
+    if constexpr (MASS) {
+        const int kind = mass_row(a, r);
+        if (kind == 1 && tid < 64) *attn_out(a, r, h * 64 + tid) = 0;
+        if (kind != 2) return;
+    }
     int keys = split_keys(a, r);
     keys = keys < kmax ? keys : kmax;  // the launch's bound holds every row's count
     const size_t base = ((size_t)split_slot(a, r) * a.n_head + h) * a.ctx_cap * 64;
@@ -2099,6 +2115,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     for (int i = 0; i < 16; i++) {
         const int row = 16 * (i & 3) + (lane >> 2), k = 64 * (4 * (i >> 2) + w) + row;
         vr[i] = *(const v4i *)(a.vc + base + (size_t)(k < keys ? k : keys - 1) * 64 + 16 * ((lane & 3) ^ vsw<4>(row & 15)));
+    }
+    uint64_t mv[4];  // the accumulators of the thread's keys
+    if constexpr (MASS) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) mv[j] = a.mass[(size_t)rh * a.ctx_cap + (tid + 256 * j < keys ? tid + 256 * j : keys - 1)];
     }
     __builtin_amdgcn_sched_barrier(0);  // every load issued before the first wait
     // the dots wait for K alone (the compiler's waits on the K registers)
@@ -2153,7 +2174,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     if (lane == 0) s_sum[w] = sum;
     __syncthreads();
     sum = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-    const double R = ldexp(1.0 / (double)sum, a.softmax_p);
+    const double R = MASS && sum == 0 ? 0.0 : ldexp(1.0 / (double)sum, a.softmax_p);
     const double sp = softmax_sp(sum, a.softmax_p);
     v4i acc[4];
 #pragma unroll
@@ -2164,7 +2185,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
 #pragma unroll
         for (int u = 0; u < 4; u++) *(v4i *)(s_v[w] + 1024 * u + 16 * lane) = vr[4 * j + u];
         // p <= 2^P <= 2^30; 0 for keys past the row (e = 0)
-        decode_pv_block<4>(s_v[w], decode_pv_digits(s_mem[w], softmax_p_of(e[j], R, sp), lane), lane, acc);
+        const uint32_t p = softmax_p_of(e[j], R, sp);
+        if (MASS && tid + 256 * j < keys) a.mass[(size_t)rh * a.ctx_cap + tid + 256 * j] = mv[j] + p;
+        decode_pv_block<4>(s_v[w], decode_pv_digits(s_mem[w], p, lane), lane, acc);
     }
     decode_pv_store<4>(s_mem[w], lane, acc);
     __syncthreads();
@@ -2181,7 +2204,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
 // 14.0, 768 row-heads at 640 keys.) Kernel time against
 // the four split launches: head_dim 128, 600 row-heads at 388 keys 35.3 -> 16.9 us; head_dim 32, 1,200
 // row-heads at 1,000 keys 41.7 -> 12.1 us.
-template <bool NOCLAMP, int HD>
+template <bool NOCLAMP, int HD, bool MASS>
 __global__ __launch_bounds__(HD > 64 ? 512 : 256) __attribute__((amdgpu_waves_per_eu(2))) void k_attend_decode_wg(
     AttnArgs a, int kmax) {
     constexpr int NW = HD > 64 ? 8 : 4, NTH = 64 * NW, KT = 1024 / NTH, QT = HD / 16;
@@ -2192,6 +2215,11 @@ __global__ __launch_bounds__(HD > 64 ? 512 : 256) __attribute__((amdgpu_waves_pe
     __shared__ uint64_t s_sum[NW];
     const int rh = blockIdx.x, tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
     const int r = rh / a.n_head, h = rh - r * a.n_head;
+    if constexpr (MASS) {
+        const int kind = mass_row(a, r);
+        if (kind == 1 && tid < HD) *attn_out(a, r, h * HD + tid) = 0;
+        if (kind != 2) return;
+    }
     int keys = split_keys(a, r);
     keys = keys < kmax ? keys : kmax;  // the launch's bound holds every row's count
     const size_t base = ((size_t)split_slot(a, r) * a.n_head + h) * a.ctx_cap * HD;
@@ -2227,6 +2255,11 @@ __global__ __launch_bounds__(HD > 64 ? 512 : 256) __attribute__((amdgpu_waves_pe
 #pragma unroll
             for (int g = 0; g < NG; g++) vr[j][g][u] = *(const v4i *)(v + 64 * g);
         }
+    }
+    uint64_t mv[KT];  // the accumulators of the thread's keys
+    if constexpr (MASS) {
+#pragma unroll
+        for (int j = 0; j < KT; j++) mv[j] = a.mass[(size_t)rh * a.ctx_cap + (tid + NTH * j < keys ? tid + NTH * j : keys - 1)];
     }
     __builtin_amdgcn_sched_barrier(0);  // every load issued before the first wait
     // the dots wait for K alone (the compiler's waits on the K registers)
@@ -2283,7 +2316,7 @@ __global__ __launch_bounds__(HD > 64 ? 512 : 256) __attribute__((amdgpu_waves_pe
     sum = 0;
 #pragma unroll
     for (int i = 0; i < NW; i++) sum += s_sum[i];
-    const double R = ldexp(1.0 / (double)sum, a.softmax_p);
+    const double R = MASS && sum == 0 ? 0.0 : ldexp(1.0 / (double)sum, a.softmax_p);
     const double sp = softmax_sp(sum, a.softmax_p);
     v4i acc[NG][NC];
 #pragma unroll
@@ -2300,7 +2333,9 @@ __global__ __launch_bounds__(HD > 64 ? 512 : 256) __attribute__((amdgpu_waves_pe
             for (int u = 0; u < NC; u++) *(v4i *)(s_v[w] + 1024 * u + 16 * lane) = vr[j][g][u];
             if (g == 0) {  // p <= 2^P <= 2^30; 0 for keys past the row (e = 0)
                 __builtin_amdgcn_sched_barrier(0);  // the weights' arithmetic covers the stores of V
-                pf = decode_pv_digits(s_mem[w], softmax_p_of(e[j], R, sp), lane);
+                const uint32_t p = softmax_p_of(e[j], R, sp);
+                if (MASS && tid + NTH * j < keys) a.mass[(size_t)rh * a.ctx_cap + tid + NTH * j] = mv[j] + p;
+                pf = decode_pv_digits(s_mem[w], p, lane);
             }
             decode_pv_block<NC>(s_v[w], pf, lane, acc[g]);
         }
@@ -2324,7 +2359,7 @@ __global__ __launch_bounds__(HD > 64 ? 512 : 256) __attribute__((amdgpu_waves_pe
 // sum and p = floor(e 2^P / S) follow the rules of the kernels above, the sums p v come from the digit
 // planes block by block. Against the four split launches, a prefill pass of 120,792 row-heads at
 // head_dim 32 and up to 400 keys: 665 -> 196 us a layer.
-template <bool NOCLAMP, int KB, int HD>
+template <bool NOCLAMP, int KB, int HD, bool MASS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k_attend_decode_wave(AttnArgs a, int n_rh,
                                                                                                      int kmax) {
     constexpr int QT = HD / 16, NC = HD < 64 ? QT : 4, NG = QT / NC, RB = 16 * NC, RL = 64 / NC, SH = NC / 2;
@@ -2332,6 +2367,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     const int rh = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (rh >= n_rh) return;
     const int r = rh / a.n_head, h = rh - r * a.n_head;
+    if constexpr (MASS) {
+        const int kind = mass_row(a, r);
+        if (kind == 1)
+            for (int c = lane; c < HD; c += 64) *attn_out(a, r, h * HD + c) = 0;
+        if (kind != 2) return;
+    }
     int keys = split_keys(a, r);
     keys = keys < kmax ? keys : kmax;
     const size_t base = ((size_t)split_slot(a, r) * a.n_head + h) * a.ctx_cap * HD;
@@ -2357,6 +2398,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
 #pragma unroll
         for (int g = 0; g < NG; g++)
             __builtin_amdgcn_global_load_lds((const void *)(v + 64 * g), (lds_void *)(sv + (g * NC * KB + i) * 1024), 16, 0, 0);
+    }
+    uint64_t mv[KB];  // the accumulators of the lane's keys
+    if constexpr (MASS) {
+#pragma unroll
+        for (int j = 0; j < KB; j++) mv[j] = a.mass[(size_t)rh * a.ctx_cap + (lane + 64 * j < keys ? lane + 64 * j : keys - 1)];
     }
     int32_t d[KB];
     int32_t dmin = INT32_MAX, dmax = INT32_MIN;
@@ -2395,7 +2441,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         }
     }
     sum = wave_sum_dpp(sum);
-    const double R = ldexp(1.0 / (double)sum, a.softmax_p);
+    const double R = MASS && sum == 0 ? 0.0 : ldexp(1.0 / (double)sum, a.softmax_p);
     const double sp = softmax_sp(sum, a.softmax_p);
     wait_vmcnt<0>();  // this wave's V rows landed in its LDS region
     v4i acc[NG][NC];
@@ -2407,7 +2453,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     for (int j = 0; j < KB; j++) {
         if (64 * j >= keys) break;
         // p <= 2^P <= 2^30; 0 for keys past the row (e = 0)
-        const v4i pf = decode_pv_digits(mem, softmax_p_of(e[j], R, sp), lane);
+        const uint32_t p = softmax_p_of(e[j], R, sp);
+        if (MASS && lane + 64 * j < keys) a.mass[(size_t)rh * a.ctx_cap + lane + 64 * j] = mv[j] + p;
+        const v4i pf = decode_pv_digits(mem, p, lane);
 #pragma unroll
         for (int g = 0; g < NG; g++) decode_pv_block<NC>(sv + (g * KB + j) * 64 * RB, pf, lane, acc[g]);
     }
@@ -2427,12 +2475,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
 // it a workgroup per row-head, up to 1,024 keys.
 static int decode_wave_keys(int hd) { return hd == 128 ? 128 : hd == 64 ? 256 : 512; }
 
-template <bool NOCLAMP, int HD>
+template <bool NOCLAMP, int HD, bool MASS>
 static hipError_t launch_decode(const AttnArgs &a, int n_rows, int kmax, hipStream_t stream) {
     const int n_rh = n_rows * a.n_head;
     if (kmax > decode_wave_keys(HD)) {
-        if constexpr (HD == 64) launch_k(k_attend_decode64<NOCLAMP>, dim3(n_rh), dim3(256), 0, stream, a, kmax);
-        else launch_k((k_attend_decode_wg<NOCLAMP, HD>), dim3(n_rh), dim3(HD > 64 ? 512 : 256), 0, stream, a, kmax);
+        if constexpr (HD == 64) launch_k((k_attend_decode64<NOCLAMP, MASS>), dim3(n_rh), dim3(256), 0, stream, a, kmax);
+        else launch_k((k_attend_decode_wg<NOCLAMP, HD, MASS>), dim3(n_rh), dim3(HD > 64 ? 512 : 256), 0, stream, a, kmax);
         return hipGetLastError();
     }
     auto run = [&](auto kernel, int kb) {
@@ -2443,23 +2491,23 @@ static hipError_t launch_decode(const AttnArgs &a, int n_rows, int kmax, hipStre
         return hipGetLastError();
     };
     const int kb = (kmax + 63) / 64;
-    if (kb <= 1) return run(k_attend_decode_wave<NOCLAMP, 1, HD>, 1);
-    if (kb == 2) return run(k_attend_decode_wave<NOCLAMP, 2, HD>, 2);
+    if (kb <= 1) return run(k_attend_decode_wave<NOCLAMP, 1, HD, MASS>, 1);
+    if (kb == 2) return run(k_attend_decode_wave<NOCLAMP, 2, HD, MASS>, 2);
     if constexpr (HD <= 64) {
-        if (kb == 3) return run(k_attend_decode_wave<NOCLAMP, 3, HD>, 3);
-        if (kb == 4) return run(k_attend_decode_wave<NOCLAMP, 4, HD>, 4);
-        if constexpr (HD < 64) return run(k_attend_decode_wave<NOCLAMP, 8, HD>, 8);
+        if (kb == 3) return run(k_attend_decode_wave<NOCLAMP, 3, HD, MASS>, 3);
+        if (kb == 4) return run(k_attend_decode_wave<NOCLAMP, 4, HD, MASS>, 4);
+        if constexpr (HD < 64) return run(k_attend_decode_wave<NOCLAMP, 8, HD, MASS>, 8);
     }
     return hipErrorInvalidValue;
 }
 
-template <bool NOCLAMP>
+template <bool NOCLAMP, bool MASS>
 static hipError_t launch_decode_hd(const AttnArgs &a, int n_rows, int kmax, hipStream_t stream) {
     switch (a.hd) {
-    case 16: return launch_decode<NOCLAMP, 16>(a, n_rows, kmax, stream);
-    case 32: return launch_decode<NOCLAMP, 32>(a, n_rows, kmax, stream);
-    case 64: return launch_decode<NOCLAMP, 64>(a, n_rows, kmax, stream);
-    case 128: return launch_decode<NOCLAMP, 128>(a, n_rows, kmax, stream);
+    case 16: return launch_decode<NOCLAMP, 16, MASS>(a, n_rows, kmax, stream);
+    case 32: return launch_decode<NOCLAMP, 32, MASS>(a, n_rows, kmax, stream);
+    case 64: return launch_decode<NOCLAMP, 64, MASS>(a, n_rows, kmax, stream);
+    case 128: return launch_decode<NOCLAMP, 128, MASS>(a, n_rows, kmax, stream);
     default: return hipErrorInvalidValue;
     }
 }
@@ -2510,22 +2558,22 @@ size_t attend_split_bytes(const AttnArgs &a, int n_rows, const SplitPlan &p) {
     return attend_split_one_launch(a.hd, a.ctx_cap, p) ? 0 : attend_split_partials(a, n_rows, p);
 }
 
-template <int HD>
+template <int HD, bool MASS>
 static void launch_split(const AttnArgs &a, int n_rows, const SplitPlan &p, void *scratch, hipStream_t stream) {
     const dim3 grid(n_rows * a.n_head, p.chunks);
     launch_k(k_split_dots<HD>, grid, dim3(64), 0, stream, a, n_rows, p, scratch);
     if (attn_noclamp(a)) {
         launch_k(k_split_sum<true>, grid, dim3(64), 0, stream, a, n_rows, p, scratch);
-        launch_k((k_split_pv<true, HD>), grid, dim3(64), 0, stream, a, n_rows, p, scratch);
+        launch_k((k_split_pv<true, HD, MASS>), grid, dim3(64), 0, stream, a, n_rows, p, scratch);
     } else {
         launch_k(k_split_sum<false>, grid, dim3(64), 0, stream, a, n_rows, p, scratch);
-        launch_k((k_split_pv<false, HD>), grid, dim3(64), 0, stream, a, n_rows, p, scratch);
+        launch_k((k_split_pv<false, HD, MASS>), grid, dim3(64), 0, stream, a, n_rows, p, scratch);
     }
 }
 
-hipError_t launch_attend_split(const AttnArgs &a, int n_rows, const SplitPlan &p, void *scratch,
-                               hipStream_t stream) {
-    if (n_rows <= 0) return hipSuccess;
+template <bool MASS>
+static hipError_t launch_attend_split_t(const AttnArgs &a, int n_rows, const SplitPlan &p, void *scratch,
+                                        hipStream_t stream) {
     if (!attend_split_ok(a.hd) || p.chunk_keys % 64 != 0 || p.chunk_keys > 4096) return hipErrorInvalidValue;
     const int kmax = p.max_keys < a.ctx_cap ? p.max_keys : a.ctx_cap;
     // one launch and no scratch up to 1,024 keys; of it a wave per (row, head) up to 256 keys at
@@ -2533,17 +2581,24 @@ hipError_t launch_attend_split(const AttnArgs &a, int n_rows, const SplitPlan &p
     // row-heads of a GPT-2-medium decode pass 37 against 42, both with the sums p v on 24-bit multiplies;
     // the wave form now takes 5.8 us for the first)
     if (attend_split_one_launch(a.hd, a.ctx_cap, p))
-        return attn_noclamp(a) ? launch_decode_hd<true>(a, n_rows, kmax, stream)
-                               : launch_decode_hd<false>(a, n_rows, kmax, stream);
+        return attn_noclamp(a) ? launch_decode_hd<true, MASS>(a, n_rows, kmax, stream)
+                               : launch_decode_hd<false, MASS>(a, n_rows, kmax, stream);
     switch (a.hd) {
-    case 16: launch_split<16>(a, n_rows, p, scratch, stream); break;
-    case 32: launch_split<32>(a, n_rows, p, scratch, stream); break;
-    case 64: launch_split<64>(a, n_rows, p, scratch, stream); break;
-    case 128: launch_split<128>(a, n_rows, p, scratch, stream); break;
-    default: launch_split<256>(a, n_rows, p, scratch, stream); break;
+    case 16: launch_split<16, MASS>(a, n_rows, p, scratch, stream); break;
+    case 32: launch_split<32, MASS>(a, n_rows, p, scratch, stream); break;
+    case 64: launch_split<64, MASS>(a, n_rows, p, scratch, stream); break;
+    case 128: launch_split<128, MASS>(a, n_rows, p, scratch, stream); break;
+    default: launch_split<256, MASS>(a, n_rows, p, scratch, stream); break;
     }
     launch_k(k_split_out, dim3(n_rows * a.n_head), dim3(a.hd), 0, stream, a, n_rows, p, scratch);
     return hipGetLastError();
+}
+
+hipError_t launch_attend_split(const AttnArgs &a, int n_rows, const SplitPlan &p, void *scratch,
+                               hipStream_t stream) {
+    if (n_rows <= 0) return hipSuccess;
+    return a.mass ? launch_attend_split_t<true>(a, n_rows, p, scratch, stream)
+                  : launch_attend_split_t<false>(a, n_rows, p, scratch, stream);
 }
 
 // =============================================================================================
@@ -4637,11 +4692,11 @@ int kernel_resources(KernelResource *out, int cap) {
         {"k_attend_short<8>", (const void *)k_attend_short<8>},
         {"k_attend_long", (const void *)k_attend_long},
         {"k_attend_mfma<noclamp, lds table>", (const void *)k_attend_mfma<true, true, false>},
-        {"k_attend_decode64<noclamp>", (const void *)k_attend_decode64<true>},
-        {"k_attend_decode_wg<noclamp, 128>", (const void *)k_attend_decode_wg<true, 128>},
-        {"k_attend_decode_wave<noclamp, 4, 64>", (const void *)k_attend_decode_wave<true, 4, 64>},
+        {"k_attend_decode64<noclamp>", (const void *)k_attend_decode64<true, false>},
+        {"k_attend_decode_wg<noclamp, 128>", (const void *)k_attend_decode_wg<true, 128, false>},
+        {"k_attend_decode_wave<noclamp, 4, 64>", (const void *)k_attend_decode_wave<true, 4, 64, false>},
         {"k_split_dots<64>", (const void *)k_split_dots<64>},
-        {"k_split_pv<noclamp, 64>", (const void *)k_split_pv<true, 64>},
+        {"k_split_pv<noclamp, 64>", (const void *)k_split_pv<true, 64, false>},
         {"k_coder_compact", (const void *)k_coder_compact<false, true, false, 256>},
         {"k_coder_compact, few rows with Decode", (const void *)k_coder_compact<false, true, true, 1024>},
         {"k_weights_compact", (const void *)k_weights_compact},
