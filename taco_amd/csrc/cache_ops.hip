@@ -19,25 +19,40 @@ struct Word<4> {
 
 // ---- commit ----------------------------------------------------------------------------------------
 // Row ctx + i takes row ctx + path[i], i < accepted. path[i] >= i, so with the rows in ascending order a
-// row is read before anything is written over it. One wave per (layer, K or V, stream, head) panel.
+// row is read before anything is written over it. A wave takes CM panels (K or V of a layer) of one (stream,
+// head): what bounds it is the chain of loads (counts, path, rows), paid once for all of them, with
+// their rows in flight together. (24 layers x 64 streams x 16 heads, 4 rows in the mean: 14.0 us a call with one panel a wave, 9.4 with eight.)
+constexpr int CM = 8;
+
 template <int W>
-__global__ __launch_bounds__(256) void k_commit(CachePtrs c, CommitArgs a, int n_panels) {
+__global__ __launch_bounds__(256) void k_commit(CachePtrs c, CommitArgs a, int layers, int n_tasks) {
     typedef typename Word<W>::type T;
-    const int lane = threadIdx.x & 63, task = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (task >= 2 * n_panels) return;
-    const int panel = task >> 1, per = a.b * a.h, layer = panel / per, sh = panel - layer * per, s = sh / a.h;
+    const int lane = threadIdx.x & 63, task = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (task >= n_tasks) return;
+    const int per = a.b * a.h, part = task / per, sh = task - part * per, s = sh / a.h;
     const uint32_t cap = (uint32_t)a.cap;
     const uint32_t ctx = a.ctx[s] < cap ? a.ctx[s] : cap;
     uint32_t acc = a.accepted[s] < (uint32_t)a.t ? a.accepted[s] : (uint32_t)a.t;
     acc = acc < cap - ctx ? acc : cap - ctx;
-    if (a.ctx_out && layer == 0 && a.first && (task & 1) == 0 && sh == s * a.h && lane == 0) a.ctx_out[s] = ctx + acc;
-    int8_t *base = ((task & 1) ? c.v[layer] : c.k[layer]) + (size_t)sh * cap * a.hd;
+    if (a.ctx_out && part == 0 && a.first && sh == s * a.h && lane == 0) a.ctx_out[s] = ctx + acc;
     const int words = a.hd / W, rows = 64 / words, r = lane / words, w = lane - r * words;
     if (r >= rows) return;
+    const size_t base = ((size_t)sh * cap + ctx) * a.hd;
     for (uint32_t i = r; i < acc; i += rows) {
         const uint32_t p = a.path[(size_t)s * a.t + i];
         if (p == i || p >= cap - ctx) continue;  // in place already; a row past the cache is left alone
-        ((T *)(base + (size_t)(ctx + i) * a.hd))[w] = ((const T *)(base + (size_t)(ctx + p) * a.hd))[w];
+        T x[CM];
+#pragma unroll
+        for (int u = 0; u < CM; u++) {
+            const int panel = CM * part + u;  // K and V of a layer in turn
+            if (panel < 2 * layers)
+                x[u] = ((const T *)((panel & 1 ? c.v : c.k)[panel >> 1] + base + (size_t)p * a.hd))[w];
+        }
+#pragma unroll
+        for (int u = 0; u < CM; u++) {
+            const int panel = CM * part + u;
+            if (panel < 2 * layers) ((T *)((panel & 1 ? c.v : c.k)[panel >> 1] + base + (size_t)i * a.hd))[w] = x[u];
+        }
     }
 }
 
@@ -48,11 +63,11 @@ static bool wide_words(const CachePtrs &c, int layers, int hd) {
 }
 
 hipError_t launch_commit(const CachePtrs &c, int layers, const CommitArgs &a, hipStream_t stream) {
-    const int panels = layers * a.b * a.h;
-    if (panels <= 0) return hipSuccess;
-    const dim3 grid((2 * panels + 3) / 4);
-    if (wide_words(c, layers, a.hd)) launch_k(k_commit<16>, grid, dim3(256), 0, stream, c, a, panels);
-    else launch_k(k_commit<4>, grid, dim3(256), 0, stream, c, a, panels);
+    const int tasks = (2 * layers + CM - 1) / CM * a.b * a.h;
+    if (tasks <= 0) return hipSuccess;
+    const dim3 grid((tasks + 3) / 4);
+    if (wide_words(c, layers, a.hd)) launch_k(k_commit<16>, grid, dim3(256), 0, stream, c, a, layers, tasks);
+    else launch_k(k_commit<4>, grid, dim3(256), 0, stream, c, a, layers, tasks);
     return hipGetLastError();
 }
 
@@ -229,12 +244,267 @@ __global__ __launch_bounds__(EV_NT) void k_evict(CachePtrs c, EvictArgs a) {
     for (int i = a.budget + tid; i < n; i += EV_NT) mass_out[i] = 0;
 }
 
+// Up to NT R keys a panel: a thread holds R masses, and everything follows from registers in a few barriers. A
+// wave owns 64 R keys in a row, so the ranks of ties, free places and movers are wave ballots and one exchange of
+// the waves' counts. The first digit of the selection is a mass's bit length and the four bits below the leading one
+// (1,040 bins in the order of the values): accumulated weights spread over orders of magnitude, so a bin
+// holds few of them, where the leading byte would hold almost all; then eight bits at a time among
+// that bin's keys, until the rest of a bin stays whole.
+constexpr int EV_BINS = 1040;
+
+__device__ __forceinline__ int mass_bin(uint64_t x) {
+    if (x == 0) return 0;
+    const int e = 63 - __builtin_clzll(x);
+    const int m = (int)(e >= 4 ? x >> (e - 4) : x << (4 - e)) & 15;
+    return 16 * (e + 1) + m;
+}
+
+// s_hist[bin] += 1 for the lanes with `on`; one addition where the whole wave has the same bin.
+__device__ __forceinline__ void count_bin(int *s_hist, int bin, bool on) {
+    const uint64_t lanes = __ballot(on);
+    if (lanes == 0) return;
+    const int lead = __builtin_ctzll(lanes), first = __shfl(bin, lead, 64);
+    if (__ballot(on && bin == first) == lanes) {
+        if ((int)(threadIdx.x & 63) == lead) atomicAdd(&s_hist[first], __popcll(lanes));
+    } else if (on) {
+        atomicAdd(&s_hist[bin], 1);
+    }
+}
+
+// The sum of v over the workgroup's threads before this one; `slots` holds a value per wave.
+template <int NT>
+__device__ __forceinline__ int scan_threads(int v, int *slots, int lane, int w) {
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(x, o, 64);
+        if (lane >= o) x += y;
+    }
+    if (lane == 63) slots[w] = x;
+    __syncthreads();
+    int before = x - v;
+    for (int i = 0; i < w; i++) before += slots[i];
+    return before;
+}
+
+template <int W, int NT, int R>
+__global__ __launch_bounds__(NT) void k_evict_regs(CachePtrs c, EvictArgs a) {
+    typedef typename Word<W>::type T;
+    constexpr int NW = NT / 64, BPT = (EV_BINS + NT - 1) / NT;
+    extern __shared__ uint32_t s_list[];  // NT R / 2 free places, then as many movers
+    __shared__ int s_hist[BPT * NT], s_slots[2][NW], s_pick[3];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), panel = blockIdx.x;
+    const int per = a.b * a.h, layer = panel / per, sh = panel - layer * per, s = sh / a.h;
+    const int cap = a.cap, n = (int)(a.ctx[s] < (uint32_t)cap ? a.ctx[s] : (uint32_t)cap);
+    const size_t at = (size_t)(a.layer0 + layer) * per + sh;
+    const uint64_t *mass = a.mass + at * cap;
+    uint64_t *mass_out = a.mass_out + at * cap;
+    uint32_t *kept = a.kept ? a.kept + at * a.budget : nullptr;
+    if (a.ctx_out && at == (size_t)s * a.h && tid == 0) a.ctx_out[s] = (uint32_t)(n < a.budget ? n : a.budget);
+    const int i0 = 64 * R * w + lane;  // the thread's keys: i0 + 64 j
+    uint64_t x[R];
+#pragma unroll
+    for (int j = 0; j < R; j++) x[j] = i0 + 64 * j < n ? mass[i0 + 64 * j] : 0;
+    if (n <= a.budget) {
+#pragma unroll
+        for (int j = 0; j < R; j++)
+            if (i0 + 64 * j < n) {
+                if (kept) kept[i0 + 64 * j] = i0 + 64 * j;
+                if (mass != mass_out) mass_out[i0 + 64 * j] = x[j];
+            }
+        return;
+    }
+    const int heavy = a.budget - a.recent, m = n - a.recent;
+    // Of the first m keys stay those with x >> sh > pre, and the first `need` of those where they are equal.
+    uint64_t pre = ~(uint64_t)0;
+    int shift = 0, need = heavy, size = 0;  // size: the keys where they are equal
+    if (heavy > 0) {
+        // the bin (from the last one down) in which the need-th key from above lies
+        auto pick = [&](int bins_a_thread) {
+            int mine = 0;
+            for (int b = 0; b < bins_a_thread; b++) mine += s_hist[bins_a_thread * NT - 1 - (bins_a_thread * tid + b)];
+            int above = scan_threads<NT>(mine, s_slots[0], lane, w);
+            if (above < need && above + mine >= need) {
+                int b = bins_a_thread * NT - 1 - bins_a_thread * tid;
+                while (above + s_hist[b] < need) above += s_hist[b--];
+                s_pick[0] = b;
+                s_pick[1] = need - above;
+                s_pick[2] = s_hist[b];
+            }
+            __syncthreads();
+            need = s_pick[1];
+            size = s_pick[2];
+            return s_pick[0];
+        };
+        for (int b = tid; b < BPT * NT; b += NT) s_hist[b] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < R; j++)
+            if (64 * (R * w + j) < m) count_bin(s_hist, mass_bin(x[j]), i0 + 64 * j < m);
+        __syncthreads();
+        const int bin = pick(BPT);
+        const int e = bin / 16 - 1;  // the bit length less one; -1: zeros
+        if (e < 0) pre = 0;
+        else if (e < 4) pre = (uint64_t)(16 + bin % 16) >> (4 - e);
+        else pre = 16 + bin % 16, shift = e - 4;
+        while (shift > 0 && size > need) {
+            const int next = shift > 8 ? shift - 8 : 0, mask = (1 << (shift - next)) - 1;
+            __syncthreads();  // (everyone has read the picked bin)
+            for (int b = tid; b < (NT < 256 ? 256 : NT); b += NT) s_hist[b] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < R; j++)
+                if (64 * (R * w + j) < m) count_bin(s_hist, (int)(x[j] >> next) & mask, i0 + 64 * j < m && x[j] >> shift == pre);
+            __syncthreads();
+            const int digit = pick(1);
+            pre = pre << (shift - next) | (uint64_t)digit;
+            shift = next;
+        }
+    }
+    // who stays; ties in order, where not all of them do
+    uint32_t in = 0;
+    {
+        int ties = 0;
+        uint64_t t[R];
+#pragma unroll
+        for (int j = 0; j < R; j++) {
+            t[j] = __ballot(i0 + 64 * j < m && heavy > 0 && x[j] >> shift == pre);
+            ties += __popcll(t[j]);
+        }
+        if (lane == 0) s_slots[1][w] = ties;
+        __syncthreads();
+        int rank = 0;
+        for (int i = 0; i < w; i++) rank += s_slots[1][i];
+#pragma unroll
+        for (int j = 0; j < R; j++) {
+            const int mine = rank + __builtin_amdgcn_mbcnt_hi((uint32_t)(t[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)t[j], 0));
+            const bool tie = (t[j] >> lane) & 1;
+            if (i0 + 64 * j < m && heavy > 0 && (x[j] >> shift > pre || (tie && mine < need))) in |= 1u << j;
+            rank += __popcll(t[j]);
+        }
+    }
+    uint32_t *s_free = s_list, *s_from = s_list + NT * R / 2;
+    int moves;
+    uint32_t from_rank[R];
+    {
+        int f = 0, q = 0;
+        uint64_t bf[R], bq[R];
+#pragma unroll
+        for (int j = 0; j < R; j++) {
+            const bool stay = (in >> j) & 1;
+            bf[j] = __ballot(i0 + 64 * j < heavy && !stay);
+            bq[j] = __ballot(i0 + 64 * j >= heavy && stay);
+            f += __popcll(bf[j]);
+            q += __popcll(bq[j]);
+        }
+        __syncthreads();
+        if (lane == 0) {
+            s_slots[0][w] = f;
+            s_slots[1][w] = q;
+        }
+        __syncthreads();
+        int fr = 0, qr = 0;
+        moves = 0;
+        for (int i = 0; i < NW; i++) {
+            fr += i < w ? s_slots[0][i] : 0;
+            qr += i < w ? s_slots[1][i] : 0;
+            moves += s_slots[1][i];
+        }
+#pragma unroll
+        for (int j = 0; j < R; j++) {
+            if ((bf[j] >> lane) & 1)
+                s_free[fr + __builtin_amdgcn_mbcnt_hi((uint32_t)(bf[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bf[j], 0))] = i0 + 64 * j;
+            from_rank[j] = qr + __builtin_amdgcn_mbcnt_hi((uint32_t)(bq[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bq[j], 0));
+            if ((bq[j] >> lane) & 1) s_from[from_rank[j]] = i0 + 64 * j;
+            fr += __popcll(bf[j]);
+            qr += __popcll(bq[j]);
+        }
+    }
+    __syncthreads();  // the lists; and every mass has been read
+    int8_t *K = c.k[layer] + (size_t)sh * cap * a.hd, *V = c.v[layer] + (size_t)sh * cap * a.hd;
+    const int words = a.hd / W, rows = NT / words, r = tid / words, wd = tid - r * words;
+    constexpr int U = 2;  // rows a thread has in flight, K and V of each
+    if (r < rows)
+        for (int j = r; j < moves; j += U * rows) {
+            T kx[U], vx[U];
+            uint32_t to[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int q = j + u * rows < moves ? j + u * rows : j;
+                to[u] = s_free[q];
+                const size_t o = (size_t)s_from[q] * a.hd;
+                kx[u] = ((const T *)(K + o))[wd];
+                vx[u] = ((const T *)(V + o))[wd];
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (j + u * rows >= moves) break;
+                const size_t o = (size_t)to[u] * a.hd;
+                ((T *)(K + o))[wd] = kx[u];
+                ((T *)(V + o))[wd] = vx[u];
+            }
+        }
+#pragma unroll
+    for (int j = 0; j < R; j++) {
+        const int i = i0 + 64 * j;
+        if (i >= n) continue;
+        int to = i;  // the key's place, if it has one
+        if (i >= m) to = heavy + (i - m);
+        else if (!((in >> j) & 1)) to = -1;
+        else if (i >= heavy) to = (int)s_free[from_rank[j]];
+        if (to >= 0) {
+            mass_out[to] = x[j];
+            if (kept) kept[to] = i;
+        }
+        if (i >= a.budget) mass_out[i] = 0;
+    }
+    // the recent rows: m .. n - 1 to heavy .. budget - 1, a tile read whole before it is written
+    const int8_t *K0 = K + (size_t)m * a.hd, *V0 = V + (size_t)m * a.hd;
+    K += (size_t)heavy * a.hd;
+    V += (size_t)heavy * a.hd;
+    for (int j0 = 0; j0 < a.recent; j0 += U * rows) {
+        T kx[U], vx[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int j = j0 + u * rows + r;
+            if (r < rows && j < a.recent) {
+                kx[u] = ((const T *)(K0 + (size_t)j * a.hd))[wd];
+                vx[u] = ((const T *)(V0 + (size_t)j * a.hd))[wd];
+            }
+        }
+        __syncthreads();  // (the first one: the movers have been read, too)
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int j = j0 + u * rows + r;
+            if (r < rows && j < a.recent) {
+                ((T *)(K + (size_t)j * a.hd))[wd] = kx[u];
+                ((T *)(V + (size_t)j * a.hd))[wd] = vx[u];
+            }
+        }
+        __syncthreads();
+    }
+}
+
+template <int W>
+static hipError_t launch_evict_w(const CachePtrs &c, int panels, const EvictArgs &a, hipStream_t stream) {
+    auto run = [&](auto kernel, int nt, int r) {
+        const size_t lds = (size_t)4 * nt * r;
+        const hipError_t e = allow_dynamic_lds((const void *)kernel, lds);
+        if (e != hipSuccess) return e;
+        launch_k(kernel, dim3(panels), dim3(nt), lds, stream, c, a);
+        return hipGetLastError();
+    };
+    if (a.cap <= 1024) return run(k_evict_regs<W, 256, 4>, 256, 4);
+    if (a.cap <= 4096) return run(k_evict_regs<W, 512, 8>, 512, 8);
+    if (a.cap <= 16384) return run(k_evict_regs<W, 1024, 16>, 1024, 16);
+    launch_k(k_evict<W>, dim3(panels), dim3(EV_NT), 0, stream, c, a);
+    return hipGetLastError();
+}
+
 hipError_t launch_evict(const CachePtrs &c, int layers, const EvictArgs &a, hipStream_t stream) {
     const int panels = layers * a.b * a.h;
     if (panels <= 0) return hipSuccess;
-    if (wide_words(c, layers, a.hd)) launch_k(k_evict<16>, dim3(panels), dim3(EV_NT), 0, stream, c, a);
-    else launch_k(k_evict<4>, dim3(panels), dim3(EV_NT), 0, stream, c, a);
-    return hipGetLastError();
+    return wide_words(c, layers, a.hd) ? launch_evict_w<16>(c, panels, a, stream) : launch_evict_w<4>(c, panels, a, stream);
 }
 
 }  // namespace hs

@@ -225,7 +225,7 @@ def test_evict_head_dims(gpu, hd):
 
 
 @pytest.mark.parametrize("cap,budget,recent", [(1, 1, 0), (2, 1, 0), (2, 1, 1), (300, 299, 0), (300, 1, 0), (300, 64, 64),
-                                               (1024, 512, 128), (1024, 1023, 700), (700, 300, 299), (5000, 1300, 17),
+                                               (1024, 512, 128), (1024, 1023, 700), (700, 300, 299), (3000, 1000, 100), (5000, 1300, 17), (16384, 9000, 1000),
                                                (20000, 6000, 511), (20000, 300, 0)])
 @pytest.mark.parametrize("alias", [False, True])
 def test_evict_budgets(gpu, cap, budget, recent, alias):
@@ -240,7 +240,7 @@ def test_evict_ties_go_to_the_lowest_index(gpu, acc):
 def test_evict_orders_of_weights(gpu):
     """Rising and falling weights (every kept key moves, none does), two values only, the top bits alone."""
     i = np.arange(1500, dtype=np.uint64)
-    for acc in (i, 1500 - i, i % 2, (i % 3) << np.uint64(62), np.where(i == 700, 2 ** 63, i).astype(np.uint64)):
+    for acc in (i, 1500 - i, i % 2, i % 7, i * i * i, i << np.uint64(20), (i % 3) << np.uint64(62), np.where(i == 700, 2 ** 63, i).astype(np.uint64)):
         check_evict(gpu, 1, 2, 1, 64, 1500, [1500, 1100], 600, 100, acc=acc)
 
 
