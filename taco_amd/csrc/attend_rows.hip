@@ -333,8 +333,14 @@ __device__ __forceinline__ void load_table(const AttnArgs &a, int32_t *s_exp, in
             s_exp[i] = a.exp_table[i < a.exp_len ? i : a.exp_len - 1];
 }
 
+// The bytes of LDS before a tile's V regions: the table, which the sums of the outputs take over.
+__host__ __device__ inline int tile_top(int qc, int table_chunks) {
+    const int acc = (8 * qc * RT_ROWS * RT_ACC + 1023) / 1024 * 1024;
+    return 1024 * table_chunks > acc ? 1024 * table_chunks : acc;
+}
+
 template <int QC, int NB, int NW, bool HI>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void k_rows_tile(RowsArgs g, int tiles, int panels) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QC == 1 && NW == 4 ? 3 : 2))) void k_rows_tile(RowsArgs g, int tiles, int panels) {
     extern __shared__ __attribute__((aligned(1024))) int8_t s_mem[];
     const AttnArgs &a = g.a;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -348,10 +354,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     if (row0 >= R.count) return;
     const int last = a.exp_len - 1, table_chunks = (a.exp_len + 255) / 256;
     int32_t *s_exp = (int32_t *)s_mem;
-    int8_t *s_v = s_mem + 1024 * table_chunks + 4096 * w;
-    int64_t *s_acc = (int64_t *)(s_mem + 1024 * table_chunks + 4096 * NW);  // [QC][16][RT_ACC]
-    uint64_t *s_sum = (uint64_t *)(s_acc + QC * RT_ROWS * RT_ACC);          // [NW][16]
-    int32_t *s_mm = (int32_t *)(s_sum + NW * RT_ROWS);                      // [2][NW][16]
+    const int top = tile_top(QC, table_chunks);
+    int64_t *s_acc = (int64_t *)s_mem;  // [QC][16][RT_ACC], over the table when that is done with
+    int8_t *s_v = s_mem + top + 4096 * w;
+    uint64_t *s_sum = (uint64_t *)(s_mem + top + 4096 * NW);  // [NW][16]
+    int32_t *s_mm = (int32_t *)(s_sum + NW * RT_ROWS);        // [2][NW][16]
 
     int keys = stream_keys(g, R);
     if (!g.mask) keys = R.base + row0 + RT_ROWS < keys ? R.base + row0 + RT_ROWS : keys;  // causal: the tile's last row
@@ -372,7 +379,6 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         const int o = 64 * c + 16 * qg;
         qf[c] = row < R.count && o < hd ? *(const v4i *)(a.q + (size_t)(R.first + row) * a.ldq + h * hd + o) : zero;
     }
-    for (int i = tid; i < QC * RT_ROWS * RT_ACC; i += 64 * NW) s_acc[i] = 0;
 
     // the dots (keys past the last reload it)
     v4i D[NB][4];
@@ -449,6 +455,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     sum = 0;
 #pragma unroll
     for (int i = 0; i < NW; i++) sum += s_sum[i * RT_ROWS + ql];
+    for (int i = tid; i < QC * RT_ROWS * RT_ACC; i += 64 * NW) s_acc[i] = 0;  // (every wave has its entries)
     const RowWeight wt(sum, a.softmax_p, row < R.count);
 #pragma unroll
     for (int j = 0; j < NB; j++)
@@ -469,6 +476,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
             if (c + 1 < QC) v_load(j, c + 1);
             block_pv(s_v, D[j], lane, acc);
         }
+        if (c == 0) lds_barrier();  // the zeros
         if (mine(0)) {
             unsigned long long *to = (unsigned long long *)s_acc + (c * RT_ROWS + ql) * RT_ACC + 4 * qg;
 #pragma unroll
@@ -493,7 +501,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
 template <int QC, int NB, int NW, bool HI>
 static hipError_t launch_tile_t(const RowsArgs &g, hipStream_t stream) {
     const int tiles = (g.t + RT_ROWS - 1) / RT_ROWS, panels = g.streams * g.a.n_head;
-    const size_t lds = (size_t)1024 * ((g.a.exp_len + 255) / 256) + 4096 * NW + 8 * QC * RT_ROWS * RT_ACC + 16 * NW * RT_ROWS;
+    const size_t lds = (size_t)tile_top(QC, (g.a.exp_len + 255) / 256) + 4096 * NW + 16 * NW * RT_ROWS;
     const hipError_t e = allow_dynamic_lds((const void *)k_rows_tile<QC, NB, NW, HI>, lds);
     if (e != hipSuccess) return e;
     launch_k((k_rows_tile<QC, NB, NW, HI>), dim3((unsigned)((panels + 7) / 8 * 8) * tiles), dim3(64 * NW), lds, stream, g, tiles, panels);
