@@ -380,24 +380,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QC == 1
         qf[c] = row < R.count && o < hd ? *(const v4i *)(a.q + (size_t)(R.first + row) * a.ldq + h * hd + o) : zero;
     }
 
-    // the dots (keys past the last reload it)
-    v4i D[NB][4];
-#pragma unroll
-    for (int j = 0; j < NB; j++) {
-        if (!mine(j)) continue;
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const int k = 64 * block(j) + 16 * t + ql;
-            const int8_t *kr = K + (size_t)(k < keys ? k : kmost) * hd + 16 * qg;
-            v4i d = zero;
-#pragma unroll
-            for (int c = 0; c < QC; c++)
-                d = __builtin_amdgcn_mfma_i32_16x16x64_i8(64 * c + 16 * qg < hd ? *(const v4i *)(kr + 64 * c) : zero, qf[c], d, 0, 0, 0);
-            D[j][t] = d;
-        }
-    }
+    // K (keys past the last reload it), then V of the first channel group, all in flight together; a block's
+    // dots need no more registers than its K did
+    v4i D[NB][4], vr[NB][4];
+    auto k_load = [&](int j, int t, int c) {
+        const int k = 64 * block(j) + 16 * t + ql, o = 64 * c + 16 * qg;
+        return o < hd ? *(const v4i *)(K + (size_t)(k < keys ? k : kmost) * hd + o) : zero;
+    };
     // V of chunk group c, block j: lane l the 16 bytes (l % 4) ^ vsw of rows 16 u + l / 4
-    v4i vr[NB][4];
     auto v_load = [&](int j, int c) {
 #pragma unroll
         for (int u = 0; u < 4; u++) {
@@ -405,9 +395,43 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QC == 1
             vr[j][u] = o < hd ? *(const v4i *)(V + (size_t)(k < keys ? k : kmost) * hd + o) : zero;
         }
     };
+    if constexpr (QC <= 2) {
+        // (no branch around the loads, so that the waits count them exactly: blocks past the keys reload the last key)
+        v4i hi[QC == 2 ? NB : 1][4];  // K's second chunk
 #pragma unroll
-    for (int j = 0; j < NB; j++)
-        if (mine(j)) v_load(j, 0);
+        for (int j = 0; j < NB; j++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                D[j][t] = k_load(j, t, 0);
+                if (QC == 2) hi[j][t] = k_load(j, t, 1);
+            }
+#pragma unroll
+        for (int j = 0; j < NB; j++) v_load(j, 0);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < NB; j++)
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+                if (mine(j)) {
+                    D[j][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(D[j][t], qf[0], zero, 0, 0, 0);
+                    if (QC == 2) D[j][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(hi[j][t], qf[QC - 1], D[j][t], 0, 0, 0);
+                }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+            if (!mine(j)) continue;
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                v4i d = zero;
+#pragma unroll
+                for (int c = 0; c < QC; c++) d = __builtin_amdgcn_mfma_i32_16x16x64_i8(k_load(j, t, c), qf[c], d, 0, 0, 0);
+                D[j][t] = d;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NB; j++)
+            if (mine(j)) v_load(j, 0);
+    }
 
     const RowSight sight = row_sight(g, R, row, keys);
     // a block whose keys every row of the tile sees
