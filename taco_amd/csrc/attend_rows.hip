@@ -121,15 +121,15 @@ constexpr int RT_ROWS = 16;
 constexpr int RT_TABLE = 16384;  // entries of the table copied to LDS at most
 constexpr int RT_ACC = 66;       // 64 channels' sums of a row and two of padding (bank spread)
 
-// Sums over the 16 rows (lanes l % 16) of p of a block's 64 keys: lane l receives the sum of key
-// 16 (l % 16 / 4) + 4 (l / 16) + l % 4. A reduce-scatter in four steps: each lane hands half of what it holds to
-// its partner and keeps the other half.
+// Sums over the 16 rows (lanes l % 16) of p of a block's 64 keys, given as p + 0x80808080: lane l receives the sum of
+// key 16 (l % 16 / 4) + 4 (l / 16) + l % 4. A reduce-scatter in four steps: each lane hands half of what it holds
+// to its partner and keeps the other half.
 __device__ __forceinline__ uint64_t row_sums(const uint32_t (&p)[16], int lane) {
     const bool b3 = lane & 8, b2 = lane & 4, b1 = lane & 2, b0 = lane & 1;
     uint32_t x[8];  // two rows: at most 2^31
 #pragma unroll
     for (int i = 0; i < 8; i++)
-        x[i] = (b3 ? p[i + 8] : p[i]) + (uint32_t)dpp_mov<0x140>((int32_t)(b3 ? p[i] : p[i + 8]));
+        x[i] = (b3 ? p[i + 8] : p[i]) + (uint32_t)dpp_mov<0x140>((int32_t)(b3 ? p[i] : p[i + 8])) - 0x01010100u;
     uint64_t y[4], z[2];
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -139,50 +139,40 @@ __device__ __forceinline__ uint64_t row_sums(const uint32_t (&p)[16], int lane) 
     return (b0 ? z[1] : z[0]) + (uint64_t)lane_move64<0>((int64_t)(b0 ? z[0] : z[1]));
 }
 
-// What a lane needs to know of its row: which keys it sees.
+// What a lane needs to know of its row (l % 16): which keys it sees.
 struct RowSight {
-    int base, lim;  // a key below base + (tree: 0, causal: row + 1) is seen: key <= lim
-    const uint64_t *bits;  // the row's mask words (tree)
-    int count;             // nodes of the stream
+    int base, lim;   // keys up to lim are seen: the context (tree), the row's own key (causal)
+    int count;       // nodes of the stream (tree; else 0)
+    uint64_t word;   // tree: word l / 16 of the row's mask
 };
 
-__device__ __forceinline__ RowSight row_sight(const RowsArgs &g, const StreamRows &R, int row, int keys) {
+__device__ __forceinline__ RowSight row_sight(const RowsArgs &g, const StreamRows &R, int row, int qg, int keys) {
     RowSight v;
-    v.base = R.base;
-    v.count = R.count;
-    v.bits = nullptr;
     const bool live = row < R.count;
-    if (g.mask) {
-        v.lim = live ? (R.base < keys ? R.base : keys) - 1 : -1;
-        v.bits = live ? R.mask + (size_t)row * g.words : nullptr;
-    } else {
-        v.lim = live ? (R.base + row < keys - 1 ? R.base + row : keys - 1) : -1;
-    }
+    v.base = R.base;
+    v.lim = live ? (g.mask ? (R.base < keys ? R.base : keys) - 1 : (R.base + row < keys - 1 ? R.base + row : keys - 1)) : -1;
+    v.count = g.mask ? R.count : 0;
+    v.word = g.mask && live && qg < g.words ? R.mask[(size_t)row * g.words + qg] : 0;
     return v;
 }
 
-// The keys 16 t + 4 qg + e of block kb that the row sees, bit 4 t + e.
-__device__ __forceinline__ uint32_t sight_bits(const RowSight &v, int kb, int qg, int keys) {
-    uint32_t ok = 0;
-    const int L = v.lim - 64 * kb - 4 * qg;
-#pragma unroll
-    for (int t = 0; t < 4; t++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) ok |= (16 * t + e <= L ? 1u : 0u) << (4 * t + e);
-    const int n0 = 64 * kb - v.base;  // the node of the block's first key
-    if (v.bits && n0 + 63 >= 0) {
+// Of the keys 64 kb + 16 t + 4 (l / 16) + e those that the row sees, bit 4 t + e. (Every lane of the wave.)
+__device__ __forceinline__ uint32_t sight_bits(const RowSight &v, int kb, int lane, int keys) {
+    const int seen = v.lim + 1 - 64 * kb;
+    uint64_t m = seen >= 64 ? ~(uint64_t)0 : (seen > 0 ? ((uint64_t)1 << seen) - 1 : 0);
+    const int n0 = 64 * kb - v.base;  // the node of the first key
+    if (v.count && n0 + 63 >= 0) {    // uniform
         // the 64 mask bits from node n0 on, those of nodes count .. and of keys past the cache cleared
         const int words = (v.count + 63) >> 6, w = n0 >> 6, o = n0 & 63;
-        uint64_t m = w >= 0 && w < words ? v.bits[w] >> o : 0;
-        if (o && w + 1 >= 0 && w + 1 < words) m |= v.bits[w + 1] << (64 - o);
-        const int most = (v.count < keys - v.base ? v.count : keys - v.base) - n0;  // nodes of the block
-        m = most <= 0 ? 0 : (most < 64 ? m & (((uint64_t)1 << most) - 1) : m);
-        if (n0 < 0) m &= ~(uint64_t)0 << -n0;
-        m >>= 4 * qg;
-#pragma unroll
-        for (int t = 0; t < 4; t++) ok |= ((uint32_t)(m >> (16 * t)) & 15u) << (4 * t);
+        const uint64_t lo = __shfl(v.word, 16 * (w & 3) + (lane & 15), 64), hi = __shfl(v.word, 16 * ((w + 1) & 3) + (lane & 15), 64);
+        uint64_t n = w >= 0 && w < words ? lo >> o : 0;
+        if (o && w + 1 < words) n |= hi << (64 - o);
+        const int most = (v.count < keys - v.base ? v.count : keys - v.base) - n0;  // nodes up to the end of the block
+        n = most <= 0 ? 0 : (most < 64 ? n & (((uint64_t)1 << most) - 1) : n);
+        m |= n0 < 0 ? n & ~(uint64_t)0 << -n0 : n;
     }
-    return ok;
+    m >>= 4 * (lane >> 4);
+    return (uint32_t)(m & 15) | (uint32_t)(m >> 12 & 0xf0) | (uint32_t)(m >> 24 & 0xf00) | (uint32_t)(m >> 36 & 0xf000);
 }
 
 // ---- The steps on a block: 64 keys x 16 rows, D[t][e] of lane l belongs to row l % 16 and key 16 t + 4 (l / 16) + e
@@ -219,6 +209,7 @@ __device__ __forceinline__ void block_extremes(const v4i (&D)[4], bool all, uint
 template <bool HI>
 struct RowIndex {
     int64_t c;  // HI: the row's addend; else M
+    __device__ __forceinline__ explicit RowIndex(int64_t row) : c(row) {}
     __device__ __forceinline__ RowIndex(const AttnArgs &a, int32_t dmax, int32_t dmin) {
         if (dmax < dmin) dmax = dmin = 0;  // a row that sees nothing
         const int64_t s0 = attn_score<HI>(a, dmax), s1 = attn_score<HI>(a, dmin);
@@ -281,10 +272,7 @@ __device__ __forceinline__ void block_digits(v4i (&D)[4], double R, double sp, u
         dg[i] = (uint32_t)__double2loint(w) + (uint32_t)(__double2hiint(r) >> 31);
     }
     if (mass) {  // uniform
-        uint32_t p[16];
-#pragma unroll
-        for (int i = 0; i < 16; i++) p[i] = dg[i] - 0x80808080u;
-        const uint64_t x = row_sums(p, lane);
+        const uint64_t x = row_sums(dg, lane);
         const int key = 16 * ((lane & 15) >> 2) + 4 * (lane >> 4) + (lane & 3);
         if (x && key < keys) atomicAdd((unsigned long long *)mass + key, (unsigned long long)x);
     }
@@ -304,12 +292,13 @@ struct RowWeight {
 };
 
 // acc[k][i] += V^T digits over a block whose V rows lie in s_v (16-byte chunk c of row r at slot 4 r + (c ^ vsw(r))):
-// channel 16 i + 4 (l / 16) + e of row l % 16.
-__device__ __forceinline__ void block_pv(const int8_t *s_v, const v4i (&pf)[4], int lane, v4i (&acc)[4][4]) {
+// channel 16 (i0 + i) + 4 (l / 16) + e of row l % 16, i < N.
+template <int N>
+__device__ __forceinline__ void block_pv(const int8_t *s_v, const v4i (&pf)[4], int i0, int lane, v4i (&acc)[4][N]) {
     const int ql = lane & 15, qg = lane >> 4, tr_k = ql >> 1, key0 = 16 * (tr_k >> 2) + 4 * qg + (tr_k & 3);
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int8_t *p0 = s_v + (4 * key0 + (i ^ vsw<4>(key0 & 15))) * 16 + 8 * (ql & 1);
+    for (int i = 0; i < N; i++) {
+        const int8_t *p0 = s_v + (4 * key0 + ((i0 + i) ^ vsw<4>(key0 & 15))) * 16 + 8 * (ql & 1);
         const v2i r0 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)p0);
         const v2i r1 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)(p0 + 32 * 64));
         const v4i vf = v4i{r0[0], r0[1], r1[0], r1[1]};
@@ -318,9 +307,38 @@ __device__ __forceinline__ void block_pv(const int8_t *s_v, const v4i (&pf)[4], 
     }
 }
 
-__device__ __forceinline__ int64_t plane_sum(const v4i (&acc)[4][4], int i, int e) {
+template <int N>
+__device__ __forceinline__ int64_t plane_sum(const v4i (&acc)[4][N], int i, int e) {
     return (int64_t)acc[0][i][e] + (int64_t)acc[1][i][e] * 256 + (int64_t)acc[2][i][e] * 65536 +
            (int64_t)acc[3][i][e] * 16777216;
+}
+
+// The rows of a (stream, head) in a cache, read by buffer loads: one offset a lane for all blocks and the block's in
+// a scalar register; rows past the cache read as zeros without an access, and so does all of a block without keys
+// (`none`), so nothing is clamped. K comes as the product's operand (chunk c: 16 bytes from 64 c + 16 (l / 16) on of
+// rows 16 t + l % 16), V in block_pv's layout (group c: the 16 bytes (l % 4) ^ vsw of rows 16 u + l / 4). Columns
+// past the head read its first ones: K's meet zeros of q there, V's outputs are not stored.
+struct Panel {
+    __amdgpu_buffer_rsrc_t rsrc;
+    int bytes;  // at most 2^30
+    __device__ __forceinline__ Panel(const int8_t *p, int cap, int hd) : bytes(cap * hd) {
+        rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, bytes, 0x00020000);
+    }
+    // the 16 bytes at lane offset `at` of the block that starts at row `row` (below cap), or zeros
+    __device__ __forceinline__ v4i load(int at, int row, int hd, bool none) const {
+        return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, none ? bytes : row * hd, 0));
+    }
+};
+template <int QC>
+__device__ __forceinline__ void load_k(const Panel &p, int row, int c, int hd, bool none, int lane, v4i (&x)[4][QC]) {
+    const int o = 64 * c + 16 * (lane >> 4), at = (lane & 15) * hd + (o < hd ? o : 0);
+#pragma unroll
+    for (int t = 0; t < 4; t++) x[t][c] = p.load(at + 16 * t * hd, row, hd, none);
+}
+__device__ __forceinline__ void load_v(const Panel &p, int row, int c, int hd, bool none, int lane, v4i (&x)[4]) {
+    const int r = lane >> 2, o = 64 * c + 16 * ((lane & 3) ^ vsw<4>(r)), at = r * hd + (o < hd ? o : 0);
+#pragma unroll
+    for (int u = 0; u < 4; u++) x[u] = p.load(at + 16 * u * hd, row, hd, none);
 }
 
 // The table to LDS: whole KiB straight, the end entry by entry (places past it repeat the last one). The caller waits.
@@ -363,9 +381,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QC == 1
     int keys = stream_keys(g, R);
     if (!g.mask) keys = R.base + row0 + RT_ROWS < keys ? R.base + row0 + RT_ROWS : keys;  // causal: the tile's last row
     keys = keys < 64 * NB * NW ? keys : 64 * NB * NW;  // (the launch's bound holds every count)
-    const int kmost = keys > 0 ? keys - 1 : 0;
     const size_t at = (size_t)R.slot * a.n_head + h, base = at * a.ctx_cap * hd;
-    const int8_t *K = a.kc + base, *V = a.vc + base;
+    const Panel K(a.kc + base, a.ctx_cap, hd), V(a.vc + base, a.ctx_cap, hd);
     auto block = [&](int j) { return NW * j + w; };
     auto mine = [&](int j) { return 64 * block(j) < keys; };  // uniform
 
@@ -380,31 +397,17 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QC == 1
         qf[c] = row < R.count && o < hd ? *(const v4i *)(a.q + (size_t)(R.first + row) * a.ldq + h * hd + o) : zero;
     }
 
-    // K (keys past the last reload it), then V of the first channel group, all in flight together; a block's
-    // dots need no more registers than its K did
+    const RowSight sight = row_sight(g, R, row, qg, keys);
+    // K, then V of the first channel group, all in flight together and no branch around them, so that the waits count
+    // them exactly; a block's dots take the registers of its K
     v4i D[NB][4], vr[NB][4];
-    auto k_load = [&](int j, int t, int c) {
-        const int k = 64 * block(j) + 16 * t + ql, o = 64 * c + 16 * qg;
-        return o < hd ? *(const v4i *)(K + (size_t)(k < keys ? k : kmost) * hd + o) : zero;
-    };
-    // V of chunk group c, block j: lane l the 16 bytes (l % 4) ^ vsw of rows 16 u + l / 4
-    auto v_load = [&](int j, int c) {
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int r = 16 * u + (lane >> 2), k = 64 * block(j) + r, o = 64 * c + 16 * ((lane & 3) ^ vsw<4>(r & 15));
-            vr[j][u] = o < hd ? *(const v4i *)(V + (size_t)(k < keys ? k : kmost) * hd + o) : zero;
-        }
-    };
+    auto v_load = [&](int j, int c) { load_v(V, 64 * block(j), c, hd, !mine(j), lane, vr[j]); };
+    v4i kr[NB][4][QC <= 2 ? QC : 1];
     if constexpr (QC <= 2) {
-        // (no branch around the loads, so that the waits count them exactly: blocks past the keys reload the last key)
-        v4i hi[QC == 2 ? NB : 1][4];  // K's second chunk
 #pragma unroll
         for (int j = 0; j < NB; j++)
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                D[j][t] = k_load(j, t, 0);
-                if (QC == 2) hi[j][t] = k_load(j, t, 1);
-            }
+            for (int c = 0; c < QC; c++) load_k<QC>(K, 64 * block(j), c, hd, !mine(j), lane, kr[j]);
 #pragma unroll
         for (int j = 0; j < NB; j++) v_load(j, 0);
         __builtin_amdgcn_sched_barrier(0);
@@ -413,27 +416,27 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QC == 1
 #pragma unroll
             for (int t = 0; t < 4; t++)
                 if (mine(j)) {
-                    D[j][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(D[j][t], qf[0], zero, 0, 0, 0);
-                    if (QC == 2) D[j][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(hi[j][t], qf[QC - 1], D[j][t], 0, 0, 0);
+                    D[j][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[j][t][0], qf[0], zero, 0, 0, 0);
+                    if (QC == 2) D[j][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[j][t][QC == 2], qf[QC == 2], D[j][t], 0, 0, 0);
                 }
     } else {
 #pragma unroll
         for (int j = 0; j < NB; j++) {
             if (!mine(j)) continue;
+            v4i k4[4][QC];
+#pragma unroll
+            for (int c = 0; c < QC; c++) load_k<QC>(K, 64 * block(j), c, hd, false, lane, k4);
 #pragma unroll
             for (int t = 0; t < 4; t++) {
-                v4i d = zero;
+                D[j][t] = zero;
 #pragma unroll
-                for (int c = 0; c < QC; c++) d = __builtin_amdgcn_mfma_i32_16x16x64_i8(k_load(j, t, c), qf[c], d, 0, 0, 0);
-                D[j][t] = d;
+                for (int c = 0; c < QC; c++) D[j][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k4[t][c], qf[c], D[j][t], 0, 0, 0);
             }
         }
 #pragma unroll
-        for (int j = 0; j < NB; j++)
-            if (mine(j)) v_load(j, 0);
+        for (int j = 0; j < NB; j++) v_load(j, 0);
     }
 
-    const RowSight sight = row_sight(g, R, row, keys);
     // a block whose keys every row of the tile sees
     const int whole = g.mask ? R.base : R.base + row0 + 1;
     auto all = [&](int j) { return 64 * block(j) + 64 <= (whole < keys ? whole : keys); };
@@ -443,7 +446,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QC == 1
     for (int j = 0; j < NB; j++) {
         ok[j] = 0;
         if (!mine(j)) continue;
-        if (!all(j)) ok[j] = sight_bits(sight, block(j), qg, keys);
+        if (!all(j)) ok[j] = sight_bits(sight, block(j), lane, keys);
         block_extremes(D[j], all(j), ok[j], dmax, dmin);
     }
 #pragma unroll
@@ -482,31 +485,45 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QC == 1
     for (int i = tid; i < QC * RT_ROWS * RT_ACC; i += 64 * NW) s_acc[i] = 0;  // (every wave has its entries)
     const RowWeight wt(sum, a.softmax_p, row < R.count);
 #pragma unroll
-    for (int j = 0; j < NB; j++)
+    for (int j = 0; j < NB; j++) {
+        __builtin_amdgcn_sched_barrier(0);  // (a block at a time: interleaved they spill)
         if (mine(j))
             block_digits(D[j], wt.R, wt.sp, g.mass ? g.mass + at * a.ctx_cap + 64 * block(j) : nullptr, keys - 64 * block(j), lane);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // The products with V, 16 N channels at a time (a lane writes its V words of those columns only). At four blocks a
+    // wave and three workgroups a CU 64 sums beside the digits and V would not fit the registers, nor would 32, and what
+    // spills are V's loads in flight: N = 1 there.
+    constexpr int N = QC == 1 && NB == 4 && NW == 4 ? 1 : 4;
+    const int column = (lane & 3) ^ vsw<4>(lane >> 2);  // of the lane's V words
 #pragma unroll
     for (int c = 0; c < QC; c++) {
-        v4i acc[4][4];
 #pragma unroll
-        for (int k = 0; k < 4; k++)
+        for (int i0 = 0; i0 < 4; i0 += N) {
+            v4i acc[4][N];
 #pragma unroll
-            for (int i = 0; i < 4; i++) acc[k][i] = zero;
+            for (int k = 0; k < 4; k++)
 #pragma unroll
-        for (int j = 0; j < NB; j++) {
-            if (!mine(j)) continue;
+                for (int i = 0; i < N; i++) acc[k][i] = zero;
 #pragma unroll
-            for (int u = 0; u < 4; u++) *(v4i *)(s_v + 1024 * u + 16 * lane) = vr[j][u];
-            if (c + 1 < QC) v_load(j, c + 1);
-            block_pv(s_v, D[j], lane, acc);
-        }
-        if (c == 0) lds_barrier();  // the zeros
-        if (mine(0)) {
-            unsigned long long *to = (unsigned long long *)s_acc + (c * RT_ROWS + ql) * RT_ACC + 4 * qg;
+            for (int j = 0; j < NB; j++) {
+                if (!mine(j)) continue;
+                __builtin_amdgcn_sched_barrier(0);
+                if (N == 4 || column / N == i0 / N) {
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+                    for (int u = 0; u < 4; u++) *(v4i *)(s_v + 1024 * u + 16 * lane) = vr[j][u];
+                }
+                if (i0 + N == 4 && c + 1 < QC) v_load(j, c + 1);
+                block_pv<N>(s_v, D[j], i0, lane, acc);
+            }
+            if (c == 0 && i0 == 0) lds_barrier();  // the zeros
+            if (mine(0)) {
+                unsigned long long *to = (unsigned long long *)s_acc + (c * RT_ROWS + ql) * RT_ACC + 16 * i0 + 4 * qg;
 #pragma unroll
-                for (int e = 0; e < 4; e++) atomicAdd(to + 16 * i + e, (unsigned long long)plane_sum(acc, i, e));
+                for (int i = 0; i < N; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) atomicAdd(to + 16 * i + e, (unsigned long long)plane_sum(acc, i, e));
+            }
         }
     }
     lds_barrier();
@@ -541,15 +558,19 @@ static hipError_t launch_tile(const RowsArgs &g, int keys, hipStream_t stream) {
 }
 
 // ---- Caches longer than a tile's registers ------------------------------------------------------------
-// Key ranges of `span` keys over workgroups of four waves: WT row tiles side by side (each wave walks the blocks
-// of its tile; the others' loads of the same rows hit the L1) and 4 / WT waves to a tile. The integer softmax
-// needs the row maximum before the entries and their sum before p, so there are three walks over the keys, each
-// forming the dots again (4 MFMAs a block, less than keeping them would cost): PHASE 1 the extreme dots, 2 the
-// sums, 3 the products with V, one launch each over all ranges, with the ranges' results in the workspace
-// and a last launch that adds the ranges' outputs. PHASE 0: all three walks in one launch, where the rows alone
-// give enough workgroups. GC: groups of 64 channels of a workgroup (a head dim above 128 takes a workgroup for each).
+// Key ranges of `span` keys over workgroups of four waves. The integer softmax needs the row maximum before the
+// entries and their sum before p, so there are three walks over the keys, each forming the dots again (4 MFMAs
+// a block and tile, less than keeping them would cost), one launch each over all ranges with the ranges' results in
+// the workspace, and a last launch that adds the ranges' outputs:
+//   k_long_scan<1> the extreme dots, <2> the sums: a wave takes blocks of keys with all WT row tiles of the group
+//     (up to four), so the four waves' loads are of different keys;
+//   k_long_pv the products with V: WT tiles side by side, 4 / WT waves to a tile, since a tile's sums are 64
+//     registers for 64 channels (the others' loads of the same rows hit the L1).
+// ALONE: k_long_pv walks all three times itself, where the rows alone give enough workgroups. A head dim above
+// 128 takes a workgroup for each 64 channels (cg).
 struct LongPlan {
-    int tiles = 0, wt = 1, groups = 1, ng = 1, span = 0, cg = 1;
+    int tiles = 0, wt = 1, groups = 1;  // row tiles; of a group; groups
+    int ng = 1, span = 0, cg = 1;        // key ranges, their keys; workgroups for the channels
 };
 struct LongScratch {
     int32_t *mm;    // [panels][rows][ng][2]: the largest and smallest dot of a range
@@ -575,16 +596,155 @@ __device__ __forceinline__ int group_keys(const RowsArgs &g, const StreamRows &R
 }
 
 template <int QC, int WT, bool HI, int PHASE>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k_rows_long(RowsArgs g, LongPlan pl, int panels, void *scratch) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k_long_scan(RowsArgs g, LongPlan pl, int panels, void *scratch) {
+    extern __shared__ __attribute__((aligned(1024))) int8_t s_mem[];  // the table
+    __shared__ uint64_t s_sum[4][WT][RT_ROWS];
+    __shared__ int32_t s_mm[2][4][WT][RT_ROWS];
+    const AttnArgs &a = g.a;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ql = lane & 15, qg = lane >> 4;
+    const int inner = pl.groups * pl.ng;
+    const int L = blockIdx.x, panel = L / (8 * inner) * 8 + (L & 7);  // a panel's workgroups on one XCD
+    const int in = (L >> 3) % inner;
+    if (panel >= panels) return;
+    const int tg = in % pl.groups, range = in / pl.groups;
+    const int s = panel / a.n_head, h = panel - s * a.n_head, hd = a.hd;
+    const StreamRows R = stream_rows(g, s);
+    const int row0 = tg * WT * RT_ROWS;
+    if (row0 >= R.count) return;
+    const int keys = group_keys(g, R, pl, tg), k0 = range * pl.span;
+    if (k0 >= keys) return;  // the ranges behind read no result of this one
+    const int k1 = k0 + pl.span < keys ? k0 + pl.span : keys, last = a.exp_len - 1;
+    int32_t *s_exp = (int32_t *)s_mem;
+    if constexpr (PHASE == 2) load_table(a, s_exp, w, 4, lane);
+    const size_t base = ((size_t)R.slot * a.n_head + h) * a.ctx_cap * hd;
+    const Panel K(a.kc + base, a.ctx_cap, hd);
+    const v4i zero = v4i{0, 0, 0, 0};
+    v4i qf[WT][QC];
+#pragma unroll
+    for (int u = 0; u < WT; u++)
+#pragma unroll
+        for (int c = 0; c < QC; c++) {
+            const int o = 64 * c + 16 * qg, row = row0 + RT_ROWS * u + ql;
+            qf[u][c] = row < R.count && o < hd ? *(const v4i *)(a.q + (size_t)(R.first + row) * a.ldq + h * hd + o) : zero;
+        }
+    const int tiles = (R.count - row0 + RT_ROWS - 1) / RT_ROWS;  // of this group with rows (uniform)
+    const LongScratch S = long_scratch(scratch, pl, panels);
+    const int rows = pl.tiles * RT_ROWS, ranges = (keys + pl.span - 1) / pl.span;
+    auto slot = [&](int u) { return ((size_t)panel * rows + row0 + RT_ROWS * u + ql) * pl.ng; };  // of a row's ranges
+
+    int32_t dmax[WT], dmin[WT];
+    uint64_t sum[WT];
+#pragma unroll
+    for (int u = 0; u < WT; u++) dmax[u] = INT32_MIN, dmin[u] = INT32_MAX, sum[u] = 0;
+    if constexpr (PHASE == 2) {
+#pragma unroll
+        for (int u = 0; u < WT; u++)
+            if (row0 + RT_ROWS * u + ql < R.count)
+                for (int c = 0; c < ranges; c++) {
+                    const int32_t x = S.mm[2 * (slot(u) + c)], y = S.mm[2 * (slot(u) + c) + 1];
+                    dmax[u] = x > dmax[u] ? x : dmax[u];
+                    dmin[u] = y < dmin[u] ? y : dmin[u];
+                }
+    }
+    int64_t index[WT];
+    if constexpr (PHASE == 2) {
+#pragma unroll
+        for (int u = 0; u < WT; u++) index[u] = RowIndex<HI>(a, dmax[u], dmin[u]).c;
+        __syncthreads();  // the table
+    }
+    typedef v4i KRows[4][QC];
+    int kb = k0 / 64 + w;
+    auto k_load = [&](int b, KRows &x) {
+#pragma unroll
+        for (int c = 0; c < QC; c++) load_k<QC>(K, 64 * b, c, hd, 64 * b >= k1, lane, x);
+    };
+    RowSight sight[WT];
+#pragma unroll
+    for (int u = 0; u < WT; u++) sight[u] = row_sight(g, R, row0 + RT_ROWS * u + ql, qg, keys);
+    auto step = [&](KRows &now, KRows &next) {
+        k_load(kb + 4, next);
+#pragma unroll
+        for (int u = 0; u < WT; u++) {
+            if (u >= tiles) break;
+            const int t0 = row0 + RT_ROWS * u;  // the tile's first row
+            int most = keys;
+            if (!g.mask) most = R.base + t0 + RT_ROWS < keys ? R.base + t0 + RT_ROWS : keys;
+            if (64 * kb >= most) continue;
+            v4i D[4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                D[t] = zero;
+#pragma unroll
+                for (int c = 0; c < QC; c++) D[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(now[t][c], qf[u][c], D[t], 0, 0, 0);
+            }
+            const int whole = g.mask ? R.base : R.base + t0 + 1;
+            const bool all = 64 * kb + 64 <= (whole < most ? whole : most);
+            const uint32_t ok = all ? 0u : sight_bits(sight[u], kb, lane, most);
+            if constexpr (PHASE == 1) {
+                block_extremes(D, all, ok, dmax[u], dmin[u]);
+            } else {
+                RowIndex<HI> ix(index[u]);
+                block_entries<HI>(a, D, ix, s_exp, last, all, ok);
+                sum[u] += block_sum(D);
+            }
+        }
+        kb += 4;
+        return 64 * kb < k1;
+    };
+    if (64 * kb < k1) {
+        KRows x, y;
+        k_load(kb, x);
+        while (step(x, y) && step(y, x)) {}
+    }
+#pragma unroll
+    for (int u = 0; u < WT; u++) {
+        if constexpr (PHASE == 1) {
+#pragma unroll
+            for (int o = 16; o < 64; o <<= 1) {
+                const int32_t x = __shfl_xor(dmax[u], o, 64), y = __shfl_xor(dmin[u], o, 64);
+                dmax[u] = x > dmax[u] ? x : dmax[u];
+                dmin[u] = y < dmin[u] ? y : dmin[u];
+            }
+            if (qg == 0) {
+                s_mm[0][w][u][ql] = dmax[u];
+                s_mm[1][w][u][ql] = dmin[u];
+            }
+        } else {
+#pragma unroll
+            for (int o = 16; o < 64; o <<= 1) sum[u] += __shfl_xor(sum[u], o, 64);
+            if (qg == 0) s_sum[w][u][ql] = sum[u];
+        }
+    }
+    __syncthreads();
+    if (tid < WT * RT_ROWS && row0 + tid < R.count) {  // a thread per row
+        const int u = tid >> 4, r = tid & 15;
+        const size_t o = ((size_t)panel * rows + row0 + tid) * pl.ng + range;
+        if constexpr (PHASE == 1) {
+            int32_t x = s_mm[0][0][u][r], y = s_mm[1][0][u][r];
+#pragma unroll
+            for (int i = 1; i < 4; i++) {
+                x = s_mm[0][i][u][r] > x ? s_mm[0][i][u][r] : x;
+                y = s_mm[1][i][u][r] < y ? s_mm[1][i][u][r] : y;
+            }
+            S.mm[2 * o] = x;
+            S.mm[2 * o + 1] = y;
+        } else {
+            S.ps[o] = s_sum[0][u][r] + s_sum[1][u][r] + s_sum[2][u][r] + s_sum[3][u][r];
+        }
+    }
+}
+
+template <int QC, int WT, bool HI, bool ALONE>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QC == 1 ? 3 : 2))) void k_long_pv(RowsArgs g, LongPlan pl, int panels, void *scratch) {
     constexpr int WK = 4 / WT, GC = QC > 2 ? 1 : QC;
-    constexpr bool SUMS = PHASE == 0 || PHASE == 2, PV = PHASE == 0 || PHASE == 3;
     extern __shared__ __attribute__((aligned(1024))) int8_t s_mem[];
     __shared__ uint64_t s_sum[4][RT_ROWS];
     __shared__ int32_t s_mm[2][4][RT_ROWS];
     const AttnArgs &a = g.a;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ql = lane & 15, qg = lane >> 4, wt = w % WT, ks = w / WT;
-    const int cgs = PV ? pl.cg : 1, inner = pl.groups * pl.ng * cgs;
+    const int cgs = pl.cg, inner = pl.groups * pl.ng * cgs;
     const int L = blockIdx.x, panel = L / (8 * inner) * 8 + (L & 7);  // a panel's workgroups on one XCD
     int in = (L >> 3) % inner;
     if (panel >= panels) return;
@@ -595,20 +755,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     const StreamRows R = stream_rows(g, s);
     if (tg * WT * RT_ROWS >= R.count) return;
     const int gkeys = group_keys(g, R, pl, tg), k0 = range * pl.span;
-    if (PHASE != 0 && k0 >= gkeys) return;  // the ranges behind read no result of this one
+    if (!ALONE && k0 >= gkeys) return;  // the last launch reads no result of this one
     const int tile = tg * WT + wt, row = tile * RT_ROWS + ql, rows = pl.tiles * RT_ROWS;
     int keys = gkeys;
     if (!g.mask) keys = R.base + (tile + 1) * RT_ROWS < keys ? R.base + (tile + 1) * RT_ROWS : keys;
     if (tile * RT_ROWS >= R.count) keys = 0;  // a tile without rows walks nothing
-    const int k1 = k0 + pl.span < keys ? k0 + pl.span : keys, kmost = k1 - 1;
-    const int last = a.exp_len - 1;
-    int32_t *s_exp = (int32_t *)s_mem;
-    int8_t *s_v = s_mem + 4096 * w;  // (its dynamic LDS: V, then the table, which the sums of the outputs take over)
-    if constexpr (SUMS || PV) s_exp = (int32_t *)(s_mem + 16384);
-    if constexpr (SUMS || PV) load_table(a, s_exp, w, 4, lane);
+    const int k1 = k0 + pl.span < keys ? k0 + pl.span : keys, last = a.exp_len - 1;
+    int8_t *s_v = s_mem + 4096 * w;
+    int32_t *s_exp = (int32_t *)(s_mem + 16384);  // the table, which the sums of the outputs take over
+    load_table(a, s_exp, w, 4, lane);
 
     const size_t at = (size_t)R.slot * a.n_head + h, base = at * a.ctx_cap * hd;
-    const int8_t *K = a.kc + base, *V = a.vc + base;
+    const Panel K(a.kc + base, a.ctx_cap, hd), V(a.vc + base, a.ctx_cap, hd);
     const v4i zero = v4i{0, 0, 0, 0};
     v4i qf[QC];
 #pragma unroll
@@ -616,53 +774,23 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         const int o = 64 * c + 16 * qg;
         qf[c] = row < R.count && o < hd ? *(const v4i *)(a.q + (size_t)(R.first + row) * a.ldq + h * hd + o) : zero;
     }
-    const RowSight sight = row_sight(g, R, row, keys);
+    const RowSight sight = row_sight(g, R, row, qg, keys);
     const int whole0 = g.mask ? R.base : R.base + tile * RT_ROWS + 1, whole = whole0 < keys ? whole0 : keys;
-    struct Loads {
-        v4i k[4][QC], v[PV ? GC : 1][4];
-    };
-    auto load = [&](int kb, Loads &x, bool v_too) {
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const int k = 64 * kb + 16 * t + ql;
-            const int8_t *kr = K + (size_t)(k < k1 ? k : kmost) * hd + 16 * qg;
-#pragma unroll
-            for (int c = 0; c < QC; c++) x.k[t][c] = 64 * c + 16 * qg < hd ? *(const v4i *)(kr + 64 * c) : zero;
-        }
-        if (!PV || !v_too) return;
-#pragma unroll
-        for (int c = 0; c < (PV ? GC : 1); c++)
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const int r = 16 * u + (lane >> 2), k = 64 * kb + r, o = 64 * (GC * cg + c) + 16 * ((lane & 3) ^ vsw<4>(r & 15));
-                x.v[c][u] = o < hd ? *(const v4i *)(V + (size_t)(k < k1 ? k : kmost) * hd + o) : zero;
-            }
-    };
-    // fn(block, its dots, its loads, whether every row sees all of it, what the row sees), the next loads in flight
-    auto walk = [&](bool v_too, auto fn) {
+    // fn(the block, its dots, whether every row sees all of it, what the row sees)
+    auto walk = [&](auto fn) {
         int kb = k0 / 64 + ks;
-        if (64 * kb >= k1) return;
-        const bool ahead = QC == 1 || !v_too;  // (K and V of two blocks beside the sums: registers for 64 channels only)
-        Loads x;
-        load(kb, x, v_too);
-        while (true) {
-            const int next = kb + WK;
-            const bool more = 64 * next < k1;
-            Loads y;
-            if (more && ahead) load(next, y, v_too);
-            v4i D[4];
+        for (; 64 * kb < k1; kb += WK) {
+            v4i x[4][QC], D[4];
+#pragma unroll
+            for (int c = 0; c < QC; c++) load_k<QC>(K, 64 * kb, c, hd, false, lane, x);
 #pragma unroll
             for (int t = 0; t < 4; t++) {
                 D[t] = zero;
 #pragma unroll
-                for (int c = 0; c < QC; c++) D[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.k[t][c], qf[c], D[t], 0, 0, 0);
+                for (int c = 0; c < QC; c++) D[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[t][c], qf[c], D[t], 0, 0, 0);
             }
             const bool all = 64 * kb + 64 <= whole;
-            fn(kb, D, x, all, all ? 0u : sight_bits(sight, kb, qg, keys));
-            if (!more) break;
-            if (ahead) x = y;
-            else load(next, x, v_too);
-            kb = next;
+            fn(kb, D, all, all ? 0u : sight_bits(sight, kb, lane, keys));
         }
     };
     const LongScratch S = long_scratch(scratch, pl, panels);
@@ -670,8 +798,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     const int ranges = (gkeys + pl.span - 1) / pl.span;
 
     int32_t dmax = INT32_MIN, dmin = INT32_MAX;
-    if constexpr (PHASE <= 1) {
-        walk(false, [&](int, v4i (&D)[4], const Loads &, bool all, uint32_t ok) { block_extremes(D, all, ok, dmax, dmin); });
+    if constexpr (ALONE) {
+        walk([&](int, v4i (&D)[4], bool all, uint32_t ok) { block_extremes(D, all, ok, dmax, dmin); });
 #pragma unroll
         for (int o = 16; o < 64; o <<= 1) {
             const int32_t x = __shfl_xor(dmax, o, 64), y = __shfl_xor(dmin, o, 64);
@@ -691,13 +819,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
                 dmin = y < dmin ? y : dmin;
             }
         }
-        if constexpr (PHASE == 1) {
-            if (ks == 0 && qg == 0 && row < R.count) {
-                S.mm[2 * (slot + range)] = dmax;
-                S.mm[2 * (slot + range) + 1] = dmin;
-            }
-            return;
-        }
     } else if (row < R.count) {
         for (int c = 0; c < ranges; c++) {
             const int32_t x = S.mm[2 * (slot + c)], y = S.mm[2 * (slot + c) + 1];
@@ -708,8 +829,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     const RowIndex<HI> ix(a, dmax, dmin);
     __syncthreads();  // the table
     uint64_t sum = 0;
-    if constexpr (SUMS) {
-        walk(false, [&](int, v4i (&D)[4], const Loads &, bool all, uint32_t ok) {
+    if constexpr (ALONE) {
+        walk([&](int, v4i (&D)[4], bool all, uint32_t ok) {
             block_entries<HI>(a, D, ix, s_exp, last, all, ok);
             sum += block_sum(D);
         });
@@ -722,82 +843,79 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
 #pragma unroll
             for (int i = 0; i < WK; i++) sum += s_sum[wt + WT * i][ql];
         }
-        if constexpr (PHASE == 2) {
-            if (ks == 0 && qg == 0 && row < R.count) S.ps[slot + range] = sum;
-            return;
-        }
     } else if (row < R.count) {
         for (int c = 0; c < ranges; c++) sum += S.ps[slot + c];
     }
-    if constexpr (PV) {
-        const RowWeight weight(sum, a.softmax_p, row < R.count);
-        v4i acc[GC][4][4];
+    const RowWeight weight(sum, a.softmax_p, row < R.count);
+    v4i acc[GC][4][4];
 #pragma unroll
-        for (int c = 0; c < GC; c++)
+    for (int c = 0; c < GC; c++)
 #pragma unroll
-            for (int k = 0; k < 4; k++)
+        for (int k = 0; k < 4; k++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) acc[c][k][i] = zero;
-        uint64_t *mass = g.mass && cg == 0 ? g.mass + at * a.ctx_cap : nullptr;
-        walk(true, [&](int kb, v4i (&D)[4], const Loads &x, bool all, uint32_t ok) {
-            block_entries<HI>(a, D, ix, s_exp, last, all, ok);
-            block_digits(D, weight.R, weight.sp, mass ? mass + 64 * kb : nullptr, k1 - 64 * kb, lane);
+            for (int i = 0; i < 4; i++) acc[c][k][i] = zero;
+    uint64_t *mass = g.mass && cg == 0 ? g.mass + at * a.ctx_cap : nullptr;
+    walk([&](int kb, v4i (&D)[4], bool all, uint32_t ok) {
+        v4i vr[GC][4];  // arrives under the weights' arithmetic
 #pragma unroll
-            for (int c = 0; c < GC; c++) {
+        for (int c = 0; c < GC; c++) load_v(V, 64 * kb, GC * cg + c, hd, false, lane, vr[c]);
+        block_entries<HI>(a, D, ix, s_exp, last, all, ok);
+        block_digits(D, weight.R, weight.sp, mass ? mass + 64 * kb : nullptr, k1 - 64 * kb, lane);
 #pragma unroll
-                for (int u = 0; u < 4; u++) *(v4i *)(s_v + 1024 * u + 16 * lane) = x.v[c][u];
-                block_pv(s_v, D, lane, acc[c]);
-            }
-        });
-        // A row's sums of one range, or the outputs themselves
-        const double mo = a.out_s > 95 ? 0.0 : ldexp((double)a.out_m, -a.out_s);
-        auto put = [&](int r, int ch, const int64_t (&x)[4]) {  // channels ch .. ch + 3 of row r
-            if (PHASE == 0) {
-                uint32_t packed = 0;
+        for (int c = 0; c < GC; c++) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) packed |= (uint32_t)(uint8_t)(int8_t)attn_out_byte(x[e], mo, a.out_m, a.out_s) << (8 * e);
-                *(uint32_t *)attn_out(a, R.first + r, h * hd + ch) = packed;
-            } else {
-                int64_t *o = S.part + (((size_t)panel * pl.ng + range) * rows + r) * hd + ch;
+            for (int u = 0; u < 4; u++) *(v4i *)(s_v + 1024 * u + 16 * lane) = vr[c][u];
+            block_pv<4>(s_v, D, 0, lane, acc[c]);
+        }
+    });
+    // A row's sums of one range, or the outputs themselves
+    const double mo = a.out_s > 95 ? 0.0 : ldexp((double)a.out_m, -a.out_s);
+    auto put = [&](int r, int ch, const int64_t (&x)[4]) {  // channels ch .. ch + 3 of row r
+        if (ALONE) {
+            uint32_t packed = 0;
 #pragma unroll
-                for (int e = 0; e < 4; e++) o[e] = x[e];
-            }
-        };
-        if constexpr (WK == 1) {
-            if (row < R.count) {
-#pragma unroll
-                for (int c = 0; c < GC; c++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int ch = 64 * (GC * cg + c) + 16 * i + 4 * qg;
-                        int64_t x[4];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) x[e] = plane_sum(acc[c], i, e);
-                        if (ch < hd) put(row, ch, x);
-                    }
-            }
+            for (int e = 0; e < 4; e++) packed |= (uint32_t)(uint8_t)(int8_t)attn_out_byte(x[e], mo, a.out_m, a.out_s) << (8 * e);
+            *(uint32_t *)attn_out(a, R.first + r, h * hd + ch) = packed;
         } else {
-            int64_t *s_acc = (int64_t *)s_exp;  // [WT][GC][16][RT_ACC], over the table
-            __syncthreads();
-            for (int i = tid; i < WT * GC * RT_ROWS * RT_ACC; i += 256) s_acc[i] = 0;
-            __syncthreads();
+            int64_t *o = S.part + (((size_t)panel * pl.ng + range) * rows + r) * hd + ch;
 #pragma unroll
-            for (int c = 0; c < GC; c++) {
-                unsigned long long *to = (unsigned long long *)s_acc + ((wt * GC + c) * RT_ROWS + ql) * RT_ACC + 4 * qg;
+            for (int e = 0; e < 4; e++) o[e] = x[e];
+        }
+    };
+    if constexpr (WK == 1) {
+        if (row < R.count) {
 #pragma unroll
-                for (int i = 0; i < 4; i++)
+            for (int c = 0; c < GC; c++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) atomicAdd(to + 16 * i + e, (unsigned long long)plane_sum(acc[c], i, e));
-            }
-            __syncthreads();
-            for (int i = tid; i < WT * GC * RT_ROWS * 16; i += 256) {
-                const int q4 = i & 15, r = (i >> 4) & 15, c = (i >> 8) % GC, u = (i >> 8) / GC;
-                const int ch = 64 * (GC * cg + c) + 4 * q4, out_row = (tg * WT + u) * RT_ROWS + r;
-                if (ch >= hd || out_row >= R.count) continue;
-                const int64_t *from = s_acc + ((u * GC + c) * RT_ROWS + r) * RT_ACC + 4 * q4;
-                const int64_t x[4] = {from[0], from[1], from[2], from[3]};
-                put(out_row, ch, x);
-            }
+                for (int i = 0; i < 4; i++) {
+                    const int ch = 64 * (GC * cg + c) + 16 * i + 4 * qg;
+                    int64_t x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[e] = plane_sum(acc[c], i, e);
+                    if (ch < hd) put(row, ch, x);
+                }
+        }
+    } else {
+        int64_t *s_acc = (int64_t *)s_exp;  // [WT][GC][16][RT_ACC], over the table
+        __syncthreads();
+        for (int i = tid; i < WT * GC * RT_ROWS * RT_ACC; i += 256) s_acc[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < GC; c++) {
+            unsigned long long *to = (unsigned long long *)s_acc + ((wt * GC + c) * RT_ROWS + ql) * RT_ACC + 4 * qg;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) atomicAdd(to + 16 * i + e, (unsigned long long)plane_sum(acc[c], i, e));
+        }
+        __syncthreads();
+        for (int i = tid; i < WT * GC * RT_ROWS * 16; i += 256) {
+            const int q4 = i & 15, r = (i >> 4) & 15, c = (i >> 8) % GC, u = (i >> 8) / GC;
+            const int ch = 64 * (GC * cg + c) + 4 * q4, out_row = (tg * WT + u) * RT_ROWS + r;
+            if (ch >= hd || out_row >= R.count) continue;
+            const int64_t *from = s_acc + ((u * GC + c) * RT_ROWS + r) * RT_ACC + 4 * q4;
+            const int64_t x[4] = {from[0], from[1], from[2], from[3]};
+            put(out_row, ch, x);
         }
     }
 }
@@ -834,10 +952,10 @@ static LongPlan long_plan(const RowsArgs &g, int keys) {
     p.wt = p.tiles >= 3 ? 4 : p.tiles;
     p.groups = (p.tiles + p.wt - 1) / p.wt;
     p.cg = g.a.hd > 128 ? (g.a.hd + 63) / 64 : 1;
-    // about LONG_WGS workgroups, at least four blocks a wave
+    // about LONG_WGS workgroups, at least two blocks a wave
     constexpr long long LONG_WGS = 1536;
     const long long wgs = (long long)g.streams * g.a.n_head * p.groups;
-    const int unit = 64 * (4 / p.wt), most = (keys + 4 * unit - 1) / (4 * unit);
+    const int unit = 256, most = (keys + 2 * unit - 1) / (2 * unit);
     long long ng = (LONG_WGS + wgs - 1) / wgs;
     ng = ng < 1 ? 1 : (ng > most ? most : ng);
     p.span = (int)(((keys + ng - 1) / ng + unit - 1) / unit) * unit;
@@ -859,10 +977,10 @@ static hipError_t launch_long_t(const RowsArgs &g, const LongPlan &p, void *scra
     };
     const size_t lds = 16384 + (table > acc ? table : acc);
     hipError_t e;
-    if (p.ng == 1) return run(k_rows_long<QC, WT, HI, 0>, grid * p.cg, lds);
-    if ((e = run(k_rows_long<QC, WT, HI, 1>, grid, 0)) != hipSuccess) return e;
-    if ((e = run(k_rows_long<QC, WT, HI, 2>, grid, 16384 + table)) != hipSuccess) return e;
-    if ((e = run(k_rows_long<QC, WT, HI, 3>, grid * p.cg, lds)) != hipSuccess) return e;
+    if (p.ng == 1) return run(k_long_pv<QC, WT, HI, true>, grid * p.cg, lds);
+    if ((e = run(k_long_scan<QC, WT, HI, 1>, grid, 0)) != hipSuccess) return e;
+    if ((e = run(k_long_scan<QC, WT, HI, 2>, grid, table)) != hipSuccess) return e;
+    if ((e = run(k_long_pv<QC, WT, HI, false>, grid * p.cg, lds)) != hipSuccess) return e;
     const size_t quads = (size_t)panels * p.tiles * RT_ROWS * (g.a.hd / 4);
     launch_k(k_rows_out, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, g, p, panels, scratch);
     return hipGetLastError();
