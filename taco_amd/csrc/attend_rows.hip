@@ -359,6 +359,7 @@ __host__ __device__ inline int tile_top(int qc, int table_chunks) {
 
 template <int QC, int NB, int NW, bool HI>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QC == 1 && NW == 4 ? 3 : 2))) void k_rows_tile(RowsArgs g, int tiles, int panels) {
+    static_assert(NB <= 4, "the plane sums of a wave's keys in 32 bits");
     extern __shared__ __attribute__((aligned(1024))) int8_t s_mem[];
     const AttnArgs &a = g.a;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -522,7 +523,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QC == 1
 #pragma unroll
                 for (int i = 0; i < N; i++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) atomicAdd(to + 16 * i + e, (unsigned long long)plane_sum(acc, i, e));
+                    for (int e = 0; e < 4; e++) {
+                        // (at most 256 keys a wave: a plane's sum is below 2^22, two planes' below 2^31)
+                        const int32_t lo = acc[0][i][e] + acc[1][i][e] * 256, hi = acc[2][i][e] + acc[3][i][e] * 256;
+                        atomicAdd(to + 16 * i + e, (unsigned long long)((int64_t)hi * 65536 + lo));
+                    }
             }
         }
     }
