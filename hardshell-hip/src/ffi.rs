@@ -67,6 +67,8 @@ pub type hs_mixer_fn = Option<unsafe extern "C" fn(user: *mut c_void, input: usi
 pub const HS_MIX_NONE: u32 = 0xFFFF_FFFF;
 /// The table of GPT-2 alone.
 pub const HS_MIX_PLAIN: u32 = 0xFFFF_FFFE;
+/// The parent of a tree's node right after the context.
+pub const HS_TREE_ROOT: u32 = 0xFFFF_FFFF;
 
 /// The values of `hs_status`.
 #[repr(i32)]
@@ -150,6 +152,30 @@ unsafe extern "C" {
     pub fn hs_batch_stream_len(batch: *const hs_batch, slot: usize) -> usize;
     pub fn hs_batch_room(batch: *const hs_batch, slot: usize) -> usize;
     pub fn hs_batch_truncate(batch: *mut hs_batch, slot: usize, len: usize) -> c_int;
+    /// No counterpart in the reference: trees of drafted tokens.
+    pub fn hs_batch_run_tree_weights(
+        batch: *mut hs_batch,
+        inputs: *const hs_input,
+        parents: *const u32,
+        n: usize,
+        out: *mut u64,
+    ) -> c_int;
+    pub fn hs_batch_run_tree_coded(
+        batch: *mut hs_batch,
+        inputs: *const hs_input,
+        parents: *const u32,
+        queries: *const hs_query,
+        n: usize,
+        freq_bits: u32,
+        out: *mut hs_interval,
+    ) -> c_int;
+    pub fn hs_batch_commit_paths(
+        batch: *mut hs_batch,
+        slots: *const u32,
+        lengths: *const u32,
+        paths: *const u32,
+        n: usize,
+    ) -> c_int;
     pub fn hs_batch_run_coded_mixed(
         batch: *mut hs_batch,
         inputs: *const hs_input,

@@ -22,7 +22,7 @@ use std::ffi::CStr;
 use hardshell::gpt2::Overlap;
 use hardshell::{ModelHash, TokenId};
 
-pub use ffi::{HS_MIX_NONE, HS_MIX_PLAIN};
+pub use ffi::{HS_MIX_NONE, HS_MIX_PLAIN, HS_TREE_ROOT};
 
 /// A result with the error of this crate.
 pub type Result<T> = std::result::Result<T, Error>;
@@ -371,6 +371,13 @@ fn inputs_of(inputs: &[(usize, TokenId)], slots: usize) -> Result<Vec<ffi::hs_in
         .collect()
 }
 
+fn parents_of(parents: &[Option<u32>], n: usize) -> Result<Vec<u32>> {
+    if parents.len() != n {
+        return Err(Error::LengthMismatch { expected: n, found: parents.len() });
+    }
+    Ok(parents.iter().map(|p| p.unwrap_or(HS_TREE_ROOT)).collect())
+}
+
 fn queries_of(queries: &[CoderQuery]) -> Result<Vec<ffi::hs_query>> {
     queries
         .iter()
@@ -545,6 +552,81 @@ impl<'m> HipBatch<'m> {
             ffi::hs_batch_run_coded(self.raw, ins.as_ptr(), qs.as_ptr(), ins.len(), freq_bits, out.as_mut_ptr())
         })?;
         Ok(self.intervals(&out))
+    }
+
+    /// The weights of every node of the slots' trees of drafted tokens: `parents[i]` is the index of
+    /// an earlier input of the same slot, or `None` for a token right after the context. No position
+    /// changes. No counterpart in the reference, which drafts chains.
+    ///
+    /// # Errors
+    /// [`Error::LengthMismatch`] if the parents do not match the inputs; [`Error::Unsupported`] for a
+    /// parent that is not an earlier input of its slot, or a tree that does not fit the pass or the rest of
+    /// the context; as [`HipBatch::run_weights`] otherwise.
+    pub fn run_tree_weights(&mut self, inputs: &[(usize, TokenId)], parents: &[Option<u32>]) -> Result<Vec<u64>> {
+        let (ins, ps) = (inputs_of(inputs, self.slots)?, parents_of(parents, inputs.len())?);
+        let mut out = vec![0u64; ins.len() * self.model.vocab_size()];
+        // SAFETY: the arrays hold n entries, `out` n * vocab values.
+        check("hs_batch_run_tree_weights", unsafe {
+            ffi::hs_batch_run_tree_weights(self.raw, ins.as_ptr(), ps.as_ptr(), ins.len(), out.as_mut_ptr())
+        })?;
+        Ok(out)
+    }
+
+    /// The coder interval of every node's query, as [`HipBatch::run_tree_weights`].
+    ///
+    /// # Errors
+    /// As [`HipBatch::run_tree_weights`] and [`HipBatch::run_coded`].
+    pub fn run_tree_coded(
+        &mut self,
+        inputs: &[(usize, TokenId)],
+        parents: &[Option<u32>],
+        queries: &[CoderQuery],
+        freq_bits: u32,
+    ) -> Result<Vec<CoderInterval>> {
+        if queries.len() != inputs.len() {
+            return Err(Error::LengthMismatch { expected: inputs.len(), found: queries.len() });
+        }
+        let (ins, ps) = (inputs_of(inputs, self.slots)?, parents_of(parents, inputs.len())?);
+        let qs = queries_of(queries)?;
+        let mut out = vec![ffi::hs_interval::default(); ins.len()];
+        // SAFETY: every array holds n entries.
+        check("hs_batch_run_tree_coded", unsafe {
+            ffi::hs_batch_run_tree_coded(
+                self.raw,
+                ins.as_ptr(),
+                ps.as_ptr(),
+                qs.as_ptr(),
+                ins.len(),
+                freq_bits,
+                out.as_mut_ptr(),
+            )
+        })?;
+        Ok(self.intervals(&out))
+    }
+
+    /// Accepts a path of the last tree of each listed slot: its node numbers, from a child of the root
+    /// down, become the slot's next inputs. An empty path accepts none.
+    ///
+    /// # Errors
+    /// [`Error::BadSlot`] for a slot that is not valid or occurs twice; [`Error::Unsupported`] for a slot
+    /// without a tree or a path that is not one of its tree. No position changes then.
+    pub fn commit_paths(&mut self, paths: &[(usize, &[u32])]) -> Result<()> {
+        if let Some(&(slot, _)) = paths.iter().find(|p| p.0 >= self.slots) {
+            return Err(Error::BadSlot { slot, slots: self.slots });
+        }
+        let slots: Vec<u32> = paths.iter().map(|p| p.0 as u32).collect();
+        let lengths: Vec<u32> = paths.iter().map(|p| p.1.len() as u32).collect();
+        let nodes: Vec<u32> = paths.iter().flat_map(|p| p.1.iter().copied()).collect();
+        // SAFETY: `slots` and `lengths` hold n entries, `nodes` the sum of the lengths.
+        check("hs_batch_commit_paths", unsafe {
+            ffi::hs_batch_commit_paths(self.raw, slots.as_ptr(), lengths.as_ptr(), nodes.as_ptr(), slots.len())
+        })?;
+        for &(slot, path) in paths {
+            if !path.is_empty() {
+                self.stepped[slot] = false;
+            }
+        }
+        Ok(())
     }
 
     /// The coder interval of each input in its table (`CudaBatch::run_coded_mixed`): GPT-2

@@ -180,6 +180,29 @@ size_t hs_batch_stream_len(const hs_batch *batch, size_t slot);
 size_t hs_batch_room(const hs_batch *batch, size_t slot);
 hs_status hs_batch_truncate(hs_batch *batch, size_t slot, size_t len);
 
+/* ---- Trees of drafts. No counterpart in the reference, which drafts chains (a call of several inputs and
+ * hs_batch_truncate). -----------------------------------------------------------------------
+ * The inputs of a slot are the nodes of a tree of tokens that may follow its context, numbered in the
+ * order in which they come: parents[i] is the index (in this call) of an earlier input of the same slot, or
+ * HS_TREE_ROOT for a token right after the context. Input i gets the weights (or the interval of
+ * queries[i]) after the context and the tokens on the path from the root to it, the results that
+ * hs_batch_run_weights and hs_batch_run_coded give for that sequence. No position changes. At most
+ * hs_batch_max_rows inputs a call and 256 a slot; a slot's tree has to fit the rest of its context (position +
+ * nodes <= n_ctx: no restart inside a tree), else HS_UNSUPPORTED. */
+#define HS_TREE_ROOT 0xFFFFFFFFu
+hs_status hs_batch_run_tree_weights(hs_batch *batch, const hs_input *inputs,
+                                    const uint32_t *parents, size_t n, uint64_t *out);
+hs_status hs_batch_run_tree_coded(hs_batch *batch, const hs_input *inputs, const uint32_t *parents,
+                                  const hs_query *queries, size_t n, uint32_t freq_bits,
+                                  hs_interval *out);
+/* Accepts a path of the last tree of each listed slot (every slot at most once): lengths[i] node numbers in
+ * `paths` (the slots' one after another), from a child of the root down, become the next inputs of the
+ * slot's context, as if they had been run. Length 0 accepts none; the tree is dropped either way, as it is by
+ * any other call that runs inputs on the slot, resets or truncates it. A slot without a tree or a
+ * path that is not one of its tree: HS_UNSUPPORTED, and no position changes. */
+hs_status hs_batch_commit_paths(hs_batch *batch, const uint32_t *slots, const uint32_t *lengths,
+                                const uint32_t *paths, size_t n);
+
 /* ---- The mixed coder op of the logs profile: crates/hardshell-cuda/src/batch/mixed.rs:23-126,
  * src/mixed.rs:24-233 (ADR 0010 section 3) ---------------------------------------------------
  * The GPU gives the statistics of each row's GPT-2 weights w; the host mixer gives q; the GPU

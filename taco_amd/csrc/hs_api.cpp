@@ -605,6 +605,18 @@ struct hs_batch {
     std::vector<StreamState> streams;
     std::vector<std::vector<uint32_t>> prev;  // [slot]: the full context before its last restart
     std::vector<uint64_t> host_w;  // [slots, vocab]: weights of the last step
+    // The tree that a slot last ran (hs_batch_run_tree_*): each node's token and parent (-1: the context's end). Its
+    // rows lie in the caches behind the context until the slot runs something else, which drops the tree.
+    struct Tree {
+        std::vector<uint32_t> tokens;
+        std::vector<int32_t> parents;
+    };
+    std::unordered_map<size_t, Tree> trees;
+    // made at the first tree call: cache positions of the pass's rows (they differ from the token positions), the
+    // rows' masks, and the context lengths, accepted counts and paths of a commit
+    RowInfo *h_kv_rows = nullptr, *d_kv_rows = nullptr;
+    uint64_t *h_mask = nullptr, *d_mask = nullptr;
+    uint32_t *h_paths = nullptr, *d_paths = nullptr;
     hipStream_t st = nullptr;
     DevMem mem;
     RowInfo *d_rows = nullptr;
@@ -654,7 +666,8 @@ struct hs_batch {
         for (auto e : event_pool) (void)hipEventDestroy(e);
         if (st) (void)hipStreamSynchronize(st);
         for (void *p : {(void *)h_rows, (void *)h_groups, (void *)h_src, (void *)h_queries, (void *)h_intervals,
-                        (void *)h_mix, (void *)h_stats, (void *)h_intervals2})
+                        (void *)h_mix, (void *)h_stats, (void *)h_intervals2, (void *)h_kv_rows, (void *)h_mask,
+                        (void *)h_paths})
             if (p) (void)hipHostFree(p);
         if (split) (void)hipFree(split);
         if (st) (void)hipStreamDestroy(st);
@@ -827,6 +840,7 @@ extern "C" void hs_batch_reset(hs_batch *b, size_t slot) {
     if (b && slot < b->slots) {
         b->pos[slot] = 0;
         b->streams[slot] = StreamState{};
+        b->trees.erase(slot);
     }
 }
 
@@ -969,8 +983,15 @@ hs_status mix_chunk(hs_batch &b, const Mixing &mx, const std::vector<int64_t> &o
     return HS_OK;
 }
 
+// The pass of a tree call: its rows lie slot by slot, each slot's in the order of its nodes (PassRow::pos is
+// the token position, context + depth).
+struct TreePass {
+    std::vector<hs::AttnGroup> groups;  // a slot each: its rows, and pos0 the context length
+    int most = 0, words = 0;            // the most nodes of a slot, the mask words of a row
+};
+
 hs_status run_pass(hs_batch &b, const std::vector<PassRow> &rows, Out out, const uint32_t *queries,
-                   uint32_t bits, uint64_t *sink, const Mixing *mx = nullptr) {
+                   uint32_t bits, uint64_t *sink, const Mixing *mx = nullptr, const TreePass *tree = nullptr) {
     const hs_model &m = *b.model;
     hipStream_t st = b.st;
     const int n = (int)rows.size();
@@ -1012,7 +1033,16 @@ hs_status run_pass(hs_batch &b, const std::vector<PassRow> &rows, Out out, const
         group_keys = std::max<int>(group_keys, std::min<int>((int)rows[r].pos + c, (int)m.C));
         r += c;
     }
-    const bool mfma_attn = m.hd == 64 && n >= 16 * n_groups;
+    const RowInfo *kv_rows = b.d_rows;  // with the cache positions
+    if (tree) {  // (the caller has staged the cache positions and the masks)
+        n_groups = (int)tree->groups.size();
+        std::copy(tree->groups.begin(), tree->groups.end(), b.h_groups);
+        kv_rows = b.d_kv_rows;
+        HIP_TRY(hipMemcpyAsync(b.d_groups, b.h_groups, n_groups * sizeof(hs::AttnGroup), hipMemcpyHostToDevice, st));
+        HIP_TRY(hipMemcpyAsync(b.d_kv_rows, b.h_kv_rows, n * sizeof(RowInfo), hipMemcpyHostToDevice, st));
+        HIP_TRY(hipMemcpyAsync(b.d_mask, b.h_mask, (size_t)n * tree->words * sizeof(uint64_t), hipMemcpyHostToDevice, st));
+    }
+    const bool mfma_attn = !tree && m.hd == 64 && n >= 16 * n_groups;
     // the largest key counts first: the persistent prefill kernel pairs long and short groups
     // in its rounds (every group writes only its own rows, so the order changes no output)
     if (mfma_attn)
@@ -1073,9 +1103,26 @@ hs_status run_pass(hs_batch &b, const std::vector<PassRow> &rows, Out out, const
     // Decode-shaped passes (short runs) and head dims that the group kernels do not take: attention in
     // one launch, or split over key chunks, as many rows at a time as 1 GiB of scratch holds; where
     // the device has no memory for that, the row kernel, which needs none.
-    bool split_attn = !mfma_attn && hs::attend_split_ok(m.hd);
+    bool split_attn = !tree && !mfma_attn && hs::attend_split_ok(m.hd);
     hs::SplitPlan split_plan;
     int split_rows = n;
+    hs::RowsArgs tree_args;  // the attention of a tree pass; a layer's caches and rules below
+    if (tree) {
+        hs::AttnArgs &a = tree_args.a;
+        a.q = b.d_qkv; a.ldq = 3 * m.d; a.kc = b.kc[0]; a.vc = b.vc[0];
+        a.n_head = m.H; a.hd = m.hd; a.ctx_cap = m.C; a.exp_table = m.attn_exp; a.exp_len = (int)m.host.attn_exp.size();
+        tree_args.streams = n_groups; tree_args.t = tree->most; tree_args.groups = b.d_groups;
+        tree_args.mask = b.d_mask; tree_args.words = tree->words;
+        const size_t need = hs::rows_workspace(tree_args);
+        if (need > b.split_bytes) {
+            HIP_TRY(hipStreamSynchronize(st));
+            if (b.split) HIP_TRY(hipFree(b.split));
+            b.split = nullptr;
+            b.split_bytes = 0;
+            HIP_TRY(hipMalloc(&b.split, need));
+            b.split_bytes = need;
+        }
+    }
     if (split_attn) {
         int max_keys = 1;
         int64_t keys = 0;
@@ -1117,14 +1164,14 @@ hs_status run_pass(hs_batch &b, const std::vector<PassRow> &rows, Out out, const
             g.bias = blk.c_attn.b; g.mult = blk.c_attn.m; g.shift = blk.c_attn.s; g.out = b.d_qkv;
             g.params_padded = 1;
             g.ldo = 3 * m.d; g.fast32 = blk.c_attn.fast32;
-            g.kv_rows = b.d_rows; g.kc = b.kc[l]; g.vc = b.vc[l];
+            g.kv_rows = kv_rows; g.kc = b.kc[l]; g.vc = b.vc[l];
             g.kv_d = m.d; g.kv_hd = m.hd; g.kv_h = m.H; g.kv_ctx = m.C;
             const uint64_t ops = 2ull * (uint64_t)n * (uint64_t)blk.c_attn.n * (uint64_t)blk.c_attn.k;
             HIP_TRY(b.launch("gemm_qkv", ops, [&] { return hs::launch_gemm(Epi::Act, g, st); }));
         } else {
             HIP_TRY(gemm("gemm_qkv", Epi::Act, blk.c_attn, b.d_a, RP, n, b.d_qkv, 3 * m.d));
             HIP_TRY(b.launch("kv_store", 0, [&] {
-                return hs::launch_kv_store(b.d_rows, n, b.d_qkv, m.d, m.H, m.hd, m.C, b.kc[l], b.vc[l], st);
+                return hs::launch_kv_store(kv_rows, n, b.d_qkv, m.d, m.H, m.hd, m.C, b.kc[l], b.vc[l], st);
             }));
         }
         hs::AttnArgs at;
@@ -1135,6 +1182,11 @@ hs_status run_pass(hs_batch &b, const std::vector<PassRow> &rows, Out out, const
         at.softmax_p = m.host.softmax_p;
         at.out = b.d_att; at.out_rows = RP;
         HIP_TRY(b.launch("attention", 4ull * attn_keys * (uint64_t)m.d, [&] {
+            if (tree) {
+                at.rows = nullptr;
+                tree_args.a = at;
+                return hs::launch_rows(tree_args, b.split, st);
+            }
             if (mfma_attn) return hs::launch_attend_groups(at, b.d_groups, n_groups, group_keys, st);
             if (!split_attn) return hs::launch_attend(at, n, st);
             for (int r0 = 0; r0 < n; r0 += split_rows) {
@@ -1293,6 +1345,8 @@ hs_status check_inputs(const hs_batch *b, const hs_input *in, size_t n) {
 hs_status run(hs_batch *b, const hs_input *in, size_t n, Out out, const uint32_t *queries,
               uint32_t bits, uint64_t *sink, const Mixing *mx = nullptr) {
     HIP_TRY(hipSetDevice(b->model->dev->ordinal));
+    if (!b->trees.empty())
+        for (size_t i = 0; i < n; i++) b->trees.erase(in[i].slot);  // their rows are written over
     static thread_local Plan plan;  // host scratch kept from call to call (one call per thread at a time)
     make_plan(*b, in, n, plan);
     for (size_t i = 0; i < plan.n_passes; i++) {
@@ -1300,6 +1354,98 @@ hs_status run(hs_batch *b, const hs_input *in, size_t n, Out out, const uint32_t
         if (s != HS_OK) return s;  // no position changes after an error
     }
     commit(*b, plan);
+    return HS_OK;
+}
+
+}  // namespace
+
+namespace {
+
+constexpr size_t HS_MAX_NODES = 256;  // drafted nodes of a stream (four mask words a row)
+
+// The checks of a tree call, its rows slot by slot, and each slot's tree.
+hs_status plan_tree(hs_batch *b, const hs_input *in, const uint32_t *parents, size_t n, std::vector<PassRow> &rows,
+                    TreePass &pass, std::unordered_map<size_t, hs_batch::Tree> &trees) {
+    if (n && !parents) return hs::fail(HS_INVALID_ARGUMENT, 0, "parents is NULL");
+    if (n > b->max_rows)
+        return hs::fail(HS_UNSUPPORTED, 0, "a tree call takes at most " + std::to_string(b->max_rows) + " inputs, a pass of the batch");
+    const size_t C = b->model->host.n_ctx;
+    std::vector<std::vector<size_t>> of;  // the inputs of each slot of the call
+    std::unordered_map<size_t, size_t> index;
+    std::vector<uint32_t> node(n), depth(n);
+    for (size_t i = 0; i < n; i++) {
+        const size_t slot = in[i].slot;
+        const auto at = index.emplace(slot, of.size());
+        if (at.second) of.emplace_back();
+        std::vector<size_t> &mine = of[at.first->second];
+        int32_t parent = -1;
+        if (parents[i] != HS_TREE_ROOT) {
+            if (parents[i] >= i || in[parents[i]].slot != slot)
+                return hs::fail(HS_UNSUPPORTED, 0, "the parent of input " + std::to_string(i) + " is not an earlier input of its slot");
+            parent = (int32_t)node[parents[i]];
+        }
+        node[i] = (uint32_t)mine.size();
+        depth[i] = parent < 0 ? 0 : depth[parents[i]] + 1;
+        mine.push_back(i);
+        if (mine.size() > HS_MAX_NODES) return hs::fail(HS_UNSUPPORTED, 0, "a tree holds at most 256 nodes");
+        if (b->pos[slot] + mine.size() > C)
+            return hs::fail(HS_UNSUPPORTED, 0, "the tree of slot " + std::to_string(slot) + " does not fit the rest of its context");
+        hs_batch::Tree &t = trees[slot];
+        t.tokens.push_back(in[i].token);
+        t.parents.push_back(parent);
+    }
+    for (const auto &mine : of) {
+        const size_t slot = in[mine[0]].slot;
+        pass.groups.push_back(hs::AttnGroup{(int32_t)rows.size(), (int32_t)mine.size(), (int32_t)slot, (int32_t)b->pos[slot]});
+        pass.most = std::max(pass.most, (int)mine.size());
+        for (size_t i : mine) rows.push_back(PassRow{(uint32_t)slot, in[i].token, (uint32_t)(b->pos[slot] + depth[i]), (int64_t)i});
+    }
+    pass.words = (pass.most + 63) / 64;
+    return HS_OK;
+}
+
+hs_status tree_buffers(hs_batch *b) {
+    if (b->h_paths) return HS_OK;
+    const size_t R = b->max_rows;
+    if (!b->d_kv_rows) HS_TRY(b->mem.alloc(b->d_kv_rows, R));
+    if (!b->d_mask) HS_TRY(b->mem.alloc(b->d_mask, R * (HS_MAX_NODES / 64)));
+    if (!b->d_paths) HS_TRY(b->mem.alloc(b->d_paths, b->slots * (2 + HS_MAX_NODES)));
+    if (!b->h_kv_rows) HIP_TRY(hipHostMalloc((void **)&b->h_kv_rows, R * sizeof(RowInfo), hipHostMallocDefault));
+    if (!b->h_mask) HIP_TRY(hipHostMalloc((void **)&b->h_mask, R * (HS_MAX_NODES / 64) * sizeof(uint64_t), hipHostMallocDefault));
+    HIP_TRY(hipHostMalloc((void **)&b->h_paths, b->slots * (2 + HS_MAX_NODES) * sizeof(uint32_t), hipHostMallocDefault));
+    return HS_OK;
+}
+
+hs_status run_tree(hs_batch *b, const hs_input *in, const uint32_t *parents, size_t n, Out out, const uint32_t *queries,
+                   uint32_t bits, uint64_t *sink) {
+    std::vector<PassRow> rows;
+    TreePass pass;
+    std::unordered_map<size_t, hs_batch::Tree> trees;
+    HS_TRY(plan_tree(b, in, parents, n, rows, pass, trees));
+    if (n == 0) return HS_OK;
+    HIP_TRY(hipSetDevice(b->model->dev->ordinal));
+    HS_TRY(tree_buffers(b));
+    if (b->inflight) {  // the staging below may still feed an earlier pass
+        HIP_TRY(hipStreamSynchronize(b->st));
+        b->inflight = false;
+    }
+    for (const hs::AttnGroup &g : pass.groups) {
+        const hs_batch::Tree &t = trees[(size_t)g.slot];
+        for (int j = 0; j < g.count; j++) {
+            const size_t r = (size_t)(g.first + j);
+            b->h_kv_rows[r] = RowInfo{g.slot, (int32_t)t.tokens[j], g.pos0 + j, -1};
+            uint64_t *m = b->h_mask + r * pass.words;
+            if (t.parents[j] < 0) std::fill(m, m + pass.words, 0);
+            else std::copy_n(b->h_mask + (size_t)(g.first + t.parents[j]) * pass.words, pass.words, m);
+            m[j >> 6] |= (uint64_t)1 << (j & 63);
+        }
+        // what a later truncation across a restart has to write again
+        StreamState &st = b->streams[(size_t)g.slot];
+        st.written = std::max<size_t>(st.written, (size_t)(g.pos0 + g.count));
+        b->trees.erase((size_t)g.slot);
+    }
+    HS_TRY(run_pass(*b, rows, out, queries, bits, sink, nullptr, &pass));
+    for (auto &t : trees) b->trees[t.first] = std::move(t.second);
     return HS_OK;
 }
 
@@ -1398,6 +1544,92 @@ extern "C" hs_status hs_batch_run_coded_dual(hs_batch *b, const hs_input *in, co
     return run(b, in, n, Out::Intervals, query_words(queries.data()), freq_bits, (uint64_t *)mixed, &mx);
 }
 
+// ---- Trees of drafts: no counterpart in the reference, which drafts chains --------------------------
+
+extern "C" hs_status hs_batch_run_tree_weights(hs_batch *b, const hs_input *in, const uint32_t *parents, size_t n,
+                                               uint64_t *out) {
+    hs::clear_error();
+    HS_TRY(check_inputs(b, in, n));
+    if (n && !out) return hs::fail(HS_INVALID_ARGUMENT, 0, "out is NULL");
+    return run_tree(b, in, parents, n, Out::Weights, nullptr, 0, out);
+}
+
+extern "C" hs_status hs_batch_run_tree_coded(hs_batch *b, const hs_input *in, const uint32_t *parents,
+                                             const hs_query *queries, size_t n, uint32_t freq_bits, hs_interval *out) {
+    hs::clear_error();
+    HS_TRY(check_inputs(b, in, n));
+    if (n && (!queries || !out)) return hs::fail(HS_INVALID_ARGUMENT, 0, "NULL argument");
+    HS_TRY(check_queries(queries, n, b->model->host.vocab, freq_bits));
+    return run_tree(b, in, parents, n, Out::Intervals, query_words(queries), freq_bits, (uint64_t *)out);
+}
+
+extern "C" hs_status hs_batch_commit_paths(hs_batch *b, const uint32_t *slots, const uint32_t *lengths,
+                                           const uint32_t *paths, size_t n) {
+    hs::clear_error();
+    if (!b || (n && (!slots || !lengths))) return hs::fail(HS_INVALID_ARGUMENT, 0, "NULL argument");
+    size_t at = 0;
+    std::vector<char> seen(b->slots, 0);
+    uint32_t most = 0;
+    bool moves = false;
+    for (size_t i = 0; i < n; at += lengths[i], i++) {
+        const size_t slot = slots[i];
+        if (slot >= b->slots || seen[slot])
+            return hs::fail(HS_BAD_SLOT, (int)slot, "slot " + std::to_string(slot) +
+                            (slot < b->slots ? " occurs two times in one call" : " is not valid in a batch of " + std::to_string(b->slots) + " slots"));
+        seen[slot] = 1;
+        if (lengths[i] == 0) continue;
+        if (!paths) return hs::fail(HS_INVALID_ARGUMENT, 0, "paths is NULL");
+        const auto t = b->trees.find(slot);
+        if (t == b->trees.end()) return hs::fail(HS_UNSUPPORTED, 0, "slot " + std::to_string(slot) + " has no tree");
+        int32_t parent = -1;
+        for (uint32_t j = 0; j < lengths[i]; j++) {
+            const uint32_t node = paths[at + j];
+            if (node >= t->second.tokens.size() || t->second.parents[node] != parent)
+                return hs::fail(HS_UNSUPPORTED, 0, "the path of slot " + std::to_string(slot) + " does not lead from its root down");
+            parent = (int32_t)node;
+            moves = moves || node != j;
+        }
+        most = std::max(most, lengths[i]);
+    }
+    if (moves) {
+        const hs_model &m = *b->model;
+        HIP_TRY(hipSetDevice(m.dev->ordinal));
+        HIP_TRY(hipStreamSynchronize(b->st));  // (a commit before may still feed from the staging)
+        uint32_t *ctx = b->h_paths, *accepted = ctx + b->slots, *path = accepted + b->slots;
+        for (size_t s = 0; s < b->slots; s++) ctx[s] = (uint32_t)b->pos[s], accepted[s] = 0;
+        at = 0;
+        for (size_t i = 0; i < n; at += lengths[i], i++) {
+            accepted[slots[i]] = lengths[i];
+            std::copy_n(paths + at, lengths[i], path + (size_t)slots[i] * most);
+        }
+        const size_t words = b->slots * (2 + (size_t)most);
+        HIP_TRY(hipMemcpyAsync(b->d_paths, b->h_paths, words * sizeof(uint32_t), hipMemcpyHostToDevice, b->st));
+        hs::CommitArgs a{b->d_paths, b->d_paths + 2 * b->slots, b->d_paths + b->slots, (int)b->slots, (int)most, m.H, m.hd, m.C, 0, nullptr};
+        for (int l0 = 0; l0 < m.L; l0 += hs::CACHE_LAYERS) {
+            const int k = std::min(hs::CACHE_LAYERS, m.L - l0);
+            hs::CachePtrs c{};
+            for (int l = 0; l < k; l++) {
+                c.k[l] = b->kc[l0 + l];
+                c.v[l] = b->vc[l0 + l];
+            }
+            HIP_TRY(b->launch("commit", 0, [&] { return hs::launch_commit(c, k, a, b->st); }));
+        }
+    }
+    at = 0;
+    const size_t C = b->model->host.n_ctx;
+    for (size_t i = 0; i < n; at += lengths[i], i++) {
+        const size_t slot = slots[i];
+        const auto t = b->trees.find(slot);
+        for (uint32_t j = 0; j < lengths[i]; j++) {
+            b->hist[slot * C + b->pos[slot]] = t->second.tokens[paths[at + j]];
+            b->streams[slot].input(b->pos[slot]);
+            b->pos[slot]++;
+        }
+        if (t != b->trees.end()) b->trees.erase(t);
+    }
+    return HS_OK;
+}
+
 extern "C" hs_status hs_batch_step(hs_batch *b, const hs_input *in, size_t n) {
     hs::clear_error();
     hs_status s = check_inputs(b, in, n);
@@ -1463,6 +1695,7 @@ extern "C" hs_status hs_batch_truncate(hs_batch *b, size_t slot, size_t len) {
     }
     commit_truncate(b->streams[slot], t, C);
     b->pos[slot] = t.pos;
+    b->trees.erase(slot);
     return HS_OK;
 }
 
@@ -1703,8 +1936,6 @@ bool aligned(size_t n, std::initializer_list<const void *> ps) {
         if ((uintptr_t)p % n) return false;
     return true;
 }
-
-constexpr size_t HS_MAX_NODES = 256;  // drafted nodes of a stream (four mask words a row)
 
 // The arguments that the entries of several rows share; on HS_OK `g` is filled but for the counts, the mask
 // and the accumulators.

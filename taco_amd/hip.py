@@ -73,6 +73,7 @@ class _Input(C.Structure):
 # The mixed coder op of the logs profile (crates/hardshell-cuda/src/mixed.rs).
 HS_MIX_NONE = 0xFFFFFFFF   # a mixed table without a prediction
 HS_MIX_PLAIN = 0xFFFFFFFE  # the table of GPT-2 alone
+HS_TREE_ROOT = 0xFFFFFFFF  # the parent of a tree's node right after the context
 
 
 class MixStats(C.Structure):
@@ -195,6 +196,9 @@ def lib() -> C.CDLL:
         L.hs_op_coder.argtypes = [P, P, S, S, P, S, P, U32, P]
         L.hs_batch_run_coded_mixed.argtypes = [P, P, P, P, S, U32, MIXER_FN, P, P]
         L.hs_batch_run_coded_dual.argtypes = [P, P, P, P, S, U32, MIXER_FN, P, P, P]
+        L.hs_batch_run_tree_weights.argtypes = [P, P, P, S, P]
+        L.hs_batch_run_tree_coded.argtypes = [P, P, P, P, S, U32, P]
+        L.hs_batch_commit_paths.argtypes = [P, P, P, P, S]
         L.hs_op_mixed_coder.argtypes = [P, P, S, S, P, P, U32, MIXER_FN, P, P, P]
         L.hs_op_mixed_coder_logits.argtypes = [P, P, S, S, P, S, P, P, U32, MIXER_FN, P, P, P]
         _lib = L
@@ -397,6 +401,40 @@ class HipBatch:
         _check(lib().hs_batch_run_coded_dual(self.h, _ptr(a), _ptr(tk), _ptr(pr), len(a), freq_bits,
                                              cb, None, _ptr(plain), _ptr(mixed)))
         return plain, mixed
+
+    def _parents(self, parents, n: int) -> np.ndarray:
+        p = np.asarray(parents, dtype=np.int64)
+        if len(p) != n:
+            raise LengthMismatch(HS_LENGTH_MISMATCH, 0, f"length mismatch: expected {n}, found {len(p)}")
+        return np.where(p < 0, HS_TREE_ROOT, p).astype(np.uint32)
+
+    def run_tree_weights(self, inputs, parents) -> np.ndarray:
+        """The weights of every node of the slots' trees of drafts (hs_batch_run_tree_weights):
+        parents[i] is the index of an earlier input of the same slot, or -1. No position changes."""
+        a = _inputs(inputs)
+        p = self._parents(parents, len(a))
+        out = np.zeros((len(a), self.vocab), np.uint64)
+        _check(lib().hs_batch_run_tree_weights(self.h, _ptr(a), _ptr(p), len(a), _ptr(out)))
+        return out
+
+    def run_tree_coded_raw(self, inputs, parents, queries, freq_bits: int = 32) -> np.ndarray:
+        """The intervals of every node's query as an [n, 3] u64 array (hs_batch_run_tree_coded)."""
+        a = _inputs(inputs)
+        p = self._parents(parents, len(a))
+        q = np.ascontiguousarray(np.asarray(queries, dtype=np.uint32).reshape(-1, 2))
+        if len(q) != len(a):
+            raise LengthMismatch(HS_LENGTH_MISMATCH, 0, f"length mismatch: expected {len(a)}, found {len(q)}")
+        out = np.zeros((len(a), 3), np.uint64)
+        _check(lib().hs_batch_run_tree_coded(self.h, _ptr(a), _ptr(p), _ptr(q), len(a), freq_bits, _ptr(out)))
+        return out
+
+    def commit_paths(self, paths) -> None:
+        """Accepts a path of the last tree of each slot: {slot: node numbers in the slot's tree, from a child
+        of the root down} (hs_batch_commit_paths)."""
+        slots = np.array(list(paths), np.uint32)
+        lengths = np.array([len(p) for p in paths.values()], np.uint32)
+        flat = np.array([int(x) for p in paths.values() for x in p], np.uint32)
+        _check(lib().hs_batch_commit_paths(self.h, _ptr(slots), _ptr(lengths), _ptr(flat), len(slots)))
 
     def step(self, inputs):
         a = _inputs(inputs)
