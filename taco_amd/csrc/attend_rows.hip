@@ -743,6 +743,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
 template <int QC, int WT, bool HI, bool ALONE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QC == 1 ? 3 : 2))) void k_long_pv(RowsArgs g, LongPlan pl, int panels, void *scratch) {
     constexpr int WK = 4 / WT, GC = QC > 2 ? 1 : QC;
+    constexpr bool AHEAD = QC == 1;  // (above 64 channels the sums or K itself leave no registers for the next block)
     extern __shared__ __attribute__((aligned(1024))) int8_t s_mem[];
     __shared__ uint64_t s_sum[4][RT_ROWS];
     __shared__ int32_t s_mm[2][4][RT_ROWS];
@@ -784,15 +785,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QC == 1 ? 3
     // fn(the block, its dots, whether every row sees all of it, what the row sees)
     auto walk = [&](auto fn) {
         int kb = k0 / 64 + ks;
-        for (; 64 * kb < k1; kb += WK) {
-            v4i x[4][QC], D[4];
+        v4i x[4][QC];
+        auto k_load = [&](int b) {
 #pragma unroll
-            for (int c = 0; c < QC; c++) load_k<QC>(K, 64 * kb, c, hd, false, lane, x);
+            for (int c = 0; c < QC; c++) load_k<QC>(K, 64 * b, c, hd, 64 * b >= k1, lane, x);
+        };
+        if (AHEAD) k_load(kb);
+        for (; 64 * kb < k1; kb += WK) {
+            v4i D[4];
+            if (!AHEAD) k_load(kb);
 #pragma unroll
             for (int t = 0; t < 4; t++) {
                 D[t] = zero;
 #pragma unroll
                 for (int c = 0; c < QC; c++) D[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[t][c], qf[c], D[t], 0, 0, 0);
+            }
+            if (AHEAD) {  // the next block's K into the registers of this one's
+                __builtin_amdgcn_sched_barrier(0);
+                k_load(kb + WK);
             }
             const bool all = 64 * kb + 64 <= whole;
             fn(kb, D, all, all ? 0u : sight_bits(sight, kb, lane, keys));
@@ -860,16 +870,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QC == 1 ? 3
 #pragma unroll
             for (int i = 0; i < 4; i++) acc[c][k][i] = zero;
     uint64_t *mass = g.mass && cg == 0 ? g.mass + at * a.ctx_cap : nullptr;
-    walk([&](int kb, v4i (&D)[4], bool all, uint32_t ok) {
-        v4i vr[GC][4];  // arrives under the weights' arithmetic
+    v4i vr[GC][4];  // arrives under the weights' arithmetic; one block ahead where K does
+    auto v_load = [&](int b) {
 #pragma unroll
-        for (int c = 0; c < GC; c++) load_v(V, 64 * kb, GC * cg + c, hd, false, lane, vr[c]);
+        for (int c = 0; c < GC; c++) load_v(V, 64 * b, GC * cg + c, hd, 64 * b >= k1, lane, vr[c]);
+    };
+    if (AHEAD) v_load(k0 / 64 + ks);
+    walk([&](int kb, v4i (&D)[4], bool all, uint32_t ok) {
+        if (!AHEAD) v_load(kb);
         block_entries<HI>(a, D, ix, s_exp, last, all, ok);
         block_digits(D, weight.R, weight.sp, mass ? mass + 64 * kb : nullptr, k1 - 64 * kb, lane);
 #pragma unroll
         for (int c = 0; c < GC; c++) {
 #pragma unroll
             for (int u = 0; u < 4; u++) *(v4i *)(s_v + 1024 * u + 16 * lane) = vr[c][u];
+            if (AHEAD) v_load(kb + WK);
             block_pv<4>(s_v, D, 0, lane, acc[c]);
         }
     });
@@ -957,11 +972,13 @@ static LongPlan long_plan(const RowsArgs &g, int keys) {
     p.wt = p.tiles >= 3 ? 4 : p.tiles;
     p.groups = (p.tiles + p.wt - 1) / p.wt;
     p.cg = g.a.hd > 128 ? (g.a.hd + 63) / 64 : 1;
-    // about LONG_WGS workgroups, at least two blocks a wave
-    constexpr long long LONG_WGS = 1536;
+    // Ranges for about four workgroups a CU, at least two blocks a wave: three are resident, and where the caches are
+    // about three quarters full (their ends' workgroups end at once) the rest is one round. 200 panels of 64 rows over up
+    // to 8,192 keys: 4 ranges 154 us a call, 5 (this rule) 130, 6 141, 8 147, 16 218.
+    constexpr long long LONG_WGS = 1024;
     const long long wgs = (long long)g.streams * g.a.n_head * p.groups;
     const int unit = 256, most = (keys + 2 * unit - 1) / (2 * unit);
-    long long ng = (LONG_WGS + wgs - 1) / wgs;
+    long long ng = LONG_WGS / wgs;
     ng = ng < 1 ? 1 : (ng > most ? most : ng);
     p.span = (int)(((keys + ng - 1) / ng + unit - 1) / unit) * unit;
     p.ng = (keys + p.span - 1) / p.span;

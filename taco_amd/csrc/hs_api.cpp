@@ -93,6 +93,10 @@ struct hs_device {
     std::string name;
     hipStream_t stream = nullptr;
     void *fixed_scratch = nullptr;  // this device's copy of `scratch` (below), a device address
+    // The workspaces of the row attention's calls without one: a pool that keeps its memory between calls (the default
+    // pool gives it back at every synchronization, which made the next call 100 us longer).
+    std::mutex pool_mu;
+    hipMemPool_t pool = nullptr;
 };
 
 // The scratch of hs_op_attend_decode_dev_noalloc: one array per GPU, loaded with the code
@@ -300,6 +304,7 @@ extern "C" hs_status hs_device_open(int ordinal, hs_device **out) {
 extern "C" void hs_device_close(hs_device *dev) {
     if (!dev) return;
     if (dev->stream) (void)hipStreamDestroy(dev->stream);
+    if (dev->pool) (void)hipMemPoolDestroy(dev->pool);
     delete dev;
 }
 
@@ -1971,8 +1976,20 @@ hs_status run_rows(hs_device *dev, const hs::RowsArgs &g, void *workspace, size_
         HIP_TRY(hs::launch_rows(g, workspace, st));
         return HS_OK;
     }
+    {
+        std::lock_guard<std::mutex> lock(dev->pool_mu);
+        if (!dev->pool) {
+            hipMemPoolProps props{};
+            props.allocType = hipMemAllocationTypePinned;
+            props.location.type = hipMemLocationTypeDevice;
+            props.location.id = dev->ordinal;
+            HIP_TRY(hipMemPoolCreate(&dev->pool, &props));
+            uint64_t keep = UINT64_MAX;
+            HIP_TRY(hipMemPoolSetAttribute(dev->pool, hipMemPoolAttrReleaseThreshold, &keep));
+        }
+    }
     void *scratch = nullptr;
-    HIP_TRY(hipMallocAsync(&scratch, need, st));
+    HIP_TRY(hipMallocFromPoolAsync(&scratch, need, dev->pool, st));
     const hipError_t e = hs::launch_rows(g, scratch, st);
     const hipError_t f = hipFreeAsync(scratch, st);
     HIP_TRY(e);
