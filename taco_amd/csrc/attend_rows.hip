@@ -292,13 +292,12 @@ struct RowWeight {
 };
 
 // acc[k][i] += V^T digits over a block whose V rows lie in s_v (16-byte chunk c of row r at slot 4 r + (c ^ vsw(r))):
-// channel 16 (i0 + i) + 4 (l / 16) + e of row l % 16, i < N.
-template <int N>
-__device__ __forceinline__ void block_pv(const int8_t *s_v, const v4i (&pf)[4], int i0, int lane, v4i (&acc)[4][N]) {
+// channel 16 i + 4 (l / 16) + e of row l % 16.
+__device__ __forceinline__ void block_pv(const int8_t *s_v, const v4i (&pf)[4], int lane, v4i (&acc)[4][4]) {
     const int ql = lane & 15, qg = lane >> 4, tr_k = ql >> 1, key0 = 16 * (tr_k >> 2) + 4 * qg + (tr_k & 3);
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        const int8_t *p0 = s_v + (4 * key0 + ((i0 + i) ^ vsw<4>(key0 & 15))) * 16 + 8 * (ql & 1);
+    for (int i = 0; i < 4; i++) {
+        const int8_t *p0 = s_v + (4 * key0 + (i ^ vsw<4>(key0 & 15))) * 16 + 8 * (ql & 1);
         const v2i r0 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)p0);
         const v2i r1 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)(p0 + 32 * 64));
         const v4i vf = v4i{r0[0], r0[1], r1[0], r1[1]};
@@ -307,8 +306,7 @@ __device__ __forceinline__ void block_pv(const int8_t *s_v, const v4i (&pf)[4], 
     }
 }
 
-template <int N>
-__device__ __forceinline__ int64_t plane_sum(const v4i (&acc)[4][N], int i, int e) {
+__device__ __forceinline__ int64_t plane_sum(const v4i (&acc)[4][4], int i, int e) {
     return (int64_t)acc[0][i][e] + (int64_t)acc[1][i][e] * 256 + (int64_t)acc[2][i][e] * 65536 +
            (int64_t)acc[3][i][e] * 16777216;
 }
@@ -358,7 +356,7 @@ __host__ __device__ inline int tile_top(int qc, int table_chunks) {
 }
 
 template <int QC, int NB, int NW, bool HI>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QC == 1 && NW == 4 ? 3 : 2))) void k_rows_tile(RowsArgs g, int tiles, int panels) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void k_rows_tile(RowsArgs g, int tiles, int panels) {
     static_assert(NB <= 4, "the plane sums of a wave's keys in 32 bits");
     extern __shared__ __attribute__((aligned(1024))) int8_t s_mem[];
     const AttnArgs &a = g.a;
@@ -492,43 +490,33 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QC == 1
             block_digits(D[j], wt.R, wt.sp, g.mass ? g.mass + at * a.ctx_cap + 64 * block(j) : nullptr, keys - 64 * block(j), lane);
     }
     __builtin_amdgcn_sched_barrier(0);
-    // The products with V, 16 N channels at a time (a lane writes its V words of those columns only). At four blocks a
-    // wave and three workgroups a CU 64 sums beside the digits and V would not fit the registers, nor would 32, and what
-    // spills are V's loads in flight: N = 1 there.
-    constexpr int N = QC == 1 && NB == 4 && NW == 4 ? 1 : 4;
-    const int column = (lane & 3) ^ vsw<4>(lane >> 2);  // of the lane's V words
 #pragma unroll
     for (int c = 0; c < QC; c++) {
+        v4i acc[4][4];
 #pragma unroll
-        for (int i0 = 0; i0 < 4; i0 += N) {
-            v4i acc[4][N];
+        for (int k = 0; k < 4; k++)
 #pragma unroll
-            for (int k = 0; k < 4; k++)
+            for (int i = 0; i < 4; i++) acc[k][i] = zero;
 #pragma unroll
-                for (int i = 0; i < N; i++) acc[k][i] = zero;
+        for (int j = 0; j < NB; j++) {
+            if (!mine(j)) continue;
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < NB; j++) {
-                if (!mine(j)) continue;
-                __builtin_amdgcn_sched_barrier(0);
-                if (N == 4 || column / N == i0 / N) {
+            for (int u = 0; u < 4; u++) *(v4i *)(s_v + 1024 * u + 16 * lane) = vr[j][u];
+            if (c + 1 < QC) v_load(j, c + 1);
+            block_pv(s_v, D[j], lane, acc);
+        }
+        if (c == 0) lds_barrier();  // the zeros
+        if (mine(0)) {
+            unsigned long long *to = (unsigned long long *)s_acc + (c * RT_ROWS + ql) * RT_ACC + 4 * qg;
 #pragma unroll
-                    for (int u = 0; u < 4; u++) *(v4i *)(s_v + 1024 * u + 16 * lane) = vr[j][u];
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    // (at most 256 keys a wave: a plane's sum is below 2^22, two planes' below 2^31)
+                    const int32_t lo = acc[0][i][e] + acc[1][i][e] * 256, hi = acc[2][i][e] + acc[3][i][e] * 256;
+                    atomicAdd(to + 16 * i + e, (unsigned long long)((int64_t)hi * 65536 + lo));
                 }
-                if (i0 + N == 4 && c + 1 < QC) v_load(j, c + 1);
-                block_pv<N>(s_v, D[j], i0, lane, acc);
-            }
-            if (c == 0 && i0 == 0) lds_barrier();  // the zeros
-            if (mine(0)) {
-                unsigned long long *to = (unsigned long long *)s_acc + (c * RT_ROWS + ql) * RT_ACC + 16 * i0 + 4 * qg;
-#pragma unroll
-                for (int i = 0; i < N; i++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        // (at most 256 keys a wave: a plane's sum is below 2^22, two planes' below 2^31)
-                        const int32_t lo = acc[0][i][e] + acc[1][i][e] * 256, hi = acc[2][i][e] + acc[3][i][e] * 256;
-                        atomicAdd(to + 16 * i + e, (unsigned long long)((int64_t)hi * 65536 + lo));
-                    }
-            }
         }
     }
     lds_barrier();
@@ -554,11 +542,20 @@ static hipError_t launch_tile_t(const RowsArgs &g, hipStream_t stream) {
     return hipGetLastError();
 }
 
+// Waves and blocks a wave by the keys the caches hold. Up to 1,024 keys eight waves of two blocks: against four of four,
+// one stream of 12 heads and 16 rows at 700 keys 9.3 us and 11.9, 64 streams 21.2 and 23.5, 128 streams 39.0 and 40.2.
+// Above 64 channels that holds while there is a workgroup a CU at most (12 panels at head_dim 128: 13.3 us and 14.9;
+// 768: 46.6 and 42.3: of the eight waves' form only one workgroup fits a CU).
 template <int QC, bool HI>
 static hipError_t launch_tile(const RowsArgs &g, int keys, hipStream_t stream) {
     if (keys <= 256) return launch_tile_t<QC, 1, 4, HI>(g, stream);
     if (keys <= 512) return launch_tile_t<QC, 2, 4, HI>(g, stream);
-    if (keys <= 1024) return launch_tile_t<QC, 4, 4, HI>(g, stream);
+    if (keys <= 1024) {
+        [[maybe_unused]] const long long wgs = (long long)g.streams * g.a.n_head * ((g.t + RT_ROWS - 1) / RT_ROWS);
+        if constexpr (QC > 1)
+            if (wgs > 256) return launch_tile_t<QC, 4, 4, HI>(g, stream);
+        return launch_tile_t<QC, 2, 8, HI>(g, stream);
+    }
     return launch_tile_t<QC, 4, 8, HI>(g, stream);
 }
 
@@ -885,7 +882,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QC == 1 ? 3
 #pragma unroll
             for (int u = 0; u < 4; u++) *(v4i *)(s_v + 1024 * u + 16 * lane) = vr[c][u];
             if (AHEAD) v_load(kb + WK);
-            block_pv<4>(s_v, D, 0, lane, acc[c]);
+            block_pv(s_v, D, lane, acc[c]);
         }
     });
     // A row's sums of one range, or the outputs themselves
