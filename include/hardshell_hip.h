@@ -317,8 +317,11 @@ hs_status hs_op_attend_decode_dev_noalloc(hs_device *dev, const int8_t *q, const
  * tree of one branch) and keeps every key until a context restarts. Device pointers throughout but
  * for the arrays of layer pointers; `stream` a hipStream_t or NULL (the device's own); nothing waits for
  * the GPU. Rules, tables and caches as in hs_op_attend_decode_dev; rows, caches, tables and counts
- * 4-byte aligned, masks and accumulators 8-byte. At most 2^22 keys a cache. Safe under graph capture
- * (with a workspace of the caller's where one is needed). ---------------------------------------- */
+ * 4-byte aligned, masks and accumulators 8-byte; table entries 0 or more. Attention takes caches of at most
+ * 2^22 keys, the others 2^30. Safe under graph capture (with a workspace of the caller's where one is
+ * needed). Arrays that a call writes overlap nothing else that it is given, but where it says so. Rows, caches
+ * and tables aligned to 16 bytes, head dims that are multiples of 16 and tables of at most 16,384
+ * entries take the fast forms. ------------------------------------------------------------------ */
 /* Attention of a tree of drafted tokens for each stream. q and out [b, t, h, hd] i8; row i < nodes[s]
  * (NULL: t for every stream) is node i of the tree of stream s, whose key and value the caller has
  * stored at cache position ctx[s] + i. mask [b, t, ceil(t / 64)] u64: bit n % 64 of word n / 64 of row i
@@ -369,7 +372,7 @@ hs_status hs_op_cache_evict_dev(hs_device *dev, int8_t *const *k_caches, int8_t 
  * path[s][i] moves to row ctx[s] + i for i < accepted[s] <= t, as if all were read before any is
  * written. path [b, t] u32 with path[s][i] >= i (any path from a root down is ascending, so it has that);
  * a row that lies past the cache is left out. ctx_out[b] (or NULL; not overlapping ctx) receives ctx[s] +
- * accepted[s]. */
+ * accepted[s] (at most ctx_cap). */
 hs_status hs_op_cache_commit_dev(hs_device *dev, int8_t *const *k_caches, int8_t *const *v_caches,
                                  size_t layers, const uint32_t *ctx, const uint32_t *path,
                                  const uint32_t *accepted, size_t b, size_t t, size_t h, size_t hd,

@@ -2003,9 +2003,9 @@ hs_status cache_args(hs_device *dev, int8_t *const *k_caches, int8_t *const *v_c
     if (!dev || (layers && (!k_caches || !v_caches))) return hs::fail(HS_INVALID_ARGUMENT, 0, "NULL argument");
     if (hd == 0 || hd % 4 != 0 || hd > 256 || h == 0 || ctx_cap == 0)
         return hs::fail(HS_UNSUPPORTED, 0, "head_dim must be a multiple of 4 in 4..=256; h and ctx_cap >= 1");
-    if (ctx_cap > (size_t)INT32_MAX || b > (size_t)INT32_MAX || h > (size_t)INT32_MAX / 128 ||
+    if (ctx_cap > (size_t)1 << 30 || b > (size_t)INT32_MAX || h > (size_t)INT32_MAX / 128 ||
         (b && h > (size_t)INT32_MAX / 128 / b))  // 64 layers of K and V in a launch
-        return hs::fail(HS_UNSUPPORTED, 0, "too many panels or keys");
+        return hs::fail(HS_UNSUPPORTED, 0, "too many panels or keys (at most 2^30 keys)");
     for (size_t l = 0; l < layers; l++) {
         if (!k_caches[l] || !v_caches[l]) return hs::fail(HS_INVALID_ARGUMENT, 0, "NULL cache");
         if (!aligned(4, {k_caches[l], v_caches[l]}))

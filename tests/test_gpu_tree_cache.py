@@ -187,9 +187,52 @@ def test_mass_steps(gpu, cap, hd):
     check_mass(gpu, 3, 1, 2, hd, cap, [cap, (cap + 1) // 2, 1])
 
 
-@pytest.mark.parametrize("t,cap", [(2, 2), (16, 1024), (17, 1100), (64, 64), (100, 100), (130, 700), (33, 4200), (40, 9000)])
+@pytest.mark.parametrize("t,cap", [(2, 2), (16, 1024), (17, 1100), (64, 64), (100, 100), (130, 700), (33, 4200), (40, 9000),
+                                   (1100, 2600), (1100, 1900)])
 def test_mass_chunks(gpu, t, cap):
     check_mass(gpu, 3, t, 2, 64, cap, [cap, t, (cap + t) // 2], [t, t, max(1, t // 2)])
+
+
+def test_unaligned_rows_and_caches(gpu):
+    """Arrays 4 bytes off a multiple of 16 (the caller's slices): the row form, the same values; and queries,
+    caches and outputs inside larger arrays, whose other bytes stay."""
+    r = np.random.default_rng(8)
+    b, t, h, hd, cap = 2, 6, 2, 64, 90
+    q, (kc, vc) = r.integers(-128, 128, (b, t, h, hd)).astype(np.int8), caches(r, b, h, cap, hd)
+    ctx, mask = np.array([70, 3], np.uint32), masks(gpu, r, b, t)
+    out, acc = np.zeros_like(q), np.zeros((b, h, cap), np.uint64)
+
+    def inside(x):
+        big = np.full(x.nbytes + 64, 55, np.int8)
+        big[4:4 + x.nbytes] = np.frombuffer(x.tobytes(), np.int8)
+        p = gpu(big)
+        return big, p, C.c_void_p(p.value + 4)
+
+    held = [inside(x) for x in (q, kc, vc, out)]
+    rule = gpu.rule(RULE, TABLE)
+    ptrs = [x[2] for x in held]
+    gpu.hip.attend_tree(gpu.dev, *ptrs[:3], gpu(ctx), None, gpu(mask), (b, t, h, hd, cap), rule, ptrs[3])
+    ref.tree(q, kc, vc, ctx, None, mask, RULE, TABLE, out)
+    big = gpu.back(held[3][1], held[3][0])
+    assert np.array_equal(big[4:4 + out.nbytes].reshape(out.shape), out)
+    assert (big[:4] == 55).all() and (big[4 + out.nbytes:] == 55).all()
+    d_acc = gpu(acc)
+    keys = ctx + np.uint32(t)
+    gpu.hip.attend_mass(gpu.dev, *ptrs[:3], gpu(keys), None, d_acc, (b, t, h, hd, cap), rule, ptrs[3])
+    ref.mass(q, kc, vc, keys, None, acc, RULE, TABLE, out)
+    assert np.array_equal(gpu.back(d_acc, acc), acc)
+    one = gpu(np.ones(b, np.uint32))
+    gpu.hip.attend_mass(gpu.dev, *ptrs[:3], gpu(keys), one, d_acc, (b, 1, h, hd, cap), rule, ptrs[3])
+    first = np.zeros((b, 1, h, hd), np.int8)
+    ref.mass(q.reshape(b * t, h, hd)[:b, None], kc, vc, keys, None, acc, RULE, TABLE, first)
+    assert np.array_equal(gpu.back(d_acc, acc), acc)
+
+
+def test_many_panels(gpu):
+    """More workgroups than fit at once, some streams without a row."""
+    check_tree(gpu, 300, 20, 4, 16, 90, [70, 0, 33], [20, 0, 17, 3])
+    check_mass(gpu, 300, 2, 4, 16, 90, [70, 2, 33, 0], [2, 0, 1, 2])
+    check_mass(gpu, 700, 1, 4, 16, 600, [70, 0, 333, 600], [1, 1, 0, 1])
 
 
 def test_mass_counts_beyond_the_cache(gpu):
@@ -352,3 +395,52 @@ def test_serving_loop(gpu):
         n = m
         assert np.array_equal(gpu.back(ctx, n), n) and np.array_equal(gpu.back(d_acc, acc), acc)
     assert n.max() == budget
+
+
+def test_caches_of_more_than_4_gib(gpu):
+    """The last of 257 streams of 2 heads and 131,072 places: its panels lie past 2^32 bytes."""
+    r = np.random.default_rng(21)
+    b, t, h, hd, cap, budget, recent = 257, 5, 2, 64, 131_072, 1000, 100
+    L = gpu.hip.lib()
+    kc, vc = caches(r, 1, h, cap, hd)
+    whole = []
+    for x in (kc, vc):
+        p = C.c_void_p()
+        gpu.hip._check(L.hs_device_alloc(gpu.dev.h, b * x.nbytes, C.byref(p)))
+        gpu.held.append(p)
+        last = C.c_void_p(p.value + (b - 1) * x.nbytes)
+        gpu.hip._check(L.hs_device_upload(gpu.dev.h, last, gpu.hip._ptr(x), x.nbytes))
+        whole.append((p, last))
+    (dk, last_k), (dv, last_v) = whole
+    q = r.integers(-128, 128, (b, t, h, hd)).astype(np.int8)
+    ctx, count = np.zeros(b, np.uint32), np.zeros(b, np.uint32)
+    ctx[-1], count[-1] = cap - t, t
+    mask = np.zeros((b, t, 1), np.uint64)
+    mask[-1] = masks(gpu, r, 1, t)[0]
+    out, acc = np.zeros_like(q), np.zeros((1, b, h, cap), np.uint64)
+    d_out, d_acc, rule = gpu(out), gpu(acc), gpu.rule(RULE, TABLE)
+    gpu.hip.attend_tree(gpu.dev, gpu(q), dk, dv, gpu(ctx), gpu(count), gpu(mask), (b, t, h, hd, cap), rule, d_out)
+    ref.tree(q[-1:], kc, vc, ctx[-1:], None, mask[-1:], RULE, TABLE, out[-1:])
+    assert np.array_equal(gpu.back(d_out, out), out)
+    keys = ctx + count
+    for rows, n in ((t, count), (1, np.minimum(count, 1))):  # a chunk of rows, then one row a stream
+        first = np.ascontiguousarray(q[:, :rows])
+        out = np.zeros_like(first)
+        d_out = gpu(out)
+        gpu.hip.attend_mass(gpu.dev, gpu(first), dk, dv, gpu(keys), gpu(n), d_acc, (b, rows, h, hd, cap), rule, d_out)
+        ref.mass(first[-1:], kc, vc, keys[-1:], None, acc[0, -1:], RULE, TABLE, out[-1:])
+        assert np.array_equal(gpu.back(d_out, out), out)
+        assert np.array_equal(gpu.back(d_acc, acc), acc)
+    path, accepted = np.zeros((b, t), np.uint32), np.zeros(b, np.uint32)
+    path[-1, :3], accepted[-1] = [1, 2, 4], 3
+    after = np.zeros(b, np.uint32)
+    d_after = gpu(after)
+    gpu.hip.cache_commit(gpu.dev, [dk], [dv], gpu(ctx), gpu(path), gpu(accepted), (b, t, h, hd, cap), d_after)
+    ref.commit([kc], [vc], ctx[-1:], path[-1:], accepted[-1:], after[-1:])
+    assert np.array_equal(gpu.back(d_after, after), after)
+    cut = np.zeros(b, np.uint32)
+    d_cut = gpu(cut)
+    gpu.hip.cache_evict(gpu.dev, [dk], [dv], d_acc, d_after, (b, h, hd, cap), budget, recent, d_acc, d_cut)
+    ref.evict([kc], [vc], acc[:, -1:], after[-1:], budget, recent, acc[:, -1:], cut[-1:], None)
+    assert np.array_equal(gpu.back(d_cut, cut), cut) and np.array_equal(gpu.back(d_acc, acc), acc)
+    assert np.array_equal(gpu.back(last_k, kc), kc) and np.array_equal(gpu.back(last_v, vc), vc)
