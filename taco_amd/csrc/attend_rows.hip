@@ -1027,11 +1027,16 @@ static bool rows_mfma_ok(const RowsArgs &g) {
     return panels * p.groups * p.ng * p.cg < (1ll << 31) && panels * tiles * RT_ROWS * (a.hd / 4) < (1ll << 38);
 }
 
-// One causal row a stream: the decode kernels, which add up the weights too.
+// One causal row a stream: the decode kernels, which add up the weights too, where one launch of them serves (768
+// row-heads of 1,024 keys 17.4 us, a tile each 36), and their split form for many row-heads over more keys than a tile
+// holds (768 row-heads of 8,000 keys 187 us, three walks 240; 192: 73 and 72). Else the forms for 16 rows: 12
+// row-heads of 2,000 keys 13.9 us, split 36; 768 of them 52 and 61; 12 of 8,000 keys 35 and 79.
 static bool rows_decode_ok(const RowsArgs &g) {
     const AttnArgs &a = g.a;
     const uintptr_t bits = (uintptr_t)a.q | (uintptr_t)a.kc | (uintptr_t)a.vc;
-    return g.t == 1 && !g.mask && !g.groups && attend_split_ok(a.hd) && bits % 16 == 0;
+    if (g.t != 1 || g.mask || g.groups || !attend_split_ok(a.hd) || bits % 16 != 0) return false;
+    return attend_split_one_launch(a.hd, a.ctx_cap, attend_split_plan(g.streams, a.n_head, a.ctx_cap)) || !rows_mfma_ok(g) ||
+           (a.ctx_cap > RT_KEYS && (long long)g.streams * a.n_head >= 512);
 }
 
 size_t rows_workspace(const RowsArgs &g) {

@@ -2020,10 +2020,15 @@ extern "C" size_t hs_op_attend_rows_workspace(size_t b, size_t t, size_t h, size
     hs::RowsArgs g;
     if (b * t * h == 0 || hd == 0 || b * t > (size_t)INT32_MAX / h || ctx_cap > (size_t)1 << 22) return 0;
     g.streams = (int)b; g.t = (int)t; g.a.n_head = (int)h; g.a.hd = (int)hd; g.a.ctx_cap = (int)ctx_cap;
-    const size_t causal = hs::rows_workspace(g);
+    // of a tree and of causal rows, with a table that the fast forms take and with a longer one
     const uint64_t some = 0;
-    g.mask = &some;  // as a tree
-    return std::max(causal, hs::rows_workspace(g));
+    size_t most = 0;
+    for (int i = 0; i < 4; i++) {
+        g.mask = i & 1 ? &some : nullptr;
+        g.a.exp_len = i & 2 ? INT32_MAX : 1;
+        most = std::max(most, hs::rows_workspace(g));
+    }
+    return most;
 }
 
 extern "C" hs_status hs_op_attend_tree_dev(hs_device *dev, const int8_t *q, const int8_t *k_cache, const int8_t *v_cache,

@@ -193,6 +193,21 @@ def test_mass_chunks(gpu, t, cap):
     check_mass(gpu, 3, t, 2, 64, cap, [cap, t, (cap + t) // 2], [t, t, max(1, t // 2)])
 
 
+def test_long_table_over_a_long_cache(gpu):
+    """A table longer than the fast forms take, and the workspace that attend_rows_workspace names for it."""
+    table = np.resize(TABLE, 20_000)
+    for t in (1, 3):
+        check_mass(gpu, 2, t, 2, 64, 2500, [2500, 700], table=table)
+    r = np.random.default_rng(3)
+    q, (kc, vc) = r.integers(-128, 128, (2, 1, 2, 64)).astype(np.int8), caches(r, 2, 2, 2500, 64)
+    ctx, acc, out = np.array([2400, 9], np.uint32), np.zeros((2, 2, 2500), np.uint64), np.zeros_like(q)
+    d_out, need = gpu(out), gpu.hip.attend_rows_workspace(2, 1, 2, 64, 2500)
+    gpu.hip.attend_mass(gpu.dev, gpu(q), gpu(kc), gpu(vc), gpu(ctx), None, gpu(acc), (2, 1, 2, 64, 2500),
+                        gpu.rule(RULE, table), d_out, gpu(np.zeros(need, np.uint8)), need)
+    ref.mass(q, kc, vc, ctx, None, acc, RULE, table, out)
+    assert np.array_equal(gpu.back(d_out, out), out)
+
+
 def test_unaligned_rows_and_caches(gpu):
     """Arrays 4 bytes off a multiple of 16 (the caller's slices): the row form, the same values; and queries,
     caches and outputs inside larger arrays, whose other bytes stay."""
@@ -233,6 +248,7 @@ def test_many_panels(gpu):
     check_tree(gpu, 300, 20, 4, 16, 90, [70, 0, 33], [20, 0, 17, 3])
     check_mass(gpu, 300, 2, 4, 16, 90, [70, 2, 33, 0], [2, 0, 1, 2])
     check_mass(gpu, 700, 1, 4, 16, 600, [70, 0, 333, 600], [1, 1, 0, 1])
+    check_mass(gpu, 130, 1, 4, 16, 2100, [2100, 0, 333, 2049, 1], [1, 1, 0, 1])
 
 
 def test_mass_counts_beyond_the_cache(gpu):
