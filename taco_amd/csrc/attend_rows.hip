@@ -1048,10 +1048,14 @@ size_t rows_workspace(const RowsArgs &g) {
     return (size_t)long_scratch(nullptr, p, panels).part + panels * p.ng * p.tiles * RT_ROWS * g.a.hd * 8;
 }
 
+// Past 1,024 keys a tile fills a CU, so three tiles and more of many panels walk the keys side by side instead (768
+// panels of 64 rows at 1,400 keys: 147 us in tiles, 103 in one launch of three walks; at 700 keys 60 and 58, 192
+// panels 19 and 32).
 template <int QC, bool HI>
 static hipError_t launch_mfma(const RowsArgs &g, void *workspace, hipStream_t stream) {
-    if (g.a.ctx_cap <= RT_KEYS) return launch_tile<QC, HI>(g, g.a.ctx_cap, stream);
-    return launch_long<QC, HI>(g, long_plan(g, g.a.ctx_cap), workspace, stream);
+    const LongPlan p = long_plan(g, g.a.ctx_cap);
+    const bool walks = g.a.ctx_cap > RT_KEYS || (g.a.ctx_cap > 1024 && p.tiles >= 3 && p.ng == 1);
+    return walks ? launch_long<QC, HI>(g, p, workspace, stream) : launch_tile<QC, HI>(g, g.a.ctx_cap, stream);
 }
 
 hipError_t launch_rows(const RowsArgs &g, void *workspace, hipStream_t stream) {

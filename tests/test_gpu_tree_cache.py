@@ -248,6 +248,7 @@ def test_many_panels(gpu):
     check_tree(gpu, 300, 20, 4, 16, 90, [70, 0, 33], [20, 0, 17, 3])
     check_mass(gpu, 300, 2, 4, 16, 90, [70, 2, 33, 0], [2, 0, 1, 2])
     check_mass(gpu, 700, 1, 4, 16, 600, [70, 0, 333, 600], [1, 1, 0, 1])
+    check_tree(gpu, 130, 40, 5, 16, 1100, [1060, 0, 33], [40, 0, 17, 3])
     check_mass(gpu, 130, 1, 4, 16, 2100, [2100, 0, 333, 2049, 1], [1, 1, 0, 1])
 
 
