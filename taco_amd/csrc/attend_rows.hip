@@ -117,6 +117,10 @@ __global__ __launch_bounds__(256) void k_rows(RowsArgs g, int n_tasks) {
 // digits, four products with V^T by transposing LDS reads; here the waves share the keys of the same rows, so the
 // extremes and the sums meet in LDS, and the output sums in 64-bit LDS atomics (integers: any order).
 // QC: 64-byte chunks of a head (the last one may be part empty: its lanes hold zeros).
+// 768 panels of 16 rows at 750 keys (76 MB): 21.3 us, 3.6 TB/s; 12 panels 6.3 us at 100 keys. Few panels are bound by
+// the chain of one workgroup (loads, two exchanges between the waves, products), many by HBM and, from three tiles a
+// panel on, by the VALU work of the scores (about 24 instructions each with a wave's fixed part): causal chunks of
+// 256 rows, 192 panels, 52 us, 27 of them VALU issue.
 constexpr int RT_ROWS = 16;
 constexpr int RT_TABLE = 16384;  // entries of the table copied to LDS at most
 constexpr int RT_ACC = 66;       // 64 channels' sums of a row and two of padding (bank spread)
@@ -569,7 +573,10 @@ static hipError_t launch_tile(const RowsArgs &g, int keys, hipStream_t stream) {
 //   k_long_pv the products with V: WT tiles side by side, 4 / WT waves to a tile, since a tile's sums are 64
 //     registers for 64 channels (the others' loads of the same rows hit the L1).
 // ALONE: k_long_pv walks all three times itself, where the rows alone give enough workgroups. A head dim above
-// 128 takes a workgroup for each 64 channels (cg).
+// 128 takes a workgroup for each 64 channels (cg). 200 panels of 64 rows at 6,100 keys, head_dim 64: 20 + 34 + 88 + 7 us
+// in the kernel trace. What bounds the products' launch: per score 4 instructions to the table index, the lookup
+// (LDS: 21 us in all, half of it bank conflicts), 6 for p and 3 for its digits (VALU: 32 us), 20 MFMAs a block (10
+// us), in chains that three waves a SIMD overlap in part; K and V come a block ahead.
 struct LongPlan {
     int tiles = 0, wt = 1, groups = 1;  // row tiles; of a group; groups
     int ng = 1, span = 0, cg = 1;        // key ranges, their keys; workgroups for the channels
@@ -977,6 +984,7 @@ static LongPlan long_plan(const RowsArgs &g, int keys) {
     const int unit = 256, most = (keys + 2 * unit - 1) / (2 * unit);
     long long ng = LONG_WGS / wgs;
     ng = ng < 1 ? 1 : (ng > most ? most : ng);
+    ng = ng < (keys + 65535) / 65536 ? (keys + 65535) / 65536 : ng;  // a wave's plane sums: at most 2^16 keys of 2^14
     p.span = (int)(((keys + ng - 1) / ng + unit - 1) / unit) * unit;
     p.ng = (keys + p.span - 1) / p.span;
     return p;

@@ -414,6 +414,33 @@ def test_serving_loop(gpu):
     assert n.max() == budget
 
 
+def test_plane_sums_of_many_keys(gpu):
+    """133,151 keys and more of equal weight, p = 8,064, whose lowest digit is -128, over values of -128: a digit plane's
+    sum over all of them passes 2^31, so no wave may add up that many (520 panels: enough for one launch else)."""
+    b, t, hd, ctx = 520, 40, 16, 133_150
+    cap = ctx + t
+    count, keys = np.zeros(b, np.uint32), np.zeros(b, np.uint32)
+    count[-1], keys[-1] = t, ctx
+    r = np.random.default_rng(2)
+    mask = np.zeros((b, t, 1), np.uint64)
+    mask[-1] = masks(gpu, r, 1, t)[0]
+    q = np.zeros((b, t, 1, hd), np.int8)
+    v = np.full((1, 1, cap, hd), -128, np.int8)
+    panels = []
+    for x in (np.zeros_like(v), v):
+        p = C.c_void_p()
+        gpu.hip._check(gpu.hip.lib().hs_device_alloc(gpu.dev.h, b * x.nbytes, C.byref(p)))
+        gpu.held.append(p)
+        gpu.hip._check(gpu.hip.lib().hs_device_upload(gpu.dev.h, C.c_void_p(p.value + (b - 1) * x.nbytes), gpu.hip._ptr(x), x.nbytes))
+        panels.append(p)
+    rule = (1 << 30, 36, 1 << 30, 60, 30)
+    out = np.full(q.shape, 77, np.int8)
+    d_out = gpu(out)
+    gpu.hip.attend_tree(gpu.dev, gpu(q), *panels, gpu(keys), gpu(count), gpu(mask), (b, t, 1, hd, cap), gpu.rule(rule, TABLE), d_out)
+    ref.tree(q[-1:], np.zeros_like(v), v, keys[-1:], None, mask[-1:], rule, TABLE, out[-1:])
+    assert np.array_equal(gpu.back(d_out, out), out) and (out[-1] < -100).all()
+
+
 def test_caches_of_more_than_4_gib(gpu):
     """The last of 257 streams of 2 heads and 131,072 places: its panels lie past 2^32 bytes."""
     r = np.random.default_rng(21)
