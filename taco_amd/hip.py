@@ -534,17 +534,21 @@ def gemm_requant_i8(dev: HipDevice, w, a, bias, mult, shift: int) -> np.ndarray:
 
 
 def _dptr(x):
-    """The device address of x: a tensor (data_ptr()), an address or a ctypes pointer, or None."""
-    return x.data_ptr() if hasattr(x, "data_ptr") else x
+    """The device address of x: a contiguous tensor on the GPU (data_ptr()), an address or a ctypes pointer, or None."""
+    if not hasattr(x, "data_ptr"):
+        return x
+    if not getattr(x, "is_cuda", True):
+        raise ValueError("a tensor in host memory where the GPU reads or writes")
+    if not x.is_contiguous():
+        raise ValueError("a tensor with strides of its own: the operators take contiguous ones")
+    return x.data_ptr()
 
 
 def _dptrs(xs):
     """The layers' device addresses as a host array, from a list of them or from one contiguous tensor
     whose first axis is the layers."""
     if hasattr(xs, "data_ptr"):
-        if not xs.is_contiguous():
-            raise ValueError("a tensor of all layers' caches must be contiguous")
-        n, at = xs.shape[0], xs.data_ptr()
+        n, at = xs.shape[0], _dptr(xs)
         step = xs.stride(0) * xs.element_size()
         return (C.c_void_p * n)(*range(at, at + n * step, step)) if step else (C.c_void_p * 0)()
     return (C.c_void_p * len(xs))(*[_dptr(x) for x in xs])

@@ -122,3 +122,31 @@ def test_tree_mask():
     for parents in ([0], [-1, 1], [-2], [-1, 5]):
         with pytest.raises(ValueError):
             hip.tree_mask(parents)
+
+
+def test_tensors_that_the_gpu_cannot_take():
+    """A tensor in host memory and one with strides of its own are refused before their address is used."""
+    torch = pytest.importorskip("torch")
+    host = torch.zeros(4, 4, dtype=torch.int8)
+
+    class Strided:
+        is_cuda = True
+        shape = (4, 4)
+        data_ptr = lambda self: BASE  # noqa: E731
+        is_contiguous = lambda self: False  # noqa: E731
+
+    dims = (2, 3, 2, 64, 100)
+    for x in (host, Strided()):
+        for i in range(6):  # q, k, v, ctx, count, mask or accumulators
+            args = [BASE] * 6
+            args[i] = x
+            for fn in (hip.attend_tree, hip.attend_mass):
+                with pytest.raises(ValueError):
+                    fn(Dev, *args, dims, RULE, BASE)
+        with pytest.raises(ValueError):
+            hip.attend_tree(Dev, *[BASE] * 6, dims, RULE, x)
+        for k in (x, [x]):
+            with pytest.raises(ValueError):
+                hip.cache_commit(Dev, k, k, BASE, BASE, BASE, dims, None)
+            with pytest.raises(ValueError):
+                hip.cache_evict(Dev, k, k, BASE, BASE, (2, 2, 64, 100), 50, 10, BASE, None)
