@@ -317,8 +317,9 @@ hs_status hs_op_attend_decode_dev_noalloc(hs_device *dev, const int8_t *q, const
  * tree of one branch) and keeps every key until a context restarts. Device pointers throughout but
  * for the arrays of layer pointers; `stream` a hipStream_t or NULL (the device's own); nothing waits for
  * the GPU. Rules, tables and caches as in hs_op_attend_decode_dev; rows, caches, tables and counts
- * 4-byte aligned, masks and accumulators 8-byte; table entries 0 or more. Attention takes caches of at most
- * 2^22 keys, the others 2^30. Safe under graph capture (with a workspace of the caller's where one is
+ * 4-byte aligned, masks and accumulators 8-byte; table entries 0 or more. Attention takes fewer than
+ * 2^26 rows of a head (b t h) and caches of at most 2^22 keys, the others fewer than 2^22 panels a layer (b h) and
+ * 2^30 keys; with no stream, row or layer a call does nothing. Safe under graph capture (with a workspace of the caller's where one is
  * needed). Arrays that a call writes overlap nothing else that it is given, but where it says so. Rows, caches
  * and tables aligned to 16 bytes, head dims that are multiples of 16 and tables of at most 16,384
  * entries take the fast forms. ------------------------------------------------------------------ */

@@ -1024,15 +1024,16 @@ constexpr int RT_KEYS = 2048;  // the most keys of a tile in one launch
 
 static bool rows_hi(const AttnArgs &a) { return a.score_s >= 32 && a.score_s <= 60 && a.score_m != INT32_MIN; }
 
-// Whether the MFMA forms take the shapes (the grids below 2^31 workgroups), the alignments and the table.
+// Whether the MFMA forms take the shapes (a grid holds fewer than 2^32 threads), the alignments and the table.
 static bool rows_mfma_ok(const RowsArgs &g) {
     const AttnArgs &a = g.a;
     const uintptr_t bits = (uintptr_t)a.q | (uintptr_t)a.kc | (uintptr_t)a.vc | (uintptr_t)a.exp_table | (uintptr_t)a.ldq | (uintptr_t)a.hd;
     const long long tiles = (g.t + RT_ROWS - 1) / RT_ROWS, panels = (long long)g.streams * a.n_head + 7;
     if (bits % 16 != 0 || a.exp_len > RT_TABLE) return false;
-    if (a.ctx_cap <= RT_KEYS) return panels * tiles < (1ll << 31);
+    if (panels * tiles >= 1ll << 23) return false;  // up to 512 threads a tile
+    if (a.ctx_cap <= RT_KEYS) return true;
     const LongPlan p = long_plan(g, a.ctx_cap);
-    return panels * p.groups * p.ng * p.cg < (1ll << 31) && panels * tiles * RT_ROWS * (a.hd / 4) < (1ll << 38);
+    return panels * p.groups * p.ng * p.cg < 1ll << 24 && panels * tiles * RT_ROWS * (a.hd / 4) < (1ll << 32) - 256;
 }
 
 // One causal row a stream: the decode kernels, which add up the weights too, where one launch of them serves (768
@@ -1043,6 +1044,7 @@ static bool rows_decode_ok(const RowsArgs &g) {
     const AttnArgs &a = g.a;
     const uintptr_t bits = (uintptr_t)a.q | (uintptr_t)a.kc | (uintptr_t)a.vc;
     if (g.t != 1 || g.mask || g.groups || !attend_split_ok(a.hd) || bits % 16 != 0) return false;
+    if ((long long)g.streams * a.n_head >= 1ll << 22) return false;  // (up to 512 threads a row-head in a grid)
     return attend_split_one_launch(a.hd, a.ctx_cap, attend_split_plan(g.streams, a.n_head, a.ctx_cap)) || !rows_mfma_ok(g) ||
            (a.ctx_cap > RT_KEYS && (long long)g.streams * a.n_head >= 512);
 }

@@ -1931,6 +1931,8 @@ extern "C" hs_status hs_op_attend_decode_dev_noalloc(hs_device *dev, const int8_
 
 namespace {
 
+constexpr size_t MAX_ROW_HEADS = ((size_t)1 << 26) - 4;  // 64 threads each in a grid of fewer than 2^32
+
 bool overlap(const void *x, size_t nx, const void *y, size_t ny) {
     const uintptr_t a = (uintptr_t)x, b = (uintptr_t)y;
     return x && y && a < b + ny && b < a + nx;
@@ -1955,8 +1957,8 @@ hs_status rows_args(hs_device *dev, const int8_t *q, const int8_t *k_cache, cons
     if (!aligned(4, {q, k_cache, v_cache, ctx, attn_exp, out}))
         return hs::fail(HS_INVALID_ARGUMENT, 0, "rows, caches, counts and the table must be 4-byte aligned");
     if (t > (size_t)INT32_MAX || h > (size_t)INT32_MAX || b > (size_t)INT32_MAX || len > (size_t)INT32_MAX ||
-        ctx_cap > (size_t)1 << 22 || h * hd > (size_t)INT32_MAX || b * t > (size_t)INT32_MAX / h)
-        return hs::fail(HS_UNSUPPORTED, 0, "too many rows, heads or keys (at most 2^22 keys)");
+        ctx_cap > (size_t)1 << 22 || h * hd > (size_t)INT32_MAX || b * t > MAX_ROW_HEADS / h)
+        return hs::fail(HS_UNSUPPORTED, 0, "too many rows, heads or keys (fewer than 2^26 rows of a head, at most 2^22 keys)");
     hs::AttnArgs &at = g.a;
     at.q = q; at.ldq = (int)(h * hd); at.kc = k_cache; at.vc = v_cache;
     at.n_head = (int)h; at.hd = (int)hd; at.ctx_cap = (int)ctx_cap; at.score_m = score_m;
@@ -2003,9 +2005,8 @@ hs_status cache_args(hs_device *dev, int8_t *const *k_caches, int8_t *const *v_c
     if (!dev || (layers && (!k_caches || !v_caches))) return hs::fail(HS_INVALID_ARGUMENT, 0, "NULL argument");
     if (hd == 0 || hd % 4 != 0 || hd > 256 || h == 0 || ctx_cap == 0)
         return hs::fail(HS_UNSUPPORTED, 0, "head_dim must be a multiple of 4 in 4..=256; h and ctx_cap >= 1");
-    if (ctx_cap > (size_t)1 << 30 || b > (size_t)INT32_MAX || h > (size_t)INT32_MAX / 128 ||
-        (b && h > (size_t)INT32_MAX / 128 / b))  // 64 layers of K and V in a launch
-        return hs::fail(HS_UNSUPPORTED, 0, "too many panels or keys (at most 2^30 keys)");
+    if (ctx_cap > (size_t)1 << 30 || h > hs::CACHE_PANELS || (b && h > hs::CACHE_PANELS / b))
+        return hs::fail(HS_UNSUPPORTED, 0, "too many heads or keys (fewer than 2^22 heads of streams, at most 2^30 keys)");
     for (size_t l = 0; l < layers; l++) {
         if (!k_caches[l] || !v_caches[l]) return hs::fail(HS_INVALID_ARGUMENT, 0, "NULL cache");
         if (!aligned(4, {k_caches[l], v_caches[l]}))
@@ -2014,11 +2015,16 @@ hs_status cache_args(hs_device *dev, int8_t *const *k_caches, int8_t *const *v_c
     return HS_OK;
 }
 
+// The layers of a launch.
+size_t launch_layers(size_t b, size_t h) { return std::min<size_t>(hs::CACHE_LAYERS, hs::CACHE_PANELS / (b * h)); }
+
 }  // namespace
 
 extern "C" size_t hs_op_attend_rows_workspace(size_t b, size_t t, size_t h, size_t hd, size_t ctx_cap) {
     hs::RowsArgs g;
-    if (b * t * h == 0 || hd == 0 || b * t > (size_t)INT32_MAX / h || ctx_cap > (size_t)1 << 22) return 0;
+    if (b == 0 || t == 0 || h == 0 || hd == 0 || hd > 256 || b > MAX_ROW_HEADS || t > MAX_ROW_HEADS ||
+        b * t > MAX_ROW_HEADS / h || ctx_cap == 0 || ctx_cap > (size_t)1 << 22)
+        return 0;  // (the call itself refuses them, or does nothing)
     g.streams = (int)b; g.t = (int)t; g.a.n_head = (int)h; g.a.hd = (int)hd; g.a.ctx_cap = (int)ctx_cap;
     // of a tree and of causal rows, with a table that the fast forms take and with a longer one
     const uint64_t some = 0;
@@ -2086,8 +2092,8 @@ extern "C" hs_status hs_op_cache_evict_dev(hs_device *dev, int8_t *const *k_cach
     HIP_TRY(hipSetDevice(dev->ordinal));
     hipStream_t st = stream ? (hipStream_t)stream : dev->stream;
     hs::EvictArgs a{mass, ctx, (int)b, (int)h, (int)hd, (int)ctx_cap, (int)budget, (int)recent, 0, mass_out, ctx_out, kept};
-    for (size_t l0 = 0; l0 < layers; l0 += hs::CACHE_LAYERS) {
-        const int n = (int)std::min<size_t>(hs::CACHE_LAYERS, layers - l0);
+    for (size_t l0 = 0, step = launch_layers(b, h); l0 < layers; l0 += step) {
+        const int n = (int)std::min(step, layers - l0);
         hs::CachePtrs c{};
         for (int l = 0; l < n; l++) {
             c.k[l] = k_caches[l0 + l];
@@ -2113,8 +2119,8 @@ extern "C" hs_status hs_op_cache_commit_dev(hs_device *dev, int8_t *const *k_cac
     HIP_TRY(hipSetDevice(dev->ordinal));
     hipStream_t st = stream ? (hipStream_t)stream : dev->stream;
     hs::CommitArgs a{ctx, path, accepted, (int)b, (int)t, (int)h, (int)hd, (int)ctx_cap, 0, ctx_out};
-    for (size_t l0 = 0; l0 < layers; l0 += hs::CACHE_LAYERS) {
-        const int n = (int)std::min<size_t>(hs::CACHE_LAYERS, layers - l0);
+    for (size_t l0 = 0, step = launch_layers(b, h); l0 < layers; l0 += step) {
+        const int n = (int)std::min(step, layers - l0);
         hs::CachePtrs c{};
         for (int l = 0; l < n; l++) {
             c.k[l] = k_caches[l0 + l];

@@ -245,6 +245,7 @@ hipError_t launch_rows(const RowsArgs &g, void *workspace, hipStream_t stream);
 
 // The caches of up to CACHE_LAYERS layers in one launch, each [b][h][cap][hd].
 constexpr int CACHE_LAYERS = 64;
+constexpr size_t CACHE_PANELS = ((size_t)1 << 22) - 1;  // (layer, stream, head) of a launch: up to 1,024 threads each
 struct CachePtrs {
     int8_t *k[CACHE_LAYERS], *v[CACHE_LAYERS];
 };

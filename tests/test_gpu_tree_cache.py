@@ -488,3 +488,54 @@ def test_caches_of_more_than_4_gib(gpu):
     ref.evict([kc], [vc], acc[:, -1:], after[-1:], budget, recent, acc[:, -1:], cut[-1:], None)
     assert np.array_equal(gpu.back(d_cut, cut), cut) and np.array_equal(gpu.back(d_acc, acc), acc)
     assert np.array_equal(gpu.back(last_k, kc), kc) and np.array_equal(gpu.back(last_v, vc), vc)
+
+
+def test_more_streams_than_a_grid_of_tiles(gpu):
+    """2^23 + 5 streams of one row and one key, which gets the whole weight: the output follows from the value
+    alone, so one row of all 256 values says what it is. As a tree and as a causal row with weights."""
+    b, hd = 2 ** 23 + 5, 16
+    r = np.random.default_rng(8)
+    every = np.arange(-128, 128).astype(np.int8).reshape(1, 1, 16, 16)  # sixteen heads of one key
+    one, out16 = np.zeros((1, 1, 16, 16), np.int8), np.zeros((1, 1, 16, 16), np.int8)
+    ref.mass(one, one.reshape(1, 16, 1, 16), every.reshape(1, 16, 1, 16), np.ones(1, np.uint32), None,
+             np.zeros((1, 16, 1), np.uint64), RULE, TABLE, out16)
+    lut = out16.reshape(256)
+    q = r.integers(-128, 128, (b, 1, 1, hd)).astype(np.int8)
+    kv = r.integers(-128, 128, (b, 1, 1, hd)).astype(np.int8)
+    expect = lut[kv.astype(np.int16) + 128]
+    d_q, d_kv, rule, dims = gpu(q), gpu(kv), gpu.rule(RULE, TABLE), (b, 1, 1, hd, 1)
+    out = np.full_like(q, 77)
+    d_out = gpu(out)
+    gpu.hip.attend_tree(gpu.dev, d_q, d_kv, d_kv, gpu(np.zeros(b, np.uint32)), None, gpu(np.ones(b, np.uint64)), dims, rule, d_out)
+    assert np.array_equal(gpu.back(d_out, out), expect)
+    d_out, d_mass = gpu(out), gpu(np.arange(b, dtype=np.uint64))
+    gpu.hip.attend_mass(gpu.dev, d_q, d_kv, d_kv, gpu(np.ones(b, np.uint32)), None, d_mass, dims, rule, d_out)
+    assert np.array_equal(gpu.back(d_out, out), expect)
+    assert np.array_equal(gpu.back(d_mass, np.empty(b, np.uint64)), np.arange(b, dtype=np.uint64) + np.uint64(2 ** 30))
+
+
+def test_more_panels_than_a_launch(gpu):
+    """64 layers of 70,000 streams, more than 2^22 panels: the layers go in two launches."""
+    layers, b, hd = 64, 70_000, 4
+    r = np.random.default_rng(9)
+    ks, vs = [[r.integers(-128, 128, (b, 1, 2, hd)).astype(np.int8) for _ in range(layers)] for _ in range(2)]
+    dk, dv = [gpu(x) for x in ks], [gpu(x) for x in vs]
+    dims, ones = (b, 1, hd, 2), gpu(np.ones(b, np.uint32))
+    mass = r.integers(0, 3, (layers, b, 1, 2)).astype(np.uint64)
+    d_mass, d_ctx, ctx = gpu(mass), gpu(np.full(b, 9, np.uint32)), np.empty(b, np.uint32)
+    gpu.hip.cache_evict(gpu.dev, dk, dv, d_mass, gpu(np.full(b, 2, np.uint32)), dims, 1, 0, d_mass, d_ctx)
+    second = mass[..., 1] > mass[..., 0]
+    for l in range(layers):
+        for x in (ks[l], vs[l]):
+            x[:, :, 0][second[l]] = x[:, :, 1][second[l]]
+    for d, x in zip(dk + dv, ks + vs):
+        assert np.array_equal(gpu.back(d, x), x)
+    mass = np.stack([mass.max(-1), np.zeros_like(mass[..., 0])], -1)
+    assert np.array_equal(gpu.back(d_mass, mass), mass)
+    assert (gpu.back(d_ctx, ctx) == 1).all()
+    d_ctx = gpu(np.full(b, 9, np.uint32))
+    gpu.hip.cache_commit(gpu.dev, dk, dv, gpu(np.zeros(b, np.uint32)), ones, ones, (b, 1, 1, hd, 2), d_ctx)
+    for d, x in zip(dk + dv, ks + vs):
+        x[:, :, 0] = x[:, :, 1]
+        assert np.array_equal(gpu.back(d, x), x)
+    assert (gpu.back(d_ctx, ctx) == 1).all()

@@ -150,3 +150,21 @@ def test_tensors_that_the_gpu_cannot_take():
                 hip.cache_commit(Dev, k, k, BASE, BASE, BASE, dims, None)
             with pytest.raises(ValueError):
                 hip.cache_evict(Dev, k, k, BASE, BASE, (2, 2, 64, 100), 50, 10, BASE, None)
+
+
+def test_more_rows_than_a_grid_holds():
+    """2^26 rows of a head and 2^22 panels a layer are past a grid of the kernels; the workspace of a call
+    that is refused, or that does nothing, is none."""
+    unsupported = hip.HS_UNSUPPORTED
+    for fn in (hip.attend_tree, hip.attend_mass):
+        rows(fn, dims=(1 << 20, 64, 1, 64, 100))(unsupported)
+        rows(fn, dims=(1 << 20, 1, 64, 64, 100))(unsupported)
+    evict(dims=(1 << 20, 4, 64, 100))(unsupported)
+    commit(dims=(1 << 12, 3, 1 << 10, 64, 100))(unsupported)
+    sizes = hip.attend_rows_workspace
+    assert sizes(8, 64, 25, 64, 8192) > 0
+    for dims in ((8, 64, 25, 1 << 33, 8192), (8, 64, 25, 1 << 31, 8192), (8, 64, 25, 272, 8192), (1 << 63, 2, 1, 64, 8192),
+                 (1 << 33, 1 << 33, 1, 64, 8192), (8, 64, 1 << 40, 64, 8192), (8, 64, 25, 64, 0),
+                 (8, 64, 25, 64, (1 << 22) + 1), (0, 64, 25, 64, 8192), (8, 0, 25, 64, 8192), (8, 64, 0, 64, 8192),
+                 (8, 64, 25, 0, 8192)):
+        assert sizes(*dims) == 0, dims
