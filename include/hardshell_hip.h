@@ -315,14 +315,15 @@ hs_status hs_op_attend_decode_dev_noalloc(hs_device *dev, const int8_t *q, const
 
 /* ---- Trees of drafts and bounded caches. No counterparts in the reference: it drafts chains (a
  * tree of one branch) and keeps every key until a context restarts. Device pointers throughout but
- * for the arrays of layer pointers; `stream` a hipStream_t or NULL (the device's own); nothing waits for
- * the GPU. Rules, tables and caches as in hs_op_attend_decode_dev; rows, caches, tables and counts
- * 4-byte aligned, masks and accumulators 8-byte; table entries 0 or more. Attention takes fewer than
- * 2^26 rows of a head (b t h) and caches of at most 2^22 keys, the others fewer than 2^22 panels a layer (b h) and
- * 2^30 keys; with no stream, row or layer a call does nothing. Safe under graph capture (with a workspace of the caller's where one is
- * needed). Arrays that a call writes overlap nothing else that it is given, but where it says so. Rows, caches
- * and tables aligned to 16 bytes, head dims that are multiples of 16 and tables of at most 16,384
- * entries take the fast forms. ------------------------------------------------------------------ */
+ * for the arrays of layer pointers; `stream` a hipStream_t or NULL (the device's own); nothing
+ * waits for the GPU. Rules, tables and caches as in hs_op_attend_decode_dev; rows, caches, tables
+ * and counts 4-byte aligned, masks and accumulators 8-byte; table entries 0 or more. Attention
+ * takes fewer than 2^26 rows of a head (b t h) and caches of at most 2^22 keys, the others fewer
+ * than 2^22 panels a layer (b h) and 2^30 keys; with no stream, row or layer a call does nothing.
+ * Safe under graph capture (with a workspace of the caller's where one is needed). Arrays that a
+ * call writes overlap nothing else that it is given, but where it says so. Rows, caches and tables
+ * aligned to 16 bytes, head dims that are multiples of 16 and tables of at most 16,384 entries take
+ * the fast forms. ------------------------------------------------------------------ */
 /* Attention of a tree of drafted tokens for each stream. q and out [b, t, h, hd] i8; row i < nodes[s]
  * (NULL: t for every stream) is node i of the tree of stream s, whose key and value the caller has
  * stored at cache position ctx[s] + i. mask [b, t, ceil(t / 64)] u64: bit n % 64 of word n / 64 of row i
@@ -351,8 +352,9 @@ hs_status hs_op_attend_mass_dev(hs_device *dev, const int8_t *q, const int8_t *k
                                 uint8_t softmax_p, int8_t *out, void *workspace,
                                 size_t workspace_bytes, void *stream);
 /* The bytes of workspace (256-byte aligned) that a call of these shapes of either needs, 0 where
- * none. A call that gets NULL allocates them on the stream. Calls that can overlap, captured graphs
- * among them, need workspaces of their own; nothing is kept in it between calls. */
+ * none. A call that gets NULL allocates them on the stream; under capture it is refused. Calls that
+ * can overlap, captured graphs among them, need workspaces of their own; nothing is kept in it
+ * between calls. */
 size_t hs_op_attend_rows_workspace(size_t b, size_t t, size_t h, size_t hd, size_t ctx_cap);
 /* Cuts the caches of each stream with n = ctx[s] > budget keys to budget keys, in place, in every
  * layer (k_caches, v_caches: host arrays of `layers` device caches [b, h, ctx_cap, hd]) and head by

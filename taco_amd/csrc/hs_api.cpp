@@ -1978,6 +1978,10 @@ hs_status run_rows(hs_device *dev, const hs::RowsArgs &g, void *workspace, size_
         HIP_TRY(hs::launch_rows(g, workspace, st));
         return HS_OK;
     }
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    HIP_TRY(hipStreamIsCapturing(st, &capture));
+    if (capture != hipStreamCaptureStatusNone)  // (the graph would hold memory that other calls get after this one)
+        return hs::fail(HS_INVALID_ARGUMENT, 0, "a captured call of these shapes needs a workspace");
     {
         std::lock_guard<std::mutex> lock(dev->pool_mu);
         if (!dev->pool) {

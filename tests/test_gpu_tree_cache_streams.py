@@ -150,3 +150,31 @@ def test_a_workspace_that_is_too_small_is_refused(gpu):
     hip.attend_tree(gpu.dev, d["q"], d["k"], d["v"], d["ctx"], None, d["mask"], s.dims, s.rule, d["tree"])  # its own
     ref.tree(s.q, s.k, s.v, s.ctx, None, s.mask, RULE, TABLE, s.tree)
     assert np.array_equal(gpu.back(d["tree"], s.tree), s.tree)
+
+
+def test_a_captured_call_without_a_workspace_is_refused(gpu):
+    rt = runtime()
+    s, stream = Step(gpu, 11, *SHAPES[1]), Stream(rt)
+    s.run(stream)
+    s.host()
+    stream.sync()
+    s.check()
+    hip, d = gpu.hip, s.d
+    refused = []
+
+    def fn():
+        for call, third in ((hip.attend_tree, d["mask"]), (hip.attend_mass, d["acc"])):
+            try:
+                call(gpu.dev, d["q"], d["k"], d["v"], d["keys"], None, third, s.dims, s.rule, d["tree"], None, 0, stream.h)
+            except hip.HipError as e:
+                refused.append(e.status)
+        s.run(stream)  # the capture goes on
+
+    run = stream.capture(fn)
+    assert refused == [hip.HS_INVALID_ARGUMENT] * 2
+    for _ in range(2):
+        ok(rt.hipGraphLaunch(run, stream.h))
+        s.host()
+        stream.sync()
+        s.check()
+    ok(rt.hipGraphExecDestroy(run))
