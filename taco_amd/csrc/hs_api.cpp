@@ -1421,6 +1421,16 @@ hs_status tree_buffers(hs_batch *b) {
     return HS_OK;
 }
 
+// What fn() gives; memory that the host lacks is a failed call, not an exception past a C entry.
+template <typename F>
+hs_status guarded(F fn) {
+    try {
+        return fn();
+    } catch (const std::bad_alloc &) {
+        return hs::fail(HS_DEVICE_ERROR, (int)hipErrorOutOfMemory, "out of host memory");
+    }
+}
+
 hs_status run_tree(hs_batch *b, const hs_input *in, const uint32_t *parents, size_t n, Out out, const uint32_t *queries,
                    uint32_t bits, uint64_t *sink) {
     std::vector<PassRow> rows;
@@ -1556,7 +1566,7 @@ extern "C" hs_status hs_batch_run_tree_weights(hs_batch *b, const hs_input *in, 
     hs::clear_error();
     HS_TRY(check_inputs(b, in, n));
     if (n && !out) return hs::fail(HS_INVALID_ARGUMENT, 0, "out is NULL");
-    return run_tree(b, in, parents, n, Out::Weights, nullptr, 0, out);
+    return guarded([&] { return run_tree(b, in, parents, n, Out::Weights, nullptr, 0, out); });
 }
 
 extern "C" hs_status hs_batch_run_tree_coded(hs_batch *b, const hs_input *in, const uint32_t *parents,
@@ -1565,12 +1575,10 @@ extern "C" hs_status hs_batch_run_tree_coded(hs_batch *b, const hs_input *in, co
     HS_TRY(check_inputs(b, in, n));
     if (n && (!queries || !out)) return hs::fail(HS_INVALID_ARGUMENT, 0, "NULL argument");
     HS_TRY(check_queries(queries, n, b->model->host.vocab, freq_bits));
-    return run_tree(b, in, parents, n, Out::Intervals, query_words(queries), freq_bits, (uint64_t *)out);
+    return guarded([&] { return run_tree(b, in, parents, n, Out::Intervals, query_words(queries), freq_bits, (uint64_t *)out); });
 }
 
-extern "C" hs_status hs_batch_commit_paths(hs_batch *b, const uint32_t *slots, const uint32_t *lengths,
-                                           const uint32_t *paths, size_t n) {
-    hs::clear_error();
+static hs_status commit_paths(hs_batch *b, const uint32_t *slots, const uint32_t *lengths, const uint32_t *paths, size_t n) {
     if (!b || (n && (!slots || !lengths))) return hs::fail(HS_INVALID_ARGUMENT, 0, "NULL argument");
     size_t at = 0;
     std::vector<char> seen(b->slots, 0);
@@ -1633,6 +1641,12 @@ extern "C" hs_status hs_batch_commit_paths(hs_batch *b, const uint32_t *slots, c
         if (t != b->trees.end()) b->trees.erase(t);
     }
     return HS_OK;
+}
+
+extern "C" hs_status hs_batch_commit_paths(hs_batch *b, const uint32_t *slots, const uint32_t *lengths,
+                                           const uint32_t *paths, size_t n) {
+    hs::clear_error();
+    return guarded([&] { return commit_paths(b, slots, lengths, paths, n); });
 }
 
 extern "C" hs_status hs_batch_step(hs_batch *b, const hs_input *in, size_t n) {
