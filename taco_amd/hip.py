@@ -406,7 +406,7 @@ class HipBatch:
         p = np.asarray(parents, dtype=np.int64)
         if len(p) != n:
             raise LengthMismatch(HS_LENGTH_MISMATCH, 0, f"length mismatch: expected {n}, found {len(p)}")
-        return np.where(p < 0, HS_TREE_ROOT, p).astype(np.uint32)
+        return np.where(p < 0, HS_TREE_ROOT, np.minimum(p, n)).astype(np.uint32)  # (n and more are no input: refused)
 
     def run_tree_weights(self, inputs, parents) -> np.ndarray:
         """The weights of every node of the slots' trees of drafts (hs_batch_run_tree_weights):

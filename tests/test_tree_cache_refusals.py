@@ -168,3 +168,11 @@ def test_more_rows_than_a_grid_holds():
                  (8, 64, 25, 64, (1 << 22) + 1), (0, 64, 25, 64, 8192), (8, 0, 25, 64, 8192), (8, 64, 0, 64, 8192),
                  (8, 64, 25, 0, 8192)):
         assert sizes(*dims) == 0, dims
+
+
+def test_parents_past_32_bits():
+    """They stay past the call's inputs (which is refused), and do not come round to one of them."""
+    p = hip.HipBatch._parents(None, [-1, 0, 2 ** 32, 2 ** 40 + 1, 3], 5)
+    assert p.dtype == np.uint32 and list(p) == [hip.HS_TREE_ROOT, 0, 5, 5, 3]
+    with pytest.raises(hip.LengthMismatch):
+        hip.HipBatch._parents(None, [-1], 2)
