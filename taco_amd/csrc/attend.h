@@ -33,6 +33,12 @@ __device__ __forceinline__ int32_t dot_key(const int *q4, const int8_t *k, int h
     return s;
 }
 
+// The keys of a decode row whose count is n: one at least, and never past the cache. (Compared unsigned: as an int
+// a count from 2^31 on would be negative, one key.)
+__device__ __forceinline__ int decode_keys(const AttnArgs &a, uint32_t n) {
+    return n < 1 ? 1 : (n > (uint32_t)a.ctx_cap ? a.ctx_cap : (int)n);
+}
+
 // score = clamp(rescale(dot, m, s), +-2^40): |dot| <= hd 2^14 <= 2^22, so |dot m| < 2^53 and one
 // multiply-add and an arithmetic shift are exact (a shift of 63 or more gives 0). With s >= 13
 // the score stays within +-2^40 and the clamp is a no-op.

@@ -1770,12 +1770,11 @@ __global__ __launch_bounds__(256) void k_attend(AttnArgs a, int n_tasks) {
     int slot, keys;
     if (a.rows) {
         slot = a.rows[r].slot;
-        keys = a.keys ? (int)a.keys[r] : a.rows[r].pos + 1;
+        keys = decode_keys(a, a.keys ? a.keys[r] : (uint32_t)(a.rows[r].pos + 1));
     } else {
         slot = r;
-        keys = (int)a.keys[r];
+        keys = decode_keys(a, a.keys[r]);
     }
-    keys = keys < 1 ? 1 : (keys > a.ctx_cap ? a.ctx_cap : keys);  // never read past the cache
     if (valid && lane < hd / 4) s_q[wave][lane] = ((const int *)(a.q + (size_t)r * a.ldq + h * hd))[lane];
     __syncthreads();
     if (!valid) return;
@@ -1876,8 +1875,7 @@ __device__ __forceinline__ SplitScratch split_scratch(void *base, int n_rows, in
 }
 
 __device__ __forceinline__ int split_keys(const AttnArgs &a, int r) {
-    int keys = a.keys ? (int)a.keys[r] : a.rows[r].pos + 1;
-    return keys < 1 ? 1 : (keys > a.ctx_cap ? a.ctx_cap : keys);
+    return decode_keys(a, a.keys ? a.keys[r] : (uint32_t)(a.rows[r].pos + 1));
 }
 
 // Of a row that keeps accumulators: 0 if it is not there, 1 if it has no key (a row of zeros), else 2.
