@@ -341,9 +341,10 @@ hs_status hs_op_attend_tree_dev(hs_device *dev, const int8_t *q, const int8_t *k
 /* Causal attention of the last rows[s] <= t tokens of each stream (NULL: t for every stream; t = 1
  * is the decode step), which also adds up how much weight each key receives: row i sees the first
  * ctx[s] - rows[s] + 1 + i of the stream's ctx[s] keys, and mass [b, h, ctx_cap] u64 gains
- * mass[s][h][j] += sum over the rows of p_j (p_j <= 2^softmax_p: 2^34 rows fit). Sums of integers: the
- * result depends on no order. A row that sees no key, or whose entries sum to 0, is 0 and adds nothing;
- * rows i >= rows[s] of out are left as they were. */
+ * mass[s][h][j] += sum over the rows of p_j (p_j <= 2^softmax_p: 2^34 rows fit). Atomic sums of
+ * integers: the result depends on no order, and calls that overlap may add to the same
+ * accumulators. A row that sees no key, or whose entries sum to 0, is 0 and adds nothing; rows i >=
+ * rows[s] of out are left as they were. */
 hs_status hs_op_attend_mass_dev(hs_device *dev, const int8_t *q, const int8_t *k_cache,
                                 const int8_t *v_cache, const uint32_t *ctx, const uint32_t *rows,
                                 uint64_t *mass, size_t b, size_t t, size_t h, size_t hd,

@@ -185,7 +185,8 @@ struct AttnArgs {
     int ldo = 0;
     int out_rows = 0;  // > 0: out is an operand in panels of out_rows rows (panel_off)
     // Decode attention that adds up each key's weights (launch_attend_split): mass [rows][H][ctx_cap] gains
-    // p. A row with keys[r] = 0 is 0 and adds nothing; one with count[r] = 0 (count may be null) is left out.
+    // p, atomically. A row with keys[r] = 0 is 0 and adds nothing; one with count[r] = 0 (count may be null) is
+    // left out.
     uint64_t *mass = nullptr;
     const uint32_t *count = nullptr;
 };

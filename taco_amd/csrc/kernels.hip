@@ -1883,6 +1883,14 @@ __device__ __forceinline__ int mass_row(const AttnArgs &a, int r) {
     return a.count && a.count[r] == 0 ? 0 : (a.keys[r] == 0 ? 1 : 2);
 }
 
+// The accumulator of key j gains p. An atomic addition, as in the forms of several rows: a call on another stream may
+// add to the same accumulators at the same time. (Loading them beside V and storing the sums lost such
+// additions, and was no faster: 768 row-heads of 1,024 keys 18.0 us at head_dim 64 and 42.4 at 128, this way 17.0 and 39.4;
+// head_dim 32 11.3 and 12.0, 8,000 keys 185 and 187.)
+__device__ __forceinline__ void add_mass(const AttnArgs &a, int rh, int j, uint64_t p) {
+    atomicAdd((unsigned long long *)a.mass + (size_t)rh * a.ctx_cap + j, (unsigned long long)p);
+}
+
 __device__ __forceinline__ int split_slot(const AttnArgs &a, int r) { return a.rows ? a.rows[r].slot : r; }
 
 // The row maximum of the scores, from every chunk's extreme dots (the score is monotone in the dot).
@@ -2040,7 +2048,7 @@ __global__ __launch_bounds__(64) void k_split_pv(AttnArgs a, int n_rows, SplitPl
                 q = __umul64hi(num, frac);  // q <= floor(num / S) <= q + 1
                 if (num - q * sum >= sum) q++;
             }
-            if (MASS && mass_row(a, r) == 2) a.mass[(size_t)rh * a.ctx_cap + kb + lane] += q;
+            if (MASS && mass_row(a, r) == 2) add_mass(a, rh, kb + lane, q);
         }
 #pragma unroll
         for (int g = 0; g < NG; g++)
@@ -2114,11 +2122,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         const int row = 16 * (i & 3) + (lane >> 2), k = 64 * (4 * (i >> 2) + w) + row;
         vr[i] = *(const v4i *)(a.vc + base + (size_t)(k < keys ? k : keys - 1) * 64 + 16 * ((lane & 3) ^ vsw<4>(row & 15)));
     }
-    uint64_t mv[4];  // the accumulators of the thread's keys
-    if constexpr (MASS) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) mv[j] = a.mass[(size_t)rh * a.ctx_cap + (tid + 256 * j < keys ? tid + 256 * j : keys - 1)];
-    }
     __builtin_amdgcn_sched_barrier(0);  // every load issued before the first wait
     // the dots wait for K alone (the compiler's waits on the K registers)
     int32_t d[4];
@@ -2184,7 +2187,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         for (int u = 0; u < 4; u++) *(v4i *)(s_v[w] + 1024 * u + 16 * lane) = vr[4 * j + u];
         // p <= 2^P <= 2^30; 0 for keys past the row (e = 0)
         const uint32_t p = softmax_p_of(e[j], R, sp);
-        if (MASS && tid + 256 * j < keys) a.mass[(size_t)rh * a.ctx_cap + tid + 256 * j] = mv[j] + p;
+        if (MASS && tid + 256 * j < keys) add_mass(a, rh, tid + 256 * j, p);
         decode_pv_block<4>(s_v[w], decode_pv_digits(s_mem[w], p, lane), lane, acc);
     }
     decode_pv_store<4>(s_mem[w], lane, acc);
@@ -2253,11 +2256,6 @@ __global__ __launch_bounds__(HD > 64 ? 512 : 256) __attribute__((amdgpu_waves_pe
 #pragma unroll
             for (int g = 0; g < NG; g++) vr[j][g][u] = *(const v4i *)(v + 64 * g);
         }
-    }
-    uint64_t mv[KT];  // the accumulators of the thread's keys
-    if constexpr (MASS) {
-#pragma unroll
-        for (int j = 0; j < KT; j++) mv[j] = a.mass[(size_t)rh * a.ctx_cap + (tid + NTH * j < keys ? tid + NTH * j : keys - 1)];
     }
     __builtin_amdgcn_sched_barrier(0);  // every load issued before the first wait
     // the dots wait for K alone (the compiler's waits on the K registers)
@@ -2332,7 +2330,7 @@ __global__ __launch_bounds__(HD > 64 ? 512 : 256) __attribute__((amdgpu_waves_pe
             if (g == 0) {  // p <= 2^P <= 2^30; 0 for keys past the row (e = 0)
                 __builtin_amdgcn_sched_barrier(0);  // the weights' arithmetic covers the stores of V
                 const uint32_t p = softmax_p_of(e[j], R, sp);
-                if (MASS && tid + NTH * j < keys) a.mass[(size_t)rh * a.ctx_cap + tid + NTH * j] = mv[j] + p;
+                if (MASS && tid + NTH * j < keys) add_mass(a, rh, tid + NTH * j, p);
                 pf = decode_pv_digits(s_mem[w], p, lane);
             }
             decode_pv_block<NC>(s_v[w], pf, lane, acc[g]);
@@ -2397,11 +2395,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         for (int g = 0; g < NG; g++)
             __builtin_amdgcn_global_load_lds((const void *)(v + 64 * g), (lds_void *)(sv + (g * NC * KB + i) * 1024), 16, 0, 0);
     }
-    uint64_t mv[KB];  // the accumulators of the lane's keys
-    if constexpr (MASS) {
-#pragma unroll
-        for (int j = 0; j < KB; j++) mv[j] = a.mass[(size_t)rh * a.ctx_cap + (lane + 64 * j < keys ? lane + 64 * j : keys - 1)];
-    }
     int32_t d[KB];
     int32_t dmin = INT32_MAX, dmax = INT32_MIN;
 #pragma unroll
@@ -2452,7 +2445,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         if (64 * j >= keys) break;
         // p <= 2^P <= 2^30; 0 for keys past the row (e = 0)
         const uint32_t p = softmax_p_of(e[j], R, sp);
-        if (MASS && lane + 64 * j < keys) a.mass[(size_t)rh * a.ctx_cap + lane + 64 * j] = mv[j] + p;
+        if (MASS && lane + 64 * j < keys) add_mass(a, rh, lane + 64 * j, p);
         const v4i pf = decode_pv_digits(mem, p, lane);
 #pragma unroll
         for (int g = 0; g < NG; g++) decode_pv_block<NC>(sv + (g * KB + j) * 64 * RB, pf, lane, acc[g]);
