@@ -83,6 +83,7 @@ const char *hs_version(void);
 /* Opens HIP device `ordinal`. HS_NO_DEVICE if there is no runtime or no such device;
  * HS_UNSUPPORTED if it is not a gfx950 (MI355X-class) GPU. */
 hs_status hs_device_open(int ordinal, hs_device **out);
+/* Waits for the GPU first where a call took a workspace from the device's pool (hs_op_attend_rows_workspace). */
 void hs_device_close(hs_device *dev);
 /* The device name ("AMD Instinct MI355X" ...), NUL-terminated, truncated to cap bytes. */
 hs_status hs_device_name(const hs_device *dev, char *buf, size_t cap);

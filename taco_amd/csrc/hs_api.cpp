@@ -303,6 +303,10 @@ extern "C" hs_status hs_device_open(int ordinal, hs_device **out) {
 
 extern "C" void hs_device_close(hs_device *dev) {
     if (!dev) return;
+    if (dev->pool) {  // calls on the caller's streams may still work in its memory
+        (void)hipSetDevice(dev->ordinal);
+        (void)hipDeviceSynchronize();
+    }
     if (dev->stream) (void)hipStreamDestroy(dev->stream);
     if (dev->pool) (void)hipMemPoolDestroy(dev->pool);
     delete dev;
