@@ -1068,17 +1068,19 @@ static hipError_t launch_mfma(const RowsArgs &g, void *workspace, hipStream_t st
     return walks ? launch_long<QC, HI>(g, p, workspace, stream) : launch_tile<QC, HI>(g, g.a.ctx_cap, stream);
 }
 
+// Without the workspace that a shape's fast form needs: the row form.
 hipError_t launch_rows(const RowsArgs &g, void *workspace, hipStream_t stream) {
     const int tasks = g.streams * g.t * g.a.n_head;
     if (tasks <= 0) return hipSuccess;
-    if (rows_decode_ok(g)) {
+    const bool fast = workspace || rows_workspace(g) == 0;
+    if (fast && rows_decode_ok(g)) {
         AttnArgs a = g.a;
         a.keys = g.ctx;
         a.count = g.count;
         a.mass = g.mass;
         return launch_attend_split(a, g.streams, attend_split_plan(g.streams, a.n_head, a.ctx_cap), workspace, stream);
     }
-    if (rows_mfma_ok(g)) {
+    if (fast && rows_mfma_ok(g)) {
         const bool hi = rows_hi(g.a);
         if (g.a.hd <= 64) return hi ? launch_mfma<1, true>(g, workspace, stream) : launch_mfma<1, false>(g, workspace, stream);
         if (g.a.hd <= 128) return hi ? launch_mfma<2, true>(g, workspace, stream) : launch_mfma<2, false>(g, workspace, stream);

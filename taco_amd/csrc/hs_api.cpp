@@ -738,6 +738,26 @@ struct hs_batch {
         span0 = nullptr;
         return hipSuccess;
     }
+    // The attention scratch (`split`) at `need` bytes or more; held: whether the device had the memory.
+    hipError_t hold_scratch(size_t need, bool &held) {
+        held = true;
+        if (need <= split_bytes) return hipSuccess;
+        if (split) {
+            hipError_t e = hipStreamSynchronize(st);
+            if (e == hipSuccess) e = hipFree(split);
+            if (e != hipSuccess) return e;
+            split = nullptr;
+            split_bytes = 0;
+        }
+        if (hipMalloc(&split, need) == hipSuccess) {
+            split_bytes = need;
+        } else {
+            (void)hipGetLastError();
+            split = nullptr;
+            held = false;
+        }
+        return hipSuccess;
+    }
     // After a stream synchronisation: adds the event times of the finished launches.
     hipError_t collect() {
         for (auto &p : pending) {
@@ -1110,12 +1130,13 @@ hs_status run_pass(hs_batch &b, const std::vector<PassRow> &rows, Out out, const
     };
     const bool kv_fused = m.hd % 16 == 0 && m.d % 16 == 0;
     // Decode-shaped passes (short runs) and head dims that the group kernels do not take: attention in
-    // one launch, or split over key chunks, as many rows at a time as 1 GiB of scratch holds; where
-    // the device has no memory for that, the row kernel, which needs none.
+    // one launch, or split over key chunks, as many rows at a time as 1 GiB of scratch holds. Where the
+    // device has no memory for the scratch of these or of a tree, the row kernels, which need none.
     bool split_attn = !tree && !mfma_attn && hs::attend_split_ok(m.hd);
     hs::SplitPlan split_plan;
     int split_rows = n;
     hs::RowsArgs tree_args;  // the attention of a tree pass; a layer's caches and rules below
+    void *tree_space = nullptr;
     if (tree) {
         hs::AttnArgs &a = tree_args.a;
         a.q = b.d_qkv; a.ldq = 3 * m.d; a.kc = b.kc[0]; a.vc = b.vc[0];
@@ -1123,14 +1144,9 @@ hs_status run_pass(hs_batch &b, const std::vector<PassRow> &rows, Out out, const
         tree_args.streams = n_groups; tree_args.t = tree->most; tree_args.groups = b.d_groups;
         tree_args.mask = b.d_mask; tree_args.words = tree->words;
         const size_t need = hs::rows_workspace(tree_args);
-        if (need > b.split_bytes) {
-            HIP_TRY(hipStreamSynchronize(st));
-            if (b.split) HIP_TRY(hipFree(b.split));
-            b.split = nullptr;
-            b.split_bytes = 0;
-            HIP_TRY(hipMalloc(&b.split, need));
-            b.split_bytes = need;
-        }
+        bool held;
+        HIP_TRY(b.hold_scratch(need, held));
+        tree_space = need && held ? b.split : nullptr;
     }
     if (split_attn) {
         int max_keys = 1;
@@ -1147,21 +1163,7 @@ hs_status run_pass(hs_batch &b, const std::vector<PassRow> &rows, Out out, const
             split_rows = std::max<int>(1, (int)((double)n * (1ull << 30) / (double)need));
             need = hs::attend_split_bytes(probe, split_rows, split_plan);
         }
-        if (need > b.split_bytes) {
-            if (b.split) {
-                HIP_TRY(hipStreamSynchronize(st));
-                HIP_TRY(hipFree(b.split));
-                b.split = nullptr;
-                b.split_bytes = 0;
-            }
-            if (hipMalloc(&b.split, need) == hipSuccess) {
-                b.split_bytes = need;
-            } else {
-                (void)hipGetLastError();
-                b.split = nullptr;
-                split_attn = false;
-            }
-        }
+        HIP_TRY(b.hold_scratch(need, split_attn));
     }
     for (int l = 0; l < m.L; l++) {
         const DevBlock &blk = m.blocks[l];
@@ -1194,7 +1196,7 @@ hs_status run_pass(hs_batch &b, const std::vector<PassRow> &rows, Out out, const
             if (tree) {
                 at.rows = nullptr;
                 tree_args.a = at;
-                return hs::launch_rows(tree_args, b.split, st);
+                return hs::launch_rows(tree_args, tree_space, st);
             }
             if (mfma_attn) return hs::launch_attend_groups(at, b.d_groups, n_groups, group_keys, st);
             if (!split_attn) return hs::launch_attend(at, n, st);
