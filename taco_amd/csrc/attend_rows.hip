@@ -50,13 +50,13 @@ __device__ __forceinline__ bool row_sees(const RowsArgs &g, const StreamRows &R,
 
 // Any head dim that is a multiple of 4, any key count and table: one wave per (row, head), three passes over
 // the keys as in k_attend (the row max, the sum of the entries, p and sum p v).
-__global__ __launch_bounds__(256) void k_rows(RowsArgs g, int n_tasks) {
+__global__ __launch_bounds__(256) void k_rows(RowsArgs g, int s0, int n_tasks) {
     __shared__ __attribute__((aligned(16))) int s_q[4][64];
     const AttnArgs &a = g.a;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int task = blockIdx.x * 4 + wave;
     const int row = task < n_tasks ? task / a.n_head : 0, h = task < n_tasks ? task % a.n_head : 0;
-    const int s = row / g.t, i = row - s * g.t, hd = a.hd;
+    const int at = row / g.t, i = row - at * g.t, s = s0 + at, hd = a.hd;  // (s0: the launch's first stream)
     const StreamRows R = stream_rows(g, s);
     const bool live = task < n_tasks && i < R.count;
     if (live && lane < hd / 4) s_q[wave][lane] = ((const int *)(a.q + (size_t)(R.first + i) * a.ldq + h * hd))[lane];
@@ -1020,6 +1020,7 @@ static hipError_t launch_long(const RowsArgs &g, const LongPlan &p, void *scratc
     return launch_long_t<QC, 4, HI>(g, p, scratch, stream);
 }
 
+constexpr int ROWS_TASKS = (1 << 26) - 4;  // of k_rows in a launch, 64 threads each
 constexpr int RT_KEYS = 2048;  // the most keys of a tile in one launch
 
 static bool rows_hi(const AttnArgs &a) { return a.score_s >= 32 && a.score_s <= 60 && a.score_m != INT32_MIN; }
@@ -1070,8 +1071,7 @@ static hipError_t launch_mfma(const RowsArgs &g, void *workspace, hipStream_t st
 
 // Without the workspace that a shape's fast form needs: the row form.
 hipError_t launch_rows(const RowsArgs &g, void *workspace, hipStream_t stream) {
-    const int tasks = g.streams * g.t * g.a.n_head;
-    if (tasks <= 0) return hipSuccess;
+    if (g.streams <= 0 || g.t <= 0 || g.a.n_head <= 0) return hipSuccess;
     const bool fast = workspace || rows_workspace(g) == 0;
     if (fast && rows_decode_ok(g)) {
         AttnArgs a = g.a;
@@ -1086,8 +1086,15 @@ hipError_t launch_rows(const RowsArgs &g, void *workspace, hipStream_t stream) {
         if (g.a.hd <= 128) return hi ? launch_mfma<2, true>(g, workspace, stream) : launch_mfma<2, false>(g, workspace, stream);
         return hi ? launch_mfma<4, true>(g, workspace, stream) : launch_mfma<4, false>(g, workspace, stream);
     }
-    launch_k(k_rows, dim3((tasks + 3) / 4), dim3(256), 0, stream, g, tasks);
-    return hipGetLastError();
+    // as many streams in a launch as a grid holds threads (fewer than 2^32) for: the batch may bring more
+    const int rows = g.t * g.a.n_head, most = ROWS_TASKS / rows < 1 ? 1 : ROWS_TASKS / rows;
+    for (int s0 = 0; s0 < g.streams; s0 += most) {
+        const int tasks = (g.streams - s0 < most ? g.streams - s0 : most) * rows;
+        launch_k(k_rows, dim3((tasks + 3) / 4), dim3(256), 0, stream, g, s0, tasks);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace hs
