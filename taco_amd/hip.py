@@ -319,9 +319,30 @@ class CoderInterval:
 ENCODE, DECODE = 0, 1
 
 
+_U32 = 0xFFFFFFFF
+
+
+def _u32(x) -> np.ndarray:
+    """x as u32. Whole numbers that 32 bits do not hold become 2^32 - 1, which is no slot, token or node (the
+    library refuses it), where a cast would bring them round to one."""
+    a = np.asarray(x)
+    b = np.ascontiguousarray(a, dtype=np.uint32) if a.dtype.kind != "O" else \
+        np.array([int(v) if 0 <= int(v) <= _U32 else _U32 for v in a.ravel()], np.uint32).reshape(a.shape)
+    if a.dtype.kind in "iu" and a.dtype.itemsize > 4 and not np.array_equal(a, b):
+        b = np.where((a < 0) | (a > _U32), _U32, a).astype(np.uint32)
+    return b
+
+
 def _inputs(inputs: Sequence[Tuple[int, int]]) -> np.ndarray:
-    a = np.asarray(inputs, dtype=np.uint32).reshape(-1, 2)
-    return np.ascontiguousarray(a)
+    return _u32(inputs).reshape(-1, 2)
+
+
+def _queries(queries) -> np.ndarray:
+    a = np.asarray(queries)
+    q = _u32(a).reshape(-1, 2)
+    if a.dtype != np.uint32 and a.size and not np.array_equal(a.reshape(-1, 2), q):
+        raise Unsupported(HS_UNSUPPORTED, 0, "a query that 32 bits do not hold")
+    return q
 
 
 class HipBatch:
@@ -366,7 +387,7 @@ class HipBatch:
     def run_coded_raw(self, inputs, queries, freq_bits: int = 32) -> np.ndarray:
         """The intervals as an [n, 3] u64 array (symbol, start, freq)."""
         a = _inputs(inputs)
-        q = np.ascontiguousarray(np.asarray(queries, dtype=np.uint32).reshape(-1, 2))
+        q = _queries(queries)
         if len(q) != len(a):
             raise LengthMismatch(HS_LENGTH_MISMATCH, 0,
                                  f"length mismatch: expected {len(a)}, found {len(q)}")
@@ -382,7 +403,7 @@ class HipBatch:
         """CudaBatch::run_coded_mixed: tables[i] is HS_MIX_PLAIN, HS_MIX_NONE or the predicted
         token; mixer(i, stats) -> q. The intervals as an [n, 3] u64 array."""
         a = _inputs(inputs)
-        q = np.ascontiguousarray(np.asarray(queries, dtype=np.uint32).reshape(-1, 2))
+        q = _queries(queries)
         t = np.ascontiguousarray(np.asarray(tables, dtype=np.uint32))
         out = np.zeros((len(a), 3), np.uint64)
         cb = _mixer(mixer)
@@ -422,7 +443,7 @@ class HipBatch:
         """The intervals of every node's query as an [n, 3] u64 array (hs_batch_run_tree_coded)."""
         a = _inputs(inputs)
         p = self._parents(parents, len(a))
-        q = np.ascontiguousarray(np.asarray(queries, dtype=np.uint32).reshape(-1, 2))
+        q = _queries(queries)
         if len(q) != len(a):
             raise LengthMismatch(HS_LENGTH_MISMATCH, 0, f"length mismatch: expected {len(a)}, found {len(q)}")
         out = np.zeros((len(a), 3), np.uint64)
@@ -432,9 +453,9 @@ class HipBatch:
     def commit_paths(self, paths) -> None:
         """Accepts a path of the last tree of each slot: {slot: node numbers in the slot's tree, from a child
         of the root down} (hs_batch_commit_paths)."""
-        slots = np.array(list(paths), np.uint32)
+        slots = _u32(list(paths))
         lengths = np.array([len(p) for p in paths.values()], np.uint32)
-        flat = np.array([int(x) for p in paths.values() for x in p], np.uint32)
+        flat = _u32([int(x) for p in paths.values() for x in p])
         _check(lib().hs_batch_commit_paths(self.h, _ptr(slots), _ptr(lengths), _ptr(flat), len(slots)))
 
     def step(self, inputs):
@@ -678,7 +699,7 @@ def mixed_intervals_of_weights(dev: HipDevice, weights: np.ndarray, queries, pre
     predicted, top) and the intervals [rows, 3] of the mixed tables of given weights."""
     w = np.ascontiguousarray(weights, dtype=np.uint64)
     rows, vocab = w.shape
-    q = np.ascontiguousarray(np.asarray(queries, dtype=np.uint32).reshape(-1, 2))
+    q = _queries(queries)
     pr = np.ascontiguousarray(np.asarray(predictions, dtype=np.uint32))
     stats = (MixStats * rows)()
     out = np.zeros((rows, 3), np.uint64)
@@ -696,7 +717,7 @@ def mixed_coder_logits(dev: HipDevice, logits: np.ndarray, table: np.ndarray, qu
     logits = np.ascontiguousarray(logits, dtype=np.int64)
     table = np.ascontiguousarray(table, dtype=np.uint64)
     rows, vocab = logits.shape
-    q = np.ascontiguousarray(np.asarray(queries, dtype=np.uint32).reshape(-1, 2))
+    q = _queries(queries)
     t = np.ascontiguousarray(np.asarray(tables, dtype=np.uint32))
     stats = (MixStats * rows)()
     out = np.zeros((rows, 3), np.uint64)
@@ -713,7 +734,7 @@ def coder(dev: HipDevice, logits: np.ndarray, table: np.ndarray, queries, freq_b
     """The coder op on given i64 logits [rows, vocab]: (symbol, start, freq) per row."""
     logits = np.ascontiguousarray(logits, dtype=np.int64)
     table = np.ascontiguousarray(table, dtype=np.uint64)
-    q = np.ascontiguousarray(np.asarray(queries, dtype=np.uint32).reshape(-1, 2))
+    q = _queries(queries)
     rows, vocab = logits.shape
     out = np.zeros((rows, 3), np.uint64)
     _check(lib().hs_op_coder(dev.h, _ptr(logits), rows, vocab, _ptr(table), len(table), _ptr(q),
