@@ -576,10 +576,7 @@ def _dptrs(xs):
     return (C.c_void_p * len(xs))(*[_dptr(x) for x in xs])
 
 
-class AttentionRule(NamedTuple):
-    """The integer rule of an attention layer: score = clamp(rescale(q . k, score_m, score_s), +-2^40),
-    weights of softmax_p bits over the device table attn_exp of `length` i32 entries, outputs rescaled
-    by (out_m, out_s)."""
+class _Rule(NamedTuple):
     score_m: int
     score_s: int
     out_m: int
@@ -587,6 +584,23 @@ class AttentionRule(NamedTuple):
     attn_exp: object
     length: int
     softmax_p: int
+
+
+class AttentionRule(_Rule):
+    """The integer rule of an attention layer: score = clamp(rescale(q . k, score_m, score_s), +-2^40),
+    weights of softmax_p bits over the device table attn_exp of `length` i32 entries, outputs rescaled
+    by (out_m, out_s). Multipliers are 32 bits, shifts and softmax_p 8 (checked here, where a call would cut them)."""
+    __slots__ = ()
+
+    def __new__(cls, score_m, score_s, out_m, out_s, attn_exp, length, softmax_p):
+        if not all(-2 ** 31 <= m < 2 ** 31 for m in (score_m, out_m)) or \
+                not all(0 <= x < 256 for x in (score_s, out_s, softmax_p)) or not 0 <= length < 2 ** 64:
+            raise Unsupported(HS_UNSUPPORTED, 0, "a rule whose multipliers (i32), shifts (u8) or table do not fit")
+        return super().__new__(cls, score_m, score_s, out_m, out_s, attn_exp, length, softmax_p)
+
+    @classmethod
+    def _make(cls, fields):
+        return cls(*fields)
 
 
 def attend_tree(dev: HipDevice, q, k_cache, v_cache, ctx, nodes, mask, dims, rule: AttentionRule, out,

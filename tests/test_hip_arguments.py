@@ -67,3 +67,14 @@ def test_one_layer_whose_stride_says_nothing():
         assert list(hip._dptrs(OnGpu(one))) == [whole.data_ptr()]
     assert list(hip._dptrs(OnGpu(whole))) == [whole.data_ptr(), whole.data_ptr() + 60]
     assert len(hip._dptrs(OnGpu(whole[:0]))) == 0
+
+
+def test_rules_that_a_call_would_cut():
+    rule = hip.AttentionRule(-2 ** 31, 255, 2 ** 31 - 1, 0, 4096, 100, 30)
+    assert rule == (-2 ** 31, 255, 2 ** 31 - 1, 0, 4096, 100, 30) and rule._replace(softmax_p=31).softmax_p == 31
+    for change in ({"score_m": 2 ** 31}, {"out_m": -2 ** 31 - 1}, {"score_s": 256}, {"score_s": -1}, {"out_s": 292},
+                   {"softmax_p": 286}, {"length": -1}, {"length": 2 ** 64}):
+        with pytest.raises(hip.Unsupported):
+            rule._replace(**change)
+        with pytest.raises(hip.Unsupported):
+            hip.AttentionRule(**{**rule._asdict(), **change})
