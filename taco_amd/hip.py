@@ -425,10 +425,15 @@ class HipBatch:
         return plain, mixed
 
     def _parents(self, parents, n: int) -> np.ndarray:
-        p = np.asarray(parents, dtype=np.int64)
+        """The parents for the library: -1 and HS_TREE_ROOT are the root, any other number that is no input of the call
+        becomes n, which is none either (the library refuses it)."""
+        p = np.asarray(parents)
         if len(p) != n:
             raise LengthMismatch(HS_LENGTH_MISMATCH, 0, f"length mismatch: expected {n}, found {len(p)}")
-        return np.where(p < 0, HS_TREE_ROOT, np.minimum(p, n)).astype(np.uint32)  # (n and more are no input: refused)
+        if p.dtype.kind not in "iuO":
+            p = p.astype(np.int64)
+        root = (p == -1) | (p == HS_TREE_ROOT)
+        return np.where(root, HS_TREE_ROOT, np.where((p < 0) | (p > n), n, p)).astype(np.uint32)
 
     def run_tree_weights(self, inputs, parents) -> np.ndarray:
         """The weights of every node of the slots' trees of drafts (hs_batch_run_tree_weights):

@@ -78,3 +78,13 @@ def test_rules_that_a_call_would_cut():
             rule._replace(**change)
         with pytest.raises(hip.Unsupported):
             hip.AttentionRule(**{**rule._asdict(), **change})
+
+
+@pytest.mark.parametrize("parents,want", [([-1, 0, 1], [LAST, 0, 1]), ([hip.HS_TREE_ROOT, -1, 2], [LAST, LAST, 2]),
+                                          ([-2, -2 ** 63, -1], [3, 3, LAST]), ([2 ** 63, 2 ** 80, -2 ** 80], [3, 3, 3]),
+                                          (np.array([2 ** 64 - 1, 2 ** 63, 1], np.uint64), [3, 3, 1]),
+                                          (np.array([LAST, 1, 3], np.uint32), [LAST, 1, 3])])
+def test_parents_that_are_none(parents, want):
+    """Only -1 and HS_TREE_ROOT are the root; what is neither that nor an input stays none."""
+    got = hip.HipBatch._parents(None, parents, 3)
+    assert got.dtype == np.uint32 and got.tolist() == want
