@@ -375,7 +375,9 @@ fn parents_of(parents: &[Option<u32>], n: usize) -> Result<Vec<u32>> {
     if parents.len() != n {
         return Err(Error::LengthMismatch { expected: n, found: parents.len() });
     }
-    Ok(parents.iter().map(|p| p.unwrap_or(HS_TREE_ROOT)).collect())
+    // An index that is no input's becomes n (or the largest index), which the library refuses: u32::MAX is the root.
+    let none = u32::try_from(n).unwrap_or(HS_TREE_ROOT - 1);
+    Ok(parents.iter().map(|p| p.map_or(HS_TREE_ROOT, |i| i.min(none))).collect())
 }
 
 fn queries_of(queries: &[CoderQuery]) -> Result<Vec<ffi::hs_query>> {
