@@ -8,7 +8,6 @@ every call fails loudly if libhardshell_hip.so is missing."""
 from __future__ import annotations
 
 import ctypes as C
-import math
 import os
 from dataclasses import dataclass
 from typing import Iterable, List, NamedTuple, Optional, Sequence, Tuple
@@ -576,7 +575,7 @@ def _dptrs(xs):
     whose first axis is the layers."""
     if hasattr(xs, "data_ptr"):
         n, at = xs.shape[0], _dptr(xs)
-        step = math.prod(xs.shape[1:]) * xs.element_size()  # (the stride of an axis of one may be anything)
+        step = xs.stride(0) * xs.element_size() if n != 1 else 1  # (the stride of an axis of one may be anything)
         return (C.c_void_p * n)(*range(at, at + n * step, step)) if step else (C.c_void_p * 0)()
     return (C.c_void_p * len(xs))(*[_dptr(x) for x in xs])
 
