@@ -597,10 +597,10 @@ class AttentionRule(_Rule):
     __slots__ = ()
 
     def __new__(cls, score_m, score_s, out_m, out_s, attn_exp, length, softmax_p):
-        if not all(-2 ** 31 <= m < 2 ** 31 for m in (score_m, out_m)) or \
-                not all(0 <= x < 256 for x in (score_s, out_s, softmax_p)) or not 0 <= length < 2 ** 64:
+        if not (-2 ** 31 <= score_m < 2 ** 31 and -2 ** 31 <= out_m < 2 ** 31 and 0 <= score_s < 256 and
+                0 <= out_s < 256 and 0 <= softmax_p < 256 and 0 <= length < 2 ** 64):
             raise Unsupported(HS_UNSUPPORTED, 0, "a rule whose multipliers (i32), shifts (u8) or table do not fit")
-        return super().__new__(cls, score_m, score_s, out_m, out_s, attn_exp, length, softmax_p)
+        return tuple.__new__(cls, (score_m, score_s, out_m, out_s, attn_exp, length, softmax_p))
 
     @classmethod
     def _make(cls, fields):
