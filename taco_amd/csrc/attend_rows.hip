@@ -49,7 +49,9 @@ __device__ __forceinline__ bool row_sees(const RowsArgs &g, const StreamRows &R,
 }
 
 // Any head dim that is a multiple of 4, any key count and table: one wave per (row, head), three passes over
-// the keys as in k_attend (the row max, the sum of the entries, p and sum p v).
+// the keys as in k_attend (the row max, the sum of the entries, p and sum p v). It is for what the other forms
+// do not take, not for speed: each row walks K and V again, and a key's weight goes through a lane move to all lanes. 768
+// panels of 16 rows at 500 to 1,000 keys: head_dim 20 625 us, 60 927 (64 in tiles 21.6); 12 panels of 8 rows at 100 keys 25.
 __global__ __launch_bounds__(256) void k_rows(RowsArgs g, int s0, int n_tasks) {
     __shared__ __attribute__((aligned(16))) int s_q[4][64];
     const AttnArgs &a = g.a;
@@ -117,10 +119,14 @@ __global__ __launch_bounds__(256) void k_rows(RowsArgs g, int s0, int n_tasks) {
 // digits, four products with V^T by transposing LDS reads; here the waves share the keys of the same rows, so the
 // extremes and the sums meet in LDS, and the output sums in 64-bit LDS atomics (integers: any order).
 // QC: 64-byte chunks of a head (the last one may be part empty: its lanes hold zeros).
-// 768 panels of 16 rows at 750 keys (76 MB): 21.3 us, 3.6 TB/s; 12 panels 6.3 us at 100 keys. Few panels are bound by
+// 768 panels of 16 rows at 750 keys (76 MB): 21.6 us, 3.5 TB/s; 12 panels 6.4 us at 100 keys. Few panels are bound by
 // the chain of one workgroup (loads, two exchanges between the waves, products), many by HBM and, from three tiles a
-// panel on, by the VALU work of the scores (about 24 instructions each with a wave's fixed part): causal chunks of
-// 256 rows, 192 panels, 52 us, 27 of them VALU issue.
+// panel on, by VALU issue. Counted at 512 and 1,024 keys: a block takes 272 VALU instructions, 17 a score; a wave's
+// fixed part 380 (320 where it has no block), which eight waves a tile pay for one or two blocks each. Causal chunks of up
+// to 256 rows, 192 panels: 52 us, of them 27 of VALU issue: 16.9 M instructions, 7.4 M for 27,200 blocks and the rest,
+// some 480 a wave with the masks, fixed. More rows a workgroup would share that part; it is not tried.
+// 65 to 128 channels: 128 panels of 23 rows at 1,500 keys (50 MB) 23.3 us; 129 to 256: 128 panels of 16 rows at 750 keys (51 MB)
+// 21.4. There the loads of a channel group leave only under the products of the one before.
 constexpr int RT_ROWS = 16;
 constexpr int RT_TABLE = 16384;  // entries of the table copied to LDS at most
 constexpr int RT_ACC = 66;       // 64 channels' sums of a row and two of padding (bank spread)
@@ -573,10 +579,15 @@ static hipError_t launch_tile(const RowsArgs &g, int keys, hipStream_t stream) {
 //   k_long_pv the products with V: WT tiles side by side, 4 / WT waves to a tile, since a tile's sums are 64
 //     registers for 64 channels (the others' loads of the same rows hit the L1).
 // ALONE: k_long_pv walks all three times itself, where the rows alone give enough workgroups. A head dim above
-// 128 takes a workgroup for each 64 channels (cg). 200 panels of 64 rows at 6,100 keys, head_dim 64: 20 + 34 + 88 + 7 us
-// in the kernel trace. What bounds the products' launch: per score 4 instructions to the table index, the lookup
-// (LDS: 21 us in all, half of it bank conflicts), 6 for p and 3 for its digits (VALU: 32 us), 20 MFMAs a block (10
-// us), in chains that three waves a SIMD overlap in part; K and V come a block ahead.
+// 128 takes a workgroup for each 64 channels (cg). 200 panels of 64 rows at 6,100 keys, head_dim 64: 139 us a call, by the
+// kernel trace (which keeps the launches apart: 146 us) 14, 23, 58 and 5% of it. What the products' launch issues:
+// per score 4 instructions to the table index, the lookup (LDS: 21 us in all, half of it bank conflicts), 6 for p and
+// 3 for its digits (VALU: 32 us), 20 MFMAs a block (10 us), in chains that three waves a SIMD (160 VGPRs) overlap in part; K
+// and V come a block ahead. A group's tile without rows leaves its wave idle: no limit, but not tried otherwise.
+// Other shapes, a call: chunks of 256 causal rows with weights, 192 panels of 4,096 keys 203 us, 48 of 8,192 127;
+// trees of 16 rows, 12 panels of 8,000 keys 38; of 64 rows and head_dim 256, 64 panels of 6,100 keys 374 (there the scans of
+// four tiles spill: 2 registers in the first, 24 in the second, 37 at score shifts outside 32 to
+// 60).
 struct LongPlan {
     int tiles = 0, wt = 1, groups = 1;  // row tiles; of a group; groups
     int ng = 1, span = 0, cg = 1;        // key ranges, their keys; workgroups for the channels
@@ -977,8 +988,15 @@ static LongPlan long_plan(const RowsArgs &g, int keys) {
     p.groups = (p.tiles + p.wt - 1) / p.wt;
     p.cg = g.a.hd > 128 ? (g.a.hd + 63) / 64 : 1;
     // Ranges for about four workgroups a CU, at least two blocks a wave: three are resident, and where the caches are
-    // about three quarters full (their ends' workgroups end at once) the rest is one round. 200 panels of 64 rows over up
-    // to 8,192 keys: 4 ranges 154 us a call, 5 (this rule) 130, 6 141, 8 147, 16 218.
+    // partly empty (their ends' workgroups end at once) the rest is one round. Workgroups in all, 256, 512, 1,024 (this
+    // rule), 2,048, 4,096, in us a call; caches of 8,192 places, all full, 6,100 and 3,000 keys in the mean:
+    //   8 x 64 rows, 25 heads of 64      262 163 152 163 262   244 157 137 153 224   111 136  92  95 119
+    //   16 x 64 rows, 25 heads of 64     321 321 284 258 284   301 301 273 219 258   148 148 212 135 152
+    //   4 x 64 rows, 12 heads of 64       65  61  79  79  79    64  59  71  72  71    62  56  58  58  58
+    //   32 x 16 rows, 12 heads of 64     120 120 143 152 161   106 106 117 122 135    54  54  75  70  76
+    //   16 x 64 rows, 25 heads of 128    852 853 547 533 587   814 815 531 451 552   391 390 404 265 304
+    //   8 x 64 rows, 25 heads of 256   2,668 1,369 1,164 1,246 1,480                  (full)
+    // The best of them differs with the panels; this one is within 1.6 of it everywhere here, and 256 up to 2.3.
     constexpr long long LONG_WGS = 1024;
     const long long wgs = (long long)g.streams * g.a.n_head * p.groups;
     const int unit = 256, most = (keys + 2 * unit - 1) / (2 * unit);
@@ -1038,9 +1056,16 @@ static bool rows_mfma_ok(const RowsArgs &g) {
 }
 
 // One causal row a stream: the decode kernels, which add up the weights too, where one launch of them serves (768
-// row-heads of 1,024 keys 17.4 us, a tile each 36), and their split form for many row-heads over more keys than a tile
-// holds (768 row-heads of 8,000 keys 187 us, three walks 240; 192: 73 and 72). Else the forms for 16 rows: 12
-// row-heads of 2,000 keys 13.9 us, split 36; 768 of them 52 and 61; 12 of 8,000 keys 35 and 79.
+// row-heads of 1,024 keys 16.9 us, a tile each 36), and their split form for many row-heads over more keys than a tile
+// holds. Else the forms for 16 rows: 12 row-heads of 2,000 keys 13.9 us, split 36; 768 of them 52 and 61; 12 of 8,000
+// keys 27 (10 MB: 2.2 us; its four launches in a chain) and 79. Split form and walks at 192, 384, 516, 768 and 1,536 row-heads,
+// all caches full:
+//   head_dim 64,  2,100 keys    38 39    43 52    52 54    72 68   123 131
+//   head_dim 64,  8,000 keys    83 90   123 148  160 227  226 313  441 621   (4,000 to 8,000: 190 and 241 at 768)
+//   head_dim 32,  8,000 keys    58 63    91 88   113 116  146 145  282 278
+//   head_dim 128, 8,000 keys   120 162  209 346  288 524  431 667  847 1,173
+//   head_dim 256, 8,000 keys   237 454  443 831  623 1,849  846 2,470  1,692 4,999
+// Above 64 channels the split form would win from fewer row-heads on than the 512 of this rule.
 static bool rows_decode_ok(const RowsArgs &g) {
     const AttnArgs &a = g.a;
     const uintptr_t bits = (uintptr_t)a.q | (uintptr_t)a.kc | (uintptr_t)a.vc;

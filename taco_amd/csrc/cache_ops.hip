@@ -78,6 +78,9 @@ hipError_t launch_commit(const CachePtrs &c, int layers, const CommitArgs &a, hi
 // keys, so only what must move moves: a kept key below `heavy` stays where it is, and the a-th free place below it
 // takes the a-th kept key from above; the recent rows follow in order. Sources of the first kind lie at or above
 // `heavy` and places below, so these copies need no order; the recent rows move down tile by tile after them.
+// (k_evict: caches of more than 16,384 places. It walks the masses up to eight times for the selection and twice
+// after it, 256 threads a panel: 256 panels of 32,768 places to 8,192 keys 635 us (531 MB: 111 at the rate of a copy), of
+// 65,536 to 16,384 1,294; 12 panels 400 and 830.)
 
 constexpr int EV_NT = 256;
 
@@ -250,6 +253,10 @@ __global__ __launch_bounds__(EV_NT) void k_evict(CachePtrs c, EvictArgs a) {
 // (1,040 bins in the order of the values): accumulated weights spread over orders of magnitude, so a bin
 // holds few of them, where the leading byte would hold almost all; then eight bits at a time among
 // that bin's keys, until the rest of a bin stays whole.
+// Copies of the kernel without a part: 9,216 panels of 1,024 places to 768 keys 107 us (375 MB), 27 without the copies of
+// rows and masses, 35 with the masses alone; 256 panels of 16,384 to 4,096 103 us (274 MB), 24 and 31. So the rows' copies
+// (half lines of 64 bytes) take 70% and start after the selection: one workgroup fills a CU at 16,384 places, and nothing
+// moves rows while it selects. That is no limit: the recent rows could be in flight by then.
 constexpr int EV_BINS = 1040;
 
 __device__ __forceinline__ int mass_bin(uint64_t x) {

@@ -1885,8 +1885,9 @@ __device__ __forceinline__ int mass_row(const AttnArgs &a, int r) {
 
 // The accumulator of key j gains p. An atomic addition, as in the forms of several rows: a call on another stream may
 // add to the same accumulators at the same time. (Loading them beside V and storing the sums lost such
-// additions, and was no faster: 768 row-heads of 1,024 keys 18.0 us at head_dim 64 and 42.4 at 128, this way 17.0 and 39.4;
-// head_dim 32 11.3 and 12.0, 8,000 keys 185 and 187.)
+// additions, and was no faster on the whole: 768 row-heads of 1,024 keys 18.0 us at head_dim 64 and 42.4 at 128, this way
+// 17.0 and 39.4; head_dim 32 11.2 and 11.9, 16 8.9 and 10.0; 1,600 row-heads at head_dim 32 20.4 and 19.2; 8,000 keys 185
+// and 187.)
 __device__ __forceinline__ void add_mass(const AttnArgs &a, int rh, int j, uint64_t p) {
     atomicAdd((unsigned long long *)a.mass + (size_t)rh * a.ctx_cap + j, (unsigned long long)p);
 }
