@@ -900,7 +900,7 @@ def main_traffic(argv):
     dims_name, W, n, _ = FOLDS[workload]
     tokens_sha = synth.sha256_tokens(synth.zipf_tokens(W * n))
     cmd = (f"rocprofv3 --pmc FETCH_SIZE (then WRITE_SIZE) --output-format csv -- python3 bench.py "
-           f"--workload {workload} --steps 1 --warmup 0 --no-cpu --batches 1 --calib-copy-mib {calib}")
+           f"--workload {workload} --steps 1 --warmup 0 --no-cpu --no-unfold --sustain-s 0 --batches 1 --calib-copy-mib {calib}")
     print(json.dumps(traffic_summary(fetch_csv, write_csv, int(calib), tokens_sha, cmd), indent=1))
 
 
