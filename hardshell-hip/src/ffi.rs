@@ -33,6 +33,21 @@ pub struct hs_input {
     pub token: u32,
 }
 
+/// One layer's pool of pages of a paged cache.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct hs_pages {
+    pub k: *mut i8,
+    pub v: *mut i8,
+    pub k_scale: *mut u32,
+    pub v_scale: *mut u32,
+    pub pages: u32,
+    pub kv_heads: u32,
+    pub page: u32,
+    pub head_dim: u32,
+    pub max_scale: u32,
+}
+
 /// A coder query: `kind` 0 is Encode(token = value), 1 is Decode(target = value).
 #[repr(C)]
 #[derive(Clone, Copy, Debug, Default)]
@@ -69,6 +84,8 @@ pub const HS_MIX_NONE: u32 = 0xFFFF_FFFF;
 pub const HS_MIX_PLAIN: u32 = 0xFFFF_FFFE;
 /// The parent of a tree's node right after the context.
 pub const HS_TREE_ROOT: u32 = 0xFFFF_FFFF;
+/// No token to score.
+pub const HS_NO_TOKEN: u32 = 0xFFFF_FFFF;
 
 /// The values of `hs_status`.
 #[repr(i32)]
@@ -168,6 +185,31 @@ unsafe extern "C" {
         n: usize,
         freq_bits: u32,
         out: *mut hs_interval,
+    ) -> c_int;
+    pub fn hs_batch_run_scored(
+        batch: *mut hs_batch,
+        inputs: *const hs_input,
+        tokens: *const u32,
+        n: usize,
+        top: usize,
+        logprob: *mut f32,
+        rank: *mut u32,
+        entropy: *mut f32,
+        top_tokens: *mut u32,
+        top_logprob: *mut f32,
+    ) -> c_int;
+    pub fn hs_batch_run_tree_scored(
+        batch: *mut hs_batch,
+        inputs: *const hs_input,
+        parents: *const u32,
+        tokens: *const u32,
+        n: usize,
+        top: usize,
+        logprob: *mut f32,
+        rank: *mut u32,
+        entropy: *mut f32,
+        top_tokens: *mut u32,
+        top_logprob: *mut f32,
     ) -> c_int;
     pub fn hs_batch_commit_paths(
         batch: *mut hs_batch,
@@ -405,6 +447,74 @@ unsafe extern "C" {
         hd: usize,
         ctx_cap: usize,
         ctx_out: *mut u32,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn hs_op_pages_append_dev(
+        dev: *mut hs_device,
+        cache: *const hs_pages,
+        k: *const c_void,
+        v: *const c_void,
+        bits: u32,
+        stride: usize,
+        table: *const u32,
+        ctx: *const u32,
+        rows: *const u32,
+        b: usize,
+        t: usize,
+        width: usize,
+        headroom: u32,
+        ctx_out: *mut u32,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn hs_op_attend_paged_dev(
+        dev: *mut hs_device,
+        cache: *const hs_pages,
+        q: *const i8,
+        q_stride: usize,
+        table: *const u32,
+        ctx: *const u32,
+        rows: *const u32,
+        b: usize,
+        t: usize,
+        h: usize,
+        width: usize,
+        keys: usize,
+        score_m: i32,
+        score_s: u8,
+        out_m: i32,
+        out_s: u8,
+        attn_exp: *const i32,
+        len: usize,
+        softmax_p: u8,
+        out: *mut i8,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn hs_op_attend_paged_workspace(
+        b: usize,
+        t: usize,
+        h: usize,
+        kv_heads: usize,
+        hd: usize,
+        keys: usize,
+    ) -> usize;
+    pub fn hs_op_score_dev(
+        dev: *mut hs_device,
+        logits: *const c_void,
+        bits: u32,
+        ld: usize,
+        tokens: *const u32,
+        table: *const u64,
+        len: usize,
+        rows: usize,
+        vocab: usize,
+        top: usize,
+        logprob: *mut f32,
+        rank: *mut u32,
+        entropy: *mut f32,
+        top_tokens: *mut u32,
+        top_logprob: *mut f32,
         stream: *mut c_void,
     ) -> c_int;
     pub fn hs_op_coder(

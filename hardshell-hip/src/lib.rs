@@ -22,7 +22,7 @@ use std::ffi::CStr;
 use hardshell::gpt2::Overlap;
 use hardshell::{ModelHash, TokenId};
 
-pub use ffi::{HS_MIX_NONE, HS_MIX_PLAIN, HS_TREE_ROOT};
+pub use ffi::{HS_MIX_NONE, HS_MIX_PLAIN, HS_NO_TOKEN, HS_TREE_ROOT};
 
 /// A result with the error of this crate.
 pub type Result<T> = std::result::Result<T, Error>;
@@ -371,6 +371,44 @@ fn inputs_of(inputs: &[(usize, TokenId)], slots: usize) -> Result<Vec<ffi::hs_in
         .collect()
 }
 
+/// What [`HipBatch::run_scored`] gives: an entry an input, `top` alternatives an input.
+#[derive(Clone, Debug, Default)]
+pub struct Scores {
+    /// ln of the token's share of the weights (0 without a token).
+    pub logprob: Vec<f32>,
+    /// How many symbols come before the token (`HS_NO_TOKEN` without one).
+    pub rank: Vec<u32>,
+    /// The entropy in nats.
+    pub entropy: Vec<f32>,
+    /// The first alternatives of each input, and their log probabilities.
+    pub top_tokens: Vec<u32>,
+    /// As `top_tokens`.
+    pub top_logprob: Vec<f32>,
+}
+
+impl Scores {
+    fn new(n: usize, top: usize) -> Result<Self> {
+        if top > 64 {
+            return Err(Error::Unsupported { reason: "top is at most 64".to_owned() });
+        }
+        Ok(Self {
+            logprob: vec![0.0; n],
+            rank: vec![0; n],
+            entropy: vec![0.0; n],
+            top_tokens: vec![0; n * top],
+            top_logprob: vec![0.0; n * top],
+        })
+    }
+}
+
+/// The tokens of a scored call as words (`None` is `HS_NO_TOKEN`; the library refuses what is not in the vocabulary).
+fn scored_of(tokens: &[Option<u32>], n: usize) -> Result<Vec<u32>> {
+    if tokens.len() != n {
+        return Err(Error::LengthMismatch { expected: n, found: tokens.len() });
+    }
+    Ok(tokens.iter().map(|t| t.map_or(HS_NO_TOKEN, |t| t.min(HS_NO_TOKEN - 1))).collect())
+}
+
 fn parents_of(parents: &[Option<u32>], n: usize) -> Result<Vec<u32>> {
     if parents.len() != n {
         return Err(Error::LengthMismatch { expected: n, found: parents.len() });
@@ -604,6 +642,66 @@ impl<'m> HipBatch<'m> {
             )
         })?;
         Ok(self.intervals(&out))
+    }
+
+    /// Runs the inputs and scores what follows each: the log probability and the rank of `tokens[i]`
+    /// (`None`: no token), the entropy, and the first `top` alternatives. No counterpart in the
+    /// reference, whose callers get whole rows of weights.
+    ///
+    /// # Errors
+    /// [`Error::LengthMismatch`] if the tokens do not match the inputs; [`Error::Unsupported`] for a token
+    /// outside the vocabulary or more than 64 alternatives; as [`HipBatch::run_weights`] otherwise.
+    pub fn run_scored(&mut self, inputs: &[(usize, TokenId)], tokens: &[Option<u32>], top: usize) -> Result<Scores> {
+        let ins = inputs_of(inputs, self.slots)?;
+        let (ts, mut out) = (scored_of(tokens, inputs.len())?, Scores::new(inputs.len(), top)?);
+        // SAFETY: the arrays hold n entries, those of the alternatives n * top.
+        check("hs_batch_run_scored", unsafe {
+            ffi::hs_batch_run_scored(
+                self.raw,
+                ins.as_ptr(),
+                ts.as_ptr(),
+                ins.len(),
+                top,
+                out.logprob.as_mut_ptr(),
+                out.rank.as_mut_ptr(),
+                out.entropy.as_mut_ptr(),
+                out.top_tokens.as_mut_ptr(),
+                out.top_logprob.as_mut_ptr(),
+            )
+        })?;
+        Ok(out)
+    }
+
+    /// The scores of every node of the slots' trees of drafts, as [`HipBatch::run_tree_weights`].
+    ///
+    /// # Errors
+    /// As [`HipBatch::run_tree_weights`] and [`HipBatch::run_scored`].
+    pub fn run_tree_scored(
+        &mut self,
+        inputs: &[(usize, TokenId)],
+        parents: &[Option<u32>],
+        tokens: &[Option<u32>],
+        top: usize,
+    ) -> Result<Scores> {
+        let (ins, ps) = (inputs_of(inputs, self.slots)?, parents_of(parents, inputs.len())?);
+        let (ts, mut out) = (scored_of(tokens, inputs.len())?, Scores::new(inputs.len(), top)?);
+        // SAFETY: the arrays hold n entries, those of the alternatives n * top.
+        check("hs_batch_run_tree_scored", unsafe {
+            ffi::hs_batch_run_tree_scored(
+                self.raw,
+                ins.as_ptr(),
+                ps.as_ptr(),
+                ts.as_ptr(),
+                ins.len(),
+                top,
+                out.logprob.as_mut_ptr(),
+                out.rank.as_mut_ptr(),
+                out.entropy.as_mut_ptr(),
+                out.top_tokens.as_mut_ptr(),
+                out.top_logprob.as_mut_ptr(),
+            )
+        })?;
+        Ok(out)
     }
 
     /// Accepts a path of the last tree of each listed slot: its node numbers, from a child of the root

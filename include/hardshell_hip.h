@@ -204,6 +204,25 @@ hs_status hs_batch_run_tree_coded(hs_batch *batch, const hs_input *inputs, const
 hs_status hs_batch_commit_paths(hs_batch *batch, const uint32_t *slots, const uint32_t *lengths,
                                 const uint32_t *paths, size_t n);
 
+/* ---- Scores: no counterpart in the reference, whose callers get whole rows of weights ------- */
+/* Runs the inputs as hs_batch_run_weights (hs_batch_run_tree_weights) does, and gives for each, of the
+ * weights w of what follows it with their sum T: logprob[i] = ln(w[tokens[i]] / T) (-logprob / ln 2
+ * bits is what coding the token costs) and rank[i], how many symbols come before the token (0: it is the
+ * first) in the order of their distance from the largest logit, min(max - l, len - 1) steps of the
+ * logits table, then of their numbers; entropy[i] = sum (w / T) ln(T / w); and the first `top` symbols of that
+ * order, top_tokens[i][..], with their log probabilities top_logprob[i][..] (drafts for a tree, say). tokens may
+ * hold HS_NO_TOKEN (log probability 0, rank HS_NO_TOKEN), and may be NULL where logprob and rank are; every
+ * result may be NULL. top is at most 64 and at most the vocabulary. Logarithms are within 2 units in the last
+ * place of 32 bits; all else is exact. */
+#define HS_NO_TOKEN 0xFFFFFFFFu
+hs_status hs_batch_run_scored(hs_batch *batch, const hs_input *inputs, const uint32_t *tokens,
+                              size_t n, size_t top, float *logprob, uint32_t *rank, float *entropy,
+                              uint32_t *top_tokens, float *top_logprob);
+hs_status hs_batch_run_tree_scored(hs_batch *batch, const hs_input *inputs, const uint32_t *parents,
+                                   const uint32_t *tokens, size_t n, size_t top, float *logprob,
+                                   uint32_t *rank, float *entropy, uint32_t *top_tokens,
+                                   float *top_logprob);
+
 /* ---- The mixed coder op of the logs profile: crates/hardshell-cuda/src/batch/mixed.rs:23-126,
  * src/mixed.rs:24-233 (ADR 0010 section 3) ---------------------------------------------------
  * The GPU gives the statistics of each row's GPT-2 weights w; the host mixer gives q; the GPU
@@ -382,6 +401,67 @@ hs_status hs_op_cache_commit_dev(hs_device *dev, int8_t *const *k_caches, int8_t
                                  size_t layers, const uint32_t *ctx, const uint32_t *path,
                                  const uint32_t *accepted, size_t b, size_t t, size_t h, size_t hd,
                                  size_t ctx_cap, uint32_t *ctx_out, void *stream);
+
+/* ---- Paged caches: keys and values in pages of a pool that streams share, 8 bits a value with a
+ * scale for each page and head. No counterpart in the reference, whose caches are one panel a slot
+ * with one scale a layer. ------------------------------------------------------------------- */
+
+/* One layer's pool. A value is its byte times the scale of its page and head. Page n of head h lies
+ * at [n][h] of k and v [pages][kv_heads][page][head_dim] and k_scale and v_scale [pages][kv_heads].
+ * head_dim is a multiple of 16 up to 256, page (the tokens of a page) a power of two from 16 to 1,024, and
+ * scales are 1 ..= max_scale <= 1,024 (others count as the nearest of these). 16-byte aligned.
+ * The table of a stream holds its pages in order: token p is in page table[p / page] at place p % page. An
+ * entry that is no page of the pool (>= pages) is a hole: its tokens are not seen, and what is
+ * appended there is dropped. Streams may share pages that none of them appends to. */
+typedef struct hs_pages {
+    int8_t *k, *v;
+    uint32_t *k_scale, *v_scale;
+    uint32_t pages, kv_heads, page, head_dim, max_scale;
+} hs_pages;
+
+/* Appends rows[s] <= t tokens (NULL: t for every stream) to the ctx[s] tokens of each stream: token i
+ * of stream s has head h of its key at k[(s t + i) stride + h head_dim], of its value in v alike, i8
+ * (bits = 8) or i16 (bits = 16); the rows may be part of a wider row (c_attn's). table [b, width].
+ * i8 values are stored as they are with scale 1. Of i16 values the FIRST row of a page sets the page's
+ * scale s = clamp(ceil(most headroom / (16 127)), 1, max_scale), most its largest magnitude in the
+ * head and headroom in sixteenths (16 ..= 64), and every row x of the page is stored as
+ * clamp(floor((2 x + s) / (2 s)), +-127). So the bytes of a token depend on that token and the first
+ * of its page alone: a stream appended token by token holds what it holds appended at once, and no
+ * token changes what an earlier one has read. Tokens past the stream's width * page are dropped. ctx_out[b]
+ * (or NULL; not overlapping ctx or rows) receives the new counts. t = 0 does nothing. Two streams must not
+ * append to one page in a call. */
+hs_status hs_op_pages_append_dev(hs_device *dev, const hs_pages *cache, const void *k, const void *v,
+                                 uint32_t bits, size_t stride, const uint32_t *table, const uint32_t *ctx,
+                                 const uint32_t *rows, size_t b, size_t t, size_t width,
+                                 uint32_t headroom, uint32_t *ctx_out, void *stream);
+/* Causal attention of the last rows[s] <= t tokens of each stream (NULL: t for every stream; t = 1 is
+ * the decode step) over its pages: row i sees the first ctx[s] - rows[s] + 1 + i of the stream's ctx[s]
+ * tokens (no more than `keys` of them count). q at [(s t + i) q_stride + h head_dim], out [b, t, h,
+ * head_dim]; head j reads head j / (h / kv_heads) of the cache. With ks and vs the scales of a key's page
+ *   score = clamp(rescale(q . k, score_m ks, score_s), +-2^40), e = attn_exp[min(M - score, len - 1)],
+ *   w = floor(e vs 2^P / S), out = clamp(rescale(sum w v, out_m, out_s), +-127)
+ * with M the largest score and S the sum of e over the keys seen; where every scale is 1 that is the rule
+ * of the other attention entries, bit for bit. score_m >= 1, score_m max_scale < 2^31 and 2^P max_scale
+ * <= 2^30 (max_scale rounded up to a power of two). A row that sees no key, or whose entries sum to 0, is
+ * 0; rows i >= rows[s] of out are left as they were. q and out 16-byte aligned, q_stride a multiple of 16. */
+hs_status hs_op_attend_paged_dev(hs_device *dev, const hs_pages *cache, const int8_t *q, size_t q_stride,
+                                 const uint32_t *table, const uint32_t *ctx, const uint32_t *rows,
+                                 size_t b, size_t t, size_t h, size_t width, size_t keys,
+                                 int32_t score_m, uint8_t score_s, int32_t out_m, uint8_t out_s,
+                                 const int32_t *attn_exp, size_t len, uint8_t softmax_p, int8_t *out,
+                                 void *workspace, size_t workspace_bytes, void *stream);
+/* The bytes of workspace that a call of these shapes needs, as hs_op_attend_rows_workspace. */
+size_t hs_op_attend_paged_workspace(size_t b, size_t t, size_t h, size_t kv_heads, size_t hd, size_t keys);
+
+/* The scores of hs_batch_run_scored for rows of logits on the device: i32 (bits = 32) or i64 (bits =
+ * 64) logits [rows, ld], of which the first vocab of a row count, and a table of `len` entries of at most
+ * 2^40 (a model's logits_exp). tokens [rows] (or NULL: none; a number that is no symbol: none, log
+ * probability 0 and rank 0xFFFFFFFF). logprob, rank, entropy [rows] and top_tokens, top_logprob [rows, top]
+ * may each be NULL. A row whose weights are all 0 has log probabilities of minus infinity and entropy 0. */
+hs_status hs_op_score_dev(hs_device *dev, const void *logits, uint32_t bits, size_t ld,
+                          const uint32_t *tokens, const uint64_t *table, size_t len, size_t rows,
+                          size_t vocab, size_t top, float *logprob, uint32_t *rank, float *entropy,
+                          uint32_t *top_tokens, float *top_logprob, void *stream);
 
 /* The coder op alone (the logits_weights + coder_interval kernels of
  * crates/hardshell-cuda/kernels/hardshell.cu:1393-1611, no public counterpart; for tests): for

@@ -626,6 +626,7 @@ struct hs_batch {
     RowInfo *h_kv_rows = nullptr, *d_kv_rows = nullptr;
     uint64_t *h_mask = nullptr, *d_mask = nullptr;
     uint32_t *h_paths = nullptr, *d_paths = nullptr;
+    float *h_scores = nullptr, *d_scores = nullptr;  // of a pass (Scoring), made at the first scored call
     hipStream_t st = nullptr;
     DevMem mem;
     RowInfo *d_rows = nullptr;
@@ -676,7 +677,7 @@ struct hs_batch {
         if (st) (void)hipStreamSynchronize(st);
         for (void *p : {(void *)h_rows, (void *)h_groups, (void *)h_src, (void *)h_queries, (void *)h_intervals,
                         (void *)h_mix, (void *)h_stats, (void *)h_intervals2, (void *)h_kv_rows, (void *)h_mask,
-                        (void *)h_paths})
+                        (void *)h_paths, (void *)h_scores})
             if (p) (void)hipHostFree(p);
         if (split) (void)hipFree(split);
         if (st) (void)hipStreamDestroy(st);
@@ -958,7 +959,7 @@ void commit(hs_batch &b, Plan &p) {
     for (auto &kv : p.prev) b.prev[kv.first] = std::move(kv.second);
 }
 
-enum class Out { Weights, Intervals, Nothing };  // Nothing: the weights, not read back
+enum class Out { Weights, Intervals, Nothing, Scores };  // Nothing: the weights, not read back
 
 // The tables of a mixed call (batch/mixed.rs:23-33): the table word of each input
 // (HS_MIX_PLAIN, HS_MIX_NONE or the predicted token), the host mixer, and for a dual call the
@@ -1012,6 +1013,18 @@ hs_status mix_chunk(hs_batch &b, const Mixing &mx, const std::vector<int64_t> &o
     return HS_OK;
 }
 
+// What a scored call asks of each input (tokens may be null) and where it goes; each result may be null.
+struct Scoring {
+    const uint32_t *tokens = nullptr;
+    size_t top = 0;
+    float *logprob = nullptr;
+    uint32_t *rank = nullptr;
+    float *entropy = nullptr;
+    uint32_t *top_tokens = nullptr;
+    float *top_logprob = nullptr;
+    size_t words() const { return 3 + 2 * top; }  // of a row, in the buffers
+};
+
 // The pass of a tree call: its rows lie slot by slot, each slot's in the order of its nodes (PassRow::pos is
 // the token position, context + depth).
 struct TreePass {
@@ -1020,7 +1033,8 @@ struct TreePass {
 };
 
 hs_status run_pass(hs_batch &b, const std::vector<PassRow> &rows, Out out, const uint32_t *queries,
-                   uint32_t bits, uint64_t *sink, const Mixing *mx = nullptr, const TreePass *tree = nullptr) {
+                   uint32_t bits, uint64_t *sink, const Mixing *mx = nullptr, const TreePass *tree = nullptr,
+                   const Scoring *sc = nullptr) {
     const hs_model &m = *b.model;
     hipStream_t st = b.st;
     const int n = (int)rows.size();
@@ -1047,6 +1061,7 @@ hs_status run_pass(hs_batch &b, const std::vector<PassRow> &rows, Out out, const
                 q[2 * n_out + 1] = queries[2 * rows[r].input + 1];
                 kinds |= q[2 * n_out];
             }
+            if (sc && sc->tokens) q[n_out] = sc->tokens[rows[r].input];
             n_out++;
         }
     }
@@ -1083,6 +1098,8 @@ hs_status run_pass(hs_batch &b, const std::vector<PassRow> &rows, Out out, const
     if (n_out) HIP_TRY(hipMemcpyAsync(b.d_src, src, n_out * sizeof(int32_t), hipMemcpyHostToDevice, st));
     if (out == Out::Intervals && n_out)
         HIP_TRY(hipMemcpyAsync(b.d_queries, q, 2 * (size_t)n_out * sizeof(uint32_t), hipMemcpyHostToDevice, st));
+    if (sc && sc->tokens && n_out)
+        HIP_TRY(hipMemcpyAsync(b.d_queries, q, (size_t)n_out * sizeof(uint32_t), hipMemcpyHostToDevice, st));
 
     uint64_t attn_keys = 0;  // sum over rows of the keys each row reads
     for (int r = 0; r < n; r++) attn_keys += (uint64_t)rows[r].pos + 1;
@@ -1242,6 +1259,21 @@ hs_status run_pass(hs_batch &b, const std::vector<PassRow> &rows, Out out, const
     head.wide32 = fits_wide((size_t)m.d, nullptr, 0, head.s);
     const size_t per_row = out == Out::Intervals ? 3 : (size_t)m.V;
     std::vector<uint64_t> host(out == Out::Weights ? (size_t)n_out * per_row : 0);
+    // the scores of output row i at [i], [n_out + i], [2 n_out + i], then the alternatives' tokens and log probabilities
+    float *const d_scores = b.d_scores;
+    auto score_args = [&](int c0) {
+        hs::ScoreArgs a;
+        a.vocab = m.V; a.table = m.logits_exp; a.table_len = (int)m.host.logits_exp.size();
+        a.tokens = sc->tokens ? b.d_queries + c0 : nullptr;
+        a.top = (int)sc->top;
+        const size_t n = (size_t)n_out;
+        a.logprob = d_scores + c0;
+        a.rank = (uint32_t *)d_scores + n + c0;
+        a.entropy = sc->entropy ? d_scores + 2 * n + c0 : nullptr;
+        a.top_tokens = (uint32_t *)d_scores + 3 * n + c0 * sc->top;
+        a.top_logprob = d_scores + (3 + sc->top) * n + c0 * sc->top;
+        return a;
+    };
     for (int c0 = 0; c0 < n_out; c0 += (int)b.chunk_rows) {
         const int cn = std::min<int>((int)b.chunk_rows, n_out - c0);
         if (m.compact) {
@@ -1258,6 +1290,12 @@ hs_status run_pass(hs_batch &b, const std::vector<PassRow> &rows, Out out, const
             const uint64_t ops = 2ull * (uint64_t)pr * cn * (uint64_t)m.V * (uint64_t)m.d;
             const Epi epi = m.wide_ln_f ? Epi::LogitsCompactWide : Epi::LogitsCompact;
             HIP_TRY(b.launch("gemm_logits", ops, [&] { return hs::launch_gemm(epi, g, st); }));
+            if (sc) {
+                hs::ScoreArgs a = score_args(c0);
+                a.src = hs::SCORE_COMPACT; a.d16 = b.d_d16; a.ld16 = m.ld16; a.tmax = b.d_tmax; a.ntiles = m.ntiles;
+                HIP_TRY(b.launch("score", 0, [&] { return hs::launch_score(a, cn, st); }));
+                continue;
+            }
             hs::CompactCoderArgs ca;
             ca.d16 = b.d_d16; ca.ld16 = m.ld16; ca.tmax = b.d_tmax; ca.ntiles = m.ntiles; ca.vocab = m.V;
             ca.table = m.logits_exp; ca.table_len = (int)m.host.logits_exp.size(); ca.d0 = m.d0;
@@ -1286,6 +1324,12 @@ hs_status run_pass(hs_batch &b, const std::vector<PassRow> &rows, Out out, const
             HIP_TRY(gemm("gemm_logits", m.wide_ln_f ? Epi::LogitsWide : Epi::Logits, head,
                          b.d_af + (size_t)pr * c0 * 64, pr * RP, cn, b.d_logits, m.V, nullptr, 0, nullptr,
                          head_group(m.wide_ln_f ? hs::plane_rows(cn) : cn)));
+            if (sc) {
+                hs::ScoreArgs a = score_args(c0);
+                a.src = hs::SCORE_I64; a.logits = b.d_logits; a.ld = (size_t)m.V;
+                HIP_TRY(b.launch("score", 0, [&] { return hs::launch_score(a, cn, st); }));
+                continue;
+            }
             hs::CoderArgs ca;
             ca.logits = b.d_logits; ca.ld = m.V; ca.vocab = m.V; ca.table = m.logits_exp;
             ca.table_len = (int)m.host.logits_exp.size();
@@ -1316,11 +1360,27 @@ hs_status run_pass(hs_batch &b, const std::vector<PassRow> &rows, Out out, const
     HIP_TRY(b.span_end());
     if (out == Out::Intervals)
         HIP_TRY(hipMemcpyAsync(b.h_intervals, b.d_intervals, (size_t)n_out * 24, hipMemcpyDeviceToHost, st));
+    if (sc)
+        HIP_TRY(hipMemcpyAsync(b.h_scores, b.d_scores, n_out * sc->words() * sizeof(float), hipMemcpyDeviceToHost, st));
     if (mx && mx->plain_sink)
         HIP_TRY(hipMemcpyAsync(b.h_intervals2, b.d_intervals2, (size_t)n_out * 24, hipMemcpyDeviceToHost, st));
     HIP_TRY(hipStreamSynchronize(st));
     if (out == Out::Nothing) {  // batch.rs:549: wait for the GPU, read nothing back
         if (b.profiling && b.pending.size() > 8192) HIP_TRY(b.collect());
+        return HS_OK;
+    }
+    if (sc) {
+        if (b.profiling && b.pending.size() > 8192) HIP_TRY(b.collect());
+        const float *h = b.h_scores;
+        const size_t k = sc->top;
+        for (size_t i = 0, n = (size_t)n_out; i < n; i++) {
+            const size_t o = (size_t)owner[i];
+            if (sc->logprob) sc->logprob[o] = h[i];
+            if (sc->rank) std::memcpy(sc->rank + o, h + n + i, sizeof(uint32_t));
+            if (sc->entropy) sc->entropy[o] = h[2 * n + i];
+            if (k && sc->top_tokens) std::memcpy(sc->top_tokens + o * k, h + 3 * n + i * k, k * sizeof(uint32_t));
+            if (k && sc->top_logprob) std::memcpy(sc->top_logprob + o * k, h + (3 + k) * n + i * k, k * sizeof(float));
+        }
         return HS_OK;
     }
     const uint64_t *res = out == Out::Intervals ? b.h_intervals : host.data();
@@ -1354,14 +1414,14 @@ hs_status check_inputs(const hs_batch *b, const hs_input *in, size_t n) {
 }
 
 hs_status run(hs_batch *b, const hs_input *in, size_t n, Out out, const uint32_t *queries,
-              uint32_t bits, uint64_t *sink, const Mixing *mx = nullptr) {
+              uint32_t bits, uint64_t *sink, const Mixing *mx = nullptr, const Scoring *sc = nullptr) {
     HIP_TRY(hipSetDevice(b->model->dev->ordinal));
     if (!b->trees.empty())
         for (size_t i = 0; i < n; i++) b->trees.erase(in[i].slot);  // their rows are written over
     static thread_local Plan plan;  // host scratch kept from call to call (one call per thread at a time)
     make_plan(*b, in, n, plan);
     for (size_t i = 0; i < plan.n_passes; i++) {
-        hs_status s = run_pass(*b, plan.passes[i], out, queries, bits, sink, mx);
+        hs_status s = run_pass(*b, plan.passes[i], out, queries, bits, sink, mx, nullptr, sc);
         if (s != HS_OK) return s;  // no position changes after an error
     }
     commit(*b, plan);
@@ -1438,7 +1498,7 @@ hs_status guarded(F fn) {
 }
 
 hs_status run_tree(hs_batch *b, const hs_input *in, const uint32_t *parents, size_t n, Out out, const uint32_t *queries,
-                   uint32_t bits, uint64_t *sink) {
+                   uint32_t bits, uint64_t *sink, const Scoring *sc = nullptr) {
     std::vector<PassRow> rows;
     TreePass pass;
     std::unordered_map<size_t, hs_batch::Tree> trees;
@@ -1465,7 +1525,7 @@ hs_status run_tree(hs_batch *b, const hs_input *in, const uint32_t *parents, siz
         st.written = std::max<size_t>(st.written, (size_t)(g.pos0 + g.count));
         b->trees.erase((size_t)g.slot);
     }
-    HS_TRY(run_pass(*b, rows, out, queries, bits, sink, nullptr, &pass));
+    HS_TRY(run_pass(*b, rows, out, queries, bits, sink, nullptr, &pass, sc));
     for (auto &t : trees) b->trees[t.first] = std::move(t.second);
     return HS_OK;
 }
@@ -1582,6 +1642,45 @@ extern "C" hs_status hs_batch_run_tree_coded(hs_batch *b, const hs_input *in, co
     if (n && (!queries || !out)) return hs::fail(HS_INVALID_ARGUMENT, 0, "NULL argument");
     HS_TRY(check_queries(queries, n, b->model->host.vocab, freq_bits));
     return guarded([&] { return run_tree(b, in, parents, n, Out::Intervals, query_words(queries), freq_bits, (uint64_t *)out); });
+}
+
+// ---- Scores: no counterpart in the reference, whose callers get whole rows of weights -----------------
+
+constexpr size_t HS_MAX_TOP = 64;
+
+// The checks of a scored call's arguments, and its buffers.
+static hs_status plan_scores(hs_batch *b, const uint32_t *tokens, size_t n, const Scoring &sc) {
+    const uint32_t V = b->model->host.vocab;
+    if (sc.top > HS_MAX_TOP || sc.top > V) return hs::fail(HS_UNSUPPORTED, 0, "top is at most 64, and at most the vocabulary");
+    if (!tokens && (sc.logprob || sc.rank)) return hs::fail(HS_INVALID_ARGUMENT, 0, "log probabilities and ranks need tokens");
+    for (size_t i = 0; tokens && i < n; i++)
+        if (tokens[i] >= V && tokens[i] != HS_NO_TOKEN) return hs::fail(HS_UNSUPPORTED, 0, "a scored token is out of range");
+    if (n == 0 || b->h_scores) return HS_OK;
+    HIP_TRY(hipSetDevice(b->model->dev->ordinal));
+    const size_t words = b->max_rows * (3 + 2 * HS_MAX_TOP);
+    if (!b->d_scores) HS_TRY(b->mem.alloc(b->d_scores, words));
+    HIP_TRY(hipHostMalloc((void **)&b->h_scores, words * sizeof(float), hipHostMallocDefault));
+    return HS_OK;
+}
+
+extern "C" hs_status hs_batch_run_scored(hs_batch *b, const hs_input *in, const uint32_t *tokens, size_t n, size_t top,
+                                         float *logprob, uint32_t *rank, float *entropy, uint32_t *top_tokens,
+                                         float *top_logprob) {
+    hs::clear_error();
+    HS_TRY(check_inputs(b, in, n));
+    const Scoring sc{tokens, top, logprob, rank, entropy, top_tokens, top_logprob};
+    HS_TRY(plan_scores(b, tokens, n, sc));
+    return guarded([&] { return run(b, in, n, Out::Scores, nullptr, 0, nullptr, nullptr, &sc); });
+}
+
+extern "C" hs_status hs_batch_run_tree_scored(hs_batch *b, const hs_input *in, const uint32_t *parents,
+                                              const uint32_t *tokens, size_t n, size_t top, float *logprob,
+                                              uint32_t *rank, float *entropy, uint32_t *top_tokens, float *top_logprob) {
+    hs::clear_error();
+    HS_TRY(check_inputs(b, in, n));
+    const Scoring sc{tokens, top, logprob, rank, entropy, top_tokens, top_logprob};
+    HS_TRY(plan_scores(b, tokens, n, sc));
+    return guarded([&] { return run_tree(b, in, parents, n, Out::Scores, nullptr, 0, nullptr, &sc); });
 }
 
 static hs_status commit_paths(hs_batch *b, const uint32_t *slots, const uint32_t *lengths, const uint32_t *paths, size_t n) {
@@ -1988,14 +2087,15 @@ hs_status rows_args(hs_device *dev, const int8_t *q, const int8_t *k_cache, cons
     return HS_OK;
 }
 
-hs_status run_rows(hs_device *dev, const hs::RowsArgs &g, void *workspace, size_t workspace_bytes, void *stream) {
-    const size_t need = hs::rows_workspace(g);
+// Runs launch(workspace, stream): the caller's workspace, or for a call without one memory of the device's pool.
+template <typename F>
+hs_status with_workspace(hs_device *dev, size_t need, void *workspace, size_t workspace_bytes, void *stream, F launch) {
     if (workspace && (workspace_bytes < need || !aligned(256, {workspace})))
         return hs::fail(HS_INVALID_ARGUMENT, 0, "the workspace needs " + std::to_string(need) + " bytes, 256-byte aligned");
     hipStream_t st = stream ? (hipStream_t)stream : dev->stream;
     HIP_TRY(hipSetDevice(dev->ordinal));
     if (need == 0 || workspace) {
-        HIP_TRY(hs::launch_rows(g, workspace, st));
+        HIP_TRY(launch(workspace, st));
         return HS_OK;
     }
     hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
@@ -2016,11 +2116,16 @@ hs_status run_rows(hs_device *dev, const hs::RowsArgs &g, void *workspace, size_
     }
     void *scratch = nullptr;
     HIP_TRY(hipMallocFromPoolAsync(&scratch, need, dev->pool, st));
-    const hipError_t e = hs::launch_rows(g, scratch, st);
+    const hipError_t e = launch(scratch, st);
     const hipError_t f = hipFreeAsync(scratch, st);
     HIP_TRY(e);
     HIP_TRY(f);
     return HS_OK;
+}
+
+hs_status run_rows(hs_device *dev, const hs::RowsArgs &g, void *workspace, size_t workspace_bytes, void *stream) {
+    return with_workspace(dev, hs::rows_workspace(g), workspace, workspace_bytes, stream,
+                          [&](void *scratch, hipStream_t st) { return hs::launch_rows(g, scratch, st); });
 }
 
 // The layer pointers of a launch, and the checks that the cache operators share.
@@ -2153,6 +2258,136 @@ extern "C" hs_status hs_op_cache_commit_dev(hs_device *dev, int8_t *const *k_cac
         a.first = l0 == 0;
         HIP_TRY(hs::launch_commit(c, n, a, st));
     }
+    return HS_OK;
+}
+
+// ---- Paged caches and scores ---------------------------------------------------------------------------
+
+namespace {
+
+hs_status pool_args(hs_device *dev, const hs_pages *c, hs::PagePool &p) {
+    if (!dev || !c || !c->k || !c->v || !c->k_scale || !c->v_scale) return hs::fail(HS_INVALID_ARGUMENT, 0, "NULL argument");
+    if (c->head_dim == 0 || c->head_dim % 16 != 0 || c->head_dim > 256)
+        return hs::fail(HS_UNSUPPORTED, 0, "head_dim must be a multiple of 16 in 16..=256");
+    if (c->page < 16 || c->page > 1024 || (c->page & (c->page - 1)))
+        return hs::fail(HS_UNSUPPORTED, 0, "a page holds a power of two of tokens, 16..=1024");
+    if (c->pages == 0 || c->pages > (uint32_t)INT32_MAX || c->kv_heads == 0 || c->kv_heads > 65535)
+        return hs::fail(HS_UNSUPPORTED, 0, "1 to 2^31 - 1 pages and 1 to 65,535 heads");
+    if (c->max_scale == 0 || c->max_scale > 1024) return hs::fail(HS_UNSUPPORTED, 0, "max_scale must be in 1..=1024");
+    if (!aligned(16, {c->k, c->v}) || !aligned(4, {c->k_scale, c->v_scale}))
+        return hs::fail(HS_INVALID_ARGUMENT, 0, "the pages must be 16-byte aligned, the scales 4-byte");
+    p.k = c->k; p.v = c->v; p.k_scale = c->k_scale; p.v_scale = c->v_scale;
+    p.pages = (int)c->pages; p.kv_heads = (int)c->kv_heads; p.page = (int)c->page; p.hd = (int)c->head_dim;
+    p.max_scale = c->max_scale;
+    return HS_OK;
+}
+
+// Of the streams, their tokens and their tables.
+hs_status paged_dims(size_t b, size_t t, size_t heads, size_t width, size_t page) {
+    if (b > (size_t)INT32_MAX || t > (size_t)INT32_MAX || heads > (size_t)INT32_MAX || width > (size_t)INT32_MAX / page)
+        return hs::fail(HS_UNSUPPORTED, 0, "too many streams, tokens or pages of a stream");
+    if (b && t && (t > MAX_ROW_HEADS / b || heads > MAX_ROW_HEADS / (b * t)))
+        return hs::fail(HS_UNSUPPORTED, 0, "too many rows (fewer than 2^26 rows of a head)");
+    return HS_OK;
+}
+
+hs_status attend_paged_args(hs_device *dev, const hs_pages *cache, size_t b, size_t t, size_t h, size_t width, size_t keys,
+                            hs::PagedArgs &g) {
+    HS_TRY(pool_args(dev, cache, g.pages));
+    HS_TRY(paged_dims(b, t, h, width, cache->page));
+    if (h == 0 || h % cache->kv_heads) return hs::fail(HS_UNSUPPORTED, 0, "the heads must be a multiple of the cache's");
+    if (keys == 0 || keys > (size_t)1 << 22 || keys > width * cache->page)
+        return hs::fail(HS_UNSUPPORTED, 0, "keys must be in 1..=2^22 and fit the pages of a stream");
+    g.streams = (int)b; g.t = (int)t; g.heads = (int)h; g.width = (int)width; g.keys = (int)keys;
+    return HS_OK;
+}
+
+}  // namespace
+
+extern "C" hs_status hs_op_pages_append_dev(hs_device *dev, const hs_pages *cache, const void *k, const void *v,
+                                            uint32_t bits, size_t stride, const uint32_t *table, const uint32_t *ctx,
+                                            const uint32_t *rows, size_t b, size_t t, size_t width, uint32_t headroom,
+                                            uint32_t *ctx_out, void *stream) {
+    hs::clear_error();
+    hs::AppendArgs a;
+    HS_TRY(pool_args(dev, cache, a.pages));
+    if (!k || !v || !table || !ctx) return hs::fail(HS_INVALID_ARGUMENT, 0, "NULL argument");
+    if (bits != 8 && bits != 16) return hs::fail(HS_UNSUPPORTED, 0, "rows of 8 or 16 bits");
+    if (headroom < 16 || headroom > 64) return hs::fail(HS_UNSUPPORTED, 0, "headroom must be in 16..=64 sixteenths");
+    HS_TRY(paged_dims(b, t, cache->kv_heads, width, cache->page));
+    const size_t values = (size_t)cache->kv_heads * cache->head_dim;
+    if (width == 0) return hs::fail(HS_UNSUPPORTED, 0, "a stream needs a page at least");
+    if (stride < values || stride > ((size_t)1 << 40) || stride * (bits / 8) % 16)
+        return hs::fail(HS_UNSUPPORTED, 0, "the stride must hold the heads of a token, in steps of 16 bytes");
+    if (!aligned(16, {k, v}) || !aligned(4, {table, ctx, rows, ctx_out}))
+        return hs::fail(HS_INVALID_ARGUMENT, 0, "rows must be 16-byte aligned, the tables and counts 4-byte");
+    if (overlap(ctx, 4 * b, ctx_out, 4 * b) || overlap(rows, 4 * b, ctx_out, 4 * b))
+        return hs::fail(HS_INVALID_ARGUMENT, 0, "ctx_out must not overlap ctx or rows");
+    if (b == 0 || t == 0) return HS_OK;
+    a.k = k; a.v = v; a.bits = (int)bits; a.stride = stride; a.table = table; a.ctx = ctx; a.rows = rows;
+    a.streams = (int)b; a.t = (int)t; a.width = (int)width; a.headroom = headroom; a.ctx_out = ctx_out;
+    HIP_TRY(hipSetDevice(dev->ordinal));
+    HIP_TRY(hs::launch_append(a, stream ? (hipStream_t)stream : dev->stream));
+    return HS_OK;
+}
+
+extern "C" size_t hs_op_attend_paged_workspace(size_t b, size_t t, size_t h, size_t kv_heads, size_t hd, size_t keys) {
+    hs::PagedArgs g;
+    if (b == 0 || t == 0 || h == 0 || kv_heads == 0 || h % kv_heads || hd == 0 || hd > 256 || keys == 0 ||
+        keys > (size_t)1 << 22 || paged_dims(b, t, h, 1, 16) != HS_OK)
+        return 0;  // (the call itself refuses them, or does nothing)
+    g.streams = (int)b; g.t = (int)t; g.heads = (int)h; g.keys = (int)keys;
+    g.pages.kv_heads = (int)kv_heads; g.pages.hd = (int)hd;
+    return hs::paged_workspace(g);
+}
+
+extern "C" hs_status hs_op_attend_paged_dev(hs_device *dev, const hs_pages *cache, const int8_t *q, size_t q_stride,
+                                            const uint32_t *table, const uint32_t *ctx, const uint32_t *rows, size_t b,
+                                            size_t t, size_t h, size_t width, size_t keys, int32_t score_m,
+                                            uint8_t score_s, int32_t out_m, uint8_t out_s, const int32_t *attn_exp,
+                                            size_t len, uint8_t softmax_p, int8_t *out, void *workspace,
+                                            size_t workspace_bytes, void *stream) {
+    hs::clear_error();
+    hs::PagedArgs g;
+    HS_TRY(attend_paged_args(dev, cache, b, t, h, width, keys, g));
+    if (!q || !table || !ctx || !attn_exp || !out) return hs::fail(HS_INVALID_ARGUMENT, 0, "NULL argument");
+    if (!aligned(16, {q, out}) || !aligned(4, {table, ctx, rows, attn_exp}))
+        return hs::fail(HS_INVALID_ARGUMENT, 0, "rows must be 16-byte aligned, the tables and counts 4-byte");
+    if (q_stride < h * cache->head_dim || q_stride > ((size_t)1 << 40) || q_stride % 16)
+        return hs::fail(HS_UNSUPPORTED, 0, "the stride must hold the heads of a token, in steps of 16 bytes");
+    uint32_t bits = 0;  // of the largest scale
+    while (((uint32_t)1 << bits) < cache->max_scale) bits++;
+    if (len == 0 || len > (size_t)INT32_MAX || score_m < 1 || (int64_t)score_m * cache->max_scale > INT32_MAX || softmax_p + bits > 30)
+        return hs::fail(HS_UNSUPPORTED, 0, "len >= 1, 1 <= score_m, score_m max_scale < 2^31 and 2^P max_scale <= 2^30");
+    if (b == 0 || t == 0) return HS_OK;
+    g.q = q; g.q_stride = q_stride; g.table = table; g.ctx = ctx; g.rows = rows;
+    g.score_m = score_m; g.score_s = score_s; g.out_m = out_m; g.out_s = out_s;
+    g.exp_table = attn_exp; g.exp_len = (int)len; g.softmax_p = softmax_p; g.out = out;
+    return with_workspace(dev, hs::paged_workspace(g), workspace, workspace_bytes, stream,
+                          [&](void *scratch, hipStream_t st) { return hs::launch_paged(g, scratch, st); });
+}
+
+extern "C" hs_status hs_op_score_dev(hs_device *dev, const void *logits, uint32_t bits, size_t ld, const uint32_t *tokens,
+                                     const uint64_t *table, size_t len, size_t rows, size_t vocab, size_t top,
+                                     float *logprob, uint32_t *rank, float *entropy, uint32_t *top_tokens,
+                                     float *top_logprob, void *stream) {
+    hs::clear_error();
+    if (!dev || !logits || !table) return hs::fail(HS_INVALID_ARGUMENT, 0, "NULL argument");
+    if (bits != 32 && bits != 64) return hs::fail(HS_UNSUPPORTED, 0, "logits of 32 or 64 bits");
+    if (vocab == 0 || vocab > (size_t)1 << 24 || len == 0 || len > (size_t)INT32_MAX || ld < vocab ||
+        ld > (size_t)1 << 40 || rows > MAX_ROW_HEADS / 16)
+        return hs::fail(HS_UNSUPPORTED, 0, "1 to 2^24 symbols a row, len >= 1 and fewer than 2^22 rows");
+    if (top > HS_MAX_TOP || top > vocab) return hs::fail(HS_UNSUPPORTED, 0, "top is at most 64, and at most the vocabulary");
+    if (!tokens && (logprob || rank)) return hs::fail(HS_INVALID_ARGUMENT, 0, "log probabilities and ranks need tokens");
+    if (!aligned(bits / 8, {logits}) || !aligned(8, {table}) || !aligned(4, {tokens, logprob, rank, entropy, top_tokens, top_logprob}))
+        return hs::fail(HS_INVALID_ARGUMENT, 0, "logits, tables and results must be aligned to their types");
+    if (rows == 0) return HS_OK;
+    hs::ScoreArgs a;
+    a.src = bits == 32 ? hs::SCORE_I32 : hs::SCORE_I64; a.logits = logits; a.ld = ld;
+    a.vocab = (int)vocab; a.table = table; a.table_len = (int)len; a.tokens = tokens; a.top = (int)top;
+    a.logprob = logprob; a.rank = rank; a.entropy = entropy; a.top_tokens = top_tokens; a.top_logprob = top_logprob;
+    HIP_TRY(hipSetDevice(dev->ordinal));
+    HIP_TRY(hs::launch_score(a, (int)rows, stream ? (hipStream_t)stream : dev->stream));
     return HS_OK;
 }
 

@@ -323,4 +323,62 @@ hipError_t launch_coder_compact(const CompactCoderArgs &a, int n_rows, hipStream
 hipError_t launch_mix_stats_compact(const CompactCoderArgs &a, int n_rows, hipStream_t stream);
 hipError_t launch_coder_compact_mixed(const CompactCoderArgs &a, int n_rows, hipStream_t stream);
 
+// Caches in pages of a pool (paged.hip): values [pages][kv_heads][page][hd], scales [pages][kv_heads].
+struct PagePool {
+    int8_t *k = nullptr, *v = nullptr;
+    uint32_t *k_scale = nullptr, *v_scale = nullptr;
+    int pages = 0, kv_heads = 0, page = 0, hd = 0;
+    uint32_t max_scale = 1;
+};
+struct AppendArgs {
+    PagePool pages;
+    const void *k = nullptr, *v = nullptr;  // token i of stream s at [(s t + i) stride + head hd], of `bits` bits
+    int bits = 8;
+    size_t stride = 0;
+    const uint32_t *table = nullptr;                     // [streams][width]
+    const uint32_t *ctx = nullptr, *rows = nullptr;      // [streams]
+    int streams = 0, t = 0, width = 0;
+    uint32_t headroom = 16;
+    uint32_t *ctx_out = nullptr;
+};
+hipError_t launch_append(const AppendArgs &a, hipStream_t stream);
+struct PagedArgs {
+    PagePool pages;
+    const int8_t *q = nullptr;  // token i of stream s at [(s t + i) q_stride + head hd]
+    size_t q_stride = 0;
+    const uint32_t *table = nullptr;
+    const uint32_t *ctx = nullptr, *rows = nullptr;
+    int streams = 0, t = 0, heads = 0, width = 0, keys = 0;  // keys: at most this many of a stream are read
+    int32_t score_m = 0;
+    int score_s = 0;
+    int32_t out_m = 0;
+    int out_s = 0;
+    const int32_t *exp_table = nullptr;
+    int exp_len = 0, softmax_p = 0;
+    int8_t *out = nullptr;  // [streams][t][heads][hd]
+};
+size_t paged_workspace(const PagedArgs &g);
+hipError_t launch_paged(const PagedArgs &g, void *workspace, hipStream_t stream);
+
+// Scores of rows of logits (score.hip): i32 or i64 logits [rows][ld], or compact ones (CompactCoderArgs).
+constexpr int SCORE_I32 = 0, SCORE_I64 = 1, SCORE_COMPACT = 2;
+struct ScoreArgs {
+    int src = SCORE_I64;
+    const void *logits = nullptr;
+    size_t ld = 0;
+    const uint16_t *d16 = nullptr;
+    int ld16 = 0;
+    const int64_t *tmax = nullptr;
+    int ntiles = 0;
+    int vocab = 0;
+    const uint64_t *table = nullptr;
+    int table_len = 0;
+    const uint32_t *tokens = nullptr;  // [rows], vocab and above: none
+    int top = 0;
+    // [rows], the alternatives [rows][top]; each may be null
+    float *logprob = nullptr, *entropy = nullptr, *top_logprob = nullptr;
+    uint32_t *rank = nullptr, *top_tokens = nullptr;
+};
+hipError_t launch_score(const ScoreArgs &a, int n_rows, hipStream_t stream);
+
 }  // namespace hs

@@ -74,6 +74,7 @@ class _Input(C.Structure):
 HS_MIX_NONE = 0xFFFFFFFF   # a mixed table without a prediction
 HS_MIX_PLAIN = 0xFFFFFFFE  # the table of GPT-2 alone
 HS_TREE_ROOT = 0xFFFFFFFF  # the parent of a tree's node right after the context
+HS_NO_TOKEN = 0xFFFFFFFF   # no token to score
 
 
 class MixStats(C.Structure):
@@ -168,6 +169,14 @@ def lib() -> C.CDLL:
         L.hs_op_attend_rows_workspace.restype = S
         L.hs_op_cache_evict_dev.argtypes = [P, P, P, S, P, P, S, S, S, S, S, S, P, P, P, P]
         L.hs_op_cache_commit_dev.argtypes = [P, P, P, S, P, P, P, S, S, S, S, S, P, P]
+        L.hs_op_pages_append_dev.argtypes = [P, P, P, P, U32, S, P, P, P, S, S, S, U32, P, P]
+        L.hs_op_attend_paged_dev.argtypes = [P, P, P, S, P, P, P, S, S, S, S, S, C.c_int32, C.c_uint8, C.c_int32,
+                                             C.c_uint8, P, S, C.c_uint8, P, P, S, P]
+        L.hs_op_attend_paged_workspace.argtypes = [S] * 6
+        L.hs_op_attend_paged_workspace.restype = S
+        L.hs_op_score_dev.argtypes = [P, P, U32, S, P, P, S, S, S, S, P, P, P, P, P, P]
+        L.hs_batch_run_scored.argtypes = [P, P, P, S, S, P, P, P, P, P]
+        L.hs_batch_run_tree_scored.argtypes = [P, P, P, P, S, S, P, P, P, P, P]
         L.hs_read_bw.argtypes = [P, S, S, C.POINTER(C.c_uint64)]
         L.hs_probe_issue.argtypes = [P, C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(C.c_uint64)]
         L.hs_model_load_with.argtypes = [P, P, S, P, C.POINTER(P)]
@@ -344,6 +353,16 @@ def _queries(queries) -> np.ndarray:
     return q
 
 
+class Scores(NamedTuple):
+    """What HipBatch.run_scored gives of each input, as arrays: float32 logprob [n] and u32 rank [n] (None without
+    tokens), float32 entropy [n], u32 top_tokens and float32 top_logprob [n, top]."""
+    logprob: Optional[np.ndarray]
+    rank: Optional[np.ndarray]
+    entropy: np.ndarray
+    top_tokens: np.ndarray
+    top_logprob: np.ndarray
+
+
 class HipBatch:
     """CudaBatch (crates/hardshell-cuda/src/batch.rs:237-476)."""
 
@@ -453,6 +472,38 @@ class HipBatch:
         out = np.zeros((len(a), 3), np.uint64)
         _check(lib().hs_batch_run_tree_coded(self.h, _ptr(a), _ptr(p), _ptr(q), len(a), freq_bits, _ptr(out)))
         return out
+
+    def _scored(self, n: int, tokens, top: int, call) -> Scores:
+        if not 0 <= top < 2 ** 31:
+            raise Unsupported(HS_UNSUPPORTED, 0, "top is at most 64, and at most the vocabulary")
+        t = None
+        if tokens is not None:
+            t = np.asarray(tokens)
+            if t.dtype.kind not in "iuO":
+                t = t.astype(np.int64)
+            if len(t) != n:
+                raise LengthMismatch(HS_LENGTH_MISMATCH, 0, f"length mismatch: expected {n}, found {len(t)}")
+            # other numbers that 32 bits do not hold become the vocabulary's size, which is no symbol either
+            none = (t == -1) | (t == HS_NO_TOKEN)
+            t = np.where(none, HS_NO_TOKEN, np.where((t < 0) | (t > self.vocab), self.vocab, t)).astype(np.uint32)
+        out = Scores(None if t is None else np.zeros(n, np.float32), None if t is None else np.zeros(n, np.uint32),
+                     np.zeros(n, np.float32), np.zeros((n, top), np.uint32), np.zeros((n, top), np.float32))
+        _check(call(None if t is None else _ptr(t), *[None if x is None else _ptr(x) for x in out]))
+        return out
+
+    def run_scored(self, inputs, tokens=None, top: int = 0) -> Scores:
+        """Runs the inputs and scores what follows each (hs_batch_run_scored): the log probability and rank of
+        tokens[i] (-1 or HS_NO_TOKEN: none), the entropy, and the first `top` alternatives."""
+        a = _inputs(inputs)
+        return self._scored(len(a), tokens, top, lambda t, *out: lib().hs_batch_run_scored(
+            self.h, _ptr(a), t, len(a), top, *out))
+
+    def run_tree_scored(self, inputs, parents, tokens=None, top: int = 0) -> Scores:
+        """run_scored for every node of the slots' trees of drafts; parents as in run_tree_weights."""
+        a = _inputs(inputs)
+        p = self._parents(parents, len(a))
+        return self._scored(len(a), tokens, top, lambda t, *out: lib().hs_batch_run_tree_scored(
+            self.h, _ptr(a), _ptr(p), t, len(a), top, *out))
 
     def commit_paths(self, paths) -> None:
         """Accepts a path of the last tree of each slot: {slot: node numbers in the slot's tree, from a child
@@ -665,6 +716,126 @@ def cache_commit(dev: HipDevice, k_caches, v_caches, ctx, path, accepted, dims, 
         raise LengthMismatch(HS_LENGTH_MISMATCH, 0, f"length mismatch: expected {len(k)}, found {len(v)}")
     _check(lib().hs_op_cache_commit_dev(dev.h, k, v, len(k), _dptr(ctx), _dptr(path), _dptr(accepted), *dims,
                                         _dptr(ctx_out), stream))
+
+
+class _Pages(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("pages", C.c_uint32), ("kv_heads", C.c_uint32), ("page", C.c_uint32), ("head_dim", C.c_uint32),
+                ("max_scale", C.c_uint32)]
+
+
+class PagedCache(NamedTuple):
+    """One layer's pool of pages (hs_pages): int8 k and v [pages, kv_heads, page, head_dim], 32-bit k_scale and
+    v_scale [pages, kv_heads], on the device; scales up to max_scale."""
+    k: object
+    v: object
+    k_scale: object
+    v_scale: object
+    pages: int
+    kv_heads: int
+    page: int
+    head_dim: int
+    max_scale: int
+
+    def _struct(self):
+        numbers = self[4:]
+        if any(not 0 <= x <= _U32 for x in numbers):
+            raise Unsupported(HS_UNSUPPORTED, 0, "a size that 32 bits do not hold")
+        return _Pages(*[_address(_dptr(x)) for x in self[:4]], *numbers)
+
+
+def _address(x):
+    return x.value if isinstance(x, C.c_void_p) else x
+
+
+def _sizes(*numbers):
+    """Sizes for the library; a negative one would come round to a large one."""
+    if any(x < 0 for x in numbers):
+        raise Unsupported(HS_UNSUPPORTED, 0, "a negative size")
+    return numbers
+
+
+def _signed(x) -> bool:
+    """Whether a tensor holds signed integers."""
+    name = str(x.dtype)
+    return "int" in name and "uint" not in name
+
+
+def _rows_of(x, stride: Optional[int], values: int):
+    """The address of rows of new tokens and the elements from one token to the next: a tensor [streams, t, heads,
+    head_dim] on the GPU whose heads of a token lie together and whose tokens at one distance, or an address with
+    `stride` (None: the rows lie together)."""
+    if not hasattr(x, "data_ptr"):
+        return x, values if stride is None else stride
+    if not getattr(x, "is_cuda", True):
+        raise ValueError("a tensor in host memory where the GPU reads or writes")
+    (b, t, h, hd), st = x.shape, x.stride()
+    step = st[1] if t > 1 else st[0] if b > 1 else values
+    if (h > 1 and st[2] != hd) or (hd > 1 and st[3] != 1) or (b > 1 and st[0] != t * step) or \
+            (stride is not None and stride != step):
+        raise ValueError("a tensor whose tokens do not lie at one distance, each with its heads together")
+    return x.data_ptr(), step
+
+
+def pages_append(dev: HipDevice, cache: PagedCache, k, v, table, ctx, rows, dims, headroom: int = 16, ctx_out=None,
+                 bits: Optional[int] = None, stride: Optional[int] = None, stream=None) -> None:
+    """Appends rows of keys and values to the streams' pages (hs_op_pages_append_dev): dims = (streams, t, width);
+    k and v are tensors [streams, t, kv_heads, head_dim] of int8 or int16, or addresses with `bits` and `stride`."""
+    b, t, width = _sizes(*dims)
+    for x in (k, v):
+        if hasattr(x, "element_size"):
+            if tuple(x.shape) != (b, t, cache.kv_heads, cache.head_dim) or bits not in (None, 8 * x.element_size()) or \
+                    not _signed(x):
+                raise ValueError("k and v: [streams, t, kv_heads, head_dim], both int8 or both int16")
+            bits = 8 * x.element_size()
+    (kp, ks), (vp, vs) = (_rows_of(x, stride, cache.kv_heads * cache.head_dim) for x in (k, v))
+    if ks != vs:
+        raise ValueError("k and v with tokens at different distances")
+    if not 0 <= headroom <= _U32:
+        raise Unsupported(HS_UNSUPPORTED, 0, "headroom must be in 16..=64 sixteenths")
+    p = cache._struct()
+    _check(lib().hs_op_pages_append_dev(dev.h, C.byref(p), kp, vp, bits or 0, *_sizes(ks), _dptr(table), _dptr(ctx),
+                                        _dptr(rows), b, t, width, headroom, _dptr(ctx_out), stream))
+
+
+def attend_paged(dev: HipDevice, cache: PagedCache, q, table, ctx, rows, dims, rule: AttentionRule, out,
+                 q_stride: Optional[int] = None, workspace=None, workspace_bytes: int = 0, stream=None) -> None:
+    """Causal attention over the streams' pages (hs_op_attend_paged_dev): dims = (streams, t, heads, width, keys);
+    q is a tensor [streams, t, heads, head_dim] of int8, or an address with `q_stride`; rows may be None (t each)."""
+    b, t, heads, width, keys = _sizes(*dims)
+    if hasattr(q, "data_ptr") and (tuple(q.shape) != (b, t, heads, cache.head_dim) or q.element_size() != 1):
+        raise ValueError("q: [streams, t, heads, head_dim] of int8")
+    qp, step = _rows_of(q, q_stride, heads * cache.head_dim)
+    m, s, om, os_, exp, length, p = rule
+    pages = cache._struct()
+    _check(lib().hs_op_attend_paged_dev(dev.h, C.byref(pages), qp, *_sizes(step), _dptr(table), _dptr(ctx), _dptr(rows),
+                                        b, t, heads, width, keys, m, s, om, os_, _dptr(exp), length, p, _dptr(out),
+                                        _dptr(workspace), workspace_bytes, stream))
+
+
+def attend_paged_workspace(streams: int, t: int, heads: int, kv_heads: int, head_dim: int, keys: int) -> int:
+    """The bytes of workspace of attend_paged (hs_op_attend_paged_workspace)."""
+    return lib().hs_op_attend_paged_workspace(*_sizes(streams, t, heads, kv_heads, head_dim, keys))
+
+
+def score_tokens(dev: HipDevice, logits, tokens, table, dims, top: int, logprob, rank, entropy, top_tokens, top_logprob,
+                 bits: Optional[int] = None, stride: Optional[int] = None, stream=None) -> None:
+    """The scores of rows of logits on the device (hs_op_score_dev): dims = (rows, vocab, table length); logits is a
+    tensor [rows, vocab] of int32 or int64 with its symbols together, or an address with `bits` and `stride`."""
+    rows, vocab, length = _sizes(*dims)
+    _sizes(top)
+    if hasattr(logits, "data_ptr"):
+        if tuple(logits.shape) != (rows, vocab) or bits not in (None, 8 * logits.element_size()) or \
+                not _signed(logits) or (vocab > 1 and logits.stride(1) != 1):
+            raise ValueError("logits: [rows, vocab] of int32 or int64, the symbols of a row together")
+        if not getattr(logits, "is_cuda", True):
+            raise ValueError("a tensor in host memory where the GPU reads or writes")
+        bits = 8 * logits.element_size()
+        stride = logits.stride(0) if rows > 1 else vocab
+        logits = logits.data_ptr()
+    _check(lib().hs_op_score_dev(dev.h, logits, bits or 0, *_sizes(vocab if stride is None else stride), _dptr(tokens),
+                                 _dptr(table), length, rows, vocab, top, _dptr(logprob), _dptr(rank), _dptr(entropy),
+                                 _dptr(top_tokens), _dptr(top_logprob), stream))
 
 
 def kernel_resources(dev: HipDevice):

@@ -1,0 +1,202 @@
+"""The refusals of the paged caches' entries and of the scores, without a GPU: every check comes before the device is
+used, so a device that is never opened serves."""
+
+import ctypes as C
+
+import pytest
+
+from taco_amd import hip
+
+FAKE = (C.c_char * 4096)()
+BASE = (C.addressof(FAKE) + 255) // 256 * 256
+BAD, UNSUPPORTED = hip.HS_INVALID_ARGUMENT, hip.HS_UNSUPPORTED
+
+
+class Dev:
+    h = BASE
+
+
+CACHE = hip.PagedCache(BASE, BASE, BASE, BASE, 10, 2, 64, 64, 64)
+RULE = hip.AttentionRule(1 << 20, 36, 1, 59, BASE, 100, 24)
+
+
+def refused(kind, fn, *args, **kw):
+    with pytest.raises(hip.HipError) as e:
+        fn(Dev, *args, **kw)
+    assert e.value.status == kind and e.value.message
+
+
+def append(kind=None, cache=CACHE, k=BASE, v=BASE, table=BASE, ctx=BASE, rows=BASE, dims=(2, 3, 4), headroom=20,
+           ctx_out=BASE + 64, bits=16, stride=None):
+    args = (cache, k, v, table, ctx, rows, dims, headroom, ctx_out, bits, stride)
+    hip.pages_append(Dev, *args) if kind is None else refused(kind, hip.pages_append, *args)
+
+
+def attend(kind=None, cache=CACHE, q=BASE, table=BASE, ctx=BASE, rows=BASE, dims=(2, 3, 4, 4, 200), rule=RULE, out=BASE, **kw):
+    args = (cache, q, table, ctx, rows, dims, rule, out)
+    hip.attend_paged(Dev, *args, **kw) if kind is None else refused(kind, hip.attend_paged, *args, **kw)
+
+
+def score(kind=None, logits=BASE, tokens=BASE, table=BASE, dims=(2, 100, 50), top=3, outs=(BASE,) * 5, bits=32, stride=None):
+    args = (logits, tokens, table, dims, top, *outs, bits, stride)
+    hip.score_tokens(Dev, *args) if kind is None else refused(kind, hip.score_tokens, *args)
+
+
+@pytest.mark.parametrize("fn", [append, attend])
+def test_pools(fn):
+    for name in ("k", "v", "k_scale", "v_scale"):
+        fn(BAD, cache=CACHE._replace(**{name: None}))
+        fn(BAD, cache=CACHE._replace(**{name: BASE + 2}))
+    fn(BAD, cache=CACHE._replace(k=BASE + 8))
+    for hd in (0, 8, 72, 272):
+        fn(UNSUPPORTED, cache=CACHE._replace(head_dim=hd))
+    for page in (0, 8, 48, 2048, 2 ** 32):
+        fn(UNSUPPORTED, cache=CACHE._replace(page=page))
+    for pages in (0, 2 ** 31, 2 ** 32 + 1, -1):
+        fn(UNSUPPORTED, cache=CACHE._replace(pages=pages))
+    for heads in (0, 65536):
+        fn(UNSUPPORTED, cache=CACHE._replace(kv_heads=heads))
+    for most in (0, 1025):
+        fn(UNSUPPORTED, cache=CACHE._replace(max_scale=most))
+
+
+def test_append_refusals():
+    for name in ("k", "v", "table", "ctx"):
+        append(BAD, **{name: None})
+    for name in ("k", "v"):
+        append(BAD, **{name: BASE + 8})
+    for name in ("table", "ctx", "rows", "ctx_out"):
+        append(BAD, **{name: BASE + 2})
+    for bits in (0, 4, 32):
+        append(UNSUPPORTED, bits=bits)
+    for headroom in (0, 15, 65, -1, 2 ** 32 + 16):
+        append(UNSUPPORTED, headroom=headroom)
+    append(UNSUPPORTED, dims=(2, 3, 0))
+    append(UNSUPPORTED, dims=(2, 3, 2 ** 25))   # 2^31 tokens of a stream
+    append(UNSUPPORTED, dims=(2 ** 20, 2 ** 6, 4))
+    append(UNSUPPORTED, dims=(-1, 3, 4))
+    for stride in (127, 132, 2 ** 41, -128):    # 128 values a token
+        append(UNSUPPORTED, stride=stride)
+    append(UNSUPPORTED, bits=8, stride=136)
+    append(BAD, ctx_out=BASE + 4)               # on the second count
+    append(BAD, ctx=BASE + 128, ctx_out=BASE)   # on rows
+    append(dims=(0, 3, 4))
+    append(dims=(2, 0, 4))
+
+
+def test_attend_refusals():
+    for name in ("q", "table", "ctx", "out"):
+        attend(BAD, **{name: None})
+    for name in ("q", "out"):
+        attend(BAD, **{name: BASE + 8})
+    for name in ("table", "ctx", "rows"):
+        attend(BAD, **{name: BASE + 2})
+    for rule in (RULE._replace(attn_exp=None), RULE._replace(attn_exp=BASE + 1)):
+        attend(BAD, rule=rule)
+    attend(UNSUPPORTED, dims=(2, 3, 0, 4, 200))
+    attend(UNSUPPORTED, dims=(2, 3, 5, 4, 200))          # 2 heads in the cache
+    attend(UNSUPPORTED, dims=(2, 3, 4, 4, 0))
+    attend(UNSUPPORTED, dims=(2, 3, 4, 4, 257))          # 4 pages of 64
+    attend(UNSUPPORTED, dims=(2, 3, 4, 2 ** 20, 2 ** 22 + 1))
+    attend(UNSUPPORTED, dims=(2 ** 12, 2 ** 12, 4, 4, 200))
+    attend(UNSUPPORTED, dims=(2, 3, 4, -1, 200))
+    for stride in (240, 264, 2 ** 41, -256):
+        attend(UNSUPPORTED, q_stride=stride)
+    for rule in (RULE._replace(length=0), RULE._replace(length=2 ** 31), RULE._replace(score_m=0), RULE._replace(score_m=-5),
+                 RULE._replace(score_m=2 ** 25), RULE._replace(softmax_p=25)):
+        attend(UNSUPPORTED, rule=rule)
+    attend(UNSUPPORTED, cache=CACHE._replace(max_scale=65))  # counts as 128: 2^24 128 is past 2^30
+    attend(BAD, workspace=BASE + 16, workspace_bytes=1 << 40)
+    attend(dims=(0, 3, 4, 4, 200))
+    attend(dims=(2, 0, 4, 4, 200))
+
+
+def test_workspaces():
+    size = hip.attend_paged_workspace
+    for dims in ((0, 1, 4, 2, 64, 200), (2, 0, 4, 2, 64, 200), (2, 1, 0, 2, 64, 200), (2, 1, 4, 0, 64, 200), (2, 1, 5, 2, 64, 200),
+                 (2, 1, 4, 2, 0, 200), (2, 1, 4, 2, 272, 200), (2, 1, 4, 2, 64, 0), (2, 1, 4, 2, 64, 2 ** 22 + 1),
+                 (2 ** 40, 1, 4, 2, 64, 200), (2 ** 20, 2 ** 20, 4, 2, 64, 200), (2, 1, 2 ** 40, 2, 64, 200)):
+        assert size(*dims) == 0, dims
+    with pytest.raises(hip.Unsupported):
+        size(-1, 1, 4, 2, 64, 200)
+
+
+def test_score_refusals():
+    score(BAD, logits=None)
+    score(BAD, table=None)
+    score(BAD, tokens=None)
+    score(BAD, logits=BASE + 2)
+    score(BAD, logits=BASE + 4, bits=64)
+    score(BAD, table=BASE + 4)
+    score(BAD, tokens=BASE + 1)
+    for i in range(5):
+        score(BAD, outs=[BASE + 2 if i == j else BASE for j in range(5)])
+    for bits in (0, 16):
+        score(UNSUPPORTED, bits=bits)
+    for dims in ((2, 0, 50), (2, 2 ** 24 + 1, 50), (2, 100, 0), (2, 100, 2 ** 31), (2 ** 22, 100, 50), (-1, 100, 50)):
+        score(UNSUPPORTED, dims=dims)
+    for top in (65, 101, -1):
+        score(UNSUPPORTED, top=top)
+    score(UNSUPPORTED, dims=(2, 2, 50))  # 3 alternatives of 2 symbols
+    for stride in (99, 2 ** 41, -100):
+        score(UNSUPPORTED, stride=stride)
+    score(dims=(0, 100, 50))
+
+
+def test_tensors():
+    """Tensors of other types, shapes and places are refused before their addresses are used."""
+    torch = pytest.importorskip("torch")
+
+    class Fake:
+        is_cuda = True
+
+        def __init__(self, x):
+            self.x, self.shape, self.dtype = x, x.shape, x.dtype
+
+        def __getattr__(self, name):
+            return getattr(self.x, name)
+
+        def data_ptr(self):
+            return BASE
+
+    rows = lambda dtype, *shape: Fake(torch.zeros(shape or (2, 3, 2, 64), dtype=dtype))  # noqa: E731
+    good = rows(torch.int16)
+    for bad in (rows(torch.float16), rows(torch.uint8), rows(torch.int16, 2, 3, 2, 32), rows(torch.int8),
+                Fake(torch.zeros(2, 3, 2, 128, dtype=torch.int16)[..., ::2]), Fake(torch.zeros(2, 2, 3, 64, dtype=torch.int16).transpose(1, 2)),
+                Fake(torch.zeros(2, 6, 2, 64, dtype=torch.int16)[:, :3]), torch.zeros(2, 3, 2, 64, dtype=torch.int16)):
+        with pytest.raises(ValueError):
+            append(k=good, v=bad, bits=None)
+        with pytest.raises(ValueError):
+            append(k=bad, v=good, bits=None)
+    with pytest.raises(ValueError):  # keys and values at different distances
+        append(k=good, v=Fake(torch.zeros(2, 3, 2, 2, 64, dtype=torch.int16)[:, :, 0]), bits=None)
+    for bad in (rows(torch.int16, 2, 3, 4, 64), rows(torch.int8, 2, 3, 2, 64), torch.zeros(2, 3, 4, 64, dtype=torch.int8)):
+        with pytest.raises(ValueError):
+            attend(q=bad)
+    for bad in (rows(torch.float32, 2, 100), rows(torch.int32, 2, 99), Fake(torch.zeros(100, 2, dtype=torch.int32).T),
+                torch.zeros(2, 100, dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            score(logits=bad, bits=None)
+    kv = torch.zeros(2, 3, 2, 2, 64, dtype=torch.int16)  # parts of wider rows
+    assert hip._rows_of(Fake(kv[:, :, 1]), None, 128) == (BASE, 256)
+    assert hip._rows_of(Fake(kv[:1, :1, 1]), None, 128) == (BASE, 128)
+
+
+def test_batch_tokens():
+    """What run_scored makes of its tokens: other numbers than symbols and `none` stay outside the vocabulary."""
+    class Batch:
+        vocab = 300
+
+    seen = []
+
+    def call(t, *out):
+        seen.extend(C.cast(t, C.POINTER(C.c_uint32))[:8])
+        return 0
+
+    out = hip.HipBatch._scored(Batch, 8, [0, -1, 299, 300, 2 ** 32 - 1, 2 ** 32, 2 ** 40, -2], 2, call)
+    none = hip.HS_NO_TOKEN
+    assert seen == [0, none, 299, 300, none, 300, 300, 300] and out.top_tokens.shape == (8, 2)
+    with pytest.raises(hip.LengthMismatch):
+        hip.HipBatch._scored(Batch, 3, [1], 2, call)
+    with pytest.raises(hip.Unsupported):
+        hip.HipBatch._scored(Batch, 3, [1, 2, 3], -1, call)
