@@ -17,7 +17,7 @@ HOST_SOURCES = {"common.cpp", "hsm.cpp", "taco/harness.cpp", "taco/tokenizer.cpp
 
 BACKEND_SOURCES = ["common.cpp", "hsm.cpp", "hs_api.cpp", "kernels.hip",
                    "gemm_rows.hip", "layernorm.hip", "attend_rows.hip", "cache_ops.hip",
-                   "paged.hip", "score.hip"]
+                   "paged.hip", "attend_paged.hip", "score.hip"]
 HARNESS_SOURCES = ["taco/harness.cpp", "taco/tokenizer.cpp"]  # hs::fail, sha256: the backend's (one error state)
 
 LIB_BACKEND = os.path.join(HERE, "libhardshell_hip.so")

@@ -2299,6 +2299,7 @@ hs_status attend_paged_args(hs_device *dev, const hs_pages *cache, size_t b, siz
     if (keys == 0 || keys > (size_t)1 << 22 || keys > width * cache->page)
         return hs::fail(HS_UNSUPPORTED, 0, "keys must be in 1..=2^22 and fit the pages of a stream");
     g.streams = (int)b; g.t = (int)t; g.heads = (int)h; g.width = (int)width; g.keys = (int)keys;
+    if (b && t && !hs::paged_fits(g)) return hs::fail(HS_UNSUPPORTED, 0, "too many rows, heads and keys (2^23 workgroups)");
     return HS_OK;
 }
 
@@ -2338,7 +2339,7 @@ extern "C" size_t hs_op_attend_paged_workspace(size_t b, size_t t, size_t h, siz
         return 0;  // (the call itself refuses them, or does nothing)
     g.streams = (int)b; g.t = (int)t; g.heads = (int)h; g.keys = (int)keys;
     g.pages.kv_heads = (int)kv_heads; g.pages.hd = (int)hd;
-    return hs::paged_workspace(g);
+    return hs::paged_fits(g) ? hs::paged_workspace(g) : 0;
 }
 
 extern "C" hs_status hs_op_attend_paged_dev(hs_device *dev, const hs_pages *cache, const int8_t *q, size_t q_stride,

@@ -355,8 +355,10 @@ struct PagedArgs {
     int out_s = 0;
     const int32_t *exp_table = nullptr;
     int exp_len = 0, softmax_p = 0;
+    int table_lds = 0;      // (set by the launch) the tiles of 16 rows copy the table to LDS
     int8_t *out = nullptr;  // [streams][t][heads][hd]
 };
+bool paged_fits(const PagedArgs &g);  // a grid holds fewer than 2^32 threads
 size_t paged_workspace(const PagedArgs &g);
 hipError_t launch_paged(const PagedArgs &g, void *workspace, hipStream_t stream);
 
