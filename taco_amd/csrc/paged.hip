@@ -10,62 +10,108 @@ __device__ __forceinline__ uint32_t page_scale(uint32_t most, const AppendArgs &
     return s < 1 ? 1 : (s > a.pages.max_scale ? a.pages.max_scale : s);
 }
 
-// The stored byte of x: round(x / s), halves up, clamped.
-__device__ __forceinline__ int8_t page_byte(int32_t x, int32_t s) {
-    const int32_t n = 2 * x + s, d = 2 * s;
-    int32_t q = n / d;
-    if (n - q * d < 0) q--;
-    return (int8_t)(q < -127 ? -127 : (q > 127 ? 127 : q));
+// floor((2 x + s) / (2 s)) = floor(x / s + 1/2), clamped to +-127, in single precision: x / s + 1/2 is a multiple of 1 / (2 s), s <=
+// 2^10, so it lies on an integer or 2^-11 from one; where the clamp does not decide, |x / s| < 128 and the roundings (1 / s, the
+// multiply-add) are below 2^-15. 2^-13 added keeps them from reaching below an integer.
+__device__ __forceinline__ int32_t page_byte(int32_t x, float inv) {
+    return (int32_t)__builtin_amdgcn_fmed3f(floorf(fmaf((float)x, inv, 0.5f + 0x1p-13f)), -127.0f, 127.0f);
 }
 
-__device__ __forceinline__ uint32_t held_scale(uint32_t s, uint32_t most) { return s < 1 ? 1 : (s > most ? most : s); }
-
-// A wave for each (stream, row, head), K and V in turn.
+// A wave for each head of a run of tokens of one stream: CR tokens of one page (a run never crosses pages), K or V. A lane takes
+// 16 channels of a row: 16 bytes of the page, so that a wave stores a whole KiB of it at a time, and reads 16 (i8) or 32
+// (i16) bytes. Every wave takes the scale from the page's first row by itself, so no wave waits for another.
 template <typename X>
-__global__ __launch_bounds__(256) void k_append(AppendArgs a, size_t n_tasks) {
-    const int lane = threadIdx.x & 63;
-    const size_t task = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (task >= n_tasks) return;
+__global__ __launch_bounds__(256) void k_append(AppendArgs a, int run, int runs, size_t n_tasks) {
     const PagePool &p = a.pages;
-    const int h = (int)(task % p.kv_heads), i = (int)(task / p.kv_heads % a.t), s = (int)(task / p.kv_heads / a.t);
+    const int lane = threadIdx.x & 63;
+    const size_t task = (size_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (task >= n_tasks) return;
+    const int which = (int)(task & 1), h = (int)((task >> 1) % p.kv_heads);
+    const size_t rest = (task >> 1) / p.kv_heads;
+    const int c = (int)(rest % runs), s = (int)(rest / runs);
     const uint32_t cap = (uint32_t)a.width * p.page, n = a.ctx[s] < cap ? a.ctx[s] : cap;
     uint32_t rows = a.rows ? a.rows[s] : (uint32_t)a.t;
     rows = rows < (uint32_t)a.t ? rows : (uint32_t)a.t;
     rows = rows < cap - n ? rows : cap - n;
-    if (a.ctx_out && i == 0 && h == 0 && lane == 0) a.ctx_out[s] = n + rows;
-    if ((uint32_t)i >= rows) return;
-    const uint32_t at = n + i, place = at % p.page, number = a.table[(size_t)s * a.width + at / p.page];
+    if (a.ctx_out && c == 0 && h == 0 && which == 0 && lane == 0) a.ctx_out[s] = n + rows;
+    // the run's tokens t0 .. t1 - 1 of the stream's
+    const uint32_t r0 = (n / run + c) * run, t0 = r0 > n ? r0 : n, t1 = r0 + run < n + rows ? r0 + run : n + rows;
+    if (t0 >= t1) return;
+    const uint32_t number = a.table[(size_t)s * a.width + t0 / p.page], start = t0 / p.page * p.page;
     if (number >= (uint32_t)p.pages) return;
     const size_t panel = (size_t)number * p.kv_heads + h;
-    for (int which = 0; which < 2; which++) {
-        const X *x = (const X *)(which ? a.v : a.k) + ((size_t)s * a.t + i) * a.stride + (size_t)h * p.hd;
-        int8_t *to = (which ? p.v : p.k) + (panel * p.page + place) * p.hd;
-        uint32_t *scales = which ? p.v_scale : p.k_scale;
-        uint32_t scale = 1;
-        if (sizeof(X) > 1) {
-            if (place <= (uint32_t)i) {  // the page's first row is of this call
-                const X *first = x - (size_t)place * a.stride;
-                int64_t most = 0;
-                for (int c = lane; c < p.hd; c += 64) {
-                    const int64_t m = first[c] < 0 ? -(int64_t)first[c] : first[c];
-                    most = m > most ? m : most;
+    const X *from = (const X *)(which ? a.v : a.k) + (size_t)s * a.t * a.stride + (size_t)h * p.hd;  // token n
+    int8_t *to = (which ? p.v : p.k) + (panel * p.page + t0 - start) * p.hd;
+    uint32_t *scales = which ? p.v_scale : p.k_scale;
+    const int units = p.hd / 16;  // of a row
+    float inv = 1.0f;
+    if constexpr (sizeof(X) > 1) {
+        uint32_t scale;
+        if (start >= n) {  // the page's first row is of this call
+            int32_t most = 0;
+            if (lane < units) {
+                const v4i *x = (const v4i *)(from + (size_t)(start - n) * a.stride + 16 * lane);
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const v4i y = x[k];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int32_t lo = (int16_t)y[e], hi = y[e] >> 16;
+                        const int32_t al = lo < 0 ? -lo : lo, ah = hi < 0 ? -hi : hi;
+                        most = al > most ? al : most;
+                        most = ah > most ? ah : most;
+                    }
                 }
-                scale = page_scale((uint32_t)wave_max64(most), a);
-            } else {
-                scale = held_scale(scales[panel], p.max_scale);
             }
+            int32_t least = 0;
+            wave_min_max(least, most);
+            scale = page_scale((uint32_t)most, a);
+            if (t0 == start && lane == 0) scales[panel] = scale;
+        } else {
+            scale = scales[panel];
+            scale = scale < 1 ? 1 : (scale > p.max_scale ? p.max_scale : scale);
         }
-        if (place == 0 && lane == 0) scales[panel] = scale;
-        for (int c = lane; c < p.hd; c += 64) to[c] = sizeof(X) > 1 ? page_byte(x[c], (int32_t)scale) : (int8_t)x[c];
+        inv = 1.0f / (float)scale;
+    } else if (t0 == start && lane == 0) {
+        scales[panel] = 1;
+    }
+    const int total = (int)(t1 - t0) * units;
+    for (int i0 = lane; i0 < total; i0 += 256) {
+        constexpr int L = sizeof(X);  // 16-byte loads of a unit
+        v4i x[4][L];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int i = i0 + 64 * k < total ? i0 + 64 * k : i0, row = i / units;
+            const v4i *y = (const v4i *)(from + (size_t)(t0 - n + row) * a.stride + 16 * (i - row * units));
+#pragma unroll
+            for (int l = 0; l < L; l++) x[k][l] = y[l];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (i0 + 64 * k >= total) break;
+            v4i out;
+            if constexpr (sizeof(X) > 1) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int32_t lo = x[k][e >> 1][2 * (e & 1)], hi = x[k][e >> 1][2 * (e & 1) + 1];
+                    const uint32_t b0 = page_byte((int16_t)lo, inv), b1 = page_byte(lo >> 16, inv), b2 = page_byte((int16_t)hi, inv),
+                                   b3 = page_byte(hi >> 16, inv);
+                    out[e] = (int32_t)((b0 & 255) | (b1 & 255) << 8 | (b2 & 255) << 16 | b3 << 24);
+                }
+            } else {
+                out = x[k][0];
+            }
+            ((v4i *)to)[i0 + 64 * k] = out;
+        }
     }
 }
 
 hipError_t launch_append(const AppendArgs &a, hipStream_t stream) {
-    const size_t tasks = (size_t)a.streams * a.t * a.pages.kv_heads;
-    if (tasks == 0) return hipSuccess;
+    const int run = a.pages.page < 64 ? a.pages.page : 64, runs = (a.t + 2 * run - 2) / run;
+    const size_t tasks = (size_t)a.streams * runs * a.pages.kv_heads * 2;
     const dim3 grid((unsigned)((tasks + 3) / 4));
-    if (a.bits == 8) launch_k(k_append<int8_t>, grid, dim3(256), 0, stream, a, tasks);
-    else launch_k(k_append<int16_t>, grid, dim3(256), 0, stream, a, tasks);
+    if (a.bits == 8) launch_k(k_append<int8_t>, grid, dim3(256), 0, stream, a, run, runs, tasks);
+    else launch_k(k_append<int16_t>, grid, dim3(256), 0, stream, a, run, runs, tasks);
     return hipGetLastError();
 }
 

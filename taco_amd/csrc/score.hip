@@ -37,75 +37,434 @@ struct ScoreRow {
     }
 };
 
-// Any vocabulary and table: a workgroup a row, which walks it for the row max, the sum, the entropy and the rank, and
-// once for each alternative (the next in the order after the one before).
-template <int SRC>
-__global__ __launch_bounds__(256) void k_score_any(ScoreArgs a) {
-    __shared__ uint64_t s_u[4];
-    __shared__ double s_d[4];
-    const int tid = threadIdx.x, r = blockIdx.x, V = a.vocab;
-    const ScoreRow<SRC> row(a, r);
-    auto all = [&](auto v, auto *slots, auto join) {  // join over the workgroup
+// What a row's results need: the token's log probability and rank, and an alternative.
+__device__ __forceinline__ void put_token(const ScoreArgs &a, size_t r, bool some, uint64_t w, uint64_t total, uint32_t rank) {
+    if (a.logprob) a.logprob[r] = some ? (float)log_share(w, total) : 0.0f;
+    if (a.rank) a.rank[r] = some ? rank : 0xffffffffu;
+}
+__device__ __forceinline__ void put_top(const ScoreArgs &a, size_t r, int i, uint32_t token, int d, uint64_t total) {
+    if (a.top_tokens) a.top_tokens[r * a.top + i] = token;
+    if (a.top_logprob) a.top_logprob[r * a.top + i] = (float)log_share(a.table[d], total);
+}
+
+// join over a workgroup of NW waves
+template <int NW, typename T, typename F>
+__device__ __forceinline__ T block_join(T v, void *slots, F join) {
+    T *s = (T *)slots;
+    const int tid = threadIdx.x;
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) v = join(v, __shfl_xor(v, o, 64));
-        __syncthreads();
-        if ((tid & 63) == 0) slots[tid >> 6] = v;
-        __syncthreads();
-        return join(join(slots[0], slots[1]), join(slots[2], slots[3]));
-    };
+    for (int o = 32; o > 0; o >>= 1) v = join(v, __shfl_xor(v, o, 64));
+    __syncthreads();
+    if ((tid & 63) == 0) s[tid >> 6] = v;
+    __syncthreads();
+    v = s[0];
+#pragma unroll
+    for (int i = 1; i < NW; i++) v = join(v, s[i]);
+    return v;
+}
+struct Add {
+    template <typename T>
+    __device__ T operator()(T x, T y) const { return x + y; }
+};
+struct Max {
+    template <typename T>
+    __device__ T operator()(T x, T y) const { return x > y ? x : y; }
+};
+struct Min {
+    template <typename T>
+    __device__ T operator()(T x, T y) const { return x < y ? x : y; }
+};
+
+// A row by itself, any vocabulary and table: the workgroup walks it for the row max, the sum, the entropy and the rank,
+// and once for each alternative (the next in the order after the one before).
+template <int SRC, int NW>
+__device__ void score_any_row(const ScoreArgs &a, size_t r, void *slots) {
+    const int tid = threadIdx.x, V = a.vocab, NT = 64 * NW;
+    const ScoreRow<SRC> row(a, r);
     int64_t mx = INT64_MIN;
-    for (int j = tid; j < row.maxima(); j += 256) {
+    for (int j = tid; j < row.maxima(); j += NT) {
         const int64_t x = row.maximum(j);
         mx = x > mx ? x : mx;
     }
-    const int64_t M = all(mx, (int64_t *)s_u, [](int64_t x, int64_t y) { return x > y ? x : y; });
-    auto add = [](uint64_t x, uint64_t y) { return x + y; };
+    const int64_t M = block_join<NW>(mx, slots, Max());
     const uint32_t token = a.tokens ? a.tokens[r] : 0xffffffffu;
-    const int td = token < (uint32_t)V ? row.index(M, (int)token) : 0;
+    const bool some = token < (uint32_t)V;
+    const int td = some ? row.index(M, (int)token) : 0;
     uint64_t sum = 0, ahead = 0;
-    for (int j = tid; j < V; j += 256) {
+    for (int j = tid; j < V; j += NT) {
         const int d = row.index(M, j);
         sum += a.table[d];
         ahead += d < td || (d == td && (uint32_t)j < token);
     }
-    const uint64_t T = all(sum, s_u, add);
-    ahead = all(ahead, s_u, add);
-    if (tid == 0) {
-        const bool some = token < (uint32_t)V;
-        if (a.logprob) a.logprob[r] = some ? (float)log_share(a.table[td], T) : 0.0f;
-        if (a.rank) a.rank[r] = some ? (uint32_t)ahead : 0xffffffffu;
-    }
+    const uint64_t T = block_join<NW>(sum, slots, Add());
+    ahead = block_join<NW>(ahead, slots, Add());
+    if (tid == 0) put_token(a, r, some, a.table[td], T, (uint32_t)ahead);
     if (a.entropy) {
         double h = 0;
-        for (int j = tid; j < V; j += 256) {
+        for (int j = tid; j < V; j += NT) {
             const uint64_t w = a.table[row.index(M, j)];
             if (w) h -= (double)w / (double)T * log_share(w, T);
         }
-        h = all(h, s_d, [](double x, double y) { return x + y; });
+        h = block_join<NW>(h, slots, Add());
         if (tid == 0) a.entropy[r] = (float)h;
     }
     int64_t before = -1;  // (d, symbol) of the last one found
     for (int i = 0; i < a.top; i++) {
         int64_t next = INT64_MAX;
-        for (int j = tid; j < V; j += 256) {
+        for (int j = tid; j < V; j += NT) {
             const int64_t x = (int64_t)row.index(M, j) << 32 | j;
             if (x > before && x < next) next = x;
         }
-        before = all(next, (int64_t *)s_u, [](int64_t x, int64_t y) { return x < y ? x : y; });
-        if (tid == 0) {
-            if (a.top_tokens) a.top_tokens[(size_t)r * a.top + i] = (uint32_t)before;
-            if (a.top_logprob) a.top_logprob[(size_t)r * a.top + i] = (float)log_share(a.table[before >> 32], T);
+        before = block_join<NW>(next, slots, Min());
+        if (tid == 0) put_top(a, r, i, (uint32_t)before, (int)(before >> 32), T);
+    }
+}
+template <int SRC>
+__global__ __launch_bounds__(512) void k_score_any(ScoreArgs a) {
+    __shared__ uint64_t slots[8];
+    score_any_row<SRC, 8>(a, blockIdx.x, slots);
+}
+
+// A row in the registers of a workgroup: read once, 4 G symbols a lane, their table indexes kept in 16 bits each and counted
+// in an LDS histogram. Symbols past the table's end (and the places of the last groups past the row) go to 64 spare bins, each
+// lane's in its own, so that no symbol needs a test and none of these many collide. The counts give T, the entropy and the
+// token's rank but for ties; one wave walks them for the index up to which the alternatives lie, and the symbols up to
+// there, few, are collected and ranked against each other.
+constexpr int SCORE_LIST = 1024;   // symbols collected; where ties make them more, the alternatives are searched one by one
+constexpr int SCORE_BINS = 16384;  // entries of the table at most
+
+template <int SRC, int G, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) void k_score_rows(ScoreArgs a) {
+    constexpr int NT = 64 * NW;
+    extern __shared__ uint32_t s_hist[];  // [table_len + 63]
+    __shared__ uint64_t slots[NW], s_list[SCORE_LIST];
+    __shared__ uint32_t s_count, s_thr, s_found;
+    const int tid = threadIdx.x, lane = tid & 63, V = a.vocab, last = a.table_len - 1;
+    const size_t r = blockIdx.x;
+    const uint32_t token = a.tokens ? a.tokens[r] : 0xffffffffu;
+    const bool some = token < (uint32_t)V;
+    const uint32_t cap = (uint32_t)(last + lane);  // this lane's bin of what lies past the table's end
+    uint32_t d2[2 * G];                            // min(d, cap), pairs
+    int off = 0;                                   // symbol of element e of group i: 4 (NT i + tid) + e - off
+    const ScoreRow<SRC> row(a, (int)r);
+    int td = 0;  // the token's index
+    auto symbol = [&](int i, int e) { return 4 * (NT * i + tid) + e - off; };
+    auto inside = [&](int j) { return j >= 0 && j < V; };
+    auto partial = [&](int i) { return symbol(i, 0) < 0 || symbol(i, 3) >= V; };  // a group not all of which is the row's
+    for (int k = tid; k < last + 64; k += NT) s_hist[k] = 0;
+    if (tid == 0) s_count = 0;
+
+    if constexpr (SRC == SCORE_COMPACT) {
+        const int64_t *tm = a.tmax + r * a.ntiles;
+        const uint16_t *p = a.d16 + r * a.ld16;  // whole tiles of 64 (the row is padded)
+        uint2 raw[G];
+        int64_t t[G];
+#pragma unroll
+        for (int i = 0; i < G; i++) {
+            const int j = symbol(i, 0) < V ? symbol(i, 0) : 0;
+            raw[i] = *(const uint2 *)(p + j);
+            t[i] = tm[j >> 6];
+        }
+        int64_t mx = INT64_MIN;
+        for (int j = tid; j < a.ntiles; j += NT) mx = tm[j] > mx ? tm[j] : mx;
+        const int64_t M = block_join<NW>(mx, slots, Max());
+        if (some) td = row.index(M, (int)token);
+#pragma unroll
+        for (int i = 0; i < G; i++) {
+            const uint64_t b = (uint64_t)M - (uint64_t)t[i];
+            const uint32_t base = b < (uint64_t)cap ? (uint32_t)b : cap;
+            uint32_t d[4] = {raw[i].x & 0xffffu, raw[i].x >> 16, raw[i].y & 0xffffu, raw[i].y >> 16};
+#pragma unroll
+            for (int e = 0; e < 4; e++) d[e] = d[e] + base < (uint32_t)last ? d[e] + base : cap;  // (a d16 may be capped at last)
+            d2[2 * i] = d[0] | d[1] << 16;
+            d2[2 * i + 1] = d[2] | d[3] << 16;
+        }
+    } else {
+        // 16-byte loads, from the 16 bytes that the row starts in to those that it ends in
+        constexpr int E = SRC == SCORE_I32 ? 4 : 8;
+        const uintptr_t at = (uintptr_t)a.logits + r * a.ld * E;
+        off = (int)(at % 16) / E;
+        const uint4 *p = (const uint4 *)(at - at % 16);
+        const int loads = (int)(((off + (size_t)V) * E + 15) / 16);
+        int32_t x[4 * G];
+        bool fits = true;
+        int64_t ref = 0;
+        const int64_t of_token = some ? row.value((int)token) : 0;
+        if constexpr (SRC == SCORE_I32) {
+#pragma unroll
+            for (int i = 0; i < G; i++) {
+                const uint4 y = p[NT * i + tid < loads ? NT * i + tid : 0];
+                x[4 * i] = (int32_t)y.x;
+                x[4 * i + 1] = (int32_t)y.y;
+                x[4 * i + 2] = (int32_t)y.z;
+                x[4 * i + 3] = (int32_t)y.w;
+            }
+        } else {
+            // differences to the row's first logit, in 32 bits
+            ref = ((const int64_t *)at)[0];
+            constexpr int B = G % 3 == 0 ? 3 : G % 4 == 0 ? 4 : 1;  // groups in flight beside those at work
+            uint4 raw[2][B][2];
+            auto fetch = [&](int i0, uint4(&y)[B][2]) {
+#pragma unroll
+                for (int i = 0; i < B; i++)
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        const int l = 2 * (NT * (i0 + i) + tid) + k;
+                        y[i][k] = p[l < loads ? l : 0];
+                    }
+            };
+            fetch(0, raw[0]);
+#pragma unroll
+            for (int i0 = 0; i0 < G; i0 += B) {
+                uint4(&y)[B][2] = raw[(i0 / B) & 1];
+                __builtin_amdgcn_sched_barrier(0);
+                if (i0 + B < G) fetch(i0 + B, raw[(i0 / B + 1) & 1]);
+#pragma unroll
+                for (int i = 0; i < B; i++) {
+                    bool in = true;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const uint4 q = y[i][e >> 1];
+                        const int64_t l = (int64_t)(e & 1 ? (uint64_t)q.w << 32 | q.z : (uint64_t)q.y << 32 | q.x);
+                        int64_t d;
+                        const bool over = __builtin_sub_overflow(l, ref, &d);
+                        in = in && !over && d == (int32_t)d;
+                        x[4 * (i0 + i) + e] = (int32_t)d;
+                    }
+                    fits = fits && (in || partial(i0 + i));
+                }
+            }
+            // (a group at the row's ends, by itself)
+#pragma unroll
+            for (int i = 0; i < G; i++)
+                if (partial(i))
+                    for (int e = 0; e < 4; e++) {
+                        int64_t d;
+                        const int j = symbol(i, e);
+                        if (inside(j)) fits = !__builtin_sub_overflow(((const int64_t *)at)[j], ref, &d) && d == (int32_t)d && fits;
+                    }
+        }
+        int32_t mx = INT32_MIN;
+#pragma unroll
+        for (int i = 0; i < G; i++) {
+            if (partial(i)) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[4 * i + e] = inside(symbol(i, e)) ? x[4 * i + e] : INT32_MIN;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) mx = x[4 * i + e] > mx ? x[4 * i + e] : mx;
+        }
+        if constexpr (SRC == SCORE_I64) {
+            if (__syncthreads_or(!fits)) {  // logits that lie further apart: uniform
+                score_any_row<SRC, NW>(a, r, slots);
+                return;
+            }
+        }
+        const int32_t m = block_join<NW>(mx, slots, Max());
+        if (some) {
+            const uint64_t d = (uint64_t)(int64_t)m + (uint64_t)ref - (uint64_t)of_token;
+            td = d < (uint64_t)last ? (int)d : last;
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * G; i++) {
+            uint32_t d[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const uint32_t y = (uint32_t)m - (uint32_t)x[2 * i + e];  // (unsigned: any two)
+                d[e] = y < cap ? y : cap;
+            }
+            d2[i] = d[0] | d[1] << 16;
         }
     }
+#pragma unroll
+    for (int i = 0; i < G; i++)
+        if (partial(i)) {
+            const uint32_t d[4] = {d2[2 * i] & 0xffffu, d2[2 * i] >> 16, d2[2 * i + 1] & 0xffffu, d2[2 * i + 1] >> 16};
+            uint32_t y[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = inside(symbol(i, e)) ? d[e] : cap;
+            d2[2 * i] = y[0] | y[1] << 16;
+            d2[2 * i + 1] = y[2] | y[3] << 16;
+        }
+    // (hides the pairs from the optimizer, which would keep every index unpacked from one walk to the next)
+    auto hide = [&] {
+#pragma unroll
+        for (int i = 0; i < 2 * G; i++) asm volatile("" : "+v"(d2[i]));
+    };
+    auto index = [&](int i, int e) { return e & 1 ? d2[2 * i + (e >> 1)] >> 16 : d2[2 * i + (e >> 1)] & 0xffffu; };
+    // fn(symbol, index) for the symbols with an index in lo ..= hi (rare ones)
+    auto those = [&](uint32_t lo, uint32_t hi, auto fn) {
+        hide();
+        if (hi >= (uint32_t)last) hi = 0xffffu;
+#pragma unroll
+        for (int i = 0; i < G; i++) {
+            uint32_t in = 0, p0 = d2[2 * i], p1 = d2[2 * i + 1];
+#pragma unroll
+            for (int e = 0; e < 4; e++) in |= index(i, e) - lo <= hi - lo ? 1u << e : 0u;
+            asm volatile("" : "+v"(p0), "+v"(p1));  // (else the choice below makes an array in memory of all pairs)
+            for (; in; in &= in - 1) {
+                const int e = __ffs(in) - 1, j = symbol(i, e);
+                const uint32_t d = ((e & 2 ? p1 : p0) >> (16 * (e & 1))) & 0xffffu;
+                if (inside(j)) fn(j, d < (uint32_t)last ? (int)d : last);
+            }
+        }
+    };
+    hide();
+#pragma unroll
+    for (int i = 0; i < G; i++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) atomicAdd(&s_hist[index(i, e)], 1u);
+        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    }
+    hide();
+    __syncthreads();
+    if (tid < 64) {  // the spare bins to the last one, without the places past the row
+        const uint32_t far = (uint32_t)wave_sum64(s_hist[last + tid]);
+        if (tid == 0) s_hist[last] = far - (uint32_t)(4 * G * NT - V);
+    }
+    __syncthreads();
+
+    // T, and the symbols that lie before the token
+    constexpr int KB = 16;  // bins of a lane kept from the sum to the entropy
+    uint64_t sum = 0;
+    uint32_t ahead = 0, n[KB];
+    float wf[KB];
+#pragma unroll
+    for (int k0 = 0; k0 < KB; k0 += 4) {
+        uint64_t w[4];
+#pragma unroll
+        for (int k = k0; k < k0 + 4; k++) {
+            const int d = tid + NT * k;
+            n[k] = d <= last ? s_hist[d] : 0;
+            w[k - k0] = n[k] ? a.table[d] : 0;
+        }
+#pragma unroll
+        for (int k = k0; k < k0 + 4; k++) {
+            sum += n[k] * w[k - k0];
+            wf[k] = (float)w[k - k0];
+            ahead += tid + NT * k < td ? n[k] : 0;
+        }
+    }
+    for (int d = tid + NT * KB; d <= last; d += NT) {
+        const uint32_t c = s_hist[d];
+        if (c) sum += c * a.table[d];
+        ahead += d < td ? c : 0;
+    }
+    const uint64_t T = block_join<NW>(sum, slots, Add());
+    if (a.entropy) {
+        // f32 terms: T / w >= 2 but for at most one symbol, whose logarithm is taken in 64 bits. Their roundings (T, w, the
+        // quotients, the logarithm, of at least ln 2) stay below 2^-21 of a term.
+        const float Tf = (float)T;
+        double hsum = 0;
+        auto term = [&](uint32_t c, float x, int d) {
+            if (!(x > 0)) return;
+            const float q = Tf / x;
+            const float l = q < 2.1f ? (float)-log_share(a.table[d], T) : __logf(q);
+            hsum += (float)c * l / q;
+        };
+#pragma unroll
+        for (int k = 0; k < KB; k++) term(n[k], wf[k], tid + NT * k);
+        for (int d = tid + NT * KB; d <= last; d += NT)
+            if (s_hist[d]) term(s_hist[d], (float)a.table[d], d);
+        hsum = block_join<NW>(hsum, slots, Add());
+        if (tid == 0) a.entropy[r] = (float)hsum;
+    }
+    if (a.rank) {  // ties of the token that come before it
+        if (some && s_hist[td] > 1) those((uint32_t)td, (uint32_t)td, [&](int j, int) { ahead += j < (int)token; });  // uniform
+        ahead = block_join<NW>(ahead, slots, Add());
+    }
+    if (tid == 0 && (a.logprob || a.rank)) put_token(a, r, some, some ? a.table[td] : 0, T, ahead);
+    if (a.top == 0 || !(a.top_tokens || a.top_logprob)) return;
+
+    // the index up to which `top` symbols lie, and how many lie up to it: one wave over 256 bins at a time
+    if (tid < 64) {
+        uint32_t before = 0;
+        for (int k0 = 0; k0 <= last; k0 += 256) {
+            uint32_t c[4], mine = 0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                c[k] = k0 + 4 * lane + k <= last ? s_hist[k0 + 4 * lane + k] : 0;
+                mine += c[k];
+            }
+            uint32_t upto = mine;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t y = __shfl_up(upto, o, 64);
+                if (lane >= o) upto += y;
+            }
+            const uint64_t reached = __ballot(before + upto >= (uint32_t)a.top);
+            if (reached) {  // (top <= vocab: some bin does)
+                if (lane == __ffsll((unsigned long long)reached) - 1) {
+                    uint32_t y = before + upto - mine;
+                    int k = -1;
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (y < (uint32_t)a.top) y += c[i], k = i;
+                    s_thr = (uint32_t)(k0 + 4 * lane + k);
+                    s_found = y;
+                }
+                break;
+            }
+            before += __shfl(upto, 63, 64);
+        }
+    }
+    __syncthreads();
+    const uint32_t thr = s_thr;
+    if (s_found <= SCORE_LIST) {  // uniform
+        those(0, thr, [&](int j, int d) { s_list[atomicAdd(&s_count, 1u)] = (uint64_t)d << 32 | (uint32_t)j; });
+        __syncthreads();
+        const int found = (int)s_found;
+        for (int i = tid; i < found; i += NT) {
+            const uint64_t x = s_list[i];
+            int place = 0;
+            for (int k = 0; k < found; k++) place += s_list[k] < x;
+            if (place < a.top) put_top(a, r, place, (uint32_t)x, (int)(x >> 32), T);
+        }
+        return;
+    }
+    int64_t one = -1;  // the last one found
+    for (int i = 0; i < a.top; i++) {
+        int64_t next = INT64_MAX;
+        those(0, thr, [&](int j, int d) {
+            const int64_t x = (int64_t)d << 32 | j;
+            if (x > one && x < next) next = x;
+        });
+        one = block_join<NW>(next, slots, Min());
+        if (tid == 0) put_top(a, r, i, (uint32_t)one, (int)(one >> 32), T);
+    }
+}
+
+template <int SRC, int G, int NW>
+static hipError_t launch_score_rows(const ScoreArgs &a, int n_rows, hipStream_t stream) {
+    const size_t lds = 4 * ((size_t)a.table_len + 63);
+    const hipError_t e = allow_dynamic_lds((const void *)k_score_rows<SRC, G, NW>, lds);
+    if (e != hipSuccess) return e;
+    launch_k((k_score_rows<SRC, G, NW>), dim3(n_rows), dim3(64 * NW), lds, stream, a);
+    return hipGetLastError();
+}
+
+template <int SRC>
+static hipError_t launch_score_src(const ScoreArgs &a, int n_rows, hipStream_t stream) {
+    if (a.table_len <= SCORE_BINS) {
+        const int v = a.vocab + 3;  // with the part of 16 bytes before a row
+        if (v <= 4 * 128 * 4) return launch_score_rows<SRC, 4, 2>(a, n_rows, stream);
+        if (v <= 4 * 512 * 8) return launch_score_rows<SRC, 8, 8>(a, n_rows, stream);
+        if constexpr (SRC == SCORE_I64) {
+            if (v <= 4 * 1024 * 15) return launch_score_rows<SRC, 15, 16>(a, n_rows, stream);
+        } else {
+            if (v <= 4 * 512 * 26) return launch_score_rows<SRC, 26, 8>(a, n_rows, stream);
+            if (v <= 4 * 1024 * 26) return launch_score_rows<SRC, 26, 16>(a, n_rows, stream);
+        }
+    }
+    launch_k(k_score_any<SRC>, dim3(n_rows), dim3(512), 0, stream, a);
+    return hipGetLastError();
 }
 
 hipError_t launch_score(const ScoreArgs &a, int n_rows, hipStream_t stream) {
     if (n_rows <= 0) return hipSuccess;
-    const dim3 grid(n_rows), block(256);
-    if (a.src == SCORE_I32) launch_k(k_score_any<SCORE_I32>, grid, block, 0, stream, a);
-    else if (a.src == SCORE_I64) launch_k(k_score_any<SCORE_I64>, grid, block, 0, stream, a);
-    else launch_k(k_score_any<SCORE_COMPACT>, grid, block, 0, stream, a);
-    return hipGetLastError();
+    if (a.src == SCORE_I32) return launch_score_src<SCORE_I32>(a, n_rows, stream);
+    if (a.src == SCORE_I64) return launch_score_src<SCORE_I64>(a, n_rows, stream);
+    return launch_score_src<SCORE_COMPACT>(a, n_rows, stream);
 }
 
 }  // namespace hs
