@@ -75,10 +75,26 @@ struct Min {
     __device__ T operator()(T x, T y) const { return x < y ? x : y; }
 };
 
-// A row by itself, any vocabulary and table: the workgroup walks it for the row max, the sum, the entropy and the rank,
-// and once for each alternative (the next in the order after the one before).
+// The alternatives of a row, one walk each: the next in the order after the one before.
 template <int SRC, int NW>
-__device__ void score_any_row(const ScoreArgs &a, size_t r, void *slots) {
+__device__ __forceinline__ void search_top(const ScoreArgs &a, size_t r, int64_t M, uint64_t T, void *slots) {
+    const ScoreRow<SRC> row(a, r);
+    int64_t before = -1;  // (d, symbol) of the last one found
+    for (int i = 0; i < a.top; i++) {
+        int64_t next = INT64_MAX;
+        for (int j = threadIdx.x; j < a.vocab; j += 64 * NW) {
+            const int64_t x = (int64_t)row.index(M, j) << 32 | j;
+            if (x > before && x < next) next = x;
+        }
+        before = block_join<NW>(next, slots, Min());
+        if (threadIdx.x == 0) put_top(a, r, i, (uint32_t)before, (int)(before >> 32), T);
+    }
+}
+
+// A row by itself, any vocabulary and table: the workgroup walks it for the row max, the sum, the entropy and the rank,
+// and for the alternatives.
+template <int SRC, int NW>
+__device__ __forceinline__ void score_any_row(const ScoreArgs &a, size_t r, void *slots) {
     const int tid = threadIdx.x, V = a.vocab, NT = 64 * NW;
     const ScoreRow<SRC> row(a, r);
     int64_t mx = INT64_MIN;
@@ -108,16 +124,7 @@ __device__ void score_any_row(const ScoreArgs &a, size_t r, void *slots) {
         h = block_join<NW>(h, slots, Add());
         if (tid == 0) a.entropy[r] = (float)h;
     }
-    int64_t before = -1;  // (d, symbol) of the last one found
-    for (int i = 0; i < a.top; i++) {
-        int64_t next = INT64_MAX;
-        for (int j = tid; j < V; j += NT) {
-            const int64_t x = (int64_t)row.index(M, j) << 32 | j;
-            if (x > before && x < next) next = x;
-        }
-        before = block_join<NW>(next, slots, Min());
-        if (tid == 0) put_top(a, r, i, (uint32_t)before, (int)(before >> 32), T);
-    }
+    search_top<SRC, NW>(a, r, M, T, slots);
 }
 template <int SRC>
 __global__ __launch_bounds__(512) void k_score_any(ScoreArgs a) {
@@ -137,20 +144,27 @@ template <int SRC, int G, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) void k_score_rows(ScoreArgs a) {
     constexpr int NT = 64 * NW;
     extern __shared__ uint32_t s_hist[];  // [table_len + 63]
-    __shared__ uint64_t slots[NW], s_list[SCORE_LIST];
-    __shared__ uint32_t s_count, s_thr, s_found;
-    const int tid = threadIdx.x, lane = tid & 63, V = a.vocab, last = a.table_len - 1;
+    __shared__ uint64_t slots[NW], s_sum[NW], s_list[SCORE_LIST];
+    __shared__ double s_ent[NW];
+    __shared__ uint32_t s_ahead[NW], s_count, s_thr, s_found;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), V = a.vocab, last = a.table_len - 1;
     const size_t r = blockIdx.x;
     const uint32_t token = a.tokens ? a.tokens[r] : 0xffffffffu;
     const bool some = token < (uint32_t)V;
     const uint32_t cap = (uint32_t)(last + lane);  // this lane's bin of what lies past the table's end
     uint32_t d2[2 * G];                            // min(d, cap), pairs
     int off = 0;                                   // symbol of element e of group i: 4 (NT i + tid) + e - off
+    int td = 0;                                    // the token's index
+    int64_t top_logit;                             // the largest
     const ScoreRow<SRC> row(a, (int)r);
-    int td = 0;  // the token's index
     auto symbol = [&](int i, int e) { return 4 * (NT * i + tid) + e - off; };
     auto inside = [&](int j) { return j >= 0 && j < V; };
-    auto partial = [&](int i) { return symbol(i, 0) < 0 || symbol(i, 3) >= V; };  // a group not all of which is the row's
+    auto edge = [&](int i) { return (i == 0 && off > 0) || 4 * NT * (i + 1) > V + off; };  // some of group i are past the row (uniform)
+    auto load = [](__amdgpu_buffer_rsrc_t x, int at, int step) { return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(x, at, step, 0)); };
+    if (a.table[0] == 0) {  // (not a table of a model: the entropy below divides by it)
+        score_any_row<SRC, NW>(a, r, slots);
+        return;
+    }
     for (int k = tid; k < last + 64; k += NT) s_hist[k] = 0;
     if (tid == 0) s_count = 0;
 
@@ -167,7 +181,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
         }
         int64_t mx = INT64_MIN;
         for (int j = tid; j < a.ntiles; j += NT) mx = tm[j] > mx ? tm[j] : mx;
-        const int64_t M = block_join<NW>(mx, slots, Max());
+        const int64_t M = top_logit = block_join<NW>(mx, slots, Max());
         if (some) td = row.index(M, (int)token);
 #pragma unroll
         for (int i = 0; i < G; i++) {
@@ -180,38 +194,51 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
             d2[2 * i + 1] = d[2] | d[3] << 16;
         }
     } else {
-        // 16-byte loads, from the 16 bytes that the row starts in to those that it ends in
+        // 16-byte loads, from the 16 bytes that the row starts in to those that it ends in; zeros past them
         constexpr int E = SRC == SCORE_I32 ? 4 : 8;
         const uintptr_t at = (uintptr_t)a.logits + r * a.ld * E;
         off = (int)(at % 16) / E;
-        const uint4 *p = (const uint4 *)(at - at % 16);
-        const int loads = (int)(((off + (size_t)V) * E + 15) / 16);
-        int32_t x[4 * G];
-        bool fits = true;
-        int64_t ref = 0;
+        const int bytes = ((off + V) * E + 15) / 16 * 16;
+        const auto from = __builtin_amdgcn_make_buffer_rsrc((void *)(at - at % 16), 0, bytes, 0x00020000);
         const int64_t of_token = some ? row.value((int)token) : 0;
+        // i32 logits as they are, i64 ones as their difference to 2^31 below the row's first one, in 32 bits
+        typedef typename std::conditional<SRC == SCORE_I32, int32_t, uint32_t>::type X;
+        constexpr X LOW = SRC == SCORE_I32 ? (X)INT32_MIN : (X)0;
+        X x[4 * G], mx = LOW;
+        uint64_t ref = 0;
+        uint32_t apart = 0;  // not 0: they do not fit
+        auto take = [&](int i) {
+            if (edge(i)) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[4 * i + e] = inside(symbol(i, e)) ? x[4 * i + e] : LOW;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) mx = x[4 * i + e] > mx ? x[4 * i + e] : mx;
+        };
         if constexpr (SRC == SCORE_I32) {
 #pragma unroll
             for (int i = 0; i < G; i++) {
-                const uint4 y = p[NT * i + tid < loads ? NT * i + tid : 0];
+                const uint4 y = load(from, 16 * tid, 16 * NT * i);
                 x[4 * i] = (int32_t)y.x;
                 x[4 * i + 1] = (int32_t)y.y;
                 x[4 * i + 2] = (int32_t)y.z;
                 x[4 * i + 3] = (int32_t)y.w;
             }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < G; i++) take(i);
         } else {
-            // differences to the row's first logit, in 32 bits
-            ref = ((const int64_t *)at)[0];
-            constexpr int B = G % 3 == 0 ? 3 : G % 4 == 0 ? 4 : 1;  // groups in flight beside those at work
+            const int64_t first = ((const int64_t *)at)[0];
+            // (a first logit at the types' ends: the differences would come round)
+            if (first >= (int64_t)1 << 62 || first < -((int64_t)1 << 62)) apart = 1;
+            ref = (uint64_t)first - 0x80000000u;
+            constexpr int B = 4;  // groups in flight beside those at work
             uint4 raw[2][B][2];
             auto fetch = [&](int i0, uint4(&y)[B][2]) {
 #pragma unroll
-                for (int i = 0; i < B; i++)
+                for (int i = 0; i < B && i0 + i < G; i++)
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const int l = 2 * (NT * (i0 + i) + tid) + k;
-                        y[i][k] = p[l < loads ? l : 0];
-                    }
+                    for (int k = 0; k < 2; k++) y[i][k] = load(from, 32 * tid + 16 * k, 32 * NT * (i0 + i));
             };
             fetch(0, raw[0]);
 #pragma unroll
@@ -219,50 +246,34 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
                 uint4(&y)[B][2] = raw[(i0 / B) & 1];
                 __builtin_amdgcn_sched_barrier(0);
                 if (i0 + B < G) fetch(i0 + B, raw[(i0 / B + 1) & 1]);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int i = 0; i < B; i++) {
-                    bool in = true;
+                for (int i = 0; i < B && i0 + i < G; i++) {
+                    uint32_t high[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const uint4 q = y[i][e >> 1];
-                        const int64_t l = (int64_t)(e & 1 ? (uint64_t)q.w << 32 | q.z : (uint64_t)q.y << 32 | q.x);
-                        int64_t d;
-                        const bool over = __builtin_sub_overflow(l, ref, &d);
-                        in = in && !over && d == (int32_t)d;
-                        x[4 * (i0 + i) + e] = (int32_t)d;
+                        const uint64_t u = (e & 1 ? (uint64_t)q.w << 32 | q.z : (uint64_t)q.y << 32 | q.x) - ref;
+                        x[4 * (i0 + i) + e] = (uint32_t)u;
+                        high[e] = (uint32_t)(u >> 32);
                     }
-                    fits = fits && (in || partial(i0 + i));
+                    if (edge(i0 + i)) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) high[e] = inside(symbol(i0 + i, e)) ? high[e] : 0;
+                    }
+                    apart |= (high[0] | high[1]) | (high[2] | high[3]);
+                    take(i0 + i);
                 }
             }
-            // (a group at the row's ends, by itself)
-#pragma unroll
-            for (int i = 0; i < G; i++)
-                if (partial(i))
-                    for (int e = 0; e < 4; e++) {
-                        int64_t d;
-                        const int j = symbol(i, e);
-                        if (inside(j)) fits = !__builtin_sub_overflow(((const int64_t *)at)[j], ref, &d) && d == (int32_t)d && fits;
-                    }
-        }
-        int32_t mx = INT32_MIN;
-#pragma unroll
-        for (int i = 0; i < G; i++) {
-            if (partial(i)) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[4 * i + e] = inside(symbol(i, e)) ? x[4 * i + e] : INT32_MIN;
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) mx = x[4 * i + e] > mx ? x[4 * i + e] : mx;
-        }
-        if constexpr (SRC == SCORE_I64) {
-            if (__syncthreads_or(!fits)) {  // logits that lie further apart: uniform
+            if (__syncthreads_or(apart != 0)) {  // logits that lie further apart: uniform
                 score_any_row<SRC, NW>(a, r, slots);
                 return;
             }
         }
-        const int32_t m = block_join<NW>(mx, slots, Max());
+        const X m = block_join<NW>(mx, slots, Max());
+        top_logit = SRC == SCORE_I32 ? (int64_t)m : (int64_t)((uint64_t)m + ref);
         if (some) {
-            const uint64_t d = (uint64_t)(int64_t)m + (uint64_t)ref - (uint64_t)of_token;
+            const uint64_t d = (uint64_t)top_logit - (uint64_t)of_token;
             td = d < (uint64_t)last ? (int)d : last;
         }
 #pragma unroll
@@ -276,13 +287,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
             d2[i] = d[0] | d[1] << 16;
         }
     }
+    auto index = [&](int i, int e) { return e & 1 ? d2[2 * i + (e >> 1)] >> 16 : d2[2 * i + (e >> 1)] & 0xffffu; };
 #pragma unroll
     for (int i = 0; i < G; i++)
-        if (partial(i)) {
-            const uint32_t d[4] = {d2[2 * i] & 0xffffu, d2[2 * i] >> 16, d2[2 * i + 1] & 0xffffu, d2[2 * i + 1] >> 16};
+        if (edge(i)) {
             uint32_t y[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = inside(symbol(i, e)) ? d[e] : cap;
+            for (int e = 0; e < 4; e++) y[e] = inside(symbol(i, e)) ? index(i, e) : cap;
             d2[2 * i] = y[0] | y[1] << 16;
             d2[2 * i + 1] = y[2] | y[3] << 16;
         }
@@ -291,24 +302,6 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
 #pragma unroll
         for (int i = 0; i < 2 * G; i++) asm volatile("" : "+v"(d2[i]));
     };
-    auto index = [&](int i, int e) { return e & 1 ? d2[2 * i + (e >> 1)] >> 16 : d2[2 * i + (e >> 1)] & 0xffffu; };
-    // fn(symbol, index) for the symbols with an index in lo ..= hi (rare ones)
-    auto those = [&](uint32_t lo, uint32_t hi, auto fn) {
-        hide();
-        if (hi >= (uint32_t)last) hi = 0xffffu;
-#pragma unroll
-        for (int i = 0; i < G; i++) {
-            uint32_t in = 0, p0 = d2[2 * i], p1 = d2[2 * i + 1];
-#pragma unroll
-            for (int e = 0; e < 4; e++) in |= index(i, e) - lo <= hi - lo ? 1u << e : 0u;
-            asm volatile("" : "+v"(p0), "+v"(p1));  // (else the choice below makes an array in memory of all pairs)
-            for (; in; in &= in - 1) {
-                const int e = __ffs(in) - 1, j = symbol(i, e);
-                const uint32_t d = ((e & 2 ? p1 : p0) >> (16 * (e & 1))) & 0xffffu;
-                if (inside(j)) fn(j, d < (uint32_t)last ? (int)d : last);
-            }
-        }
-    };
     hide();
 #pragma unroll
     for (int i = 0; i < G; i++) {
@@ -316,68 +309,66 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
         for (int e = 0; e < 4; e++) atomicAdd(&s_hist[index(i, e)], 1u);
         if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
-    hide();
-    __syncthreads();
-    if (tid < 64) {  // the spare bins to the last one, without the places past the row
-        const uint32_t far = (uint32_t)wave_sum64(s_hist[last + tid]);
-        if (tid == 0) s_hist[last] = far - (uint32_t)(4 * G * NT - V);
+    // fn(symbol, index) for the symbols with an index in lo ..= hi, few: a test a group of four
+    auto those = [&](uint32_t lo, uint32_t hi, auto fn) {
+        hide();
+        const uint32_t span = (hi >= (uint32_t)last ? 0xffffu : hi) - lo;
+#pragma unroll
+        for (int i = 0; i < G; i++) {
+            uint32_t p0 = d2[2 * i], p1 = d2[2 * i + 1], least = 0xffffffffu;
+#pragma unroll
+            for (int e = 0; e < 4; e++) least = index(i, e) - lo < least ? index(i, e) - lo : least;
+            if (least > span) continue;
+            asm volatile("" : "+v"(p0), "+v"(p1));  // (else the choice below makes an array in memory of all pairs)
+#pragma unroll 1
+            for (int e = 0; e < 4; e++) {
+                const uint32_t d = ((e & 2 ? p1 : p0) >> (16 * (e & 1))) & 0xffffu;
+                if (d - lo <= span && inside(symbol(i, e))) fn(symbol(i, e), d < (uint32_t)last ? (int)d : last);
+            }
+        }
+    };
+    __syncthreads();  // the counts are there
+    if (w == 0) {     // the spare bins to the last one, without the places past the row
+        const uint32_t far = (uint32_t)wave_sum64(s_hist[last + lane]);
+        if (lane == 0) s_hist[last] = far - (uint32_t)(4 * G * NT - V);
     }
+    uint32_t ahead = 0;  // symbols before the token
     __syncthreads();
-
-    // T, and the symbols that lie before the token
-    constexpr int KB = 16;  // bins of a lane kept from the sum to the entropy
+    if (a.rank && some && s_hist[td] > 1) those((uint32_t)td, (uint32_t)td, [&](int j, int) { ahead += j < (int)token; });  // its ties
+    // T and the entropy from the counts, in one pass: with w0 = table[0], the largest weight there is, the entropy
+    // sum (w / T) ln(T / w) = ln(T / w0) + (sum w ln(w0 / w)) / T, two terms that are not negative (log_share takes the first,
+    // exact where T is close to w0). In f32 the logarithms of the second are some 2^-22 off, which the first outweighs: it is
+    // at least the share of all symbols but the largest.
+    const uint64_t w0 = a.table[0];
+    const float w0f = (float)w0;
     uint64_t sum = 0;
-    uint32_t ahead = 0, n[KB];
-    float wf[KB];
+    float spread = 0;
+    for (int d0 = tid; d0 <= last; d0 += 8 * NT) {
+        uint32_t n[8];
+        uint64_t x[8];
 #pragma unroll
-    for (int k0 = 0; k0 < KB; k0 += 4) {
-        uint64_t w[4];
-#pragma unroll
-        for (int k = k0; k < k0 + 4; k++) {
-            const int d = tid + NT * k;
+        for (int k = 0; k < 8; k++) {
+            const int d = d0 + NT * k;
             n[k] = d <= last ? s_hist[d] : 0;
-            w[k - k0] = n[k] ? a.table[d] : 0;
+            x[k] = n[k] ? a.table[d] : 0;
         }
 #pragma unroll
-        for (int k = k0; k < k0 + 4; k++) {
-            sum += n[k] * w[k - k0];
-            wf[k] = (float)w[k - k0];
-            ahead += tid + NT * k < td ? n[k] : 0;
+        for (int k = 0; k < 8; k++) {
+            sum += n[k] * x[k];
+            const float y = (float)x[k], l = __builtin_amdgcn_logf(w0f * __builtin_amdgcn_rcpf(y));
+            spread += x[k] ? (float)n[k] * y * l : 0.0f;
+            ahead += d0 + NT * k < td ? n[k] : 0;
         }
     }
-    for (int d = tid + NT * KB; d <= last; d += NT) {
-        const uint32_t c = s_hist[d];
-        if (c) sum += c * a.table[d];
-        ahead += d < td ? c : 0;
-    }
-    const uint64_t T = block_join<NW>(sum, slots, Add());
-    if (a.entropy) {
-        // f32 terms: T / w >= 2 but for at most one symbol, whose logarithm is taken in 64 bits. Their roundings (T, w, the
-        // quotients, the logarithm, of at least ln 2) stay below 2^-21 of a term.
-        const float Tf = (float)T;
-        double hsum = 0;
-        auto term = [&](uint32_t c, float x, int d) {
-            if (!(x > 0)) return;
-            const float q = Tf / x;
-            const float l = q < 2.1f ? (float)-log_share(a.table[d], T) : __logf(q);
-            hsum += (float)c * l / q;
-        };
+    double h = (double)spread * 0.693147180559945309;
 #pragma unroll
-        for (int k = 0; k < KB; k++) term(n[k], wf[k], tid + NT * k);
-        for (int d = tid + NT * KB; d <= last; d += NT)
-            if (s_hist[d]) term(s_hist[d], (float)a.table[d], d);
-        hsum = block_join<NW>(hsum, slots, Add());
-        if (tid == 0) a.entropy[r] = (float)hsum;
-    }
-    if (a.rank) {  // ties of the token that come before it
-        if (some && s_hist[td] > 1) those((uint32_t)td, (uint32_t)td, [&](int j, int) { ahead += j < (int)token; });  // uniform
-        ahead = block_join<NW>(ahead, slots, Add());
-    }
-    if (tid == 0 && (a.logprob || a.rank)) put_token(a, r, some, some ? a.table[td] : 0, T, ahead);
-    if (a.top == 0 || !(a.top_tokens || a.top_logprob)) return;
-
-    // the index up to which `top` symbols lie, and how many lie up to it: one wave over 256 bins at a time
-    if (tid < 64) {
+    for (int o = 32; o > 0; o >>= 1) h += __shfl_xor(h, o, 64);
+    sum = wave_sum_dpp(sum);
+    ahead = (uint32_t)wave_sum_dpp(ahead);
+    if (lane == 0) s_sum[w] = sum, s_ahead[w] = ahead, s_ent[w] = h;
+    const bool tops = a.top > 0 && (a.top_tokens || a.top_logprob);
+    // the index up to which `top` symbols lie, and how many lie up to it: the last wave over 256 bins at a time
+    if (tops && w == NW - 1) {
         uint32_t before = 0;
         for (int k0 = 0; k0 <= last; k0 += 256) {
             uint32_t c[4], mine = 0;
@@ -409,6 +400,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
         }
     }
     __syncthreads();
+    uint64_t T = 0;
+#pragma unroll
+    for (int i = 0; i < NW; i++) T += s_sum[i];
+    if (tid == 0) {
+        for (int i = 1; i < NW; i++) ahead += s_ahead[i], h += s_ent[i];
+        if (a.logprob || a.rank) put_token(a, r, some, some ? a.table[td] : 0, T, ahead);
+        if (a.entropy) a.entropy[r] = (float)(h / (double)T - log_share(w0, T));
+    }
+    if (!tops) return;
     const uint32_t thr = s_thr;
     if (s_found <= SCORE_LIST) {  // uniform
         those(0, thr, [&](int j, int d) { s_list[atomicAdd(&s_count, 1u)] = (uint64_t)d << 32 | (uint32_t)j; });
@@ -422,16 +422,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
         }
         return;
     }
-    int64_t one = -1;  // the last one found
-    for (int i = 0; i < a.top; i++) {
-        int64_t next = INT64_MAX;
-        those(0, thr, [&](int j, int d) {
-            const int64_t x = (int64_t)d << 32 | j;
-            if (x > one && x < next) next = x;
-        });
-        one = block_join<NW>(next, slots, Min());
-        if (tid == 0) put_top(a, r, i, (uint32_t)one, (int)(one >> 32), T);
-    }
+    search_top<SRC, NW>(a, r, top_logit, T, slots);
 }
 
 template <int SRC, int G, int NW>
@@ -450,7 +441,7 @@ static hipError_t launch_score_src(const ScoreArgs &a, int n_rows, hipStream_t s
         if (v <= 4 * 128 * 4) return launch_score_rows<SRC, 4, 2>(a, n_rows, stream);
         if (v <= 4 * 512 * 8) return launch_score_rows<SRC, 8, 8>(a, n_rows, stream);
         if constexpr (SRC == SCORE_I64) {
-            if (v <= 4 * 1024 * 15) return launch_score_rows<SRC, 15, 16>(a, n_rows, stream);
+            if (v <= 4 * 1024 * 13) return launch_score_rows<SRC, 13, 16>(a, n_rows, stream);
         } else {
             if (v <= 4 * 512 * 26) return launch_score_rows<SRC, 26, 8>(a, n_rows, stream);
             if (v <= 4 * 1024 * 26) return launch_score_rows<SRC, 26, 16>(a, n_rows, stream);
