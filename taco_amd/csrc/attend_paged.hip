@@ -15,30 +15,32 @@ struct PagedPlan {
     int group = 1, tiles = 1;  // query heads of a cache head; row tiles of a panel
     int panels = 0;            // (stream, cache head)
     int ng = 1, span = 0;      // key ranges, their keys
+    int store = 0;             // the ranges' scores are kept in the scratch
+    int rows = 0, chunks = 1;  // rows of a tile with scores there; of PG_CHUNK keys, with a sum each
     int page_log = 4;
 };
+constexpr int PG_CHUNK = 4096;
 
-// The ranges' results: the largest score, the sum of the entries and the sums w v of each row of each tile, and the
-// dots (tiles of four rows).
+// What the ranges leave for the next launch, for each tile of each panel.
 struct PagedScratch {
-    int64_t *mx;    // [tiles of all panels][ng][rt]
-    uint64_t *sum;  // the same
-    int64_t *part;  // [..][ng][rt][hd]
-    v4i *dots;      // [..][ng][keys of a range]
+    int64_t *mx;    // [ng][rt]: the largest score
+    uint64_t *sum;  // [chunks or ng][rt]: the sum of the entries
+    int64_t *part;  // [ng][rt][hd]: sum w v
+    int64_t *keep;  // [rows][ng span]: the scores, then the entries, as i32 in half of it where they fit
 };
 __host__ __device__ inline size_t pg256(size_t x) { return (x + 255) / 256 * 256; }
 __host__ __device__ inline PagedScratch paged_scratch(void *base, const PagedPlan &p, int hd, size_t *bytes = nullptr) {
-    const size_t n = (size_t)p.panels * p.tiles * p.ng;
+    const size_t n = (size_t)p.panels * p.tiles;
     PagedScratch s;
     size_t at = 0;
     s.mx = (int64_t *)base;
-    at += pg256(n * p.rt * 8);
+    at += pg256(n * p.ng * p.rt * 8);
     s.sum = (uint64_t *)((char *)base + at);
-    at += pg256(n * p.rt * 8);
+    at += pg256(n * p.chunks * p.rt * 8);
     s.part = (int64_t *)((char *)base + at);
-    at += pg256(n * p.rt * hd * 8);
-    s.dots = (v4i *)((char *)base + at);
-    if (p.rt == 4) at += pg256(n * p.span * 16);
+    at += pg256(n * p.ng * p.rt * hd * 8);
+    s.keep = (int64_t *)((char *)base + at);
+    if (p.store) at += pg256(n * p.rows * p.ng * p.span * 8);
     if (bytes) *bytes = at;
     return s;
 }
@@ -77,15 +79,18 @@ struct PagedRule {
 // with keys 4 (l / 16) + e of a group. With 16 rows a column is a row and D[t] holds group t. With 4 rows column 4 t + r is
 // row r with group t: the products of the four groups add up in one accumulator, each with q in its own columns and
 // zeros in the others, so that no lane idles; the product with V takes the rows' four digit planes as its 16 columns.
-// PHASE 0: all in one launch. Else the ranges meet in the scratch: 1 the largest scores (and the dots of 4 rows), 2 the sums
-// of the entries, 3 the products with V.
-template <int RT, int QC, int NB, int NW, bool HI, int PHASE>
+// PHASE 0: all in one launch. Else the ranges meet in the scratch: 1 the largest scores, 2 the sums of the entries, 3 the
+// products with V. KEEP: launch 1 leaves all scores there (0x80.. where a row does not see a key), k_paged_entries makes them
+// entries and sums, and launch 3 reads those; else each launch forms the dots again.
+template <int RT, int QC, int NB, int NW, bool HI, int PHASE, bool KEEP>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 ? 4 : 2))) void k_paged_tile(PagedArgs g, PagedPlan pl, void *scratch) {
     static_assert(NB <= 16, "a lane for each group of the wave's blocks");
     static_assert(RT == 4 || NB <= 4, "two planes' sums of a wave's keys in 32 bits");
     constexpr int TU = RT / 4;  // accumulators of a block
     constexpr int KD = QC == 1 ? (NB < 4 ? NB : NW > 8 ? 2 : 4) : QC == 2 && NB > 1 && NW <= 8 ? 2 : 1;  // blocks of K in flight, and of V
-    constexpr bool DOTS = PHASE < 2 || RT == 16;  // whether the launch forms the dots
+    constexpr bool DOTS = !(KEEP && PHASE == 3);  // whether the launch forms the dots
+    typedef typename std::conditional<HI, int32_t, int64_t>::type Score;
+    constexpr Score LOW = HI ? (Score)INT32_MIN : (Score)INT64_MIN;
     extern __shared__ __attribute__((aligned(1024))) int8_t s_mem[];
     const PagePool &p = g.pages;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -111,7 +116,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
     const uint32_t last = (uint32_t)g.exp_len - 1;
 
     // LDS: the table (of 16 rows), which the sums of the outputs take over, each wave's V, what the waves exchange
-    const bool in_lds = RT == 16 && PHASE != 1 && g.table_lds;
+    const bool in_lds = RT == 16 && PHASE != 1 && !(KEEP && PHASE == 3) && g.table_lds;
     constexpr int ACC_BYTES = (8 * QC * RT * PG_ACC + 1023) / 1024 * 1024;
     const int table_bytes = in_lds ? 1024 * ((g.exp_len + 255) / 256) : 0;
     const int top = table_bytes > ACC_BYTES ? table_bytes : ACC_BYTES;
@@ -141,8 +146,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
     const uint64_t there = __ballot(held);  // of the groups, those with keys and a page
     if (held) {
         const size_t at = (size_t)number * p.kv_heads + h;
-        mul = p.k_scale[at];
-        vs = p.v_scale[at];
+        if (DOTS) mul = p.k_scale[at];
+        if (PHASE == 0 || PHASE == 3) vs = p.v_scale[at];
     }
     auto group_rows = [&](const int8_t *pool, int j, int t) {  // the 16 rows of a group; no access where they are not there
         const bool in_page = (there >> (4 * j + t)) & 1;
@@ -173,8 +178,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
     const v4i zero = v4i{0, 0, 0, 0};
     const int row = RT == 16 ? ql : ql & 3, near = row < live ? row : live - 1;  // rows that are not there: as the last one
     const int64_t first = (int64_t)s * g.t;                                      // the stream's first token
-    const size_t slot = ((size_t)panel * pl.tiles + tile) * pl.ng;                // of the tile's ranges
+    const size_t place = (size_t)panel * pl.tiles + tile, slot = place * pl.ng;   // of the tile, of its ranges
     const PagedScratch S = paged_scratch(scratch, pl, hd);
+    // a lane's scores or entries of block j, accumulator u in the scratch: four keys of its row
+    auto kept = [&](int j, int u) {
+        const int key = key_of(j) + 16 * (RT == 16 ? u : ql >> 2) + 4 * qg;
+        return (Score *)S.keep + (place * pl.rows + row) * ((size_t)pl.ng * pl.span) + key;
+    };
     v4i D[NB][TU];
     v4i vr[KD][4];
     if constexpr (DOTS) {
@@ -219,7 +229,17 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
     } else {
 #pragma unroll
         for (int j = 0; j < NB; j++)
-            if (mine(j)) D[j][0] = S.dots[(slot + range) * pl.span + (size_t)64 * (NW * j + w) + lane];
+#pragma unroll
+            for (int u = 0; u < TU; u++) {
+                D[j][u] = zero;
+                if (!mine(j) || row >= live) continue;
+                if constexpr (HI) {
+                    D[j][u] = *(const v4i *)kept(j, u);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) D[j][u][e] = (int32_t)kept(j, u)[e];
+                }
+            }
     }
     if constexpr ((PHASE == 0 && NB > KD) || PHASE == 3) {
 #pragma unroll
@@ -243,16 +263,31 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
     const PagedRule<HI> rule(g);
     int64_t M = INT64_MIN;
     if constexpr (PHASE < 2) {
-        typedef typename std::conditional<HI, int32_t, int64_t>::type Score;
-        Score mx = HI ? (Score)INT32_MIN : (Score)INT64_MIN;
+        Score mx = LOW;
 #pragma unroll
         for (int j = 0; j < NB; j++) {
             if (!mine(j)) continue;
-            if constexpr (PHASE == 1 && RT == 4) S.dots[(slot + range) * pl.span + (size_t)64 * (NW * j + w) + lane] = D[j][0];
             const bool whole_block = all(j);
 #pragma unroll
             for (int u = 0; u < TU; u++) {
                 const int m = scale_of(mul, j, u), k = whole_block ? 4 : seen(j, u);
+                if constexpr (PHASE == 1 && KEEP) {
+                    Score x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        x[e] = e < k ? (Score)rule.score(D[j][u][e], m) : LOW;
+                        mx = x[e] > mx ? x[e] : mx;
+                    }
+                    if (row < live) {
+                        if constexpr (HI) {
+                            *(v4i *)kept(j, u) = v4i{(int)x[0], (int)x[1], (int)x[2], (int)x[3]};
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; e++) kept(j, u)[e] = x[e];
+                        }
+                    }
+                    continue;
+                }
                 int32_t d = INT32_MIN;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
@@ -268,7 +303,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
             const Score x = __shfl_xor(mx, o, 64);
             mx = x > mx ? x : mx;
         }
-        if (lane < RT) s_mx[w * RT + lane] = HI && mx == (Score)INT32_MIN ? INT64_MIN : (int64_t)mx;
+        if (lane < RT) s_mx[w * RT + lane] = mx == LOW ? INT64_MIN : (int64_t)mx;
         if (PHASE == 0 && !mine(0)) wait_vmcnt<0>();  // (no K to wait for)
         lds_barrier();                                // not the fence of __syncthreads, which would wait for V too
         if constexpr (PHASE == 1) {
@@ -281,7 +316,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
         }
 #pragma unroll
         for (int i = 0; i < NW; i++) M = s_mx[i * RT + row] > M ? s_mx[i * RT + row] : M;
-    } else {
+    } else if constexpr (DOTS) {
         for (int i = 0; i < ranges; i++) {
             const int64_t x = S.mx[(slot + i) * RT + row];
             M = x > M ? x : M;
@@ -294,7 +329,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
     uint64_t sum = 0;
 #pragma unroll
     for (int j = 0; j < NB; j++) {
-        if (!mine(j)) continue;
+        if (!DOTS || !mine(j)) continue;
         const bool whole_block = all(j);
 #pragma unroll
         for (int u = 0; u < TU; u++) {
@@ -339,7 +374,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
                 sum = 0;
 #pragma unroll
                 for (int i = 0; i < NW; i++) sum += s_sum[i * RT + tid];
-                S.sum[(slot + range) * RT + tid] = sum;
+                S.sum[(place * pl.chunks + range) * RT + tid] = sum;
             }
             return;
         }
@@ -347,7 +382,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
 #pragma unroll
         for (int i = 0; i < NW; i++) sum += s_sum[i * RT + row];
     } else {
-        for (int i = 0; i < ranges; i++) sum += S.sum[(slot + i) * RT + row];
+        const int sums = KEEP ? (keys + PG_CHUNK - 1) / PG_CHUNK : ranges;
+        for (int i = 0; i < sums; i++) sum += S.sum[(place * pl.chunks + i) * RT + row];
         lds_barrier();  // every wave has its entries
     }
     for (int i = tid; i < QC * RT * PG_ACC; i += 64 * NW) s_acc[i] = 0;
@@ -477,6 +513,78 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
     }
 }
 
+// The scores of a row over PG_CHUNK keys to their entries, in place, and the entries' sum.
+template <bool HI>
+__global__ __launch_bounds__(256) void k_paged_entries(PagedArgs g, PagedPlan pl, void *scratch) {
+    typedef typename std::conditional<HI, int32_t, int64_t>::type Score;
+    constexpr Score LOW = HI ? (Score)INT32_MIN : (Score)INT64_MIN;
+    constexpr int N = PG_CHUNK / 256;
+    __shared__ uint64_t s_sum[4];
+    const PagePool &p = g.pages;
+    const int tid = threadIdx.x;
+    // (row fastest, then the chunk)
+    const int r = blockIdx.x % pl.rows, chunk = blockIdx.x / pl.rows % pl.chunks;
+    const size_t place = blockIdx.x / pl.rows / pl.chunks;
+    const int tile = (int)(place % pl.tiles), s = (int)(place / pl.tiles) / p.kv_heads;
+    const int n = (int)(g.ctx[s] < (uint32_t)g.keys ? g.ctx[s] : (uint32_t)g.keys);
+    uint32_t count = g.rows ? g.rows[s] : (uint32_t)g.t;
+    count = count < (uint32_t)g.t ? count : (uint32_t)g.t;
+    const int rows = (int)count * pl.group, row0 = pl.rt * tile, live = rows - row0 < pl.rt ? rows - row0 : pl.rt;
+    if (r >= live) return;
+    const int keys = n - (int)count + (row0 + live - 1) / pl.group + 1;  // of the tile: those have scores, in whole blocks
+    const int k0 = chunk * PG_CHUNK, k1 = (keys + 63) / 64 * 64 < k0 + PG_CHUNK ? (keys + 63) / 64 * 64 : k0 + PG_CHUNK;
+    if (k0 >= keys) return;
+    const PagedScratch S = paged_scratch(scratch, pl, p.hd);
+    Score *at = (Score *)S.keep + (place * pl.rows + r) * ((size_t)pl.ng * pl.span);
+    Score x[N];
+#pragma unroll
+    for (int i = 0; i < N / 4; i++) {
+        const int key = k0 + 1024 * i + 4 * tid;
+        if constexpr (HI) {
+            const v4i y = key < k1 ? *(const v4i *)(at + key) : v4i{LOW, LOW, LOW, LOW};
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[4 * i + e] = y[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[4 * i + e] = key < k1 ? at[key + e] : LOW;
+        }
+    }
+    const int ranges = (keys + pl.span - 1) / pl.span;
+    int64_t M = INT64_MIN;
+    for (int i = tid & 63; i < ranges; i += 64) {
+        const int64_t y = S.mx[(place * pl.ng + i) * pl.rt + r];
+        M = y > M ? y : M;
+    }
+    M = wave_max64(M);
+    const uint32_t last = (uint32_t)g.exp_len - 1;
+    uint64_t sum = 0;
+    int32_t y[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        uint32_t d;
+        if constexpr (HI) d = (uint32_t)((int32_t)M - x[i]);
+        else d = (uint64_t)(M - x[i]) < last ? (uint32_t)(M - x[i]) : last;
+        y[i] = x[i] == LOW ? 0 : g.exp_table[d < last ? d : last];
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) sum += (uint32_t)y[i];
+#pragma unroll
+    for (int i = 0; i < N / 4; i++) {
+        const int key = k0 + 1024 * i + 4 * tid;
+        if (key >= k1) continue;
+        if constexpr (HI) {
+            *(v4i *)(at + key) = v4i{y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) at[key + e] = y[4 * i + e];
+        }
+    }
+    sum = wave_sum_dpp(sum);
+    if ((tid & 63) == 0) s_sum[tid >> 6] = sum;
+    __syncthreads();
+    if (tid == 0) S.sum[(place * pl.chunks + chunk) * pl.rt + r] = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+}
+
 // The outputs from the ranges' sums: a thread per four channels.
 __global__ __launch_bounds__(256) void k_paged_out(PagedArgs g, PagedPlan pl, void *scratch) {
     const PagePool &p = g.pages;
@@ -496,10 +604,17 @@ __global__ __launch_bounds__(256) void k_paged_out(PagedArgs g, PagedPlan pl, vo
     const int ranges = keys > pl.span ? (keys + pl.span - 1) / pl.span : 1;
     const PagedScratch S = paged_scratch(scratch, pl, p.hd);
     int64_t x[4] = {0, 0, 0, 0};
-    for (int c = 0; c < ranges; c++) {
-        const int64_t *from = S.part + ((tiles * pl.ng + c) * pl.rt + r) * p.hd + ch;
+    const int64_t *from = S.part + (tiles * pl.ng * pl.rt + r) * p.hd + ch;
+    for (int c0 = 0; c0 < ranges; c0 += 8) {  // eight in flight
+        int64_t y[8][4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) x[e] += from[e];
+        for (int c = 0; c < 8; c++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[c][e] = from[(size_t)(c0 + c < ranges ? c0 + c : c0) * pl.rt * p.hd + e];
+#pragma unroll
+        for (int c = 0; c < 8; c++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] += c0 + c < ranges ? y[c][e] : 0;
     }
     const double mo = g.out_s > 95 ? 0.0 : ldexp((double)g.out_m, -g.out_s);
     uint32_t packed = 0;
@@ -509,15 +624,19 @@ __global__ __launch_bounds__(256) void k_paged_out(PagedArgs g, PagedPlan pl, vo
     *(uint32_t *)(g.out + (((size_t)s * g.t + tok) * g.heads + head) * p.hd + ch) = packed;
 }
 
+constexpr size_t PG_KEEP = (size_t)128 << 20;  // bytes of scores that a call keeps at most (tiles of 16 rows)
+
 static PagedPlan paged_plan(const PagedArgs &g) {
     PagedPlan p;
     p.group = g.heads / g.pages.kv_heads;
     const long long rows = (long long)g.t * p.group;
     p.rt = rows <= 4 ? 4 : 16;
+    p.rows = rows < p.rt ? (int)rows : p.rt;
     p.tiles = (int)((rows + p.rt - 1) / p.rt);
     p.panels = g.streams * g.pages.kv_heads;
     while (1 << p.page_log < g.pages.page) p.page_log++;
     const int most = p.rt == 4 ? 4096 : 2048;  // keys of a tile in one launch
+    p.span = (g.keys + 63) / 64 * 64;
     if (g.keys > most) {
         const long long wgs = (long long)p.panels * p.tiles;
         long long ng = (1024 + wgs - 1) / wgs;
@@ -525,15 +644,15 @@ static PagedPlan paged_plan(const PagedArgs &g) {
         ng = ng < least ? least : (ng > more ? more : ng);
         p.span = (int)(((g.keys + ng - 1) / ng + 255) / 256) * 256;
         p.ng = (g.keys + p.span - 1) / p.span;
-    } else {
-        p.span = (g.keys + 63) / 64 * 64;
+        p.store = p.rt == 4 || (size_t)wgs * p.rows * p.ng * p.span * 8 <= PG_KEEP;
+        p.chunks = p.store ? (g.keys + PG_CHUNK - 1) / PG_CHUNK : p.ng;
     }
     return p;
 }
 
 bool paged_fits(const PagedArgs &g) {
     const PagedPlan p = paged_plan(g);
-    return ((long long)p.panels + 7) * p.tiles < (1ll << 23) / p.ng && (long long)p.panels * p.tiles * p.rt < (1ll << 31) / (g.pages.hd / 4);
+    return ((long long)p.panels + 7) * p.tiles < (1ll << 23) / p.ng && (long long)p.panels * p.tiles * p.rows < (1ll << 23) / p.chunks && (long long)p.panels * p.tiles * p.rt < (1ll << 31) / (g.pages.hd / 4);
 }
 
 size_t paged_workspace(const PagedArgs &g) {
@@ -543,14 +662,14 @@ size_t paged_workspace(const PagedArgs &g) {
     return bytes;
 }
 
-template <int RT, int QC, int NB, int NW, bool HI, int PHASE>
+template <int RT, int QC, int NB, int NW, bool HI, int PHASE, bool KEEP = false>
 static hipError_t launch_paged_t(const PagedArgs &g, const PagedPlan &p, void *scratch, hipStream_t stream) {
     const int acc = (8 * QC * RT * PG_ACC + 1023) / 1024 * 1024;
-    const int table = RT == 16 && PHASE != 1 && g.table_lds ? 1024 * ((g.exp_len + 255) / 256) : 0;
+    const int table = RT == 16 && PHASE != 1 && !(KEEP && PHASE == 3) && g.table_lds ? 1024 * ((g.exp_len + 255) / 256) : 0;
     const size_t lds = (size_t)(table > acc ? table : acc) + 4096 * NW + 16 * NW * RT;
-    const hipError_t e = allow_dynamic_lds((const void *)k_paged_tile<RT, QC, NB, NW, HI, PHASE>, lds);
+    const hipError_t e = allow_dynamic_lds((const void *)k_paged_tile<RT, QC, NB, NW, HI, PHASE, KEEP>, lds);
     if (e != hipSuccess) return e;
-    launch_k((k_paged_tile<RT, QC, NB, NW, HI, PHASE>), dim3((unsigned)((p.panels + 7) / 8 * 8) * p.tiles * p.ng), dim3(64 * NW), lds, stream, g, p, scratch);
+    launch_k((k_paged_tile<RT, QC, NB, NW, HI, PHASE, KEEP>), dim3((unsigned)((p.panels + 7) / 8 * 8) * p.tiles * p.ng), dim3(64 * NW), lds, stream, g, p, scratch);
     return hipGetLastError();
 }
 
@@ -558,9 +677,16 @@ template <int RT, int QC, bool HI>
 static hipError_t launch_paged_q(const PagedArgs &g, const PagedPlan &p, void *scratch, hipStream_t stream) {
     if (p.ng > 1) {
         hipError_t e;
-        if ((e = launch_paged_t<RT, QC, 4, 4, HI, 1>(g, p, scratch, stream)) != hipSuccess) return e;
-        if ((e = launch_paged_t<RT, QC, 4, 4, HI, 2>(g, p, scratch, stream)) != hipSuccess) return e;
-        if ((e = launch_paged_t<RT, QC, 4, 4, HI, 3>(g, p, scratch, stream)) != hipSuccess) return e;
+        if (p.store) {
+            if ((e = launch_paged_t<RT, QC, 4, 4, HI, 1, true>(g, p, scratch, stream)) != hipSuccess) return e;
+            launch_k(k_paged_entries<HI>, dim3((unsigned)p.panels * p.tiles * p.chunks * p.rows), dim3(256), 0, stream, g, p, scratch);
+            if ((e = hipGetLastError()) != hipSuccess) return e;
+            if ((e = launch_paged_t<RT, QC, 4, 4, HI, 3, true>(g, p, scratch, stream)) != hipSuccess) return e;
+        } else if constexpr (RT == 16) {
+            if ((e = launch_paged_t<RT, QC, 4, 4, HI, 1>(g, p, scratch, stream)) != hipSuccess) return e;
+            if ((e = launch_paged_t<RT, QC, 4, 4, HI, 2>(g, p, scratch, stream)) != hipSuccess) return e;
+            if ((e = launch_paged_t<RT, QC, 4, 4, HI, 3>(g, p, scratch, stream)) != hipSuccess) return e;
+        }
         const size_t quads = (size_t)p.panels * p.tiles * p.rt * (g.pages.hd / 4);
         launch_k(k_paged_out, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, g, p, scratch);
         return hipGetLastError();

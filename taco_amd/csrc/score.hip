@@ -132,205 +132,262 @@ __global__ __launch_bounds__(512) void k_score_any(ScoreArgs a) {
     score_any_row<SRC, 8>(a, blockIdx.x, slots);
 }
 
-// A row in the registers of a workgroup: read once, 4 G symbols a lane, their table indexes kept in 16 bits each and counted
-// in an LDS histogram. Symbols past the table's end (and the places of the last groups past the row) go to 64 spare bins, each
-// lane's in its own, so that no symbol needs a test and none of these many collide. The counts give T, the entropy and the
-// token's rank but for ties; one wave walks them for the index up to which the alternatives lie, and the symbols up to
-// there, few, are collected and ranked against each other.
+// A row by a workgroup of NW waves, its symbols four to a lane in groups of 256 NW. Each symbol's table index is counted in an
+// LDS histogram; those past the table's end (and the places of the last group past the row) go to 64 spare bins, each lane's in
+// its own, so that no symbol needs a test and none of these many collide. The counts give T, the entropy and the token's
+// rank but for ties; one wave walks them for the index up to which the alternatives lie, and the symbols up to there, few, are
+// collected and ranked against each other.
+// G > 0: the row is read once, G groups at most, and its indexes stay in registers, 16 bits each. G = 0, longer rows: read for
+// the max, for the counts, and once each for ties and alternatives.
 constexpr int SCORE_LIST = 1024;   // symbols collected; where ties make them more, the alternatives are searched one by one
 constexpr int SCORE_BINS = 16384;  // entries of the table at most
 
 template <int SRC, int G, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) void k_score_rows(ScoreArgs a) {
-    constexpr int NT = 64 * NW;
+    constexpr int NT = 64 * NW, LIST = NW == 1 ? 256 : SCORE_LIST, GS = G ? G : 1;
     extern __shared__ uint32_t s_hist[];  // [table_len + 63]
-    __shared__ uint64_t slots[NW], s_sum[NW], s_list[SCORE_LIST];
+    __shared__ uint64_t slots[NW], s_sum[NW], s_list[LIST], s_best[64];
     __shared__ double s_ent[NW];
     __shared__ uint32_t s_ahead[NW], s_count, s_thr, s_found;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), V = a.vocab, last = a.table_len - 1;
     const size_t r = blockIdx.x;
-    const uint32_t token = a.tokens ? a.tokens[r] : 0xffffffffu;
-    const bool some = token < (uint32_t)V;
     const uint32_t cap = (uint32_t)(last + lane);  // this lane's bin of what lies past the table's end
-    uint32_t d2[2 * G];                            // min(d, cap), pairs
-    int off = 0;                                   // symbol of element e of group i: 4 (NT i + tid) + e - off
-    int td = 0;                                    // the token's index
-    int64_t top_logit;                             // the largest
     const ScoreRow<SRC> row(a, (int)r);
+
+    // i32 logits as they are, i64 ones as their difference to 2^31 below the row's first one, in 32 bits; read 16 bytes at a
+    // time, from the 16 bytes that the row starts in to those that it ends in (zeros past them). Compact ones in whole tiles.
+    typedef typename std::conditional<SRC == SCORE_I64, uint32_t, int32_t>::type X;
+    constexpr X LOW = SRC == SCORE_I64 ? (X)0 : (X)INT32_MIN;
+    constexpr int E = SRC == SCORE_I64 ? 8 : SRC == SCORE_I32 ? 4 : 2;
+    const uintptr_t at = SRC == SCORE_COMPACT ? (uintptr_t)(a.d16 + r * a.ld16) : (uintptr_t)a.logits + r * a.ld * E;
+    const int off = SRC == SCORE_COMPACT ? 0 : (int)(at % 16) / E;  // symbol of element e of group i: 4 (NT i + tid) + e - off
+    const auto from = __builtin_amdgcn_make_buffer_rsrc((void *)(at - at % 16), 0, SRC == SCORE_COMPACT ? (V + 63) / 64 * 128 : ((off + V) * E + 15) / 16 * 16, 0x00020000);
+    const int groups = (V + off + 4 * NT - 1) / (4 * NT);
     auto symbol = [&](int i, int e) { return 4 * (NT * i + tid) + e - off; };
     auto inside = [&](int j) { return j >= 0 && j < V; };
     auto edge = [&](int i) { return (i == 0 && off > 0) || 4 * NT * (i + 1) > V + off; };  // some of group i are past the row (uniform)
-    auto load = [](__amdgpu_buffer_rsrc_t x, int at, int step) { return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(x, at, step, 0)); };
-    if (a.table[0] == 0) {  // (not a table of a model: the entropy below divides by it)
+    typedef typename std::conditional<SRC == SCORE_I64, v4i[2], typename std::conditional<SRC == SCORE_I32, v4i[1], v2i[1]>::type>::type Raw;
+    auto fetch = [&](int i, Raw &y) {
+        if constexpr (SRC == SCORE_COMPACT) {
+            y[0] = __builtin_bit_cast(v2i, __builtin_amdgcn_raw_buffer_load_b64(from, 8 * tid, 8 * NT * i, 0));
+        } else {
+#pragma unroll
+            for (int k = 0; k < E / 4; k++)
+                y[k] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(from, 4 * E * tid + 16 * k, 4 * E * NT * i, 0));
+        }
+    };
+    uint64_t ref = 0;
+    uint32_t apart = 0;  // not 0: the differences do not fit
+    auto start = [&] {   // (behind the first loads)
+        if constexpr (SRC == SCORE_I64) {
+            const int64_t first = *(const int64_t *)at;
+            if (first >= (int64_t)1 << 62 || first < -((int64_t)1 << 62)) apart = 1;  // (they would come round)
+            ref = (uint64_t)first - 0x80000000u;
+        }
+        for (int k = tid; k < last + 64; k += NT) s_hist[k] = 0;
+        if (tid == 0) s_count = 0;
+    };
+    X mx = LOW;
+    auto values = [&](int i, const Raw &y, X (&x)[4]) {
+        if constexpr (SRC == SCORE_I64) {
+            uint32_t high[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint64_t u = ((uint64_t)(uint32_t)y[e >> 1][2 * (e & 1) + 1] << 32 | (uint32_t)y[e >> 1][2 * (e & 1)]) - ref;
+                x[e] = (X)u;
+                high[e] = (uint32_t)(u >> 32);
+            }
+            if (edge(i)) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) high[e] = inside(symbol(i, e)) ? high[e] : 0;
+            }
+            apart |= (high[0] | high[1]) | (high[2] | high[3]);
+        } else if constexpr (SRC == SCORE_I32) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = y[0][e];
+        }
+        if (edge(i)) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = inside(symbol(i, e)) ? x[e] : LOW;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) mx = x[e] > mx ? x[e] : mx;
+    };
+
+    X x[GS][4];
+    Raw raw[SRC == SCORE_COMPACT ? GS : 1];
+    int64_t tile[SRC == SCORE_COMPACT ? GS : 1];
+    const int64_t *tm = a.tmax + r * a.ntiles;
+    auto tile_of = [&](int i) { return tm[symbol(i, 0) < V ? symbol(i, 0) >> 6 : 0]; };
+    if constexpr (SRC == SCORE_COMPACT) {
+        if constexpr (G > 0) {
+#pragma unroll
+            for (int i = 0; i < G; i++) {
+                fetch(i, raw[i]);
+                tile[i] = tile_of(i);
+            }
+        }
+        start();
+    } else if constexpr (G > 0) {
+        constexpr int B = SRC == SCORE_I32 ? G : 4;  // groups in flight, besides those at work (i32: all)
+        Raw y[2][B];
+#pragma unroll
+        for (int i = 0; i < B && i < G; i++) fetch(i, y[0][i]);
+        __builtin_amdgcn_sched_barrier(0);
+        start();
+#pragma unroll
+        for (int i0 = 0; i0 < G; i0 += B) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = i0 + B; i < i0 + 2 * B && i < G; i++) fetch(i, y[(i0 / B + 1) & 1][i - i0 - B]);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = i0; i < i0 + B && i < G; i++) values(i, y[(i0 / B) & 1][i - i0], x[i]);
+        }
+    } else {
+        start();
+        for (int i0 = 0; i0 < groups; i0 += 8) {
+            Raw y[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) fetch(i0 + i, y[i]);
+#pragma unroll
+            for (int i = 0; i < 8; i++) values(i0 + i, y[i], x[0]);
+        }
+    }
+    const uint64_t w0 = a.table[0];
+    const uint32_t token = a.tokens ? a.tokens[r] : 0xffffffffu;
+    const bool some = token < (uint32_t)V;
+    const int64_t of_token = SRC != SCORE_COMPACT && some ? row.value((int)token) : 0;
+    int64_t M;
+    if constexpr (SRC == SCORE_COMPACT) {
+        int64_t most = INT64_MIN;
+        for (int j = tid; j < a.ntiles; j += NT) most = tm[j] > most ? tm[j] : most;
+        M = block_join<NW>(most, slots, Max());
+    } else {
+        mx = block_join<NW>(mx, slots, Max());  // (its barriers: the histogram is clear)
+        M = SRC == SCORE_I32 ? (int64_t)mx : (int64_t)((uint64_t)(uint32_t)mx + ref);
+    }
+    // logits that lie further apart; and a table that is not a model's (the entropy below divides by w0): uniform
+    if (w0 == 0 || (SRC == SCORE_I64 && __syncthreads_or(apart != 0))) {
         score_any_row<SRC, NW>(a, r, slots);
         return;
     }
-    for (int k = tid; k < last + 64; k += NT) s_hist[k] = 0;
-    if (tid == 0) s_count = 0;
-
-    if constexpr (SRC == SCORE_COMPACT) {
-        const int64_t *tm = a.tmax + r * a.ntiles;
-        const uint16_t *p = a.d16 + r * a.ld16;  // whole tiles of 64 (the row is padded)
-        uint2 raw[G];
-        int64_t t[G];
-#pragma unroll
-        for (int i = 0; i < G; i++) {
-            const int j = symbol(i, 0) < V ? symbol(i, 0) : 0;
-            raw[i] = *(const uint2 *)(p + j);
-            t[i] = tm[j >> 6];
-        }
-        int64_t mx = INT64_MIN;
-        for (int j = tid; j < a.ntiles; j += NT) mx = tm[j] > mx ? tm[j] : mx;
-        const int64_t M = top_logit = block_join<NW>(mx, slots, Max());
-        if (some) td = row.index(M, (int)token);
-#pragma unroll
-        for (int i = 0; i < G; i++) {
-            const uint64_t b = (uint64_t)M - (uint64_t)t[i];
-            const uint32_t base = b < (uint64_t)cap ? (uint32_t)b : cap;
-            uint32_t d[4] = {raw[i].x & 0xffffu, raw[i].x >> 16, raw[i].y & 0xffffu, raw[i].y >> 16};
-#pragma unroll
-            for (int e = 0; e < 4; e++) d[e] = d[e] + base < (uint32_t)last ? d[e] + base : cap;  // (a d16 may be capped at last)
-            d2[2 * i] = d[0] | d[1] << 16;
-            d2[2 * i + 1] = d[2] | d[3] << 16;
-        }
-    } else {
-        // 16-byte loads, from the 16 bytes that the row starts in to those that it ends in; zeros past them
-        constexpr int E = SRC == SCORE_I32 ? 4 : 8;
-        const uintptr_t at = (uintptr_t)a.logits + r * a.ld * E;
-        off = (int)(at % 16) / E;
-        const int bytes = ((off + V) * E + 15) / 16 * 16;
-        const auto from = __builtin_amdgcn_make_buffer_rsrc((void *)(at - at % 16), 0, bytes, 0x00020000);
-        const int64_t of_token = some ? row.value((int)token) : 0;
-        // i32 logits as they are, i64 ones as their difference to 2^31 below the row's first one, in 32 bits
-        typedef typename std::conditional<SRC == SCORE_I32, int32_t, uint32_t>::type X;
-        constexpr X LOW = SRC == SCORE_I32 ? (X)INT32_MIN : (X)0;
-        X x[4 * G], mx = LOW;
-        uint64_t ref = 0;
-        uint32_t apart = 0;  // not 0: they do not fit
-        auto take = [&](int i) {
-            if (edge(i)) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[4 * i + e] = inside(symbol(i, e)) ? x[4 * i + e] : LOW;
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) mx = x[4 * i + e] > mx ? x[4 * i + e] : mx;
-        };
-        if constexpr (SRC == SCORE_I32) {
-#pragma unroll
-            for (int i = 0; i < G; i++) {
-                const uint4 y = load(from, 16 * tid, 16 * NT * i);
-                x[4 * i] = (int32_t)y.x;
-                x[4 * i + 1] = (int32_t)y.y;
-                x[4 * i + 2] = (int32_t)y.z;
-                x[4 * i + 3] = (int32_t)y.w;
-            }
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int i = 0; i < G; i++) take(i);
+    int td = 0;  // the token's index
+    if (some) {
+        if constexpr (SRC == SCORE_COMPACT) {
+            td = row.index(M, (int)token);
         } else {
-            const int64_t first = ((const int64_t *)at)[0];
-            // (a first logit at the types' ends: the differences would come round)
-            if (first >= (int64_t)1 << 62 || first < -((int64_t)1 << 62)) apart = 1;
-            ref = (uint64_t)first - 0x80000000u;
-            constexpr int B = 4;  // groups in flight beside those at work
-            uint4 raw[2][B][2];
-            auto fetch = [&](int i0, uint4(&y)[B][2]) {
-#pragma unroll
-                for (int i = 0; i < B && i0 + i < G; i++)
-#pragma unroll
-                    for (int k = 0; k < 2; k++) y[i][k] = load(from, 32 * tid + 16 * k, 32 * NT * (i0 + i));
-            };
-            fetch(0, raw[0]);
-#pragma unroll
-            for (int i0 = 0; i0 < G; i0 += B) {
-                uint4(&y)[B][2] = raw[(i0 / B) & 1];
-                __builtin_amdgcn_sched_barrier(0);
-                if (i0 + B < G) fetch(i0 + B, raw[(i0 / B + 1) & 1]);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int i = 0; i < B && i0 + i < G; i++) {
-                    uint32_t high[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const uint4 q = y[i][e >> 1];
-                        const uint64_t u = (e & 1 ? (uint64_t)q.w << 32 | q.z : (uint64_t)q.y << 32 | q.x) - ref;
-                        x[4 * (i0 + i) + e] = (uint32_t)u;
-                        high[e] = (uint32_t)(u >> 32);
-                    }
-                    if (edge(i0 + i)) {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) high[e] = inside(symbol(i0 + i, e)) ? high[e] : 0;
-                    }
-                    apart |= (high[0] | high[1]) | (high[2] | high[3]);
-                    take(i0 + i);
-                }
-            }
-            if (__syncthreads_or(apart != 0)) {  // logits that lie further apart: uniform
-                score_any_row<SRC, NW>(a, r, slots);
-                return;
-            }
-        }
-        const X m = block_join<NW>(mx, slots, Max());
-        top_logit = SRC == SCORE_I32 ? (int64_t)m : (int64_t)((uint64_t)m + ref);
-        if (some) {
-            const uint64_t d = (uint64_t)top_logit - (uint64_t)of_token;
+            const uint64_t d = (uint64_t)M - (uint64_t)of_token;
             td = d < (uint64_t)last ? (int)d : last;
         }
+    }
+    // the indexes of a group, cap for what lies past the table and the row
+    auto indexes = [&](int i, const Raw &y, const X (&v)[4], int64_t t, uint32_t (&d)[4]) {
+        if constexpr (SRC == SCORE_COMPACT) {
+            const uint64_t b = (uint64_t)M - (uint64_t)t;
+            const uint32_t base = b < (uint64_t)cap ? (uint32_t)b : cap;
 #pragma unroll
-        for (int i = 0; i < 2 * G; i++) {
-            uint32_t d[2];
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const uint32_t y = (uint32_t)m - (uint32_t)x[2 * i + e];  // (unsigned: any two)
-                d[e] = y < cap ? y : cap;
+            for (int e = 0; e < 4; e++) {
+                d[e] = base + (e & 1 ? (uint32_t)y[0][e >> 1] >> 16 : (uint32_t)y[0][e >> 1] & 0xffffu);
+                d[e] = d[e] < (uint32_t)last ? d[e] : cap;  // (a d16 may be capped at last)
             }
-            d2[i] = d[0] | d[1] << 16;
-        }
-    }
-    auto index = [&](int i, int e) { return e & 1 ? d2[2 * i + (e >> 1)] >> 16 : d2[2 * i + (e >> 1)] & 0xffffu; };
+        } else {
 #pragma unroll
-    for (int i = 0; i < G; i++)
+            for (int e = 0; e < 4; e++) {
+                d[e] = (uint32_t)mx - (uint32_t)v[e];  // (unsigned: any two)
+                d[e] = d[e] < cap ? d[e] : cap;
+            }
+        }
         if (edge(i)) {
-            uint32_t y[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = inside(symbol(i, e)) ? index(i, e) : cap;
-            d2[2 * i] = y[0] | y[1] << 16;
-            d2[2 * i + 1] = y[2] | y[3] << 16;
+            for (int e = 0; e < 4; e++) d[e] = inside(symbol(i, e)) ? d[e] : cap;
         }
-    // (hides the pairs from the optimizer, which would keep every index unpacked from one walk to the next)
-    auto hide = [&] {
-#pragma unroll
-        for (int i = 0; i < 2 * G; i++) asm volatile("" : "+v"(d2[i]));
     };
-    hide();
-#pragma unroll
-    for (int i = 0; i < G; i++) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) atomicAdd(&s_hist[index(i, e)], 1u);
-        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-    }
-    // fn(symbol, index) for the symbols with an index in lo ..= hi, few: a test a group of four
-    auto those = [&](uint32_t lo, uint32_t hi, auto fn) {
-        hide();
-        const uint32_t span = (hi >= (uint32_t)last ? 0xffffu : hi) - lo;
+    uint32_t d2[2 * GS];  // G > 0: the indexes, pairs
+    uint32_t places = 0;  // counted
+    if constexpr (G > 0) {
 #pragma unroll
         for (int i = 0; i < G; i++) {
-            uint32_t p0 = d2[2 * i], p1 = d2[2 * i + 1], least = 0xffffffffu;
+            uint32_t d[4];
+            indexes(i, raw[SRC == SCORE_COMPACT ? i : 0], x[i], tile[SRC == SCORE_COMPACT ? i : 0], d);
 #pragma unroll
-            for (int e = 0; e < 4; e++) least = index(i, e) - lo < least ? index(i, e) - lo : least;
-            if (least > span) continue;
-            asm volatile("" : "+v"(p0), "+v"(p1));  // (else the choice below makes an array in memory of all pairs)
+            for (int e = 0; e < 4; e++) atomicAdd(&s_hist[d[e]], 1u);
+            d2[2 * i] = d[0] | d[1] << 16;
+            d2[2 * i + 1] = d[2] | d[3] << 16;
+            if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+        places = 4 * G * NT;
+    }
+    // fn(i, y): the loads of each group (G = 0), eight at a time, and its values and tile maxes
+    auto walk = [&](auto fn) {
+        for (int i0 = 0; i0 < groups; i0 += 8) {
+            Raw y[8];
+            int64_t t[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                fetch(i0 + i, y[i]);
+                if constexpr (SRC == SCORE_COMPACT) t[i] = tile_of(i0 + i);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                uint32_t d[4];
+                X v[4];
+                if (i0 + i >= groups) break;  // uniform
+                if constexpr (SRC != SCORE_COMPACT) values(i0 + i, y[i], v);
+                indexes(i0 + i, y[i], v, t[i], d);
+                fn(i0 + i, d);
+            }
+        }
+    };
+    if constexpr (G == 0) {
+        walk([&](int, uint32_t (&d)[4]) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) atomicAdd(&s_hist[d[e]], 1u);
+        });
+        places = 4 * NT * groups;
+    }
+    // fn(symbol, index) for the symbols with an index in lo ..= hi, few: a test for eight at once
+    auto those = [&](uint32_t lo, uint32_t hi, auto fn) {
+        const uint32_t span = (hi >= (uint32_t)last ? 0xffffu : hi) - lo;
+        auto take = [&](int i, int e, uint32_t d) {
+            if (d - lo <= span && inside(symbol(i, e))) fn(symbol(i, e), d < (uint32_t)last ? (int)d : last);
+        };
+        if constexpr (G == 0) {
+            walk([&](int i, uint32_t (&d)[4]) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) take(i, e, d[e]);
+            });
+        } else {
+            const us2 base = {(unsigned short)lo, (unsigned short)lo}, most = {(unsigned short)span, (unsigned short)span};
+#pragma unroll
+            for (int i = 0; i < G; i += 2) {
+                uint32_t q[4];
+                us2 least = {0xffff, 0xffff};
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    q[k] = 2 * i + k < 2 * G ? d2[2 * i + k] : 0xffffffffu;
+                    // (hidden from the optimizer: it would keep the indexes unpacked from one walk to the next, or make an array
+                    // in memory for the choice below)
+                    asm volatile("" : "+v"(q[k]));
+                    us2 p;
+                    __builtin_memcpy(&p, &q[k], 4);
+                    p -= base;
+                    least = __builtin_elementwise_min(least, p);
+                }
+                const us2 over = __builtin_elementwise_sub_sat(least, most);  // 0: one of the four lies in the span
+                if (over.x && over.y) continue;
 #pragma unroll 1
-            for (int e = 0; e < 4; e++) {
-                const uint32_t d = ((e & 2 ? p1 : p0) >> (16 * (e & 1))) & 0xffffu;
-                if (d - lo <= span && inside(symbol(i, e))) fn(symbol(i, e), d < (uint32_t)last ? (int)d : last);
+                for (int e = 0; e < 8; e++) {
+                    const uint32_t pair = e & 4 ? (e & 2 ? q[3] : q[2]) : (e & 2 ? q[1] : q[0]);
+                    take(i + (e >> 2), e & 3, (pair >> (16 * (e & 1))) & 0xffffu);
+                }
             }
         }
     };
     __syncthreads();  // the counts are there
     if (w == 0) {     // the spare bins to the last one, without the places past the row
         const uint32_t far = (uint32_t)wave_sum64(s_hist[last + lane]);
-        if (lane == 0) s_hist[last] = far - (uint32_t)(4 * G * NT - V);
+        if (lane == 0) s_hist[last] = far - (places - (uint32_t)V);
     }
     uint32_t ahead = 0;  // symbols before the token
     __syncthreads();
@@ -339,24 +396,24 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
     // sum (w / T) ln(T / w) = ln(T / w0) + (sum w ln(w0 / w)) / T, two terms that are not negative (log_share takes the first,
     // exact where T is close to w0). In f32 the logarithms of the second are some 2^-22 off, which the first outweighs: it is
     // at least the share of all symbols but the largest.
-    const uint64_t w0 = a.table[0];
     const float w0f = (float)w0;
     uint64_t sum = 0;
     float spread = 0;
     for (int d0 = tid; d0 <= last; d0 += 8 * NT) {
         uint32_t n[8];
-        uint64_t x[8];
+        uint64_t z[8];
 #pragma unroll
         for (int k = 0; k < 8; k++) {
             const int d = d0 + NT * k;
             n[k] = d <= last ? s_hist[d] : 0;
-            x[k] = n[k] ? a.table[d] : 0;
+            z[k] = n[k] ? a.table[d] : 0;
         }
 #pragma unroll
         for (int k = 0; k < 8; k++) {
-            sum += n[k] * x[k];
-            const float y = (float)x[k], l = __builtin_amdgcn_logf(w0f * __builtin_amdgcn_rcpf(y));
-            spread += x[k] ? (float)n[k] * y * l : 0.0f;
+            sum += n[k] * z[k];
+            const float y = fmaf((float)(uint32_t)(z[k] >> 32), 0x1p32f, (float)(uint32_t)z[k]);
+            const float l = __builtin_amdgcn_logf(w0f * __builtin_amdgcn_rcpf(y));
+            spread += z[k] ? (float)n[k] * y * l : 0.0f;
             ahead += d0 + NT * k < td ? n[k] : 0;
         }
     }
@@ -403,26 +460,40 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
     uint64_t T = 0;
 #pragma unroll
     for (int i = 0; i < NW; i++) T += s_sum[i];
-    if (tid == 0) {
-        for (int i = 1; i < NW; i++) ahead += s_ahead[i], h += s_ent[i];
-        if (a.logprob || a.rank) put_token(a, r, some, some ? a.table[td] : 0, T, ahead);
-        if (a.entropy) a.entropy[r] = (float)(h / (double)T - log_share(w0, T));
-    }
-    if (!tops) return;
-    const uint32_t thr = s_thr;
-    if (s_found <= SCORE_LIST) {  // uniform
-        those(0, thr, [&](int j, int d) { s_list[atomicAdd(&s_count, 1u)] = (uint64_t)d << 32 | (uint32_t)j; });
+    int best = 0;  // alternatives in s_best
+    if (tops && s_found <= LIST) {  // uniform
+        those(0, s_thr, [&](int j, int d) { s_list[atomicAdd(&s_count, 1u)] = (uint64_t)d << 32 | (uint32_t)j; });
         __syncthreads();
         const int found = (int)s_found;
         for (int i = tid; i < found; i += NT) {
-            const uint64_t x = s_list[i];
+            const uint64_t one = s_list[i];
             int place = 0;
-            for (int k = 0; k < found; k++) place += s_list[k] < x;
-            if (place < a.top) put_top(a, r, place, (uint32_t)x, (int)(x >> 32), T);
+            for (int k = 0; k < found; k++) place += s_list[k] < one;
+            if (place < a.top) s_best[place] = one;
         }
-        return;
+        __syncthreads();
+        best = a.top;
     }
-    search_top<SRC, NW>(a, r, top_logit, T, slots);
+    // one logarithm a lane: the alternatives', the token's, the entropy's
+    for (int i = tid; i < best + 2; i += NT) {
+        const uint64_t one = i < best ? s_best[i] : 0;
+        const uint64_t weight = i < best ? a.table[one >> 32] : i == best ? (some ? a.table[td] : 1) : w0;
+        const double l = log_share(weight, T);
+        if (i < best) {
+            if (a.top_tokens) a.top_tokens[r * a.top + i] = (uint32_t)one;
+            if (a.top_logprob) a.top_logprob[r * a.top + i] = (float)l;
+        } else if (i == best) {
+            uint32_t n = 0;
+            for (int k = 0; k < NW; k++) n += s_ahead[k];
+            if (a.logprob) a.logprob[r] = some ? (float)l : 0.0f;
+            if (a.rank) a.rank[r] = some ? n : 0xffffffffu;
+        } else if (a.entropy) {
+            double x = 0;
+            for (int k = 0; k < NW; k++) x += s_ent[k];
+            a.entropy[r] = (float)(x / (double)T - l);
+        }
+    }
+    if (tops && best == 0) search_top<SRC, NW>(a, r, M, T, slots);
 }
 
 template <int SRC, int G, int NW>
@@ -438,14 +509,16 @@ template <int SRC>
 static hipError_t launch_score_src(const ScoreArgs &a, int n_rows, hipStream_t stream) {
     if (a.table_len <= SCORE_BINS) {
         const int v = a.vocab + 3;  // with the part of 16 bytes before a row
-        if (v <= 4 * 128 * 4) return launch_score_rows<SRC, 4, 2>(a, n_rows, stream);
+        if (v <= 4 * 64 * 4) return launch_score_rows<SRC, 4, 1>(a, n_rows, stream);
         if (v <= 4 * 512 * 8) return launch_score_rows<SRC, 8, 8>(a, n_rows, stream);
         if constexpr (SRC == SCORE_I64) {
             if (v <= 4 * 1024 * 13) return launch_score_rows<SRC, 13, 16>(a, n_rows, stream);
         } else {
+            // a row a CU: 64 rows 18 us (26 groups of 8 waves 21); more rows share a CU, one at its loads while another counts
+            if (n_rows <= 256 && v <= 4 * 1024 * 13) return launch_score_rows<SRC, 13, 16>(a, n_rows, stream);
             if (v <= 4 * 512 * 26) return launch_score_rows<SRC, 26, 8>(a, n_rows, stream);
-            if (v <= 4 * 1024 * 26) return launch_score_rows<SRC, 26, 16>(a, n_rows, stream);
         }
+        return launch_score_rows<SRC, 0, 16>(a, n_rows, stream);
     }
     launch_k(k_score_any<SRC>, dim3(n_rows), dim3(512), 0, stream, a);
     return hipGetLastError();

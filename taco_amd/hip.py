@@ -610,12 +610,20 @@ def gemm_requant_i8(dev: HipDevice, w, a, bias, mult, shift: int) -> np.ndarray:
     return out
 
 
+def _on_gpu(x) -> bool:
+    """Whether x is a tensor, on the GPU (one in host memory is refused)."""
+    cuda = getattr(x, "is_cuda", None)
+    if cuda is None:
+        return hasattr(x, "data_ptr")
+    if not cuda:
+        raise ValueError("a tensor in host memory where the GPU reads or writes")
+    return True
+
+
 def _dptr(x):
     """The device address of x: a contiguous tensor on the GPU (data_ptr()), an address or a ctypes pointer, or None."""
-    if not hasattr(x, "data_ptr"):
+    if not _on_gpu(x):
         return x
-    if not getattr(x, "is_cuda", True):
-        raise ValueError("a tensor in host memory where the GPU reads or writes")
     if not x.is_contiguous():
         raise ValueError("a tensor with strides of its own: the operators take contiguous ones")
     return x.data_ptr()
@@ -738,43 +746,46 @@ class PagedCache(NamedTuple):
     max_scale: int
 
     def _struct(self):
-        numbers = self[4:]
-        if any(not 0 <= x <= _U32 for x in numbers):
+        k, v, ks, vs, *numbers = self
+        if min(numbers) < 0 or max(numbers) > _U32:
             raise Unsupported(HS_UNSUPPORTED, 0, "a size that 32 bits do not hold")
-        return _Pages(*[_address(_dptr(x)) for x in self[:4]], *numbers)
-
-
-def _address(x):
-    return x.value if isinstance(x, C.c_void_p) else x
+        return _Pages(_dptr(k), _dptr(v), _dptr(ks), _dptr(vs), *numbers)
 
 
 def _sizes(*numbers):
     """Sizes for the library; a negative one would come round to a large one."""
-    if any(x < 0 for x in numbers):
+    if min(numbers) < 0:
         raise Unsupported(HS_UNSUPPORTED, 0, "a negative size")
     return numbers
 
 
-def _signed(x) -> bool:
-    """Whether a tensor holds signed integers."""
-    name = str(x.dtype)
-    return "int" in name and "uint" not in name
+_types = {}  # the bits of a tensor's type, 0 where it does not hold signed integers
 
 
-def _rows_of(x, stride: Optional[int], values: int):
-    """The address of rows of new tokens and the elements from one token to the next: a tensor [streams, t, heads,
+def _bits_of(x) -> int:
+    dtype = x.dtype
+    bits = _types.get(dtype)
+    if bits is None:
+        name = str(dtype)
+        bits = _types[dtype] = 8 * x.element_size() if "int" in name and "uint" not in name else 0
+    return bits
+
+
+def _rows_of(x, bits: Optional[int], stride: Optional[int], shape):
+    """Rows of new tokens as (address, bits of a value, elements from one token to the next): a tensor [streams, t, heads,
     head_dim] on the GPU whose heads of a token lie together and whose tokens at one distance, or an address with
-    `stride` (None: the rows lie together)."""
-    if not hasattr(x, "data_ptr"):
-        return x, values if stride is None else stride
-    if not getattr(x, "is_cuda", True):
-        raise ValueError("a tensor in host memory where the GPU reads or writes")
-    (b, t, h, hd), st = x.shape, x.stride()
-    step = st[1] if t > 1 else st[0] if b > 1 else values
+    `bits` and `stride` (None: the rows lie together)."""
+    b, t, h, hd = shape
+    if not _on_gpu(x):
+        return x, bits or 0, h * hd if stride is None else stride
+    st, own = x.stride(), _bits_of(x)
+    if x.shape != shape or own == 0 or (bits is not None and bits != own):
+        raise ValueError(f"a tensor that does not hold {tuple(shape)} integers of the operator's types")
+    step = st[1] if t > 1 else st[0] if b > 1 else h * hd
     if (h > 1 and st[2] != hd) or (hd > 1 and st[3] != 1) or (b > 1 and st[0] != t * step) or \
             (stride is not None and stride != step):
         raise ValueError("a tensor whose tokens do not lie at one distance, each with its heads together")
-    return x.data_ptr(), step
+    return x.data_ptr(), own, step
 
 
 def pages_append(dev: HipDevice, cache: PagedCache, k, v, table, ctx, rows, dims, headroom: int = 16, ctx_out=None,
@@ -782,19 +793,14 @@ def pages_append(dev: HipDevice, cache: PagedCache, k, v, table, ctx, rows, dims
     """Appends rows of keys and values to the streams' pages (hs_op_pages_append_dev): dims = (streams, t, width);
     k and v are tensors [streams, t, kv_heads, head_dim] of int8 or int16, or addresses with `bits` and `stride`."""
     b, t, width = _sizes(*dims)
-    for x in (k, v):
-        if hasattr(x, "element_size"):
-            if tuple(x.shape) != (b, t, cache.kv_heads, cache.head_dim) or bits not in (None, 8 * x.element_size()) or \
-                    not _signed(x):
-                raise ValueError("k and v: [streams, t, kv_heads, head_dim], both int8 or both int16")
-            bits = 8 * x.element_size()
-    (kp, ks), (vp, vs) = (_rows_of(x, stride, cache.kv_heads * cache.head_dim) for x in (k, v))
-    if ks != vs:
-        raise ValueError("k and v with tokens at different distances")
+    shape = (b, t, cache.kv_heads, cache.head_dim)
+    kp, kb, ks = _rows_of(k, bits, stride, shape)
+    vp, vb, vs = _rows_of(v, bits, stride, shape)
+    if ks != vs or kb != vb:
+        raise ValueError("k and v of different types, or with tokens at different distances")
     if not 0 <= headroom <= _U32:
         raise Unsupported(HS_UNSUPPORTED, 0, "headroom must be in 16..=64 sixteenths")
-    p = cache._struct()
-    _check(lib().hs_op_pages_append_dev(dev.h, C.byref(p), kp, vp, bits or 0, *_sizes(ks), _dptr(table), _dptr(ctx),
+    _check(lib().hs_op_pages_append_dev(dev.h, C.byref(cache._struct()), kp, vp, kb, *_sizes(ks), _dptr(table), _dptr(ctx),
                                         _dptr(rows), b, t, width, headroom, _dptr(ctx_out), stream))
 
 
@@ -803,14 +809,13 @@ def attend_paged(dev: HipDevice, cache: PagedCache, q, table, ctx, rows, dims, r
     """Causal attention over the streams' pages (hs_op_attend_paged_dev): dims = (streams, t, heads, width, keys);
     q is a tensor [streams, t, heads, head_dim] of int8, or an address with `q_stride`; rows may be None (t each)."""
     b, t, heads, width, keys = _sizes(*dims)
-    if hasattr(q, "data_ptr") and (tuple(q.shape) != (b, t, heads, cache.head_dim) or q.element_size() != 1):
+    qp, bits, step = _rows_of(q, None, q_stride, (b, t, heads, cache.head_dim))
+    if bits not in (0, 8):
         raise ValueError("q: [streams, t, heads, head_dim] of int8")
-    qp, step = _rows_of(q, q_stride, heads * cache.head_dim)
     m, s, om, os_, exp, length, p = rule
-    pages = cache._struct()
-    _check(lib().hs_op_attend_paged_dev(dev.h, C.byref(pages), qp, *_sizes(step), _dptr(table), _dptr(ctx), _dptr(rows),
-                                        b, t, heads, width, keys, m, s, om, os_, _dptr(exp), length, p, _dptr(out),
-                                        _dptr(workspace), workspace_bytes, stream))
+    _check(lib().hs_op_attend_paged_dev(dev.h, C.byref(cache._struct()), qp, *_sizes(step), _dptr(table), _dptr(ctx),
+                                        _dptr(rows), b, t, heads, width, keys, m, s, om, os_, _dptr(exp), length, p,
+                                        _dptr(out), _dptr(workspace), workspace_bytes, stream))
 
 
 def attend_paged_workspace(streams: int, t: int, heads: int, kv_heads: int, head_dim: int, keys: int) -> int:
@@ -823,19 +828,16 @@ def score_tokens(dev: HipDevice, logits, tokens, table, dims, top: int, logprob,
     """The scores of rows of logits on the device (hs_op_score_dev): dims = (rows, vocab, table length); logits is a
     tensor [rows, vocab] of int32 or int64 with its symbols together, or an address with `bits` and `stride`."""
     rows, vocab, length = _sizes(*dims)
-    _sizes(top)
-    if hasattr(logits, "data_ptr"):
-        if tuple(logits.shape) != (rows, vocab) or bits not in (None, 8 * logits.element_size()) or \
-                not _signed(logits) or (vocab > 1 and logits.stride(1) != 1):
+    if _on_gpu(logits):
+        own, st = _bits_of(logits), logits.stride()
+        if logits.shape != (rows, vocab) or own == 0 or (bits is not None and bits != own) or (vocab > 1 and st[1] != 1):
             raise ValueError("logits: [rows, vocab] of int32 or int64, the symbols of a row together")
-        if not getattr(logits, "is_cuda", True):
-            raise ValueError("a tensor in host memory where the GPU reads or writes")
-        bits = 8 * logits.element_size()
-        stride = logits.stride(0) if rows > 1 else vocab
-        logits = logits.data_ptr()
-    _check(lib().hs_op_score_dev(dev.h, logits, bits or 0, *_sizes(vocab if stride is None else stride), _dptr(tokens),
-                                 _dptr(table), length, rows, vocab, top, _dptr(logprob), _dptr(rank), _dptr(entropy),
-                                 _dptr(top_tokens), _dptr(top_logprob), stream))
+        bits, stride, logits = own, st[0] if rows > 1 else vocab, logits.data_ptr()
+    elif stride is None:
+        stride = vocab
+    _sizes(top, stride)
+    _check(lib().hs_op_score_dev(dev.h, logits, bits or 0, stride, _dptr(tokens), _dptr(table), length, rows, vocab, top,
+                                 _dptr(logprob), _dptr(rank), _dptr(entropy), _dptr(top_tokens), _dptr(top_logprob), stream))
 
 
 def kernel_resources(dev: HipDevice):

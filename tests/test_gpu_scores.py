@@ -233,3 +233,31 @@ def test_wide_models_and_long_tables(dev):
         weights = plain.run_weights(inputs)
         tokens = likely(r, weights)
         check_scores(scored.run_scored(inputs, tokens, 5), weights, tokens, 5)
+
+
+@pytest.mark.parametrize("dtype", [np.int32, np.int64])
+@pytest.mark.parametrize("vocab", [1021, 1022, 16381, 16382, 53245, 53246, 131_072])
+def test_around_the_forms(gpu, vocab, dtype):
+    """Vocabularies at the ends of what a wave's and a workgroup's registers hold, every alignment of a row, and ties."""
+    r = np.random.default_rng(vocab)
+    logits = normal(r, 4, vocab, dtype, std=300)
+    logits[1, vocab // 3::5] = logits[1].max()
+    check(gpu, logits, WEIGHTS, [vocab - 1, vocab - 2, 0, int(logits[3].argmax())], 9, 1)
+
+
+def test_rows_that_do_not_start_at_16_bytes(gpu):
+    r = np.random.default_rng(8)
+    for dtype in (np.int32, np.int64):
+        logits, tokens = normal(r, 3, 501, dtype), np.array([0, 250, 500], np.uint32)
+        size = dtype().itemsize
+        for skip in range(1, 16 // size):
+            flat = np.concatenate([np.full(skip, np.iinfo(dtype).max, dtype), logits.ravel()])
+            outs = [np.zeros(3, np.float32), np.zeros(3, np.uint32), np.zeros(3, np.float32)]
+            held = [gpu(x) for x in outs]
+            gpu.hip.score_tokens(gpu.dev, gpu(flat).value + skip * size, gpu(tokens), gpu(WEIGHTS), (3, 501, 8192), 0, *held, None, None,
+                                 bits=8 * size)
+            got = [gpu.back(p, x) for p, x in zip(held, outs)]
+            lp, rank, entropy, _, _ = ref.scores(logits, WEIGHTS, tokens, 0)
+            assert np.array_equal(got[1], rank)
+            ref.close(got[0], lp, 1)
+            ref.close(got[2], entropy, 8)

@@ -178,8 +178,8 @@ def test_tensors():
         with pytest.raises(ValueError):
             score(logits=bad, bits=None)
     kv = torch.zeros(2, 3, 2, 2, 64, dtype=torch.int16)  # parts of wider rows
-    assert hip._rows_of(Fake(kv[:, :, 1]), None, 128) == (BASE, 256)
-    assert hip._rows_of(Fake(kv[:1, :1, 1]), None, 128) == (BASE, 128)
+    assert hip._rows_of(Fake(kv[:, :, 1]), None, None, (2, 3, 2, 64)) == (BASE, 16, 256)
+    assert hip._rows_of(Fake(kv[:1, :1, 1]), None, None, (1, 1, 2, 64)) == (BASE, 16, 128)
 
 
 def test_batch_tokens():
