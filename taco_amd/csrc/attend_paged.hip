@@ -10,6 +10,17 @@ constexpr int PG_TABLE = 16384;  // entries of the table copied to LDS at most
 constexpr int PG_ACC = 66;       // 64 channels' sums of a row and two of padding (bank spread)
 constexpr int PG_NONE = 0x7fffffff;  // a lane's offset past any page: the buffer load gives zeros
 
+// n / d without a division: m = ceil(2^32 / d) makes the high word of n m the quotient or one more.
+struct PagedDiv {
+    uint32_t d = 1, m = 0;
+    PagedDiv() = default;
+    explicit PagedDiv(uint32_t n) : d(n), m(n > 1 ? 0xffffffffu / n + 1 : 0) {}
+    __device__ __forceinline__ int of(int n) const {
+        const uint32_t q = m ? __umulhi((uint32_t)n, m) : (uint32_t)n;
+        return (int)(q * d > (uint32_t)n ? q - 1 : q);
+    }
+};
+
 struct PagedPlan {
     int rt = 16;               // rows of a tile
     int group = 1, tiles = 1;  // query heads of a cache head; row tiles of a panel
@@ -18,6 +29,7 @@ struct PagedPlan {
     int store = 0;             // the ranges' scores are kept in the scratch
     int rows = 0, chunks = 1;  // rows of a tile with scores there; of PG_CHUNK keys, with a sum each
     int page_log = 4;
+    PagedDiv by_group, by_tiles, by_heads, by_inner;  // group, tiles, cache heads, 8 tiles ng
 };
 constexpr int PG_CHUNK = 4096;
 
@@ -73,50 +85,292 @@ struct PagedRule {
     }
 };
 
+// The table to LDS: whole KiB straight, the rest entry by entry (places past it repeat the last one). The caller waits.
+__device__ __forceinline__ void paged_table(const PagedArgs &g, int32_t *s_exp, int w, int waves, int lane) {
+    w = __builtin_amdgcn_readfirstlane(w);
+    for (int ch = w; ch < g.exp_len / 256; ch += waves)
+        __builtin_amdgcn_global_load_lds((const void *)(g.exp_table + ch * 256 + 4 * lane), (lds_void *)(s_exp + ch * 256), 16, 0, 0);
+    if (w == 0)
+        for (int i = g.exp_len / 256 * 256 + lane; i < (g.exp_len + 255) / 256 * 256; i += 64)
+            s_exp[i] = g.exp_table[i < g.exp_len ? i : g.exp_len - 1];
+}
+
+// The tile and key range of a workgroup. Workgroup L runs on XCD L % 8: the tiles of a panel stay on one XCD and share K and V in
+// its L2.
+struct PagedTile {
+    int s, h, tile, range, panel;
+    int row0, live;        // its first row, of those that are there
+    int before;            // token i of the stream sees keys up to before + i
+    int whole, keys;       // the keys that its first row sees, its last
+    size_t place, slot;    // of the tile, of its ranges in the scratch
+    bool there;
+    __device__ __forceinline__ PagedTile() {}
+    __device__ __forceinline__ PagedTile(const PagedArgs &g, const PagedPlan &pl, int L) {
+        const int inner = pl.tiles * pl.ng, group = pl.by_inner.of(L);
+        panel = 8 * group + (L & 7);
+        const int in = (L - 8 * inner * group) >> 3;
+        range = pl.by_tiles.of(in);
+        tile = in - range * pl.tiles;
+        there = panel < pl.panels;
+        if (!there) return;
+        s = pl.by_heads.of(panel);
+        h = panel - s * g.pages.kv_heads;
+        place = (size_t)panel * pl.tiles + tile;
+        slot = place * pl.ng;
+    }
+    // with the stream's counts
+    __device__ __forceinline__ void rows(const PagedArgs &g, const PagedPlan &pl, uint32_t ctx, uint32_t count) {
+        const int n = (int)(ctx < (uint32_t)g.keys ? ctx : (uint32_t)g.keys);
+        count = count < (uint32_t)g.t ? count : (uint32_t)g.t;
+        const int all = (int)count * pl.group;
+        row0 = pl.rt * tile;
+        live = all - row0 < pl.rt ? all - row0 : pl.rt;
+        before = n - (int)count;
+        whole = before + pl.by_group.of(row0) + 1;
+        keys = live > 0 ? before + pl.by_group.of(row0 + live - 1) + 1 : 0;
+    }
+};
+
+// The pages of a wave's blocks of 64 keys (the wave's block j starts at key first + step j, at most 16 of them): lane 4 j + t
+// knows the page of group t, the 16 keys from 16 t on.
+struct PagedBlocks {
+    uint32_t number;
+    uint64_t there;  // the groups with keys and a page
+    int first, step;
+    // (before the stream's counts are known: entries up to `keys` are there for every stream)
+    __device__ __forceinline__ PagedBlocks(const PagedArgs &g, const PagedPlan &pl, int s, int k0, int st, int blocks, int lane) : first(k0), step(st) {
+        const int key = key_of(lane >> 2) + 16 * (lane & 3);
+        number = 0xffffffffu;
+        if ((lane >> 2) < blocks && key < g.keys) number = g.table[(size_t)s * g.width + (key >> pl.page_log)];
+    }
+    __device__ __forceinline__ void until(const PagedArgs &g, int k1, int lane) {
+        if (key_of(lane >> 2) + 16 * (lane & 3) >= k1) number = 0xffffffffu;
+        there = __ballot(number < (uint32_t)g.pages.pages);
+    }
+    __device__ __forceinline__ int key_of(int j) const { return first + step * j; }
+    __device__ __forceinline__ bool has(int j, int t) const { return (there >> (4 * j + t)) & 1; }
+    // this lane's page's scale, 1 ..= max_scale (1 without a page)
+    __device__ __forceinline__ uint32_t scale(const PagedArgs &g, const uint32_t *scales, int h) const {
+        uint32_t x = 1;
+        if (number < (uint32_t)g.pages.pages) x = scales[(size_t)number * g.pages.kv_heads + h];
+        return x < 1 ? 1 : (x > g.pages.max_scale ? g.pages.max_scale : x);
+    }
+    // the 16 rows of a group; loads of one that is not there give zeros without an access
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows(const PagedArgs &g, const PagedPlan &pl, const int8_t *pool, int h, int j, int t) const {
+        const PagePool &p = g.pages;
+        const uint32_t page = has(j, t) ? (uint32_t)__builtin_amdgcn_readlane((int)number, 4 * j + t) : 0;
+        const size_t row = (((size_t)page * p.kv_heads + h) << pl.page_log) + ((key_of(j) + 16 * t) & (p.page - 1));
+        return __builtin_amdgcn_make_buffer_rsrc((void *)(pool + row * p.hd), 0, has(j, t) ? 16 * p.hd : 0, 0x00020000);
+    }
+};
+__device__ __forceinline__ v4i paged_load(__amdgpu_buffer_rsrc_t r, int at) {
+    return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
+}
+// K as the product's operand (chunk c: bytes 64 c + 16 (l / 16) .. of row l % 16); channels past the head are zeros
+template <int QC>
+__device__ __forceinline__ void paged_k(const PagedArgs &g, const PagedPlan &pl, const PagedBlocks &b, int h, int j, int lane, v4i (&x)[4][QC]) {
+    const int hd = g.pages.hd;
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        const auto r = b.rows(g, pl, g.pages.k, h, j, t);
+#pragma unroll
+        for (int c = 0; c < QC; c++) {
+            const int o = 64 * c + 16 * (lane >> 4);
+            x[t][c] = paged_load(r, o < hd ? (lane & 15) * hd + o : PG_NONE);
+        }
+    }
+}
+// 64 channels of V for paged_pv: lane l has 16-byte chunk l % 4, swizzled, of row l / 4 of each group
+__device__ __forceinline__ void paged_v(const PagedArgs &g, const PagedPlan &pl, const PagedBlocks &b, int h, int j, int c, int lane, v4i (&x)[4]) {
+    const int hd = g.pages.hd, r = lane >> 2, o = 64 * c + 16 * ((lane & 3) ^ vsw<4>(r)), at = o < hd ? r * hd + o : PG_NONE;
+#pragma unroll
+    for (int t = 0; t < 4; t++) x[t] = paged_load(b.rows(g, pl, g.pages.v, h, j, t), at);
+}
+// q of a tile's rows as the product's operand: with 16 rows a column is a row; with 4, operand t has row r in column 4 t + r.
+template <int RT, int QC>
+__device__ __forceinline__ void paged_q(const PagedArgs &g, const PagedPlan &pl, const PagedTile &T, int lane, v4i (&q)[RT == 16 ? 1 : 4][QC]) {
+    const int ql = lane & 15, row = RT == 16 ? ql : ql & 3, tok = pl.by_group.of(T.row0 + row);
+    const int head = T.h * pl.group + T.row0 + row - tok * pl.group;
+    const v4i zero = v4i{0, 0, 0, 0};
+#pragma unroll
+    for (int c = 0; c < QC; c++) {
+        const int o = 64 * c + 16 * (lane >> 4);
+        const v4i x = row < T.live && o < g.pages.hd
+                          ? *(const v4i *)(g.q + ((size_t)T.s * g.t + tok) * g.q_stride + (size_t)head * g.pages.hd + o) : zero;
+        if constexpr (RT == 16) {
+            q[0][c] = x;
+        } else {
+#pragma unroll
+            for (int t = 0; t < 4; t++) q[t][c] = (ql >> 2) == t ? x : zero;
+        }
+    }
+}
+// The dots of a block.
+template <int RT, int QC>
+__device__ __forceinline__ void paged_dots(const v4i (&x)[4][QC], const v4i (&q)[RT == 16 ? 1 : 4][QC], v4i (&D)[RT / 4]) {
+#pragma unroll
+    for (int u = 0; u < RT / 4; u++) D[u] = v4i{0, 0, 0, 0};
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int c = 0; c < QC; c++) {
+            v4i &d = D[RT == 16 ? t : 0];
+            d = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[t][c], q[RT == 16 ? 0 : t][c], d, 0, 0, 0);
+        }
+}
+// Of a value that lane 4 j + t holds, that of this lane's group of accumulator u.
+template <int RT>
+__device__ __forceinline__ int paged_of(uint32_t x, int j, int u, int lane) {
+    return RT == 16 ? __builtin_amdgcn_readlane((int)x, 4 * j + u) : __shfl((int)x, 4 * j + ((lane & 15) >> 2), 64);
+}
+
+// The digits of w = floor(E 2^P / S) for E = e vs, exactly (softmax_p_of, which holds for E < 2^53 with w <= 2^30), with
+// 0x80808080 inside the rounding constant: the low word of the sum is w + 0x80808080, whose bytes xor 0x80 are balanced
+// digits. From the entries D[u][e]: D[k] word t the digit k of group t's keys (16 rows); D[0] word t digit l % 4 of row
+// l / 4 % 4 of group t's keys (4 rows: the lanes transpose through 1 KiB of LDS).
+struct PagedWeight {
+    double R, sp;  // rows that are not there and rows without weight: w = 0 (R = 0)
+    __device__ __forceinline__ PagedWeight(uint64_t sum, int P, bool live)
+        : R(sum > 0 && live ? ldexp(1.0 / (double)sum, P) : 0.0), sp(softmax_sp(sum, P)) {}
+};
+template <int RT>
+__device__ __forceinline__ void paged_digits(const PagedWeight &wt, uint32_t vs, int j, int lane, int8_t *mem, v4i (&D)[RT / 4]) {
+    constexpr double magic = 6755399441055744.0 + 2155905152.0;  // 1.5 2^52 + 0x80808080
+    constexpr int TU = RT / 4;
+    const int ql = lane & 15, qg = lane >> 4;
+    uint32_t o[TU][4];
+#pragma unroll
+    for (int u = 0; u < TU; u++) {
+        const double scale = (double)(uint32_t)paged_of<RT>(vs, j, u, lane);
+        uint32_t dg[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const double ed = (double)(uint32_t)D[u][e] * scale, x = fma(ed, wt.R, magic), r = fma(x - magic, wt.sp, ed);
+            dg[e] = (uint32_t)__double2loint(x) + (uint32_t)(__double2hiint(r) >> 31);
+        }
+        byte_transpose(dg[0], dg[1], dg[2], dg[3], o[u]);
+        if (RT == 16) __builtin_amdgcn_sched_barrier(0);  // (interleaved they spill)
+    }
+    if constexpr (RT == 16) {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) D[k][t] = (int32_t)(o[t][k] ^ 0x80808080u);
+    } else {
+        int *to = (int *)mem + 64 * (ql & 3) + 4 * qg + (ql >> 2);  // [row][digit][l / 16][group]
+#pragma unroll
+        for (int k = 0; k < 4; k++) to[16 * k] = (int)(o[0][k] ^ 0x80808080u);
+        D[0] = *(const v4i *)((const int *)mem + 16 * ql + 4 * qg);
+    }
+}
+// acc += V^T digits over a block, 64 channels of V through 4 KiB of LDS: channels 16 i + 4 (l / 16) + e of digit k of row l % 16
+// in acc[k][i][e] (16 rows), of digit l % 4 of row l / 4 % 4 in acc[0][i][e] (4 rows).
+// `then` runs when x has left the registers.
+template <int RT, typename F>
+__device__ __forceinline__ void paged_pv(const v4i (&x)[4], const v4i (&D)[RT / 4], int lane, int8_t *mem, v4i (&acc)[RT / 4][4], F then) {
+    const int ql = lane & 15, qg = lane >> 4, tr_k = ql >> 1, key = 16 * (tr_k >> 2) + 4 * qg + (tr_k & 3);
+#pragma unroll
+    for (int u = 0; u < 4; u++) *(v4i *)(mem + 1024 * u + 16 * lane) = x[u];
+    then();
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int8_t *p0 = mem + (4 * key + (i ^ vsw<4>(key & 15))) * 16 + 8 * (ql & 1);
+        const v2i r0 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)p0);
+        const v2i r1 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)(p0 + 32 * 64));
+        const v4i vf = v4i{r0[0], r0[1], r1[0], r1[1]};
+#pragma unroll
+        for (int k = 0; k < RT / 4; k++) acc[k][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf, D[k], acc[k][i], 0, 0, 0);
+    }
+}
+// The planes' sums of 64 channels of a wave added to the rows' sums s_acc[RT][PG_ACC]; SMALL: at most 256 keys, two planes' sums
+// below 2^31.
+template <int RT, bool SMALL>
+__device__ __forceinline__ void paged_add(const v4i (&acc)[RT / 4][4], int live, int lane, int64_t *s_acc) {
+    const int ql = lane & 15, qg = lane >> 4;
+    if constexpr (RT == 16) {
+        unsigned long long *to = (unsigned long long *)s_acc + ql * PG_ACC + 4 * qg;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                int64_t x;
+                if constexpr (SMALL) {
+                    const int32_t lo = acc[0][i][e] + acc[1][i][e] * 256, hi = acc[2][i][e] + acc[3][i][e] * 256;
+                    x = (int64_t)hi * 65536 + lo;
+                } else {
+                    const int64_t lo = (int64_t)acc[1][i][e] * 256 + acc[0][i][e], hi = (int64_t)acc[3][i][e] * 256 + acc[2][i][e];
+                    x = hi * 65536 + lo;
+                }
+                atomicAdd(to + 16 * i + e, (unsigned long long)x);
+            }
+    } else {
+        // lane l % 4 = i keeps the four planes' sum of channels 16 i ..: the quad's lanes exchange halves twice
+        const bool b0 = lane & 1, b1 = lane & 2;
+        int64_t y[2][4], z[4];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int32_t keep = b0 ? acc[0][2 * i + 1][e] : acc[0][2 * i][e], give = b0 ? acc[0][2 * i][e] : acc[0][2 * i + 1][e];
+                const int32_t got = dpp_mov<0xB1>(give);  // of the plane next to this lane's
+                y[i][e] = b0 ? (int64_t)keep * 256 + got : (int64_t)got * 256 + keep;
+            }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int64_t keep = b1 ? y[1][e] : y[0][e], got = lane_move64<1>(b1 ? y[0][e] : y[1][e]);
+            z[e] = b1 ? keep * 65536 + got : got * 65536 + keep;
+        }
+        unsigned long long *to = (unsigned long long *)s_acc + (ql >> 2) * PG_ACC + 16 * (lane & 3) + 4 * qg;
+        if ((ql >> 2) < live) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) atomicAdd(to + e, (unsigned long long)z[e]);
+        }
+    }
+}
+// Four output bytes of a row.
+__device__ __forceinline__ void paged_put(const PagedArgs &g, const PagedPlan &pl, int s, int h, int row, int ch, const int64_t *x) {
+    const double mo = g.out_s > 95 ? 0.0 : ldexp((double)g.out_m, -g.out_s);
+    uint32_t packed = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) packed |= (uint32_t)(uint8_t)(int8_t)attn_out_byte(x[e], mo, g.out_m, g.out_s) << (8 * e);
+    const int tok = pl.by_group.of(row), head = h * pl.group + row - tok * pl.group;
+    *(uint32_t *)(g.out + (((size_t)s * g.t + tok) * g.heads + head) * g.pages.hd + ch) = packed;
+}
+
 // Tiles of RT rows (16, or 4 where there are no more) of one (stream, cache head): row r is query head r % group of
 // token r / group. Wave w takes the blocks of 64 keys w, w + NW, .. of the range, NB at most, each in four groups of 16
 // keys that lie in one page. K is the first operand of v_mfma_i32_16x16x64_i8, so lane l holds dots of column l % 16
 // with keys 4 (l / 16) + e of a group. With 16 rows a column is a row and D[t] holds group t. With 4 rows column 4 t + r is
 // row r with group t: the products of the four groups add up in one accumulator, each with q in its own columns and
 // zeros in the others, so that no lane idles; the product with V takes the rows' four digit planes as its 16 columns.
-// PHASE 0: all in one launch. Else the ranges meet in the scratch: 1 the largest scores, 2 the sums of the entries, 3 the
-// products with V. KEEP: launch 1 leaves all scores there (0x80.. where a row does not see a key), k_paged_entries makes them
-// entries and sums, and launch 3 reads those; else each launch forms the dots again.
-template <int RT, int QC, int NB, int NW, bool HI, int PHASE, bool KEEP>
+// PHASE 0: all in one launch, the dots in registers from the one product to the other. Else the key ranges meet in the
+// scratch, each launch forming the dots again: 1 the largest scores, 2 the sums of the entries, 3 the products with V.
+template <int RT, int QC, int NB, int NW, bool HI, int PHASE>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 ? 4 : 2))) void k_paged_tile(PagedArgs g, PagedPlan pl, void *scratch) {
     static_assert(NB <= 16, "a lane for each group of the wave's blocks");
     static_assert(RT == 4 || NB <= 4, "two planes' sums of a wave's keys in 32 bits");
     constexpr int TU = RT / 4;  // accumulators of a block
-    constexpr int KD = QC == 1 ? (NB < 4 ? NB : NW > 8 ? 2 : 4) : QC == 2 && NB > 1 && NW <= 8 ? 2 : 1;  // blocks of K in flight, and of V
-    constexpr bool DOTS = !(KEEP && PHASE == 3);  // whether the launch forms the dots
+    constexpr int KD = QC == 1 ? (NB < 4 ? NB : NW > 8 || NB > 4 ? 2 : 4) : QC == 2 && NB > 1 && NW <= 8 ? 2 : 1;  // blocks of K in flight, and of V
     typedef typename std::conditional<HI, int32_t, int64_t>::type Score;
     constexpr Score LOW = HI ? (Score)INT32_MIN : (Score)INT64_MIN;
     extern __shared__ __attribute__((aligned(1024))) int8_t s_mem[];
     const PagePool &p = g.pages;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ql = lane & 15, qg = lane >> 4, hd = p.hd;
-    // workgroup L runs on XCD L % 8: the tiles of a panel stay on one XCD and share K and V in its L2
-    const int inner = pl.tiles * pl.ng;
-    const int L = blockIdx.x, panel = L / (8 * inner) * 8 + (L & 7), in = (L >> 3) % inner;
-    if (panel >= pl.panels) return;
-    const int tile = in % pl.tiles, range = in / pl.tiles;
-    const int s = panel / p.kv_heads, h = panel - s * p.kv_heads;
-    const int n = (int)(g.ctx[s] < (uint32_t)g.keys ? g.ctx[s] : (uint32_t)g.keys);  // the stream's keys
-    uint32_t count = g.rows ? g.rows[s] : (uint32_t)g.t;
-    count = count < (uint32_t)g.t ? count : (uint32_t)g.t;
-    const int rows = (int)count * pl.group, row0 = RT * tile;
-    if (row0 >= rows) return;
-    const int live = rows - row0 < RT ? rows - row0 : RT;
-    const int before = n - (int)count;  // token i sees keys up to before + i
-    const int whole = before + row0 / pl.group + 1, keys = before + (row0 + live - 1) / pl.group + 1;
-    const int k0 = PHASE ? range * pl.span : 0;
-    if (PHASE && k0 >= keys && range > 0) return;  // the launches behind read no result of this range
-    const int k1 = PHASE && k0 + pl.span < keys ? k0 + pl.span : keys;
-    const int ranges = PHASE && keys > pl.span ? (keys + pl.span - 1) / pl.span : 1;
+    PagedTile T(g, pl, blockIdx.x);
+    if (!T.there) return;
+    const int k0 = PHASE ? T.range * pl.span : 0;
+    const uint32_t ctx = g.ctx[T.s], count = g.rows ? g.rows[T.s] : (uint32_t)g.t;
+    PagedBlocks B(g, pl, T.s, k0 + 64 * w, 64 * NW, NB, lane);
+    T.rows(g, pl, ctx, count);
+    if (T.live <= 0) return;
+    if (PHASE && k0 >= T.keys && T.range > 0) return;  // the launches behind read no result of this range
+    const int k1 = PHASE && k0 + pl.span < T.keys ? k0 + pl.span : T.keys;
+    const int ranges = PHASE && T.keys > pl.span ? (T.keys + pl.span - 1) / pl.span : 1;
     const uint32_t last = (uint32_t)g.exp_len - 1;
 
     // LDS: the table (of 16 rows), which the sums of the outputs take over, each wave's V, what the waves exchange
-    const bool in_lds = RT == 16 && PHASE != 1 && !(KEEP && PHASE == 3) && g.table_lds;
+    const bool in_lds = RT == 16 && PHASE != 1 && g.table_lds;
     constexpr int ACC_BYTES = (8 * QC * RT * PG_ACC + 1023) / 1024 * 1024;
     const int table_bytes = in_lds ? 1024 * ((g.exp_len + 255) / 256) : 0;
     const int top = table_bytes > ACC_BYTES ? table_bytes : ACC_BYTES;
@@ -126,139 +380,45 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
     uint64_t *s_sum = (uint64_t *)(s_mem + top + 4096 * NW);  // [NW][RT]
     int64_t *s_mx = (int64_t *)(s_sum + NW * RT);             // [NW][RT]
     if (in_lds) {
-        for (int ch = w; ch < g.exp_len / 256; ch += NW)
-            __builtin_amdgcn_global_load_lds((const void *)(g.exp_table + ch * 256 + 4 * lane), (lds_void *)(s_exp + ch * 256), 16, 0, 0);
-        if (w == 0)
-            for (int i = g.exp_len / 256 * 256 + lane; i < table_bytes / 4; i += 64) s_exp[i] = g.exp_table[i < g.exp_len ? i : g.exp_len - 1];
+        paged_table(g, s_exp, w, NW, lane);
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);  // the table's loads before those of K: who has K has the table
     }
-
-    // lane 4 j + t: the page of group t of the wave's block j, and its scales
-    auto key_of = [&](int j) { return k0 + 64 * (NW * j + w); };
-    auto mine = [&](int j) { return key_of(j) < k1; };  // uniform
-    uint32_t number = 0xffffffffu, mul = 0, vs = 1;
-    {
-        const int key = key_of(lane >> 2) + 16 * (lane & 3);
-        if ((lane >> 2) < NB && key < k1) number = g.table[(size_t)s * g.width + (key >> pl.page_log)];
-    }
-    const bool held = number < (uint32_t)p.pages;
-    const uint64_t there = __ballot(held);  // of the groups, those with keys and a page
-    if (held) {
-        const size_t at = (size_t)number * p.kv_heads + h;
-        if (DOTS) mul = p.k_scale[at];
-        if (PHASE == 0 || PHASE == 3) vs = p.v_scale[at];
-    }
-    auto group_rows = [&](const int8_t *pool, int j, int t) {  // the 16 rows of a group; no access where they are not there
-        const bool in_page = (there >> (4 * j + t)) & 1;
-        const uint32_t page = in_page ? (uint32_t)__builtin_amdgcn_readlane((int)number, 4 * j + t) : 0;
-        const size_t row = (((size_t)page * p.kv_heads + h) << pl.page_log) + ((key_of(j) + 16 * t) & (p.page - 1));
-        return __builtin_amdgcn_make_buffer_rsrc((void *)(pool + row * hd), 0, in_page ? 16 * hd : 0, 0x00020000);
-    };
-    auto load = [&](__amdgpu_buffer_rsrc_t r, int at) { return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0)); };
-    // K as the product's operand (chunk c: bytes 64 c + 16 (l / 16) .. of row l % 16), V as block_pv's (16-byte chunk
-    // l % 4, swizzled, of row l / 4); channels past the head are zeros
-    auto k_load = [&](int j, v4i (&x)[4][QC]) {
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const auto r = group_rows(p.k, j, t);
-#pragma unroll
-            for (int c = 0; c < QC; c++) {
-                const int o = 64 * c + 16 * qg;
-                x[t][c] = load(r, o < hd ? ql * hd + o : PG_NONE);
-            }
-        }
-    };
-    auto v_load = [&](int j, int c, v4i (&x)[4]) {
-        const int r = lane >> 2, o = 64 * c + 16 * ((lane & 3) ^ vsw<4>(r)), at = o < hd ? r * hd + o : PG_NONE;
-#pragma unroll
-        for (int t = 0; t < 4; t++) x[t] = load(group_rows(p.v, j, t), at);
-    };
-
-    const v4i zero = v4i{0, 0, 0, 0};
-    const int row = RT == 16 ? ql : ql & 3, near = row < live ? row : live - 1;  // rows that are not there: as the last one
-    const int64_t first = (int64_t)s * g.t;                                      // the stream's first token
-    const size_t place = (size_t)panel * pl.tiles + tile, slot = place * pl.ng;   // of the tile, of its ranges
+    B.until(g, k1, lane);
+    auto mine = [&](int j) { return B.key_of(j) < k1; };  // uniform
+    const int row = RT == 16 ? ql : ql & 3, near = row < T.live ? row : T.live - 1;  // rows that are not there: as the last one
     const PagedScratch S = paged_scratch(scratch, pl, hd);
-    // a lane's scores or entries of block j, accumulator u in the scratch: four keys of its row
-    auto kept = [&](int j, int u) {
-        const int key = key_of(j) + 16 * (RT == 16 ? u : ql >> 2) + 4 * qg;
-        return (Score *)S.keep + (place * pl.rows + row) * ((size_t)pl.ng * pl.span) + key;
-    };
-    v4i D[NB][TU];
-    v4i vr[KD][4];
-    if constexpr (DOTS) {
-        v4i qf[RT == 16 ? 1 : 4][QC];
-        const int tok = (row0 + row) / pl.group, head = h * pl.group + (row0 + row) % pl.group;
+    v4i D[NB][TU], vr[KD][4], qf[RT == 16 ? 1 : 4][QC];
+    // all loads without a branch around them, so that the waits count them exactly
+    v4i kr[KD][4][QC];
 #pragma unroll
-        for (int c = 0; c < QC; c++) {
-            const int o = 64 * c + 16 * qg;
-            const v4i x = row < live && o < hd ? *(const v4i *)(g.q + (first + tok) * g.q_stride + (size_t)head * hd + o) : zero;
-            if constexpr (RT == 16) {
-                qf[0][c] = x;
-            } else {
+    for (int j = 0; j < KD; j++) paged_k<QC>(g, pl, B, T.h, j, lane, kr[j]);
+    paged_q<RT, QC>(g, pl, T, lane, qf);
+    uint32_t mul = B.scale(g, p.k_scale, T.h) * (uint32_t)g.score_m, vs = 1;
+    if constexpr (PHASE == 0 || PHASE == 3) vs = B.scale(g, p.v_scale, T.h);
+    if constexpr (PHASE == 0 && NB <= KD) {
 #pragma unroll
-                for (int t = 0; t < 4; t++) qf[t][c] = (ql >> 2) == t ? x : zero;
-            }
-        }
-        // all loads without a branch around them, so that the waits count them exactly
-        v4i kr[KD][4][QC];
+        for (int j = 0; j < NB; j++) paged_v(g, pl, B, T.h, j, 0, lane, vr[j]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < KD; j++) k_load(j, kr[j]);
-        if constexpr (PHASE == 0 && NB <= KD) {
-#pragma unroll
-            for (int j = 0; j < NB; j++) v_load(j, 0, vr[j]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int j = 0; j < NB; j++) {
-            v4i(&x)[4][QC] = kr[j % KD];
-            if (mine(j)) {
-#pragma unroll
-                for (int u = 0; u < TU; u++) D[j][u] = zero;
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-#pragma unroll
-                    for (int c = 0; c < QC; c++) {
-                        v4i &d = D[j][RT == 16 ? t : 0];
-                        d = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[t][c], qf[RT == 16 ? 0 : t][c], d, 0, 0, 0);
-                    }
-            }
-            if (j + KD < NB) k_load(j + KD, x);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < NB; j++)
-#pragma unroll
-            for (int u = 0; u < TU; u++) {
-                D[j][u] = zero;
-                if (!mine(j) || row >= live) continue;
-                if constexpr (HI) {
-                    D[j][u] = *(const v4i *)kept(j, u);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) D[j][u][e] = (int32_t)kept(j, u)[e];
-                }
-            }
+    for (int j = 0; j < NB; j++) {
+        if (mine(j)) paged_dots<RT, QC>(kr[j % KD], qf, D[j]);
+        if (j + KD < NB) paged_k<QC>(g, pl, B, T.h, j + KD, lane, kr[j % KD]);
+        if (NB > 4) __builtin_amdgcn_sched_barrier(0);
     }
     if constexpr ((PHASE == 0 && NB > KD) || PHASE == 3) {
 #pragma unroll
-        for (int j = 0; j < KD; j++) v_load(j, 0, vr[j]);
+        for (int j = 0; j < KD; j++) paged_v(g, pl, B, T.h, j, 0, lane, vr[j]);
     }
 
     // which of a lane's keys its row sees, where not all do
-    mul = (mul < 1 ? 1 : (mul > p.max_scale ? p.max_scale : mul)) * (uint32_t)g.score_m;
-    vs = vs < 1 ? 1 : (vs > p.max_scale ? p.max_scale : vs);
-    const int most = whole < k1 ? whole : k1;
-    auto all = [&](int j) { return key_of(j) + 64 <= most && ((there >> (4 * j)) & 15) == 15; };  // uniform
-    const int sees = before + (row0 + near) / pl.group + 1, lim = sees < k1 ? sees : k1;
-    auto group_of = [&](int u) { return RT == 16 ? u : ql >> 2; };
+    const int most = T.whole < k1 ? T.whole : k1;
+    auto all = [&](int j) { return B.key_of(j) + 64 <= most && ((B.there >> (4 * j)) & 15) == 15; };  // uniform
+    const int sees = T.before + pl.by_group.of(T.row0 + near) + 1, lim = sees < k1 ? sees : k1;
     auto seen = [&](int j, int u) {  // how many of the lane's four keys
-        const int x = lim - (key_of(j) + 16 * group_of(u) + 4 * qg);
-        return (there >> (4 * j + group_of(u))) & 1 ? x : 0;
-    };
-    auto scale_of = [&](uint32_t x, int j, int u) {
-        return RT == 16 ? __builtin_amdgcn_readlane((int)x, 4 * j + u) : __shfl((int)x, 4 * j + (ql >> 2), 64);
+        const int t = RT == 16 ? u : ql >> 2;
+        return B.has(j, t) ? lim - (B.key_of(j) + 16 * t + 4 * qg) : 0;
     };
     const PagedRule<HI> rule(g);
     int64_t M = INT64_MIN;
@@ -270,24 +430,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
             const bool whole_block = all(j);
 #pragma unroll
             for (int u = 0; u < TU; u++) {
-                const int m = scale_of(mul, j, u), k = whole_block ? 4 : seen(j, u);
-                if constexpr (PHASE == 1 && KEEP) {
-                    Score x[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        x[e] = e < k ? (Score)rule.score(D[j][u][e], m) : LOW;
-                        mx = x[e] > mx ? x[e] : mx;
-                    }
-                    if (row < live) {
-                        if constexpr (HI) {
-                            *(v4i *)kept(j, u) = v4i{(int)x[0], (int)x[1], (int)x[2], (int)x[3]};
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 4; e++) kept(j, u)[e] = x[e];
-                        }
-                    }
-                    continue;
-                }
+                const int m = paged_of<RT>(mul, j, u, lane), k = whole_block ? 4 : seen(j, u);
                 int32_t d = INT32_MIN;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
@@ -310,15 +453,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
             if (tid < RT) {
 #pragma unroll
                 for (int i = 0; i < NW; i++) M = s_mx[i * RT + tid] > M ? s_mx[i * RT + tid] : M;
-                S.mx[(slot + range) * RT + tid] = M;
+                S.mx[(T.slot + T.range) * RT + tid] = M;
             }
             return;
         }
 #pragma unroll
         for (int i = 0; i < NW; i++) M = s_mx[i * RT + row] > M ? s_mx[i * RT + row] : M;
-    } else if constexpr (DOTS) {
+    } else {
         for (int i = 0; i < ranges; i++) {
-            const int64_t x = S.mx[(slot + i) * RT + row];
+            const int64_t x = S.mx[(T.slot + i) * RT + row];
             M = x > M ? x : M;
         }
         if (!mine(0)) wait_vmcnt<0>();
@@ -329,11 +472,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
     uint64_t sum = 0;
 #pragma unroll
     for (int j = 0; j < NB; j++) {
-        if (!DOTS || !mine(j)) continue;
+        if (!mine(j)) continue;
         const bool whole_block = all(j);
 #pragma unroll
         for (int u = 0; u < TU; u++) {
-            const int m = scale_of(mul, j, u);
+            const int m = paged_of<RT>(mul, j, u, lane);
 #pragma unroll
             for (int e = 0; e < 4; e++) D[j][u][e] = (int32_t)rule.index(D[j][u][e], m, c0, last);
         }
@@ -342,7 +485,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
             for (int u = 0; u < TU; u++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) D[j][u][e] = s_exp[D[j][u][e]];
-        } else if (row < live) {
+        } else if (row < T.live) {
 #pragma unroll
             for (int u = 0; u < TU; u++)
 #pragma unroll
@@ -369,147 +512,226 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
         for (int o = RT == 16 ? 16 : 4; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
         if (lane < RT) s_sum[w * RT + lane] = sum;
         lds_barrier();
+        sum = 0;
         if constexpr (PHASE == 2) {
             if (tid < RT) {
-                sum = 0;
 #pragma unroll
                 for (int i = 0; i < NW; i++) sum += s_sum[i * RT + tid];
-                S.sum[(place * pl.chunks + range) * RT + tid] = sum;
+                S.sum[(T.slot + T.range) * RT + tid] = sum;
             }
             return;
         }
-        sum = 0;
 #pragma unroll
         for (int i = 0; i < NW; i++) sum += s_sum[i * RT + row];
     } else {
-        const int sums = KEEP ? (keys + PG_CHUNK - 1) / PG_CHUNK : ranges;
-        for (int i = 0; i < sums; i++) sum += S.sum[(place * pl.chunks + i) * RT + row];
+        for (int i = 0; i < ranges; i++) sum += S.sum[(T.slot + i) * RT + row];
         lds_barrier();  // every wave has its entries
     }
     for (int i = tid; i < QC * RT * PG_ACC; i += 64 * NW) s_acc[i] = 0;
-
-    // The digits of w = floor(E 2^P / S) for E = e vs, exactly (softmax_p_of, which holds for E < 2^53 with w <= 2^30), with
-    // 0x80808080 inside the rounding constant: the low word of the sum is w + 0x80808080, whose bytes xor 0x80 are
-    // balanced digits. D[j][k] word t: digit k of group t's keys (16 rows); D[j][0] word t: digit l % 4 of row l / 4 % 4
-    // of group t's keys (4 rows: the lanes transpose through LDS).
-    {
-        constexpr double magic = 6755399441055744.0 + 2155905152.0;  // 1.5 2^52 + 0x80808080
-        const double R = sum > 0 && row < live ? ldexp(1.0 / (double)sum, g.softmax_p) : 0.0, sp = softmax_sp(sum, g.softmax_p);
+    const PagedWeight wt(sum, g.softmax_p, row < T.live);
 #pragma unroll
-        for (int j = 0; j < NB; j++) {
-            __builtin_amdgcn_sched_barrier(0);  // (a block at a time: interleaved they spill)
-            if (!mine(j)) continue;
-            uint32_t o[TU][4];
-#pragma unroll
-            for (int u = 0; u < TU; u++) {
-                const double scale = (double)(uint32_t)scale_of(vs, j, u);
-                uint32_t dg[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const double ed = (double)(uint32_t)D[j][u][e] * scale, x = fma(ed, R, magic), r = fma(x - magic, sp, ed);
-                    dg[e] = (uint32_t)__double2loint(x) + (uint32_t)(__double2hiint(r) >> 31);
-                }
-                byte_transpose(dg[0], dg[1], dg[2], dg[3], o[u]);
-            }
-            if constexpr (RT == 16) {
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-#pragma unroll
-                    for (int t = 0; t < 4; t++) D[j][k][t] = (int32_t)(o[t][k] ^ 0x80808080u);
-            } else {
-                // [row][digit][l / 16][group]
-                int *to = (int *)s_v + 64 * (ql & 3) + 4 * qg + (ql >> 2);
-#pragma unroll
-                for (int k = 0; k < 4; k++) to[16 * k] = (int)(o[0][k] ^ 0x80808080u);
-                D[j][0] = *(const v4i *)((const int *)s_v + 16 * ql + 4 * qg);
-            }
-        }
+    for (int j = 0; j < NB; j++) {
+        __builtin_amdgcn_sched_barrier(0);  // (a block at a time: interleaved they spill)
+        if (mine(j)) paged_digits<RT>(wt, vs, j, lane, s_v, D[j]);
     }
     __builtin_amdgcn_sched_barrier(0);
-
-    // sum w v: channels 64 c + 16 i + 4 (l / 16) + e of digit k of row l % 16 in acc[k][i][e] (16 rows), of digit l % 4 of row
-    // l / 4 % 4 in acc[0][i][e] (4 rows)
 #pragma unroll
     for (int c = 0; c < QC; c++) {
         v4i acc[TU][4];
 #pragma unroll
         for (int k = 0; k < TU; k++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) acc[k][i] = zero;
+            for (int i = 0; i < 4; i++) acc[k][i] = v4i{0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < NB; j++) {
             const int f = c * NB + j;  // the loads run ahead over the channels
-            v4i(&x)[4] = vr[f % KD];
             __builtin_amdgcn_sched_barrier(0);
-            if (mine(j)) {
-#pragma unroll
-                for (int u = 0; u < 4; u++) *(v4i *)(s_v + 1024 * u + 16 * lane) = x[u];
-            }
-            if (f + KD < QC * NB) v_load((f + KD) % NB, (f + KD) / NB, x);
-            if (!mine(j)) continue;
-            const int tr_k = ql >> 1, key = 16 * (tr_k >> 2) + 4 * qg + (tr_k & 3);
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int8_t *p0 = s_v + (4 * key + (i ^ vsw<4>(key & 15))) * 16 + 8 * (ql & 1);
-                const v2i r0 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)p0);
-                const v2i r1 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)(p0 + 32 * 64));
-                const v4i vf = v4i{r0[0], r0[1], r1[0], r1[1]};
-#pragma unroll
-                for (int k = 0; k < TU; k++) acc[k][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf, D[j][k], acc[k][i], 0, 0, 0);
-            }
+            if (mine(j)) paged_pv<RT>(vr[f % KD], D[j], lane, s_v, acc, [] {});
+            if (f + KD < QC * NB) paged_v(g, pl, B, T.h, (f + KD) % NB, (f + KD) / NB, lane, vr[f % KD]);
         }
         if (c == 0) lds_barrier();  // the zeros
-        if (!mine(0)) continue;
-        if constexpr (RT == 16) {
-            unsigned long long *to = (unsigned long long *)s_acc + (c * RT + ql) * PG_ACC + 4 * qg;
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    // (at most 256 keys a wave: a plane's sum is below 2^22, two planes' below 2^31)
-                    const int32_t lo = acc[0][i][e] + acc[1][i][e] * 256, hi = acc[2][i][e] + acc[3][i][e] * 256;
-                    atomicAdd(to + 16 * i + e, (unsigned long long)((int64_t)hi * 65536 + lo));
-                }
-        } else {
-            // lane l % 4 = i keeps the four planes' sum of channels 16 i ..: the quad's lanes exchange halves twice
-            const bool b0 = lane & 1, b1 = lane & 2;
-            int64_t y[2][4], z[4];
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int32_t keep = b0 ? acc[0][2 * i + 1][e] : acc[0][2 * i][e], give = b0 ? acc[0][2 * i][e] : acc[0][2 * i + 1][e];
-                    const int32_t got = dpp_mov<0xB1>(give);  // of the plane next to this lane's
-                    y[i][e] = b0 ? (int64_t)keep * 256 + got : (int64_t)got * 256 + keep;
-                }
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int64_t keep = b1 ? y[1][e] : y[0][e], got = lane_move64<1>(b1 ? y[0][e] : y[1][e]);
-                z[e] = b1 ? keep * 65536 + got : got * 65536 + keep;
-            }
-            unsigned long long *to = (unsigned long long *)s_acc + (c * RT + (ql >> 2)) * PG_ACC + 16 * (lane & 3) + 4 * qg;
-            if ((ql >> 2) < live) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) atomicAdd(to + e, (unsigned long long)z[e]);
-            }
-        }
+        if (mine(0)) paged_add<RT, (NB <= 4)>(acc, T.live, lane, s_acc + c * RT * PG_ACC);
     }
     lds_barrier();
-    const double mo = g.out_s > 95 ? 0.0 : ldexp((double)g.out_m, -g.out_s);
-    for (int i = tid; i < live * (hd / 4); i += 64 * NW) {
+    for (int i = tid; i < T.live * (hd / 4); i += 64 * NW) {
         const int r = i / (hd / 4), ch = 4 * (i - r * (hd / 4));
         const int64_t *x = s_acc + ((ch >> 6) * RT + r) * PG_ACC + (ch & 63);
         if constexpr (PHASE == 3) {
-            int64_t *to = S.part + ((slot + range) * RT + r) * hd + ch;
+            int64_t *to = S.part + ((T.slot + T.range) * RT + r) * hd + ch;
 #pragma unroll
             for (int e = 0; e < 4; e++) to[e] = x[e];
         } else {
-            uint32_t packed = 0;
-#pragma unroll
-            for (int e = 0; e < 4; e++) packed |= (uint32_t)(uint8_t)(int8_t)attn_out_byte(x[e], mo, g.out_m, g.out_s) << (8 * e);
-            const int tok = (row0 + r) / pl.group, head = h * pl.group + (row0 + r) % pl.group;
-            *(uint32_t *)(g.out + ((first + tok) * g.heads + head) * hd + ch) = packed;
+            paged_put(g, pl, T.s, T.h, T.row0 + r, ch, x);
         }
+    }
+}
+
+// ---- Ranges that leave their scores in the scratch ------------------------------------------------------
+// Three launches and a join: the scores of every key (K once), their entries and sums, the products with V (V once). Four waves
+// walk a range's blocks, at most 16 each, with the next blocks' loads under way; what a workgroup has to find out first (counts,
+// pages, scales) is spread over up to 4,096 keys.
+template <int RT, int QC, bool HI>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QC == 4 ? 2 : 4))) void k_paged_scores(PagedArgs g, PagedPlan pl, void *scratch) {
+    typedef typename std::conditional<HI, int32_t, int64_t>::type Score;
+    constexpr Score LOW = HI ? (Score)INT32_MIN : (Score)INT64_MIN;
+    constexpr int TU = RT / 4;
+    __shared__ int64_t s_mx[4][RT];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ql = lane & 15, qg = lane >> 4;
+    PagedTile T(g, pl, blockIdx.x);
+    if (!T.there) return;
+    const int k0 = T.range * pl.span;
+    const uint32_t ctx = g.ctx[T.s], count = g.rows ? g.rows[T.s] : (uint32_t)g.t;
+    PagedBlocks B(g, pl, T.s, k0 + 64 * w, 256, 16, lane);
+    T.rows(g, pl, ctx, count);
+    if (T.live <= 0 || k0 >= T.keys) return;  // the launches behind read no result of this range
+    const int k1 = k0 + pl.span < T.keys ? k0 + pl.span : T.keys;
+    B.until(g, k1, lane);
+    const int row = RT == 16 ? ql : ql & 3, near = row < T.live ? row : T.live - 1;
+    const PagedScratch S = paged_scratch(scratch, pl, g.pages.hd);
+    constexpr int KD = QC == 1 ? 3 : 2;  // blocks of K in flight, with the one at work
+    v4i x[KD][4][QC], qf[RT == 16 ? 1 : 4][QC];
+#pragma unroll
+    for (int j = 0; j + 1 < KD; j++) paged_k<QC>(g, pl, B, T.h, j, lane, x[j]);
+    paged_q<RT, QC>(g, pl, T, lane, qf);
+    const uint32_t mul = B.scale(g, g.pages.k_scale, T.h) * (uint32_t)g.score_m;
+    const int sees = T.before + pl.by_group.of(T.row0 + near) + 1, lim = sees < k1 ? sees : k1, most = T.whole < k1 ? T.whole : k1;
+    const PagedRule<HI> rule(g);
+    Score mx = LOW;
+    Score *to = (Score *)S.keep + (T.place * pl.rows + row) * ((size_t)pl.ng * pl.span) + 4 * qg + (RT == 16 ? 0 : 16 * (ql >> 2));
+    auto step = [&](int j, v4i (&now)[4][QC], v4i (&next)[4][QC]) {
+        if (j + KD - 1 < 16) paged_k<QC>(g, pl, B, T.h, j + KD - 1, lane, next);  // (past the range: no access)
+        v4i D[TU];
+        paged_dots<RT, QC>(now, qf, D);
+        const int key = B.key_of(j);
+        const bool whole = key + 64 <= most && ((B.there >> (4 * j)) & 15) == 15;  // uniform
+#pragma unroll
+        for (int u = 0; u < TU; u++) {
+            const int t = RT == 16 ? u : ql >> 2, m = paged_of<RT>(mul, j, u, lane);
+            const int k = whole ? 4 : B.has(j, t) ? lim - (key + 16 * t + 4 * qg) : 0;
+            Score y[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                y[e] = whole || e < k ? (Score)rule.score(D[u][e], m) : LOW;
+                mx = y[e] > mx ? y[e] : mx;
+            }
+            if (row < T.live) {
+                Score *at = to + key + (RT == 16 ? 16 * u : 0);
+                if constexpr (HI) {
+                    *(v4i *)at = v4i{(int)y[0], (int)y[1], (int)y[2], (int)y[3]};
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) at[e] = y[e];
+                }
+            }
+        }
+        return B.key_of(j + 1) < k1;
+    };
+    if (B.key_of(0) < k1)
+        for (int j = 0;; j += KD) {
+            if (!step(j, x[0], x[KD - 1]) || !step(j + 1, x[1], x[0])) break;
+            if constexpr (KD == 3)
+                if (!step(j + 2, x[2], x[1])) break;
+        }
+#pragma unroll
+    for (int o = RT == 16 ? 16 : 4; o < 64; o <<= 1) {
+        const Score y = __shfl_xor(mx, o, 64);
+        mx = y > mx ? y : mx;
+    }
+    if (lane < RT) s_mx[w][lane] = mx == LOW ? INT64_MIN : (int64_t)mx;
+    __syncthreads();
+    if (tid < RT) {
+        int64_t M = s_mx[0][tid];
+#pragma unroll
+        for (int i = 1; i < 4; i++) M = s_mx[i][tid] > M ? s_mx[i][tid] : M;
+        S.mx[(T.slot + T.range) * RT + tid] = M;
+    }
+}
+
+// GC chunks of 64 channels from chunk GC blockIdx.y on.
+template <int RT, int GC, bool HI>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RT == 16 && GC > 1 ? 2 : 3))) void k_paged_products(PagedArgs g, PagedPlan pl, void *scratch) {
+    typedef typename std::conditional<HI, int32_t, int64_t>::type Score;
+    constexpr int TU = RT / 4;
+    __shared__ __attribute__((aligned(1024))) int8_t s_mem[4][4096];
+    __shared__ int64_t s_acc[GC * RT * PG_ACC];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ql = lane & 15, qg = lane >> 4, hd = g.pages.hd, c0 = GC * blockIdx.y;
+    PagedTile T(g, pl, blockIdx.x);
+    if (!T.there) return;
+    const int k0 = T.range * pl.span;
+    const uint32_t ctx = g.ctx[T.s], count = g.rows ? g.rows[T.s] : (uint32_t)g.t;
+    PagedBlocks B(g, pl, T.s, k0 + 64 * w, 256, 16, lane);
+    for (int i = tid; i < GC * RT * PG_ACC; i += 256) s_acc[i] = 0;
+    T.rows(g, pl, ctx, count);
+    if (T.live <= 0 || (k0 >= T.keys && T.range > 0)) return;  // the join reads no result of this range
+    const int k1 = k0 + pl.span < T.keys ? k0 + pl.span : T.keys;
+    B.until(g, k1, lane);
+    const int row = RT == 16 ? ql : ql & 3;
+    const bool live = row < T.live;
+    const PagedScratch S = paged_scratch(scratch, pl, hd);
+    const Score *from = (const Score *)S.keep + (T.place * pl.rows + (live ? row : 0)) * ((size_t)pl.ng * pl.span) + 4 * qg + (RT == 16 ? 0 : 16 * (ql >> 2));
+    auto entries = [&](int j, v4i (&D)[TU]) {
+        const int key = B.key_of(j) < k1 ? B.key_of(j) : k0;
+#pragma unroll
+        for (int u = 0; u < TU; u++) {
+            const Score *at = from + key + (RT == 16 ? 16 * u : 0);
+            if constexpr (HI) {
+                D[u] = *(const v4i *)at;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) D[u][e] = (int32_t)at[e];
+            }
+        }
+    };
+    v4i x[GC][4], D[TU];
+    const bool any = B.key_of(0) < k1;
+    if (any) entries(0, D);
+#pragma unroll
+    for (int c = 0; c < GC; c++) paged_v(g, pl, B, T.h, 0, c0 + c, lane, x[c]);
+    const uint32_t vs = B.scale(g, g.pages.v_scale, T.h);
+    uint64_t sum = 0;
+    const int sums = (T.keys + PG_CHUNK - 1) / PG_CHUNK;
+    for (int i = 0; i < sums; i++) sum += S.sum[(T.place * pl.chunks + i) * RT + (live ? row : 0)];
+    const PagedWeight wt(sum, g.softmax_p, live);
+    v4i acc[GC][TU][4];
+#pragma unroll
+    for (int c = 0; c < GC; c++)
+#pragma unroll
+        for (int k = 0; k < TU; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[c][k][i] = v4i{0, 0, 0, 0};
+    // (one step a turn, the entries copied: with two and an exit between them the sums are held twice and spill)
+    for (int j = 0; B.key_of(j) < k1; j++) {
+        v4i E[TU];
+#pragma unroll
+        for (int u = 0; u < TU; u++) E[u] = D[u];
+        entries(j + 1, D);
+        __builtin_amdgcn_sched_barrier(0);
+        paged_digits<RT>(wt, vs, j, lane, s_mem[w], E);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = 0; c < GC; c++) {
+            paged_pv<RT>(x[c], E, lane, s_mem[w], acc[c], [&] {
+                __builtin_amdgcn_sched_barrier(0);
+                if (j + 1 < 16) paged_v(g, pl, B, T.h, j + 1, c0 + c, lane, x[c]);  // (past the range: no access)
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        }
+    }
+    __syncthreads();  // the zeros
+    if (any) {
+#pragma unroll
+        for (int c = 0; c < GC; c++) paged_add<RT, false>(acc[c], T.live, lane, s_acc + c * RT * PG_ACC);
+    }
+    __syncthreads();
+    const int chs = hd - 64 * c0 < 64 * GC ? hd - 64 * c0 : 64 * GC;  // channels here
+    for (int i = tid; i < T.live * (chs / 4); i += 256) {
+        const int r = i / (chs / 4), ch = 4 * (i - r * (chs / 4));
+        const int64_t *y = s_acc + ((ch >> 6) * RT + r) * PG_ACC + (ch & 63);
+        int64_t *to = S.part + ((T.slot + T.range) * RT + r) * hd + 64 * c0 + ch;
+#pragma unroll
+        for (int e = 0; e < 4; e++) to[e] = y[e];
     }
 }
 
@@ -519,19 +741,22 @@ __global__ __launch_bounds__(256) void k_paged_entries(PagedArgs g, PagedPlan pl
     typedef typename std::conditional<HI, int32_t, int64_t>::type Score;
     constexpr Score LOW = HI ? (Score)INT32_MIN : (Score)INT64_MIN;
     constexpr int N = PG_CHUNK / 256;
+    extern __shared__ __attribute__((aligned(1024))) int32_t s_exp[];  // the table, where it fits
     __shared__ uint64_t s_sum[4];
     const PagePool &p = g.pages;
     const int tid = threadIdx.x;
+    if (g.table_lds) paged_table(g, s_exp, tid >> 6, 4, tid & 63);
     // (row fastest, then the chunk)
     const int r = blockIdx.x % pl.rows, chunk = blockIdx.x / pl.rows % pl.chunks;
-    const size_t place = blockIdx.x / pl.rows / pl.chunks;
-    const int tile = (int)(place % pl.tiles), s = (int)(place / pl.tiles) / p.kv_heads;
-    const int n = (int)(g.ctx[s] < (uint32_t)g.keys ? g.ctx[s] : (uint32_t)g.keys);
-    uint32_t count = g.rows ? g.rows[s] : (uint32_t)g.t;
-    count = count < (uint32_t)g.t ? count : (uint32_t)g.t;
-    const int rows = (int)count * pl.group, row0 = pl.rt * tile, live = rows - row0 < pl.rt ? rows - row0 : pl.rt;
-    if (r >= live) return;
-    const int keys = n - (int)count + (row0 + live - 1) / pl.group + 1;  // of the tile: those have scores, in whole blocks
+    PagedTile T;
+    T.place = blockIdx.x / pl.rows / pl.chunks;
+    T.panel = pl.by_tiles.of((int)T.place);
+    T.tile = (int)T.place - T.panel * pl.tiles;
+    T.s = pl.by_heads.of(T.panel);
+    T.rows(g, pl, g.ctx[T.s], g.rows ? g.rows[T.s] : (uint32_t)g.t);
+    if (r >= T.live) return;
+    const size_t place = T.place;
+    const int keys = T.keys;  // of the tile: those have scores, in whole blocks
     const int k0 = chunk * PG_CHUNK, k1 = (keys + 63) / 64 * 64 < k0 + PG_CHUNK ? (keys + 63) / 64 * 64 : k0 + PG_CHUNK;
     if (k0 >= keys) return;
     const PagedScratch S = paged_scratch(scratch, pl, p.hd);
@@ -564,8 +789,18 @@ __global__ __launch_bounds__(256) void k_paged_entries(PagedArgs g, PagedPlan pl
         uint32_t d;
         if constexpr (HI) d = (uint32_t)((int32_t)M - x[i]);
         else d = (uint64_t)(M - x[i]) < last ? (uint32_t)(M - x[i]) : last;
-        y[i] = x[i] == LOW ? 0 : g.exp_table[d < last ? d : last];
+        y[i] = (int32_t)(d < last ? d : last);
     }
+    __syncthreads();  // the table
+    if (g.table_lds) {
+#pragma unroll
+        for (int i = 0; i < N; i++) y[i] = s_exp[y[i]];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) y[i] = g.exp_table[y[i]];
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) y[i] = x[i] == LOW ? 0 : y[i];
 #pragma unroll
     for (int i = 0; i < N; i++) sum += (uint32_t)y[i];
 #pragma unroll
@@ -587,41 +822,35 @@ __global__ __launch_bounds__(256) void k_paged_entries(PagedArgs g, PagedPlan pl
 
 // The outputs from the ranges' sums: a thread per four channels.
 __global__ __launch_bounds__(256) void k_paged_out(PagedArgs g, PagedPlan pl, void *scratch) {
-    const PagePool &p = g.pages;
-    const int quads = p.hd / 4;
+    const int hd = g.pages.hd, quads = hd / 4;
     const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, at = i / quads;  // (tile of a panel, row)
-    const int ch = 4 * (int)(i - at * quads), r = (int)(at % pl.rt);
-    const size_t tiles = at / pl.rt;
-    if (tiles >= (size_t)pl.panels * pl.tiles) return;
-    const int tile = (int)(tiles % pl.tiles), panel = (int)(tiles / pl.tiles), s = panel / p.kv_heads, h = panel - s * p.kv_heads;
-    const int n = (int)(g.ctx[s] < (uint32_t)g.keys ? g.ctx[s] : (uint32_t)g.keys);
-    uint32_t count = g.rows ? g.rows[s] : (uint32_t)g.t;
-    count = count < (uint32_t)g.t ? count : (uint32_t)g.t;
-    const int rows = (int)count * pl.group, row0 = pl.rt * tile;
-    if (row0 + r >= rows) return;
-    const int end = rows - row0 < pl.rt ? rows - row0 : pl.rt;
-    const int keys = n - (int)count + (row0 + end - 1) / pl.group + 1;
-    const int ranges = keys > pl.span ? (keys + pl.span - 1) / pl.span : 1;
-    const PagedScratch S = paged_scratch(scratch, pl, p.hd);
+    const int ch = 4 * (int)(i - at * quads);
+    PagedTile T;
+    T.place = at / pl.rows;
+    const int r = (int)(at - T.place * pl.rows);
+    if (T.place >= (size_t)pl.panels * pl.tiles) return;
+    T.panel = pl.by_tiles.of((int)T.place);
+    T.tile = (int)T.place - T.panel * pl.tiles;
+    T.s = pl.by_heads.of(T.panel);
+    T.h = T.panel - T.s * g.pages.kv_heads;
+    T.rows(g, pl, g.ctx[T.s], g.rows ? g.rows[T.s] : (uint32_t)g.t);
+    if (r >= T.live) return;
+    const int ranges = T.keys > pl.span ? (T.keys + pl.span - 1) / pl.span : 1;
+    const PagedScratch S = paged_scratch(scratch, pl, hd);
     int64_t x[4] = {0, 0, 0, 0};
-    const int64_t *from = S.part + (tiles * pl.ng * pl.rt + r) * p.hd + ch;
+    const int64_t *from = S.part + (T.place * pl.ng * pl.rt + r) * hd + ch;
     for (int c0 = 0; c0 < ranges; c0 += 8) {  // eight in flight
         int64_t y[8][4];
 #pragma unroll
         for (int c = 0; c < 8; c++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) y[c][e] = from[(size_t)(c0 + c < ranges ? c0 + c : c0) * pl.rt * p.hd + e];
+            for (int e = 0; e < 4; e++) y[c][e] = from[(size_t)(c0 + c < ranges ? c0 + c : c0) * pl.rt * hd + e];
 #pragma unroll
         for (int c = 0; c < 8; c++)
 #pragma unroll
             for (int e = 0; e < 4; e++) x[e] += c0 + c < ranges ? y[c][e] : 0;
     }
-    const double mo = g.out_s > 95 ? 0.0 : ldexp((double)g.out_m, -g.out_s);
-    uint32_t packed = 0;
-#pragma unroll
-    for (int e = 0; e < 4; e++) packed |= (uint32_t)(uint8_t)(int8_t)attn_out_byte(x[e], mo, g.out_m, g.out_s) << (8 * e);
-    const int tok = (row0 + r) / pl.group, head = h * pl.group + (row0 + r) % pl.group;
-    *(uint32_t *)(g.out + (((size_t)s * g.t + tok) * g.heads + head) * p.hd + ch) = packed;
+    paged_put(g, pl, T.s, T.h, T.row0 + r, ch, x);
 }
 
 constexpr size_t PG_KEEP = (size_t)128 << 20;  // bytes of scores that a call keeps at most (tiles of 16 rows)
@@ -639,14 +868,23 @@ static PagedPlan paged_plan(const PagedArgs &g) {
     p.span = (g.keys + 63) / 64 * 64;
     if (g.keys > most) {
         const long long wgs = (long long)p.panels * p.tiles;
-        long long ng = (1024 + wgs - 1) / wgs;
-        const long long least = (g.keys + 1023) / 1024, more = (g.keys + 255) / 256;  // of 1,024 keys, of 256
-        ng = ng < least ? least : (ng > more ? more : ng);
-        p.span = (int)(((g.keys + ng - 1) / ng + 255) / 256) * 256;
-        p.ng = (g.keys + p.span - 1) / p.span;
+        auto ranges = [&](int least_keys, int most_keys, long long all) {
+            long long ng = (all + wgs - 1) / wgs;
+            const long long least = (g.keys + most_keys - 1) / most_keys, more = (g.keys + least_keys - 1) / least_keys;
+            ng = ng < least ? least : (ng > more ? more : ng);
+            p.span = (int)(((g.keys + ng - 1) / ng + 255) / 256) * 256;
+            p.ng = (g.keys + p.span - 1) / p.span;
+        };
+        if (p.rt == 4) ranges(1024, 4096, 3072);
+        else ranges(512, 4096, 512);
         p.store = p.rt == 4 || (size_t)wgs * p.rows * p.ng * p.span * 8 <= PG_KEEP;
+        if (!p.store) ranges(256, 1024, 1024);
         p.chunks = p.store ? (g.keys + PG_CHUNK - 1) / PG_CHUNK : p.ng;
     }
+    p.by_group = PagedDiv((uint32_t)p.group);
+    p.by_tiles = PagedDiv((uint32_t)p.tiles);
+    p.by_heads = PagedDiv((uint32_t)g.pages.kv_heads);
+    p.by_inner = PagedDiv((uint32_t)(8 * p.tiles * p.ng));
     return p;
 }
 
@@ -662,14 +900,14 @@ size_t paged_workspace(const PagedArgs &g) {
     return bytes;
 }
 
-template <int RT, int QC, int NB, int NW, bool HI, int PHASE, bool KEEP = false>
+template <int RT, int QC, int NB, int NW, bool HI, int PHASE>
 static hipError_t launch_paged_t(const PagedArgs &g, const PagedPlan &p, void *scratch, hipStream_t stream) {
     const int acc = (8 * QC * RT * PG_ACC + 1023) / 1024 * 1024;
-    const int table = RT == 16 && PHASE != 1 && !(KEEP && PHASE == 3) && g.table_lds ? 1024 * ((g.exp_len + 255) / 256) : 0;
+    const int table = RT == 16 && PHASE != 1 && g.table_lds ? 1024 * ((g.exp_len + 255) / 256) : 0;
     const size_t lds = (size_t)(table > acc ? table : acc) + 4096 * NW + 16 * NW * RT;
-    const hipError_t e = allow_dynamic_lds((const void *)k_paged_tile<RT, QC, NB, NW, HI, PHASE, KEEP>, lds);
+    const hipError_t e = allow_dynamic_lds((const void *)k_paged_tile<RT, QC, NB, NW, HI, PHASE>, lds);
     if (e != hipSuccess) return e;
-    launch_k((k_paged_tile<RT, QC, NB, NW, HI, PHASE, KEEP>), dim3((unsigned)((p.panels + 7) / 8 * 8) * p.tiles * p.ng), dim3(64 * NW), lds, stream, g, p, scratch);
+    launch_k((k_paged_tile<RT, QC, NB, NW, HI, PHASE>), dim3((unsigned)((p.panels + 7) / 8 * 8) * p.tiles * p.ng), dim3(64 * NW), lds, stream, g, p, scratch);
     return hipGetLastError();
 }
 
@@ -677,17 +915,23 @@ template <int RT, int QC, bool HI>
 static hipError_t launch_paged_q(const PagedArgs &g, const PagedPlan &p, void *scratch, hipStream_t stream) {
     if (p.ng > 1) {
         hipError_t e;
+        const unsigned grid = (unsigned)((p.panels + 7) / 8 * 8) * p.tiles * p.ng;
         if (p.store) {
-            if ((e = launch_paged_t<RT, QC, 4, 4, HI, 1, true>(g, p, scratch, stream)) != hipSuccess) return e;
-            launch_k(k_paged_entries<HI>, dim3((unsigned)p.panels * p.tiles * p.chunks * p.rows), dim3(256), 0, stream, g, p, scratch);
+            constexpr int GC = QC == 4 ? 2 : QC;  // (the sums of more channels do not fit the registers)
+            launch_k(k_paged_scores<RT, QC, HI>, dim3(grid), dim3(256), 0, stream, g, p, scratch);
             if ((e = hipGetLastError()) != hipSuccess) return e;
-            if ((e = launch_paged_t<RT, QC, 4, 4, HI, 3, true>(g, p, scratch, stream)) != hipSuccess) return e;
+            const size_t table = g.table_lds ? (size_t)1024 * ((g.exp_len + 255) / 256) : 0;
+            if ((e = allow_dynamic_lds((const void *)k_paged_entries<HI>, table)) != hipSuccess) return e;
+            launch_k(k_paged_entries<HI>, dim3((unsigned)p.panels * p.tiles * p.chunks * p.rows), dim3(256), table, stream, g, p, scratch);
+            if ((e = hipGetLastError()) != hipSuccess) return e;
+            launch_k(k_paged_products<RT, GC, HI>, dim3(grid, QC / GC), dim3(256), 0, stream, g, p, scratch);
+            if ((e = hipGetLastError()) != hipSuccess) return e;
         } else if constexpr (RT == 16) {
             if ((e = launch_paged_t<RT, QC, 4, 4, HI, 1>(g, p, scratch, stream)) != hipSuccess) return e;
             if ((e = launch_paged_t<RT, QC, 4, 4, HI, 2>(g, p, scratch, stream)) != hipSuccess) return e;
             if ((e = launch_paged_t<RT, QC, 4, 4, HI, 3>(g, p, scratch, stream)) != hipSuccess) return e;
         }
-        const size_t quads = (size_t)p.panels * p.tiles * p.rt * (g.pages.hd / 4);
+        const size_t quads = (size_t)p.panels * p.tiles * p.rows * (g.pages.hd / 4);
         launch_k(k_paged_out, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, g, p, scratch);
         return hipGetLastError();
     }
