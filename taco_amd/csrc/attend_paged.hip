@@ -135,7 +135,8 @@ struct PagedTile {
 // knows the page of group t, the 16 keys from 16 t on.
 struct PagedBlocks {
     uint32_t number;
-    uint64_t there;  // the groups with keys and a page
+    uint32_t at_lo, at_hi;  // where the group's rows start in the pools
+    uint64_t there;         // the groups with keys and a page
     int first, step;
     // (before the stream's counts are known: entries up to `keys` are there for every stream)
     __device__ __forceinline__ PagedBlocks(const PagedArgs &g, const PagedPlan &pl, int s, int k0, int st, int blocks, int lane) : first(k0), step(st) {
@@ -143,9 +144,15 @@ struct PagedBlocks {
         number = 0xffffffffu;
         if ((lane >> 2) < blocks && key < g.keys) number = g.table[(size_t)s * g.width + (key >> pl.page_log)];
     }
-    __device__ __forceinline__ void until(const PagedArgs &g, int k1, int lane) {
-        if (key_of(lane >> 2) + 16 * (lane & 3) >= k1) number = 0xffffffffu;
-        there = __ballot(number < (uint32_t)g.pages.pages);
+    __device__ __forceinline__ void until(const PagedArgs &g, const PagedPlan &pl, int h, int k1, int lane) {
+        const PagePool &p = g.pages;
+        const int key = key_of(lane >> 2) + 16 * (lane & 3);
+        if (key >= k1) number = 0xffffffffu;
+        there = __ballot(number < (uint32_t)p.pages);
+        const uint64_t row = (((uint64_t)number * (uint32_t)p.kv_heads + h) << pl.page_log) + (key & (p.page - 1));
+        const uint64_t at = row * (uint32_t)p.hd;
+        at_lo = (uint32_t)at;
+        at_hi = (uint32_t)(at >> 32);
     }
     __device__ __forceinline__ int key_of(int j) const { return first + step * j; }
     __device__ __forceinline__ bool has(int j, int t) const { return (there >> (4 * j + t)) & 1; }
@@ -156,11 +163,9 @@ struct PagedBlocks {
         return x < 1 ? 1 : (x > g.pages.max_scale ? g.pages.max_scale : x);
     }
     // the 16 rows of a group; loads of one that is not there give zeros without an access
-    __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows(const PagedArgs &g, const PagedPlan &pl, const int8_t *pool, int h, int j, int t) const {
-        const PagePool &p = g.pages;
-        const uint32_t page = has(j, t) ? (uint32_t)__builtin_amdgcn_readlane((int)number, 4 * j + t) : 0;
-        const size_t row = (((size_t)page * p.kv_heads + h) << pl.page_log) + ((key_of(j) + 16 * t) & (p.page - 1));
-        return __builtin_amdgcn_make_buffer_rsrc((void *)(pool + row * p.hd), 0, has(j, t) ? 16 * p.hd : 0, 0x00020000);
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows(const PagedArgs &g, const int8_t *pool, int j, int t) const {
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)at_lo, 4 * j + t), hi = (uint32_t)__builtin_amdgcn_readlane((int)at_hi, 4 * j + t);
+        return __builtin_amdgcn_make_buffer_rsrc((void *)(pool + ((uint64_t)hi << 32 | lo)), 0, has(j, t) ? 16 * g.pages.hd : 0, 0x00020000);
     }
 };
 __device__ __forceinline__ v4i paged_load(__amdgpu_buffer_rsrc_t r, int at) {
@@ -168,11 +173,11 @@ __device__ __forceinline__ v4i paged_load(__amdgpu_buffer_rsrc_t r, int at) {
 }
 // K as the product's operand (chunk c: bytes 64 c + 16 (l / 16) .. of row l % 16); channels past the head are zeros
 template <int QC>
-__device__ __forceinline__ void paged_k(const PagedArgs &g, const PagedPlan &pl, const PagedBlocks &b, int h, int j, int lane, v4i (&x)[4][QC]) {
+__device__ __forceinline__ void paged_k(const PagedArgs &g, const PagedBlocks &b, int j, int lane, v4i (&x)[4][QC]) {
     const int hd = g.pages.hd;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
-        const auto r = b.rows(g, pl, g.pages.k, h, j, t);
+        const auto r = b.rows(g, g.pages.k, j, t);
 #pragma unroll
         for (int c = 0; c < QC; c++) {
             const int o = 64 * c + 16 * (lane >> 4);
@@ -181,10 +186,10 @@ __device__ __forceinline__ void paged_k(const PagedArgs &g, const PagedPlan &pl,
     }
 }
 // 64 channels of V for paged_pv: lane l has 16-byte chunk l % 4, swizzled, of row l / 4 of each group
-__device__ __forceinline__ void paged_v(const PagedArgs &g, const PagedPlan &pl, const PagedBlocks &b, int h, int j, int c, int lane, v4i (&x)[4]) {
+__device__ __forceinline__ void paged_v(const PagedArgs &g, const PagedBlocks &b, int j, int c, int lane, v4i (&x)[4]) {
     const int hd = g.pages.hd, r = lane >> 2, o = 64 * c + 16 * ((lane & 3) ^ vsw<4>(r)), at = o < hd ? r * hd + o : PG_NONE;
 #pragma unroll
-    for (int t = 0; t < 4; t++) x[t] = paged_load(b.rows(g, pl, g.pages.v, h, j, t), at);
+    for (int t = 0; t < 4; t++) x[t] = paged_load(b.rows(g, g.pages.v, j, t), at);
 }
 // q of a tile's rows as the product's operand: with 16 rows a column is a row; with 4, operand t has row r in column 4 t + r.
 template <int RT, int QC>
@@ -346,11 +351,11 @@ __device__ __forceinline__ void paged_put(const PagedArgs &g, const PagedPlan &p
 // PHASE 0: all in one launch, the dots in registers from the one product to the other. Else the key ranges meet in the
 // scratch, each launch forming the dots again: 1 the largest scores, 2 the sums of the entries, 3 the products with V.
 template <int RT, int QC, int NB, int NW, bool HI, int PHASE>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 ? 4 : 2))) void k_paged_tile(PagedArgs g, PagedPlan pl, void *scratch) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 ? 4 : QC == 1 && RT == 16 ? 3 : 2))) void k_paged_tile(PagedArgs g, PagedPlan pl, void *scratch) {
     static_assert(NB <= 16, "a lane for each group of the wave's blocks");
     static_assert(RT == 4 || NB <= 4, "two planes' sums of a wave's keys in 32 bits");
     constexpr int TU = RT / 4;  // accumulators of a block
-    constexpr int KD = QC == 1 ? (NB < 4 ? NB : NW > 8 || NB > 4 ? 2 : 4) : QC == 2 && NB > 1 && NW <= 8 ? 2 : 1;  // blocks of K in flight, and of V
+    constexpr int KD = QC == 1 ? (NB < 2 ? NB : RT == 16 || NW > 8 || NB > 4 ? 2 : NB < 4 ? NB : 4) : QC == 2 && NB > 1 && NW <= 8 ? 2 : 1;  // blocks of K in flight, and of V
     typedef typename std::conditional<HI, int32_t, int64_t>::type Score;
     constexpr Score LOW = HI ? (Score)INT32_MIN : (Score)INT64_MIN;
     extern __shared__ __attribute__((aligned(1024))) int8_t s_mem[];
@@ -384,7 +389,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);  // the table's loads before those of K: who has K has the table
     }
-    B.until(g, k1, lane);
+    B.until(g, pl, T.h, k1, lane);
     auto mine = [&](int j) { return B.key_of(j) < k1; };  // uniform
     const int row = RT == 16 ? ql : ql & 3, near = row < T.live ? row : T.live - 1;  // rows that are not there: as the last one
     const PagedScratch S = paged_scratch(scratch, pl, hd);
@@ -392,24 +397,24 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
     // all loads without a branch around them, so that the waits count them exactly
     v4i kr[KD][4][QC];
 #pragma unroll
-    for (int j = 0; j < KD; j++) paged_k<QC>(g, pl, B, T.h, j, lane, kr[j]);
+    for (int j = 0; j < KD; j++) paged_k<QC>(g, B, j, lane, kr[j]);
     paged_q<RT, QC>(g, pl, T, lane, qf);
     uint32_t mul = B.scale(g, p.k_scale, T.h) * (uint32_t)g.score_m, vs = 1;
     if constexpr (PHASE == 0 || PHASE == 3) vs = B.scale(g, p.v_scale, T.h);
     if constexpr (PHASE == 0 && NB <= KD) {
 #pragma unroll
-        for (int j = 0; j < NB; j++) paged_v(g, pl, B, T.h, j, 0, lane, vr[j]);
+        for (int j = 0; j < NB; j++) paged_v(g, B, j, 0, lane, vr[j]);
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int j = 0; j < NB; j++) {
         if (mine(j)) paged_dots<RT, QC>(kr[j % KD], qf, D[j]);
-        if (j + KD < NB) paged_k<QC>(g, pl, B, T.h, j + KD, lane, kr[j % KD]);
+        if (j + KD < NB) paged_k<QC>(g, B, j + KD, lane, kr[j % KD]);
         if (NB > 4) __builtin_amdgcn_sched_barrier(0);
     }
     if constexpr ((PHASE == 0 && NB > KD) || PHASE == 3) {
 #pragma unroll
-        for (int j = 0; j < KD; j++) paged_v(g, pl, B, T.h, j, 0, lane, vr[j]);
+        for (int j = 0; j < KD; j++) paged_v(g, B, j, 0, lane, vr[j]);
     }
 
     // which of a lane's keys its row sees, where not all do
@@ -547,7 +552,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
             const int f = c * NB + j;  // the loads run ahead over the channels
             __builtin_amdgcn_sched_barrier(0);
             if (mine(j)) paged_pv<RT>(vr[f % KD], D[j], lane, s_v, acc, [] {});
-            if (f + KD < QC * NB) paged_v(g, pl, B, T.h, (f + KD) % NB, (f + KD) / NB, lane, vr[f % KD]);
+            if (f + KD < QC * NB) paged_v(g, B, (f + KD) % NB, (f + KD) / NB, lane, vr[f % KD]);
         }
         if (c == 0) lds_barrier();  // the zeros
         if (mine(0)) paged_add<RT, (NB <= 4)>(acc, T.live, lane, s_acc + c * RT * PG_ACC);
@@ -586,13 +591,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QC == 4 ? 2
     T.rows(g, pl, ctx, count);
     if (T.live <= 0 || k0 >= T.keys) return;  // the launches behind read no result of this range
     const int k1 = k0 + pl.span < T.keys ? k0 + pl.span : T.keys;
-    B.until(g, k1, lane);
+    B.until(g, pl, T.h, k1, lane);
     const int row = RT == 16 ? ql : ql & 3, near = row < T.live ? row : T.live - 1;
     const PagedScratch S = paged_scratch(scratch, pl, g.pages.hd);
     constexpr int KD = QC == 1 ? 3 : 2;  // blocks of K in flight, with the one at work
     v4i x[KD][4][QC], qf[RT == 16 ? 1 : 4][QC];
 #pragma unroll
-    for (int j = 0; j + 1 < KD; j++) paged_k<QC>(g, pl, B, T.h, j, lane, x[j]);
+    for (int j = 0; j + 1 < KD; j++) paged_k<QC>(g, B, j, lane, x[j]);
     paged_q<RT, QC>(g, pl, T, lane, qf);
     const uint32_t mul = B.scale(g, g.pages.k_scale, T.h) * (uint32_t)g.score_m;
     const int sees = T.before + pl.by_group.of(T.row0 + near) + 1, lim = sees < k1 ? sees : k1, most = T.whole < k1 ? T.whole : k1;
@@ -600,7 +605,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QC == 4 ? 2
     Score mx = LOW;
     Score *to = (Score *)S.keep + (T.place * pl.rows + row) * ((size_t)pl.ng * pl.span) + 4 * qg + (RT == 16 ? 0 : 16 * (ql >> 2));
     auto step = [&](int j, v4i (&now)[4][QC], v4i (&next)[4][QC]) {
-        if (j + KD - 1 < 16) paged_k<QC>(g, pl, B, T.h, j + KD - 1, lane, next);  // (past the range: no access)
+        if (j + KD - 1 < 16) paged_k<QC>(g, B, j + KD - 1, lane, next);  // (past the range: no access)
         v4i D[TU];
         paged_dots<RT, QC>(now, qf, D);
         const int key = B.key_of(j);
@@ -666,7 +671,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RT == 16 &&
     T.rows(g, pl, ctx, count);
     if (T.live <= 0 || (k0 >= T.keys && T.range > 0)) return;  // the join reads no result of this range
     const int k1 = k0 + pl.span < T.keys ? k0 + pl.span : T.keys;
-    B.until(g, k1, lane);
+    B.until(g, pl, T.h, k1, lane);
     const int row = RT == 16 ? ql : ql & 3;
     const bool live = row < T.live;
     const PagedScratch S = paged_scratch(scratch, pl, hd);
@@ -688,7 +693,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RT == 16 &&
     const bool any = B.key_of(0) < k1;
     if (any) entries(0, D);
 #pragma unroll
-    for (int c = 0; c < GC; c++) paged_v(g, pl, B, T.h, 0, c0 + c, lane, x[c]);
+    for (int c = 0; c < GC; c++) paged_v(g, B, 0, c0 + c, lane, x[c]);
     const uint32_t vs = B.scale(g, g.pages.v_scale, T.h);
     uint64_t sum = 0;
     const int sums = (T.keys + PG_CHUNK - 1) / PG_CHUNK;
@@ -714,7 +719,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RT == 16 &&
         for (int c = 0; c < GC; c++) {
             paged_pv<RT>(x[c], E, lane, s_mem[w], acc[c], [&] {
                 __builtin_amdgcn_sched_barrier(0);
-                if (j + 1 < 16) paged_v(g, pl, B, T.h, j + 1, c0 + c, lane, x[c]);  // (past the range: no access)
+                if (j + 1 < 16) paged_v(g, B, j + 1, c0 + c, lane, x[c]);  // (past the range: no access)
                 __builtin_amdgcn_sched_barrier(0);
             });
         }
