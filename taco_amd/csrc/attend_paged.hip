@@ -26,7 +26,8 @@ struct PagedPlan {
     int group = 1, tiles = 1;  // query heads of a cache head; row tiles of a panel
     int panels = 0;            // (stream, cache head)
     int ng = 1, span = 0;      // key ranges, their keys
-    int store = 0;             // the ranges' scores are kept in the scratch
+    int split = 0;             // several launches, which meet in the scratch
+    int store = 0;             // the scores of the ranges are kept there
     int rows = 0, chunks = 1;  // rows of a tile with scores there; of PG_CHUNK keys, with a sum each
     int page_log = 4;
     PagedDiv by_group, by_tiles, by_heads, by_inner;  // group, tiles, cache heads, 8 tiles ng
@@ -191,10 +192,10 @@ __device__ __forceinline__ void paged_v(const PagedArgs &g, const PagedBlocks &b
 #pragma unroll
     for (int t = 0; t < 4; t++) x[t] = paged_load(b.rows(g, g.pages.v, j, t), at);
 }
-// q of a tile's rows as the product's operand: with 16 rows a column is a row; with 4, operand t has row r in column 4 t + r.
+// q of a tile's rows from row r0 on as the product's operand: with 16 rows a column is a row; with 4, operand t has row r in column 4 t + r.
 template <int RT, int QC>
-__device__ __forceinline__ void paged_q(const PagedArgs &g, const PagedPlan &pl, const PagedTile &T, int lane, v4i (&q)[RT == 16 ? 1 : 4][QC]) {
-    const int ql = lane & 15, row = RT == 16 ? ql : ql & 3, tok = pl.by_group.of(T.row0 + row);
+__device__ __forceinline__ void paged_q(const PagedArgs &g, const PagedPlan &pl, const PagedTile &T, int r0, int lane, v4i (&q)[RT == 16 ? 1 : 4][QC]) {
+    const int ql = lane & 15, row = r0 + (RT == 16 ? ql : ql & 3), tok = pl.by_group.of(T.row0 + row);
     const int head = T.h * pl.group + T.row0 + row - tok * pl.group;
     const v4i zero = v4i{0, 0, 0, 0};
 #pragma unroll
@@ -348,10 +349,9 @@ __device__ __forceinline__ void paged_put(const PagedArgs &g, const PagedPlan &p
 // with keys 4 (l / 16) + e of a group. With 16 rows a column is a row and D[t] holds group t. With 4 rows column 4 t + r is
 // row r with group t: the products of the four groups add up in one accumulator, each with q in its own columns and
 // zeros in the others, so that no lane idles; the product with V takes the rows' four digit planes as its 16 columns.
-// PHASE 0: all in one launch, the dots in registers from the one product to the other. Else the key ranges meet in the
-// scratch, each launch forming the dots again: 1 the largest scores, 2 the sums of the entries, 3 the products with V.
-template <int RT, int QC, int NB, int NW, bool HI, int PHASE>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 ? 4 : QC == 1 && RT == 16 ? 3 : 2))) void k_paged_tile(PagedArgs g, PagedPlan pl, void *scratch) {
+// All in one launch, the dots in registers from the one product to the other.
+template <int RT, int QC, int NB, int NW, bool HI>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 ? 4 : QC == 1 && RT == 16 ? 3 : 2))) void k_paged_tile(PagedArgs g, PagedPlan pl) {
     static_assert(NB <= 16, "a lane for each group of the wave's blocks");
     static_assert(RT == 4 || NB <= 4, "two planes' sums of a wave's keys in 32 bits");
     constexpr int TU = RT / 4;  // accumulators of a block
@@ -364,18 +364,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
     const int ql = lane & 15, qg = lane >> 4, hd = p.hd;
     PagedTile T(g, pl, blockIdx.x);
     if (!T.there) return;
-    const int k0 = PHASE ? T.range * pl.span : 0;
     const uint32_t ctx = g.ctx[T.s], count = g.rows ? g.rows[T.s] : (uint32_t)g.t;
-    PagedBlocks B(g, pl, T.s, k0 + 64 * w, 64 * NW, NB, lane);
+    PagedBlocks B(g, pl, T.s, 64 * w, 64 * NW, NB, lane);
     T.rows(g, pl, ctx, count);
     if (T.live <= 0) return;
-    if (PHASE && k0 >= T.keys && T.range > 0) return;  // the launches behind read no result of this range
-    const int k1 = PHASE && k0 + pl.span < T.keys ? k0 + pl.span : T.keys;
-    const int ranges = PHASE && T.keys > pl.span ? (T.keys + pl.span - 1) / pl.span : 1;
+    const int k1 = T.keys;
     const uint32_t last = (uint32_t)g.exp_len - 1;
 
     // LDS: the table (of 16 rows), which the sums of the outputs take over, each wave's V, what the waves exchange
-    const bool in_lds = RT == 16 && PHASE != 1 && g.table_lds;
+    const bool in_lds = RT == 16 && g.table_lds;
     constexpr int ACC_BYTES = (8 * QC * RT * PG_ACC + 1023) / 1024 * 1024;
     const int table_bytes = in_lds ? 1024 * ((g.exp_len + 255) / 256) : 0;
     const int top = table_bytes > ACC_BYTES ? table_bytes : ACC_BYTES;
@@ -392,16 +389,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
     B.until(g, pl, T.h, k1, lane);
     auto mine = [&](int j) { return B.key_of(j) < k1; };  // uniform
     const int row = RT == 16 ? ql : ql & 3, near = row < T.live ? row : T.live - 1;  // rows that are not there: as the last one
-    const PagedScratch S = paged_scratch(scratch, pl, hd);
     v4i D[NB][TU], vr[KD][4], qf[RT == 16 ? 1 : 4][QC];
     // all loads without a branch around them, so that the waits count them exactly
     v4i kr[KD][4][QC];
 #pragma unroll
     for (int j = 0; j < KD; j++) paged_k<QC>(g, B, j, lane, kr[j]);
-    paged_q<RT, QC>(g, pl, T, lane, qf);
-    uint32_t mul = B.scale(g, p.k_scale, T.h) * (uint32_t)g.score_m, vs = 1;
-    if constexpr (PHASE == 0 || PHASE == 3) vs = B.scale(g, p.v_scale, T.h);
-    if constexpr (PHASE == 0 && NB <= KD) {
+    paged_q<RT, QC>(g, pl, T, 0, lane, qf);
+    const uint32_t mul = B.scale(g, p.k_scale, T.h) * (uint32_t)g.score_m, vs = B.scale(g, p.v_scale, T.h);
+    if constexpr (NB <= KD) {
 #pragma unroll
         for (int j = 0; j < NB; j++) paged_v(g, B, j, 0, lane, vr[j]);
     }
@@ -412,7 +407,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
         if (j + KD < NB) paged_k<QC>(g, B, j + KD, lane, kr[j % KD]);
         if (NB > 4) __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr ((PHASE == 0 && NB > KD) || PHASE == 3) {
+    if constexpr (NB > KD) {
 #pragma unroll
         for (int j = 0; j < KD; j++) paged_v(g, B, j, 0, lane, vr[j]);
     }
@@ -426,52 +421,37 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
         return B.has(j, t) ? lim - (B.key_of(j) + 16 * t + 4 * qg) : 0;
     };
     const PagedRule<HI> rule(g);
-    int64_t M = INT64_MIN;
-    if constexpr (PHASE < 2) {
-        Score mx = LOW;
+    Score mx = LOW;
 #pragma unroll
-        for (int j = 0; j < NB; j++) {
-            if (!mine(j)) continue;
-            const bool whole_block = all(j);
+    for (int j = 0; j < NB; j++) {
+        if (!mine(j)) continue;
+        const bool whole_block = all(j);
 #pragma unroll
-            for (int u = 0; u < TU; u++) {
-                const int m = paged_of<RT>(mul, j, u, lane), k = whole_block ? 4 : seen(j, u);
-                int32_t d = INT32_MIN;
+        for (int u = 0; u < TU; u++) {
+            const int m = paged_of<RT>(mul, j, u, lane);
+            v4i y = D[j][u];
+            int k = 4;
+            if (!whole_block) {
+                k = seen(j, u);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int32_t x = e < k ? D[j][u][e] : INT32_MIN;
-                    d = x > d ? x : d;
-                }
-                const Score x = (Score)rule.score(d, m);  // the score grows with the dot
-                if (k > 0) mx = x > mx ? x : mx;
+                for (int e = 1; e < 4; e++) y[e] = e < k ? y[e] : y[0];  // (with none the result is not used)
             }
+            const int32_t a = y[0] > y[1] ? y[0] : y[1], b = y[2] > y[3] ? y[2] : y[3];
+            const Score x = (Score)rule.score(a > b ? a : b, m);  // the score grows with the dot
+            if (whole_block || k > 0) mx = x > mx ? x : mx;
         }
-#pragma unroll
-        for (int o = RT == 16 ? 16 : 4; o < 64; o <<= 1) {  // the lanes of the row
-            const Score x = __shfl_xor(mx, o, 64);
-            mx = x > mx ? x : mx;
-        }
-        if (lane < RT) s_mx[w * RT + lane] = mx == LOW ? INT64_MIN : (int64_t)mx;
-        if (PHASE == 0 && !mine(0)) wait_vmcnt<0>();  // (no K to wait for)
-        lds_barrier();                                // not the fence of __syncthreads, which would wait for V too
-        if constexpr (PHASE == 1) {
-            if (tid < RT) {
-#pragma unroll
-                for (int i = 0; i < NW; i++) M = s_mx[i * RT + tid] > M ? s_mx[i * RT + tid] : M;
-                S.mx[(T.slot + T.range) * RT + tid] = M;
-            }
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < NW; i++) M = s_mx[i * RT + row] > M ? s_mx[i * RT + row] : M;
-    } else {
-        for (int i = 0; i < ranges; i++) {
-            const int64_t x = S.mx[(T.slot + i) * RT + row];
-            M = x > M ? x : M;
-        }
-        if (!mine(0)) wait_vmcnt<0>();
-        if (in_lds) lds_barrier();
     }
+#pragma unroll
+    for (int o = RT == 16 ? 16 : 4; o < 64; o <<= 1) {  // the lanes of the row
+        const Score x = __shfl_xor(mx, o, 64);
+        mx = x > mx ? x : mx;
+    }
+    if (lane < RT) s_mx[w * RT + lane] = mx == LOW ? INT64_MIN : (int64_t)mx;
+    if (!mine(0)) wait_vmcnt<0>();  // (no K to wait for)
+    lds_barrier();                  // not the fence of __syncthreads, which would wait for V too
+    int64_t M = INT64_MIN;
+#pragma unroll
+    for (int i = 0; i < NW; i++) M = s_mx[i * RT + row] > M ? s_mx[i * RT + row] : M;
     // the entries, in place of the dots
     const int64_t c0 = rule.constant(M == INT64_MIN ? 0 : M);
     uint64_t sum = 0;
@@ -505,33 +485,20 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
             }
         }
     }
-    if constexpr (PHASE != 3) {
 #pragma unroll
-        for (int j = 0; j < NB; j++) {
-            if (!mine(j)) continue;
+    for (int j = 0; j < NB; j++) {
+        if (!mine(j)) continue;
 #pragma unroll
-            for (int u = 0; u < TU; u++)  // (entries are below 2^31: a pair sums in 32 bits)
-                sum += (uint64_t)((uint32_t)D[j][u][0] + (uint32_t)D[j][u][1]) + ((uint32_t)D[j][u][2] + (uint32_t)D[j][u][3]);
-        }
-#pragma unroll
-        for (int o = RT == 16 ? 16 : 4; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
-        if (lane < RT) s_sum[w * RT + lane] = sum;
-        lds_barrier();
-        sum = 0;
-        if constexpr (PHASE == 2) {
-            if (tid < RT) {
-#pragma unroll
-                for (int i = 0; i < NW; i++) sum += s_sum[i * RT + tid];
-                S.sum[(T.slot + T.range) * RT + tid] = sum;
-            }
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < NW; i++) sum += s_sum[i * RT + row];
-    } else {
-        for (int i = 0; i < ranges; i++) sum += S.sum[(T.slot + i) * RT + row];
-        lds_barrier();  // every wave has its entries
+        for (int u = 0; u < TU; u++)  // (entries are below 2^31: a pair sums in 32 bits)
+            sum += (uint64_t)((uint32_t)D[j][u][0] + (uint32_t)D[j][u][1]) + ((uint32_t)D[j][u][2] + (uint32_t)D[j][u][3]);
     }
+#pragma unroll
+    for (int o = RT == 16 ? 16 : 4; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane < RT) s_sum[w * RT + lane] = sum;
+    lds_barrier();
+    sum = 0;
+#pragma unroll
+    for (int i = 0; i < NW; i++) sum += s_sum[i * RT + row];
     for (int i = tid; i < QC * RT * PG_ACC; i += 64 * NW) s_acc[i] = 0;
     const PagedWeight wt(sum, g.softmax_p, row < T.live);
 #pragma unroll
@@ -561,13 +528,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
     for (int i = tid; i < T.live * (hd / 4); i += 64 * NW) {
         const int r = i / (hd / 4), ch = 4 * (i - r * (hd / 4));
         const int64_t *x = s_acc + ((ch >> 6) * RT + r) * PG_ACC + (ch & 63);
-        if constexpr (PHASE == 3) {
-            int64_t *to = S.part + ((T.slot + T.range) * RT + r) * hd + ch;
-#pragma unroll
-            for (int e = 0; e < 4; e++) to[e] = x[e];
-        } else {
-            paged_put(g, pl, T.s, T.h, T.row0 + r, ch, x);
-        }
+        paged_put(g, pl, T.s, T.h, T.row0 + r, ch, x);
     }
 }
 
@@ -598,7 +559,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QC == 4 ? 2
     v4i x[KD][4][QC], qf[RT == 16 ? 1 : 4][QC];
 #pragma unroll
     for (int j = 0; j + 1 < KD; j++) paged_k<QC>(g, B, j, lane, x[j]);
-    paged_q<RT, QC>(g, pl, T, lane, qf);
+    paged_q<RT, QC>(g, pl, T, 0, lane, qf);
     const uint32_t mul = B.scale(g, g.pages.k_scale, T.h) * (uint32_t)g.score_m;
     const int sees = T.before + pl.by_group.of(T.row0 + near) + 1, lim = sees < k1 ? sees : k1, most = T.whole < k1 ? T.whole : k1;
     const PagedRule<HI> rule(g);
@@ -740,6 +701,232 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RT == 16 &&
     }
 }
 
+// ---- Many rows over long caches ------------------------------------------------------------------------
+// Groups of 64 rows, four tiles of 16: three walks over a range's keys, each forming the dots again (4 MFMAs a block and tile,
+// less than keeping 16 scores a key and tile would cost): the largest scores, the sums of the entries, the products with V.
+// In the first two a wave takes blocks of keys with all four tiles, so that the four waves' loads are of different keys; in
+// the third a wave takes a tile over all blocks, since a tile's sums are 64 registers for 64 channels (the waves' loads of
+// the same rows meet in the L1).
+template <int QC, bool HI, int PHASE>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QC == 4 ? 2 : 3))) void k_paged_scan(PagedArgs g, PagedPlan pl, void *scratch) {
+    extern __shared__ __attribute__((aligned(1024))) int32_t s_exp[];  // the table
+    __shared__ int64_t s_x[4][64];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ql = lane & 15, qg = lane >> 4;
+    PagedTile T(g, pl, blockIdx.x);
+    if (!T.there) return;
+    if (PHASE == 2 && g.table_lds) paged_table(g, s_exp, w, 4, lane);
+    const int k0 = T.range * pl.span;
+    const uint32_t ctx = g.ctx[T.s], count = g.rows ? g.rows[T.s] : (uint32_t)g.t;
+    PagedBlocks B(g, pl, T.s, k0 + 64 * w, 256, 16, lane);
+    T.rows(g, pl, ctx, count);
+    if (T.live <= 0 || k0 >= T.keys) return;  // the launches behind read no result of this range
+    const int k1 = k0 + pl.span < T.keys ? k0 + pl.span : T.keys, tiles = (T.live + 15) / 16;
+    B.until(g, pl, T.h, k1, lane);
+    const PagedScratch S = paged_scratch(scratch, pl, g.pages.hd);
+    v4i x[4][QC], qf[4][1][QC];
+    paged_k<QC>(g, B, 0, lane, x);
+    const uint32_t mul = B.scale(g, g.pages.k_scale, T.h) * (uint32_t)g.score_m;
+    const PagedRule<HI> rule(g);
+    int lim[4];
+    int64_t v[4];  // the largest score; then the row's constant
+    uint64_t sum[4];
+    const int ranges = (T.keys + pl.span - 1) / pl.span;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        const int r = 16 * u + ql, near = r < T.live ? r : T.live - 1;
+        paged_q<16, QC>(g, pl, T, 16 * u, lane, qf[u]);
+        const int sees = T.before + pl.by_group.of(T.row0 + near) + 1;
+        lim[u] = sees < k1 ? sees : k1;
+        v[u] = INT64_MIN;
+        sum[u] = 0;
+        if constexpr (PHASE == 2) {
+            for (int i = 0; i < ranges; i++) {
+                const int64_t y = S.mx[(T.slot + i) * 64 + near];
+                v[u] = y > v[u] ? y : v[u];
+            }
+            v[u] = rule.constant(v[u] == INT64_MIN ? 0 : v[u]);
+        }
+    }
+    const uint32_t last = (uint32_t)g.exp_len - 1;
+    if constexpr (PHASE == 2) __syncthreads();  // the table
+    for (int j = 0; B.key_of(j) < k1; j++) {
+        const int key = B.key_of(j);
+        const bool pages = ((B.there >> (4 * j)) & 15) == 15;
+        v4i next[4][QC];
+        paged_k<QC>(g, B, j + 1 < 16 ? j + 1 : 15, lane, next);  // (past the range: no access)
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (u >= tiles) break;
+            __builtin_amdgcn_sched_barrier(0);
+            v4i D[4];
+            paged_dots<16, QC>(x, qf[u], D);
+            const int whole = T.before + pl.by_group.of(T.row0 + 16 * u) + 1;
+            const bool all = pages && key + 64 <= (whole < k1 ? whole : k1);  // uniform
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const int m = paged_of<16>(mul, j, t, lane), k = all ? 4 : B.has(j, t) ? lim[u] - (key + 16 * t + 4 * qg) : 0;
+                v4i y = D[t];
+                if constexpr (PHASE == 1) {
+                    if (!all) {
+#pragma unroll
+                        for (int e = 1; e < 4; e++) y[e] = e < k ? y[e] : y[0];
+                    }
+                    const int32_t a = y[0] > y[1] ? y[0] : y[1], b = y[2] > y[3] ? y[2] : y[3];
+                    const int64_t z = rule.score(a > b ? a : b, m);
+                    if (all || k > 0) v[u] = z > v[u] ? z : v[u];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) y[e] = (int32_t)rule.index(y[e], m, v[u], last);
+                    if (g.table_lds) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) y[e] = s_exp[y[e]];
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) y[e] = g.exp_table[y[e]];
+                    }
+                    if (!all) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) y[e] = e < k ? y[e] : 0;
+                    }
+                    sum[u] += (uint64_t)((uint32_t)y[0] + (uint32_t)y[1]) + ((uint32_t)y[2] + (uint32_t)y[3]);
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int c = 0; c < QC; c++) x[t][c] = next[t][c];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        if constexpr (PHASE == 1) {
+#pragma unroll
+            for (int o = 16; o < 64; o <<= 1) {
+                const int64_t y = __shfl_xor(v[u], o, 64);
+                v[u] = y > v[u] ? y : v[u];
+            }
+            if (qg == 0) s_x[w][16 * u + ql] = v[u];
+        } else {
+#pragma unroll
+            for (int o = 16; o < 64; o <<= 1) sum[u] += __shfl_xor(sum[u], o, 64);
+            if (qg == 0) s_x[w][16 * u + ql] = (int64_t)sum[u];
+        }
+    }
+    __syncthreads();
+    if (tid < 64) {
+        int64_t y = s_x[0][tid];
+#pragma unroll
+        for (int i = 1; i < 4; i++) y = PHASE == 2 ? y + s_x[i][tid] : (s_x[i][tid] > y ? s_x[i][tid] : y);
+        if constexpr (PHASE == 1) S.mx[(T.slot + T.range) * 64 + tid] = y;
+        else S.sum[(T.slot + T.range) * 64 + tid] = (uint64_t)y;
+    }
+}
+
+// 64 channels from chunk blockIdx.y on. With one range the outputs themselves.
+template <int QC, bool HI>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QC == 1 ? 3 : 2))) void k_paged_walk(PagedArgs g, PagedPlan pl, void *scratch) {
+    extern __shared__ __attribute__((aligned(1024))) int8_t s_mem[];  // 4 KiB of V a wave, the table
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ql = lane & 15, qg = lane >> 4, hd = g.pages.hd, c = blockIdx.y;
+    int8_t *s_v = s_mem + 4096 * w;
+    int32_t *s_exp = (int32_t *)(s_mem + 16384);
+    PagedTile T(g, pl, blockIdx.x);
+    if (!T.there) return;
+    if (g.table_lds) paged_table(g, s_exp, w, 4, lane);
+    const int k0 = T.range * pl.span;
+    T.rows(g, pl, g.ctx[T.s], g.rows ? g.rows[T.s] : (uint32_t)g.t);
+    if (T.live <= 0 || (k0 >= T.keys && T.range > 0)) return;  // the join reads no result of this range
+    const int gk1 = k0 + pl.span < T.keys ? k0 + pl.span : T.keys;
+    const PagedScratch S = paged_scratch(scratch, pl, hd);
+    const int r = 16 * w + ql, near = r < T.live ? r : T.live - 1;
+    // the tile's last row sees no more than this
+    const int end = 16 * w + 15 < T.live ? 16 * w + 15 : T.live - 1, sees_end = T.before + pl.by_group.of(T.row0 + end) + 1;
+    const int k1 = 16 * w >= T.live ? k0 : (sees_end < gk1 ? sees_end : gk1);
+    const int sees = T.before + pl.by_group.of(T.row0 + near) + 1, lim = sees < k1 ? sees : k1;
+    const int whole0 = T.before + pl.by_group.of(T.row0 + 16 * w) + 1, whole = whole0 < k1 ? whole0 : k1;
+    const PagedRule<HI> rule(g);
+    const int ranges = (T.keys + pl.span - 1) / pl.span;
+    int64_t M = INT64_MIN;
+    uint64_t sum = 0;
+    for (int i = 0; i < ranges; i++) {
+        const int64_t y = S.mx[(T.slot + i) * 64 + near];
+        M = y > M ? y : M;
+        sum += S.sum[(T.slot + i) * 64 + near];
+    }
+    const int64_t c0 = rule.constant(M == INT64_MIN ? 0 : M);
+    const PagedWeight wt(sum, g.softmax_p, r < T.live);
+    const uint32_t last = (uint32_t)g.exp_len - 1;
+    v4i qf[1][QC], acc[4][4];
+    paged_q<16, QC>(g, pl, T, 16 * w, lane, qf);
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[k][i] = v4i{0, 0, 0, 0};
+    __syncthreads();  // the table
+    for (int b0 = k0; b0 < k1; b0 += 1024) {  // 16 blocks with one look at the pages
+        PagedBlocks B(g, pl, T.s, b0, 64, 16, lane);
+        const int e1 = b0 + 1024 < k1 ? b0 + 1024 : k1;
+        B.until(g, pl, T.h, e1, lane);
+        v4i x[4][QC], y[4];
+        paged_k<QC>(g, B, 0, lane, x);
+        const uint32_t mul = B.scale(g, g.pages.k_scale, T.h) * (uint32_t)g.score_m, vs = B.scale(g, g.pages.v_scale, T.h);
+        paged_v(g, B, 0, c, lane, y);
+        for (int j = 0; B.key_of(j) < e1; j++) {
+            v4i D[4];
+            paged_dots<16, QC>(x, qf, D);
+            __builtin_amdgcn_sched_barrier(0);
+            if (j + 1 < 16) paged_k<QC>(g, B, j + 1, lane, x);  // (past the range: no access)
+            const int key = B.key_of(j);
+            const bool all = ((B.there >> (4 * j)) & 15) == 15 && key + 64 <= whole;  // uniform
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const int m = paged_of<16>(mul, j, t, lane);
+#pragma unroll
+                for (int e = 0; e < 4; e++) D[t][e] = (int32_t)rule.index(D[t][e], m, c0, last);
+                if (g.table_lds) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) D[t][e] = s_exp[D[t][e]];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) D[t][e] = g.exp_table[D[t][e]];
+                }
+            }
+            if (!all) {
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const int k = B.has(j, t) ? lim - (key + 16 * t + 4 * qg) : 0;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) D[t][e] = e < k ? D[t][e] : 0;
+                }
+            }
+            paged_digits<16>(wt, vs, j, lane, s_v, D);
+            paged_pv<16>(y, D, lane, s_v, acc, [&] {
+                __builtin_amdgcn_sched_barrier(0);
+                if (j + 1 < 16) paged_v(g, B, j + 1, c, lane, y);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        }
+    }
+    if (r >= T.live) return;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int ch = 64 * c + 16 * i + 4 * qg;
+        if (ch >= hd) continue;
+        int64_t z[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            z[e] = (int64_t)acc[0][i][e] + (int64_t)acc[1][i][e] * 256 + (int64_t)acc[2][i][e] * 65536 + (int64_t)acc[3][i][e] * 16777216;
+        if (pl.ng == 1) {
+            paged_put(g, pl, T.s, T.h, T.row0 + r, ch, z);
+        } else {
+            int64_t *to = S.part + ((T.slot + T.range) * 64 + r) * hd + ch;
+#pragma unroll
+            for (int e = 0; e < 4; e++) to[e] = z[e];
+        }
+    }
+}
+
 // The scores of a row over PG_CHUNK keys to their entries, in place, and the entries' sum.
 template <bool HI>
 __global__ __launch_bounds__(256) void k_paged_entries(PagedArgs g, PagedPlan pl, void *scratch) {
@@ -858,32 +1045,31 @@ __global__ __launch_bounds__(256) void k_paged_out(PagedArgs g, PagedPlan pl, vo
     paged_put(g, pl, T.s, T.h, T.row0 + r, ch, x);
 }
 
-constexpr size_t PG_KEEP = (size_t)128 << 20;  // bytes of scores that a call keeps at most (tiles of 16 rows)
-
 static PagedPlan paged_plan(const PagedArgs &g) {
     PagedPlan p;
     p.group = g.heads / g.pages.kv_heads;
     const long long rows = (long long)g.t * p.group;
-    p.rt = rows <= 4 ? 4 : 16;
+    const int most = rows <= 4 ? 4096 : 2048;  // keys of a tile in one launch
+    p.rt = rows <= 4 ? 4 : (rows > 16 && g.keys > most ? 64 : 16);
     p.rows = rows < p.rt ? (int)rows : p.rt;
     p.tiles = (int)((rows + p.rt - 1) / p.rt);
     p.panels = g.streams * g.pages.kv_heads;
     while (1 << p.page_log < g.pages.page) p.page_log++;
-    const int most = p.rt == 4 ? 4096 : 2048;  // keys of a tile in one launch
     p.span = (g.keys + 63) / 64 * 64;
     if (g.keys > most) {
         const long long wgs = (long long)p.panels * p.tiles;
-        auto ranges = [&](int least_keys, int most_keys, long long all) {
+        auto ranges = [&](int least_keys, long long all) {
             long long ng = (all + wgs - 1) / wgs;
-            const long long least = (g.keys + most_keys - 1) / most_keys, more = (g.keys + least_keys - 1) / least_keys;
+            const long long least = (g.keys + 4095) / 4096, more = (g.keys + least_keys - 1) / least_keys;
             ng = ng < least ? least : (ng > more ? more : ng);
             p.span = (int)(((g.keys + ng - 1) / ng + 255) / 256) * 256;
             p.ng = (g.keys + p.span - 1) / p.span;
         };
-        if (p.rt == 4) ranges(1024, 4096, 3072);
-        else ranges(512, 4096, 512);
-        p.store = p.rt == 4 || (size_t)wgs * p.rows * p.ng * p.span * 8 <= PG_KEEP;
-        if (!p.store) ranges(256, 1024, 1024);
+        if (p.rt == 4) ranges(1024, 3072);
+        else if (p.rt == 16) ranges(512, 512);
+        else ranges(512, 1024);
+        p.store = p.rt < 64;
+        p.split = 1;
         p.chunks = p.store ? (g.keys + PG_CHUNK - 1) / PG_CHUNK : p.ng;
     }
     p.by_group = PagedDiv((uint32_t)p.group);
@@ -901,49 +1087,51 @@ bool paged_fits(const PagedArgs &g) {
 size_t paged_workspace(const PagedArgs &g) {
     const PagedPlan p = paged_plan(g);
     size_t bytes = 0;
-    if (p.ng > 1) paged_scratch(nullptr, p, g.pages.hd, &bytes);
+    if (p.split) paged_scratch(nullptr, p, g.pages.hd, &bytes);
     return bytes;
 }
 
-template <int RT, int QC, int NB, int NW, bool HI, int PHASE>
-static hipError_t launch_paged_t(const PagedArgs &g, const PagedPlan &p, void *scratch, hipStream_t stream) {
+template <int RT, int QC, int NB, int NW, bool HI>
+static hipError_t launch_paged_t(const PagedArgs &g, const PagedPlan &p, hipStream_t stream) {
     const int acc = (8 * QC * RT * PG_ACC + 1023) / 1024 * 1024;
-    const int table = RT == 16 && PHASE != 1 && g.table_lds ? 1024 * ((g.exp_len + 255) / 256) : 0;
+    const int table = RT == 16 && g.table_lds ? 1024 * ((g.exp_len + 255) / 256) : 0;
     const size_t lds = (size_t)(table > acc ? table : acc) + 4096 * NW + 16 * NW * RT;
-    const hipError_t e = allow_dynamic_lds((const void *)k_paged_tile<RT, QC, NB, NW, HI, PHASE>, lds);
+    const hipError_t e = allow_dynamic_lds((const void *)k_paged_tile<RT, QC, NB, NW, HI>, lds);
     if (e != hipSuccess) return e;
-    launch_k((k_paged_tile<RT, QC, NB, NW, HI, PHASE>), dim3((unsigned)((p.panels + 7) / 8 * 8) * p.tiles * p.ng), dim3(64 * NW), lds, stream, g, p, scratch);
+    launch_k((k_paged_tile<RT, QC, NB, NW, HI>), dim3((unsigned)((p.panels + 7) / 8 * 8) * p.tiles * p.ng), dim3(64 * NW), lds, stream, g, p);
     return hipGetLastError();
 }
 
 template <int RT, int QC, bool HI>
 static hipError_t launch_paged_q(const PagedArgs &g, const PagedPlan &p, void *scratch, hipStream_t stream) {
-    if (p.ng > 1) {
+    if (p.split) {
         hipError_t e;
         const unsigned grid = (unsigned)((p.panels + 7) / 8 * 8) * p.tiles * p.ng;
+        const size_t table = g.table_lds ? (size_t)1024 * ((g.exp_len + 255) / 256) : 0;
+        auto run = [&](auto kernel, dim3 n, size_t lds) {
+            const hipError_t f = allow_dynamic_lds((const void *)kernel, lds);
+            if (f != hipSuccess) return f;
+            launch_k(kernel, n, dim3(256), lds, stream, g, p, scratch);
+            return hipGetLastError();
+        };
         if (p.store) {
             constexpr int GC = QC == 4 ? 2 : QC;  // (the sums of more channels do not fit the registers)
-            launch_k(k_paged_scores<RT, QC, HI>, dim3(grid), dim3(256), 0, stream, g, p, scratch);
-            if ((e = hipGetLastError()) != hipSuccess) return e;
-            const size_t table = g.table_lds ? (size_t)1024 * ((g.exp_len + 255) / 256) : 0;
-            if ((e = allow_dynamic_lds((const void *)k_paged_entries<HI>, table)) != hipSuccess) return e;
-            launch_k(k_paged_entries<HI>, dim3((unsigned)p.panels * p.tiles * p.chunks * p.rows), dim3(256), table, stream, g, p, scratch);
-            if ((e = hipGetLastError()) != hipSuccess) return e;
-            launch_k(k_paged_products<RT, GC, HI>, dim3(grid, QC / GC), dim3(256), 0, stream, g, p, scratch);
-            if ((e = hipGetLastError()) != hipSuccess) return e;
+            if ((e = run(k_paged_scores<RT, QC, HI>, dim3(grid), 0)) != hipSuccess) return e;
+            if ((e = run(k_paged_entries<HI>, dim3((unsigned)p.panels * p.tiles * p.chunks * p.rows), table)) != hipSuccess) return e;
+            if ((e = run(k_paged_products<RT, GC, HI>, dim3(grid, QC / GC), 0)) != hipSuccess) return e;
         } else if constexpr (RT == 16) {
-            if ((e = launch_paged_t<RT, QC, 4, 4, HI, 1>(g, p, scratch, stream)) != hipSuccess) return e;
-            if ((e = launch_paged_t<RT, QC, 4, 4, HI, 2>(g, p, scratch, stream)) != hipSuccess) return e;
-            if ((e = launch_paged_t<RT, QC, 4, 4, HI, 3>(g, p, scratch, stream)) != hipSuccess) return e;
+            if ((e = run(k_paged_scan<QC, HI, 1>, dim3(grid), 0)) != hipSuccess) return e;
+            if ((e = run(k_paged_scan<QC, HI, 2>, dim3(grid), table)) != hipSuccess) return e;
+            if ((e = run(k_paged_walk<QC, HI>, dim3(grid, (g.pages.hd + 63) / 64), 16384 + table)) != hipSuccess) return e;
+            if (p.ng == 1) return hipSuccess;
         }
         const size_t quads = (size_t)p.panels * p.tiles * p.rows * (g.pages.hd / 4);
-        launch_k(k_paged_out, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, g, p, scratch);
-        return hipGetLastError();
+        return run(k_paged_out, dim3((unsigned)((quads + 255) / 256)), 0);
     }
-    if (p.span <= 256) return launch_paged_t<RT, QC, 1, 4, HI, 0>(g, p, scratch, stream);
-    if (p.span <= 1024) return launch_paged_t<RT, QC, 4, 4, HI, 0>(g, p, scratch, stream);
-    if (p.span <= 2048) return launch_paged_t<RT, QC, 4, 8, HI, 0>(g, p, scratch, stream);
-    if constexpr (RT == 4) return launch_paged_t<RT, QC, 8, 8, HI, 0>(g, p, scratch, stream);
+    if (p.span <= 256) return launch_paged_t<RT, QC, 1, 4, HI>(g, p, stream);
+    if (p.span <= 1024) return launch_paged_t<RT, QC, 4, 4, HI>(g, p, stream);
+    if (p.span <= 2048) return launch_paged_t<RT, QC, 4, 8, HI>(g, p, stream);
+    if constexpr (RT == 4) return launch_paged_t<RT, QC, 4, 16, HI>(g, p, stream);
     return hipErrorInvalidValue;
 }
 
