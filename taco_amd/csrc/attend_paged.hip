@@ -1049,7 +1049,7 @@ static PagedPlan paged_plan(const PagedArgs &g) {
     PagedPlan p;
     p.group = g.heads / g.pages.kv_heads;
     const long long rows = (long long)g.t * p.group;
-    const int most = rows <= 4 ? 4096 : 2048;  // keys of a tile in one launch
+    const int most = rows > 4 ? 2048 : g.pages.hd > 128 ? 4096 : 8192;  // keys of a tile in one launch
     p.rt = rows <= 4 ? 4 : (rows > 16 && g.keys > most ? 64 : 16);
     p.rows = rows < p.rt ? (int)rows : p.rt;
     p.tiles = (int)((rows + p.rt - 1) / p.rt);
@@ -1130,8 +1130,13 @@ static hipError_t launch_paged_q(const PagedArgs &g, const PagedPlan &p, void *s
     }
     if (p.span <= 256) return launch_paged_t<RT, QC, 1, 4, HI>(g, p, stream);
     if (p.span <= 1024) return launch_paged_t<RT, QC, 4, 4, HI>(g, p, stream);
-    if (p.span <= 2048) return launch_paged_t<RT, QC, 4, 8, HI>(g, p, stream);
-    if constexpr (RT == 4) return launch_paged_t<RT, QC, 4, 16, HI>(g, p, stream);
+    if constexpr (RT == 16) {
+        if (p.span <= 2048) return launch_paged_t<RT, QC, 4, 8, HI>(g, p, stream);
+    } else {
+        if (p.span <= 2048) return launch_paged_t<RT, QC, 2, 16, HI>(g, p, stream);
+        if (p.span <= 4096) return launch_paged_t<RT, QC, 4, 16, HI>(g, p, stream);
+        if constexpr (QC <= 2) return launch_paged_t<RT, QC, 8, 16, HI>(g, p, stream);
+    }
     return hipErrorInvalidValue;
 }
 
