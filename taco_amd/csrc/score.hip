@@ -148,7 +148,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
     extern __shared__ uint32_t s_hist[];  // [table_len + 63]
     __shared__ uint64_t slots[NW], s_sum[NW], s_list[LIST], s_best[64];
     __shared__ double s_ent[NW];
-    __shared__ uint32_t s_ahead[NW], s_count, s_thr, s_found;
+    __shared__ uint32_t s_ahead[NW], s_count, s_thr, s_found, s_below;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), V = a.vocab, last = a.table_len - 1;
     const size_t r = blockIdx.x;
     const uint32_t cap = (uint32_t)(last + lane);  // this lane's bin of what lies past the table's end
@@ -162,14 +162,19 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
     const uintptr_t at = SRC == SCORE_COMPACT ? (uintptr_t)(a.d16 + r * a.ld16) : (uintptr_t)a.logits + r * a.ld * E;
     const int off = SRC == SCORE_COMPACT ? 0 : (int)(at % 16) / E;  // symbol of element e of group i: 4 (NT i + tid) + e - off
     const auto from = __builtin_amdgcn_make_buffer_rsrc((void *)(at - at % 16), 0, SRC == SCORE_COMPACT ? (V + 63) / 64 * 128 : ((off + V) * E + 15) / 16 * 16, 0x00020000);
-    const int groups = (V + off + 4 * NT - 1) / (4 * NT);
-    auto symbol = [&](int i, int e) { return 4 * (NT * i + tid) + e - off; };
+    const int groups = SRC == SCORE_COMPACT ? 2 * ((V + 8 * NT - 1) / (8 * NT)) : (V + off + 4 * NT - 1) / (4 * NT);
+    // (compact ones eight together, two groups: they share a tile)
+    auto symbol = [&](int i, int e) {
+        return SRC == SCORE_COMPACT ? 8 * (NT * (i >> 1) + tid) + 4 * (i & 1) + e : 4 * (NT * i + tid) + e - off;
+    };
     auto inside = [&](int j) { return j >= 0 && j < V; };
-    auto edge = [&](int i) { return (i == 0 && off > 0) || 4 * NT * (i + 1) > V + off; };  // some of group i are past the row (uniform)
+    auto edge = [&](int i) {  // some of group i are past the row (uniform)
+        return SRC == SCORE_COMPACT ? 8 * NT * ((i >> 1) + 1) > V : (i == 0 && off > 0) || 4 * NT * (i + 1) > V + off;
+    };
     typedef typename std::conditional<SRC == SCORE_I64, v4i[2], typename std::conditional<SRC == SCORE_I32, v4i[1], v2i[1]>::type>::type Raw;
     auto fetch = [&](int i, Raw &y) {
         if constexpr (SRC == SCORE_COMPACT) {
-            y[0] = __builtin_bit_cast(v2i, __builtin_amdgcn_raw_buffer_load_b64(from, 8 * tid, 8 * NT * i, 0));
+            y[0] = __builtin_bit_cast(v2i, __builtin_amdgcn_raw_buffer_load_b64(from, 16 * tid + 8 * (i & 1), 16 * NT * (i >> 1), 0));
         } else {
 #pragma unroll
             for (int k = 0; k < E / 4; k++)
@@ -224,7 +229,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
 #pragma unroll
             for (int i = 0; i < G; i++) {
                 fetch(i, raw[i]);
-                tile[i] = tile_of(i);
+                tile[i] = i & 1 ? tile[i - 1] : tile_of(i);
             }
         }
         start();
@@ -285,11 +290,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
     auto indexes = [&](int i, const Raw &y, const X (&v)[4], int64_t t, uint32_t (&d)[4]) {
         if constexpr (SRC == SCORE_COMPACT) {
             const uint64_t b = (uint64_t)M - (uint64_t)t;
-            const uint32_t base = b < (uint64_t)cap ? (uint32_t)b : cap;
+            const unsigned short base = (unsigned short)(b < (uint64_t)cap ? (uint32_t)b : cap);
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                d[e] = base + (e & 1 ? (uint32_t)y[0][e >> 1] >> 16 : (uint32_t)y[0][e >> 1] & 0xffffu);
-                d[e] = d[e] < (uint32_t)last ? d[e] : cap;  // (a d16 may be capped at last)
+            for (int k = 0; k < 2; k++) {  // (a d16 may be capped at last: past the table too)
+                const int two = y[0][k];
+                us2 p;
+                __builtin_memcpy(&p, &two, 4);
+                p = __builtin_elementwise_min(__builtin_elementwise_add_sat(p, us2{base, base}), us2{(unsigned short)cap, (unsigned short)cap});
+                d[2 * k] = p.x;
+                d[2 * k + 1] = p.y;
             }
         } else {
 #pragma unroll
@@ -326,7 +335,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 fetch(i0 + i, y[i]);
-                if constexpr (SRC == SCORE_COMPACT) t[i] = tile_of(i0 + i);
+                if constexpr (SRC == SCORE_COMPACT) t[i] = i & 1 ? t[i - 1] : tile_of(i0 + i);
             }
 #pragma unroll
             for (int i = 0; i < 8; i++) {
@@ -386,12 +395,28 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
     };
     __syncthreads();  // the counts are there
     if (w == 0) {     // the spare bins to the last one, without the places past the row
-        const uint32_t far = (uint32_t)wave_sum64(s_hist[last + lane]);
+        const uint32_t far = (uint32_t)wave_sum_dpp(s_hist[last + lane]);
         if (lane == 0) s_hist[last] = far - (places - (uint32_t)V);
     }
     uint32_t ahead = 0;  // symbols before the token
     __syncthreads();
-    if (a.rank && some && s_hist[td] > 1) those((uint32_t)td, (uint32_t)td, [&](int j, int) { ahead += j < (int)token; });  // its ties
+    if (a.rank && some && s_hist[td] > 1) {  // its ties (uniform)
+        if (G > 0 && s_hist[td] > 512) {     // many, those past the table say: without a branch
+            const uint32_t span = (td >= last ? 0xffffu : (uint32_t)td) - (uint32_t)td;
+#pragma unroll
+            for (int i = 0; i < G; i++) {
+                uint32_t q[2] = {d2[2 * i], d2[2 * i + 1]};
+                asm volatile("" : "+v"(q[0]), "+v"(q[1]));
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t d = e & 1 ? q[e >> 1] >> 16 : q[e >> 1] & 0xffffu;
+                    ahead += d - (uint32_t)td <= span && (uint32_t)symbol(i, e) < token;
+                }
+            }
+        } else {
+            those((uint32_t)td, (uint32_t)td, [&](int j, int) { ahead += j < (int)token; });
+        }
+    }
     // T and the entropy from the counts, in one pass: with w0 = table[0], the largest weight there is, the entropy
     // sum (w / T) ln(T / w) = ln(T / w0) + (sum w ln(w0 / w)) / T, two terms that are not negative (log_share takes the first,
     // exact where T is close to w0). In f32 the logarithms of the second are some 2^-22 off, which the first outweighs: it is
@@ -424,14 +449,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
     ahead = (uint32_t)wave_sum_dpp(ahead);
     if (lane == 0) s_sum[w] = sum, s_ahead[w] = ahead, s_ent[w] = h;
     const bool tops = a.top > 0 && (a.top_tokens || a.top_logprob);
-    // the index up to which `top` symbols lie, and how many lie up to it: the last wave over 256 bins at a time
+    // the index up to which `top` symbols lie, and how many lie up to it: the last wave over 1,024 bins at a time
     if (tops && w == NW - 1) {
         uint32_t before = 0;
-        for (int k0 = 0; k0 <= last; k0 += 256) {
-            uint32_t c[4], mine = 0;
+        for (int k0 = 0; k0 <= last; k0 += 1024) {
+            uint32_t c[16], mine = 0;
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                c[k] = k0 + 4 * lane + k <= last ? s_hist[k0 + 4 * lane + k] : 0;
+            for (int k = 0; k < 16; k++) {
+                c[k] = k0 + 16 * lane + k <= last ? s_hist[k0 + 16 * lane + k] : 0;
                 mine += c[k];
             }
             uint32_t upto = mine;
@@ -443,13 +468,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
             const uint64_t reached = __ballot(before + upto >= (uint32_t)a.top);
             if (reached) {  // (top <= vocab: some bin does)
                 if (lane == __ffsll((unsigned long long)reached) - 1) {
-                    uint32_t y = before + upto - mine;
+                    uint32_t y = before + upto - mine, under = 0;
                     int k = -1;
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (y < (uint32_t)a.top) y += c[i], k = i;
-                    s_thr = (uint32_t)(k0 + 4 * lane + k);
+                    for (int i = 0; i < 16; i++)
+                        if (y < (uint32_t)a.top) under = y, y += c[i], k = i;
+                    s_thr = (uint32_t)(k0 + 16 * lane + k);
                     s_found = y;
+                    s_below = under;
                 }
                 break;
             }
@@ -461,15 +487,34 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
 #pragma unroll
     for (int i = 0; i < NW; i++) T += s_sum[i];
     int best = 0;  // alternatives in s_best
-    if (tops && s_found <= LIST) {  // uniform
-        those(0, s_thr, [&](int j, int d) { s_list[atomicAdd(&s_count, 1u)] = (uint64_t)d << 32 | (uint32_t)j; });
+    if (tops) {
+        const uint32_t thr = s_thr;
+        const bool ties = s_found > LIST;  // more than the list holds, so most of them equal: those of thr apart (uniform)
+        if (!ties || thr > 0)
+            those(0, ties ? thr - 1 : thr, [&](int j, int d) { s_list[atomicAdd(&s_count, 1u)] = (uint64_t)d << 32 | (uint32_t)j; });
         __syncthreads();
-        const int found = (int)s_found;
+        const int found = (int)(ties ? s_below : s_found);
         for (int i = tid; i < found; i += NT) {
             const uint64_t one = s_list[i];
             int place = 0;
             for (int k = 0; k < found; k++) place += s_list[k] < one;
             if (place < a.top) s_best[place] = one;
+        }
+        if (ties) {  // the first of the equal ones, in the symbols' order
+            for (int j0 = 0, got = found; got < a.top && j0 < V; j0 += NT) {
+                const bool in = j0 + tid < V && row.index(M, j0 + tid < V ? j0 + tid : 0) == (int)thr;
+                const uint64_t m = __ballot(in);
+                if (lane == 0) slots[w] = (uint64_t)__popcll(m);
+                __syncthreads();
+                int place = got + __popcll(m & (((uint64_t)1 << lane) - 1));
+#pragma unroll
+                for (int i = 0; i < NW; i++) {
+                    place += i < w ? (int)slots[i] : 0;
+                    got += (int)slots[i];
+                }
+                if (in && place < a.top) s_best[place] = (uint64_t)thr << 32 | (uint32_t)(j0 + tid);
+                __syncthreads();
+            }
         }
         __syncthreads();
         best = a.top;
@@ -493,7 +538,6 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
             a.entropy[r] = (float)(x / (double)T - l);
         }
     }
-    if (tops && best == 0) search_top<SRC, NW>(a, r, M, T, slots);
 }
 
 template <int SRC, int G, int NW>
@@ -515,7 +559,7 @@ static hipError_t launch_score_src(const ScoreArgs &a, int n_rows, hipStream_t s
             if (v <= 4 * 1024 * 13) return launch_score_rows<SRC, 13, 16>(a, n_rows, stream);
         } else {
             // a row a CU: 64 rows 18 us (26 groups of 8 waves 21); more rows share a CU, one at its loads while another counts
-            if (n_rows <= 256 && v <= 4 * 1024 * 13) return launch_score_rows<SRC, 13, 16>(a, n_rows, stream);
+            if (n_rows <= 256 && v <= 4 * 1024 * 13) return launch_score_rows<SRC, SRC == SCORE_COMPACT ? 14 : 13, 16>(a, n_rows, stream);
             if (v <= 4 * 512 * 26) return launch_score_rows<SRC, 26, 8>(a, n_rows, stream);
         }
         return launch_score_rows<SRC, 0, 16>(a, n_rows, stream);

@@ -79,6 +79,24 @@ def test_ties(gpu):
         check(gpu, logits, WEIGHTS, [0, vocab - 1, 77, vocab - 2, vocab // 2], 64)
 
 
+def test_more_ties_than_a_list(gpu):
+    """Thousands of equal symbols at the border of the alternatives, some before them, and past the table's end; the token
+    one of them."""
+    r = np.random.default_rng(12)
+    for vocab in (700, 5000, 50257, 120_000):
+        logits = np.full((6, vocab), -700, np.int32)
+        logits[0, r.integers(0, vocab, 20)] = r.integers(0, 300, 20)
+        logits[1, :] = -9000
+        logits[1, vocab - 5:] = np.arange(5)
+        logits[2, : vocab // 2] = -20_000
+        logits[2, vocab // 2] = 0
+        logits[3, r.random(vocab) < 0.5] = -701
+        logits[4, -1] = 5
+        logits[5] = r.integers(-100_000, 0, vocab)
+        for dtype in (np.int32, np.int64):
+            check(gpu, logits.astype(dtype), WEIGHTS, r.integers(0, vocab, 6), 64)
+
+
 def test_weights_of_zero(gpu):
     """A table that ends in zeros: alternatives and tokens without weight have log probability minus infinity."""
     r = np.random.default_rng(2)
