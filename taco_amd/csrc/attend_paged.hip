@@ -1129,7 +1129,11 @@ static hipError_t launch_paged_q(const PagedArgs &g, const PagedPlan &p, void *s
         return run(k_paged_out, dim3((unsigned)((quads + 255) / 256)), 0);
     }
     if (p.span <= 256) return launch_paged_t<RT, QC, 1, 4, HI>(g, p, stream);
-    if (p.span <= 1024) return launch_paged_t<RT, QC, 4, 4, HI>(g, p, stream);
+    if (p.span <= 1024) {
+        if constexpr (RT == 4)
+            if ((long long)p.panels <= 256) return launch_paged_t<RT, QC, 1, 16, HI>(g, p, stream);
+        return launch_paged_t<RT, QC, 4, 4, HI>(g, p, stream);
+    }
     if constexpr (RT == 16) {
         if (p.span <= 2048) return launch_paged_t<RT, QC, 4, 8, HI>(g, p, stream);
     } else {

@@ -622,8 +622,11 @@ def _on_gpu(x) -> bool:
 
 def _dptr(x):
     """The device address of x: a contiguous tensor on the GPU (data_ptr()), an address or a ctypes pointer, or None."""
-    if not _on_gpu(x):
+    cuda = getattr(x, "is_cuda", None)
+    if cuda is None and not hasattr(x, "data_ptr"):
         return x
+    if cuda is not None and not cuda:
+        raise ValueError("a tensor in host memory where the GPU reads or writes")
     if not x.is_contiguous():
         raise ValueError("a tensor with strides of its own: the operators take contiguous ones")
     return x.data_ptr()
