@@ -351,11 +351,11 @@ __device__ __forceinline__ void paged_put(const PagedArgs &g, const PagedPlan &p
 // zeros in the others, so that no lane idles; the product with V takes the rows' four digit planes as its 16 columns.
 // All in one launch, the dots in registers from the one product to the other.
 template <int RT, int QC, int NB, int NW, bool HI>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 ? 4 : QC == 1 && RT == 16 ? 3 : 2))) void k_paged_tile(PagedArgs g, PagedPlan pl) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 || (RT == 4 && NW == 8 && QC <= 2) ? 4 : QC == 1 && RT == 16 ? 3 : 2))) void k_paged_tile(PagedArgs g, PagedPlan pl) {
     static_assert(NB <= 16, "a lane for each group of the wave's blocks");
     static_assert(RT == 4 || NB <= 4, "two planes' sums of a wave's keys in 32 bits");
     constexpr int TU = RT / 4;  // accumulators of a block
-    constexpr int KD = QC == 1 ? (NB < 2 ? NB : RT == 16 || NW > 8 || NB > 4 ? 2 : NB < 4 ? NB : 4) : QC == 2 && NB > 1 && NW <= 8 ? 2 : 1;  // blocks of K in flight, and of V
+    constexpr int KD = QC == 1 ? (NB < 2 ? NB : RT == 16 || NW >= 8 ? 2 : NB < 4 ? NB : 4) : QC == 2 && NB > 1 && NW <= 8 ? 2 : 1;  // blocks of K in flight, and of V
     typedef typename std::conditional<HI, int32_t, int64_t>::type Score;
     constexpr Score LOW = HI ? (Score)INT32_MIN : (Score)INT64_MIN;
     extern __shared__ __attribute__((aligned(1024))) int8_t s_mem[];
@@ -1065,6 +1065,9 @@ static PagedPlan paged_plan(const PagedArgs &g) {
             p.span = (int)(((g.keys + ng - 1) / ng + 255) / 256) * 256;
             p.ng = (g.keys + p.span - 1) / p.span;
         };
+        // workgroups in all, of 512, 768, 1,024, 2,048 and 3,072, in us of the scores' launch and the products':
+        //   200 panels of one row, 8,192 to 16,384 keys     41 + 41   41 + 41   40 + 41   38 + 38   36 + 39
+        //   128 panels of eight rows, 128 channels, 4,000   15 + 17   17 + 23   15 + 22   17 + 30   17 + 30
         if (p.rt == 4) ranges(1024, 3072);
         else if (p.rt == 16) ranges(512, 512);
         else ranges(512, 1024);
@@ -1081,7 +1084,7 @@ static PagedPlan paged_plan(const PagedArgs &g) {
 
 bool paged_fits(const PagedArgs &g) {
     const PagedPlan p = paged_plan(g);
-    return ((long long)p.panels + 7) * p.tiles < (1ll << 23) / p.ng && (long long)p.panels * p.tiles * p.rows < (1ll << 23) / p.chunks && (long long)p.panels * p.tiles * p.rt < (1ll << 31) / (g.pages.hd / 4);
+    return ((long long)p.panels + 7) * p.tiles < (1ll << 23) / p.ng && (!p.store || (long long)p.panels * p.tiles * p.rows < (1ll << 23) / p.chunks) && (long long)p.panels * p.tiles * p.rt < (1ll << 31) / (g.pages.hd / 4);
 }
 
 size_t paged_workspace(const PagedArgs &g) {
@@ -1128,20 +1131,22 @@ static hipError_t launch_paged_q(const PagedArgs &g, const PagedPlan &p, void *s
         const size_t quads = (size_t)p.panels * p.tiles * p.rows * (g.pages.hd / 4);
         return run(k_paged_out, dim3((unsigned)((quads + 255) / 256)), 0);
     }
+    // Blocks a wave and waves, by the keys a call may read. One row a panel: a workgroup a CU and less takes 16 waves, whose
+    // chains are short (12 panels of 1,000 keys 8.6 us, in four waves 9.3); 768 panels one round of three workgroups a CU (18.9
+    // us at 1,024 keys); more keys two workgroups of eight waves a CU, one at its loads while the other works (2,048 keys
+    // 37.9 us, in one of 16 waves 46.0; 4,096 keys 62.8 and 70.2, and with 128 channels 166 and 141, where eight blocks spill).
     if (p.span <= 256) return launch_paged_t<RT, QC, 1, 4, HI>(g, p, stream);
     if (p.span <= 1024) {
         if constexpr (RT == 4)
-            if ((long long)p.panels <= 256) return launch_paged_t<RT, QC, 1, 16, HI>(g, p, stream);
+            if (p.panels <= 256) return launch_paged_t<RT, QC, 1, 16, HI>(g, p, stream);
         return launch_paged_t<RT, QC, 4, 4, HI>(g, p, stream);
     }
-    if constexpr (RT == 16) {
-        if (p.span <= 2048) return launch_paged_t<RT, QC, 4, 8, HI>(g, p, stream);
-    } else {
-        if (p.span <= 2048) return launch_paged_t<RT, QC, 2, 16, HI>(g, p, stream);
-        if (p.span <= 4096) return launch_paged_t<RT, QC, 4, 16, HI>(g, p, stream);
+    if (p.span <= 2048) return launch_paged_t<RT, QC, 4, 8, HI>(g, p, stream);
+    if constexpr (RT == 4) {
+        if (p.span <= 4096) return launch_paged_t<RT, QC, QC == 2 ? 4 : 8, QC == 2 ? 16 : 8, HI>(g, p, stream);
         if constexpr (QC <= 2) return launch_paged_t<RT, QC, 8, 16, HI>(g, p, stream);
     }
-    return hipErrorInvalidValue;
+    return hipErrorInvalidValue;  // (the plan splits longer ones)
 }
 
 template <int RT>
