@@ -212,8 +212,9 @@ hs_status hs_batch_commit_paths(hs_batch *batch, const uint32_t *slots, const ui
  * logits table, then of their numbers; entropy[i] = sum (w / T) ln(T / w); and the first `top` symbols of that
  * order, top_tokens[i][..], with their log probabilities top_logprob[i][..] (drafts for a tree, say). tokens may
  * hold HS_NO_TOKEN (log probability 0, rank HS_NO_TOKEN), and may be NULL where logprob and rank are; every
- * result may be NULL. top is at most 64 and at most the vocabulary. Logarithms are within 2 units in the last
- * place of 32 bits; all else is exact. */
+ * result may be NULL and may not overlap another. top is at most 64 and at most the vocabulary. Log
+ * probabilities are within one unit in the last place of 32 bits and entropies within 2^-20 of themselves, for
+ * tables that do not increase (a model's logits_exp); all else is exact. */
 #define HS_NO_TOKEN 0xFFFFFFFFu
 hs_status hs_batch_run_scored(hs_batch *batch, const hs_input *inputs, const uint32_t *tokens,
                               size_t n, size_t top, float *logprob, uint32_t *rank, float *entropy,
@@ -443,7 +444,8 @@ hs_status hs_op_pages_append_dev(hs_device *dev, const hs_pages *cache, const vo
  * with M the largest score and S the sum of e over the keys seen; where every scale is 1 that is the rule
  * of the other attention entries, bit for bit. score_m >= 1, score_m max_scale < 2^31 and 2^P max_scale
  * <= 2^30 (max_scale rounded up to a power of two). A row that sees no key, or whose entries sum to 0, is
- * 0; rows i >= rows[s] of out are left as they were. q and out 16-byte aligned, q_stride a multiple of 16. */
+ * 0; rows i >= rows[s] of out are left as they were. q and out 16-byte aligned and not overlapping, q_stride a
+ * multiple of 16. */
 hs_status hs_op_attend_paged_dev(hs_device *dev, const hs_pages *cache, const int8_t *q, size_t q_stride,
                                  const uint32_t *table, const uint32_t *ctx, const uint32_t *rows,
                                  size_t b, size_t t, size_t h, size_t width, size_t keys,
@@ -454,10 +456,11 @@ hs_status hs_op_attend_paged_dev(hs_device *dev, const hs_pages *cache, const in
 size_t hs_op_attend_paged_workspace(size_t b, size_t t, size_t h, size_t kv_heads, size_t hd, size_t keys);
 
 /* The scores of hs_batch_run_scored for rows of logits on the device: i32 (bits = 32) or i64 (bits =
- * 64) logits [rows, ld], of which the first vocab of a row count, and a table of `len` entries of at most
- * 2^40 (a model's logits_exp). tokens [rows] (or NULL: none; a number that is no symbol: none, log
+ * 64) logits [rows, ld], of which the first vocab < 2^24 of a row count, and a table of `len` entries
+ * of at most 2^40 (a model's logits_exp). tokens [rows] (or NULL: none; a number that is no symbol: none, log
  * probability 0 and rank 0xFFFFFFFF). logprob, rank, entropy [rows] and top_tokens, top_logprob [rows, top]
- * may each be NULL. A row whose weights are all 0 has log probabilities of minus infinity and entropy 0. */
+ * may each be NULL and must not overlap. A row whose weights are all 0 has log probabilities of minus
+ * infinity and entropy 0. */
 hs_status hs_op_score_dev(hs_device *dev, const void *logits, uint32_t bits, size_t ld,
                           const uint32_t *tokens, const uint64_t *table, size_t len, size_t rows,
                           size_t vocab, size_t top, float *logprob, uint32_t *rank, float *entropy,

@@ -1078,13 +1078,16 @@ static PagedPlan paged_plan(const PagedArgs &g) {
     p.by_group = PagedDiv((uint32_t)p.group);
     p.by_tiles = PagedDiv((uint32_t)p.tiles);
     p.by_heads = PagedDiv((uint32_t)g.pages.kv_heads);
-    p.by_inner = PagedDiv((uint32_t)(8 * p.tiles * p.ng));
+    p.by_inner = PagedDiv((uint32_t)(8ll * p.tiles * p.ng));
     return p;
 }
 
+// A grid has fewer than 2^32 threads: workgroups of up to 1,024 in one launch, and 256 in each of several.
 bool paged_fits(const PagedArgs &g) {
     const PagedPlan p = paged_plan(g);
-    return ((long long)p.panels + 7) * p.tiles < (1ll << 23) / p.ng && (!p.store || (long long)p.panels * p.tiles * p.rows < (1ll << 23) / p.chunks) && (long long)p.panels * p.tiles * p.rt < (1ll << 31) / (g.pages.hd / 4);
+    const long long tiles = (long long)p.panels * p.tiles;
+    return ((long long)p.panels + 7) * p.tiles < (1ll << 22) / p.ng && (!p.store || tiles * p.rows < (1ll << 23) / p.chunks) &&
+           tiles * p.rt < (1ll << 31) / (g.pages.hd / 4);
 }
 
 size_t paged_workspace(const PagedArgs &g) {

@@ -2299,7 +2299,7 @@ hs_status attend_paged_args(hs_device *dev, const hs_pages *cache, size_t b, siz
     if (keys == 0 || keys > (size_t)1 << 22 || keys > width * cache->page)
         return hs::fail(HS_UNSUPPORTED, 0, "keys must be in 1..=2^22 and fit the pages of a stream");
     g.streams = (int)b; g.t = (int)t; g.heads = (int)h; g.width = (int)width; g.keys = (int)keys;
-    if (b && t && !hs::paged_fits(g)) return hs::fail(HS_UNSUPPORTED, 0, "too many rows, heads and keys (2^23 workgroups)");
+    if (b && t && !hs::paged_fits(g)) return hs::fail(HS_UNSUPPORTED, 0, "too many rows, heads and keys (2^22 workgroups)");
     return HS_OK;
 }
 
@@ -2327,6 +2327,7 @@ extern "C" hs_status hs_op_pages_append_dev(hs_device *dev, const hs_pages *cach
     if (b == 0 || t == 0) return HS_OK;
     a.k = k; a.v = v; a.bits = (int)bits; a.stride = stride; a.table = table; a.ctx = ctx; a.rows = rows;
     a.streams = (int)b; a.t = (int)t; a.width = (int)width; a.headroom = headroom; a.ctx_out = ctx_out;
+    if (!hs::append_fits(a)) return hs::fail(HS_UNSUPPORTED, 0, "too many streams, tokens and heads (2^25 runs of a head)");
     HIP_TRY(hipSetDevice(dev->ordinal));
     HIP_TRY(hs::launch_append(a, stream ? (hipStream_t)stream : dev->stream));
     return HS_OK;
@@ -2361,6 +2362,9 @@ extern "C" hs_status hs_op_attend_paged_dev(hs_device *dev, const hs_pages *cach
     if (len == 0 || len > (size_t)INT32_MAX || score_m < 1 || (int64_t)score_m * cache->max_scale > INT32_MAX || softmax_p + bits > 30)
         return hs::fail(HS_UNSUPPORTED, 0, "len >= 1, 1 <= score_m, score_m max_scale < 2^31 and 2^P max_scale <= 2^30");
     if (b == 0 || t == 0) return HS_OK;
+    const size_t far = (size_t)1 << 46;  // (past any allocation)
+    if (overlap(q, b * t > far / q_stride ? far : b * t * q_stride, out, b * t * h * cache->head_dim))
+        return hs::fail(HS_INVALID_ARGUMENT, 0, "out must not overlap q");
     g.q = q; g.q_stride = q_stride; g.table = table; g.ctx = ctx; g.rows = rows;
     g.score_m = score_m; g.score_s = score_s; g.out_m = out_m; g.out_s = out_s;
     g.exp_table = attn_exp; g.exp_len = (int)len; g.softmax_p = softmax_p; g.out = out;
@@ -2375,9 +2379,9 @@ extern "C" hs_status hs_op_score_dev(hs_device *dev, const void *logits, uint32_
     hs::clear_error();
     if (!dev || !logits || !table) return hs::fail(HS_INVALID_ARGUMENT, 0, "NULL argument");
     if (bits != 32 && bits != 64) return hs::fail(HS_UNSUPPORTED, 0, "logits of 32 or 64 bits");
-    if (vocab == 0 || vocab > (size_t)1 << 24 || len == 0 || len > (size_t)INT32_MAX || ld < vocab ||
+    if (vocab == 0 || vocab >= (size_t)1 << 24 || len == 0 || len > (size_t)INT32_MAX || ld < vocab ||
         ld > (size_t)1 << 40 || rows > MAX_ROW_HEADS / 16)
-        return hs::fail(HS_UNSUPPORTED, 0, "1 to 2^24 symbols a row, len >= 1 and fewer than 2^22 rows");
+        return hs::fail(HS_UNSUPPORTED, 0, "1 to 2^24 - 1 symbols a row (their weights add up below 2^64), len >= 1 and fewer than 2^22 rows");
     if (top > HS_MAX_TOP || top > vocab) return hs::fail(HS_UNSUPPORTED, 0, "top is at most 64, and at most the vocabulary");
     if (!tokens && (logprob || rank)) return hs::fail(HS_INVALID_ARGUMENT, 0, "log probabilities and ranks need tokens");
     if (!aligned(bits / 8, {logits}) || !aligned(8, {table}) || !aligned(4, {tokens, logprob, rank, entropy, top_tokens, top_logprob}))

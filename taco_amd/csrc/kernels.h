@@ -341,6 +341,7 @@ struct AppendArgs {
     uint32_t headroom = 16;
     uint32_t *ctx_out = nullptr;
 };
+bool append_fits(const AppendArgs &a);
 hipError_t launch_append(const AppendArgs &a, hipStream_t stream);
 struct PagedArgs {
     PagePool pages;

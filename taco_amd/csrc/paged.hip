@@ -106,8 +106,16 @@ __global__ __launch_bounds__(256) void k_append(AppendArgs a, int run, int runs,
     }
 }
 
+// Runs of up to 64 tokens: the most that t tokens of a stream touch.
+static int append_run(const AppendArgs &a) { return a.pages.page < 64 ? a.pages.page : 64; }
+static int append_runs(const AppendArgs &a) { return (a.t + 2 * append_run(a) - 2) / append_run(a); }
+
+bool append_fits(const AppendArgs &a) {  // a wave a task, a grid of fewer than 2^32 threads
+    return (size_t)a.streams * append_runs(a) * a.pages.kv_heads * 2 < ((size_t)1 << 26) - 4;
+}
+
 hipError_t launch_append(const AppendArgs &a, hipStream_t stream) {
-    const int run = a.pages.page < 64 ? a.pages.page : 64, runs = (a.t + 2 * run - 2) / run;
+    const int run = append_run(a), runs = append_runs(a);
     const size_t tasks = (size_t)a.streams * runs * a.pages.kv_heads * 2;
     const dim3 grid((unsigned)((tasks + 3) / 4));
     if (a.bits == 8) launch_k(k_append<int8_t>, grid, dim3(256), 0, stream, a, run, runs, tasks);

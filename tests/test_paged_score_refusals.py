@@ -32,7 +32,7 @@ def append(kind=None, cache=CACHE, k=BASE, v=BASE, table=BASE, ctx=BASE, rows=BA
     hip.pages_append(Dev, *args) if kind is None else refused(kind, hip.pages_append, *args)
 
 
-def attend(kind=None, cache=CACHE, q=BASE, table=BASE, ctx=BASE, rows=BASE, dims=(2, 3, 4, 4, 200), rule=RULE, out=BASE, **kw):
+def attend(kind=None, cache=CACHE, q=BASE, table=BASE, ctx=BASE, rows=BASE, dims=(2, 3, 4, 4, 200), rule=RULE, out=BASE + 2048, **kw):
     args = (cache, q, table, ctx, rows, dims, rule, out)
     hip.attend_paged(Dev, *args, **kw) if kind is None else refused(kind, hip.attend_paged, *args, **kw)
 
@@ -80,6 +80,8 @@ def test_append_refusals():
     append(UNSUPPORTED, bits=8, stride=136)
     append(BAD, ctx_out=BASE + 4)               # on the second count
     append(BAD, ctx=BASE + 128, ctx_out=BASE)   # on rows
+    append(UNSUPPORTED, dims=(2 ** 25 - 8, 1, 4), ctx_out=BASE + 2 ** 40)    # 2^26 waves for keys and values
+    append(UNSUPPORTED, dims=(2 ** 23, 3, 4), ctx_out=BASE + 2 ** 40)        # two runs of a stream
     append(dims=(0, 3, 4))
     append(dims=(2, 0, 4))
 
@@ -106,7 +108,10 @@ def test_attend_refusals():
                  RULE._replace(score_m=2 ** 25), RULE._replace(softmax_p=25)):
         attend(UNSUPPORTED, rule=rule)
     attend(UNSUPPORTED, cache=CACHE._replace(max_scale=65))  # counts as 128: 2^24 128 is past 2^30
+    attend(UNSUPPORTED, dims=(2 ** 21, 1, 4, 4, 200), out=BASE + 2 ** 40)    # 2^22 workgroups
     attend(BAD, workspace=BASE + 16, workspace_bytes=1 << 40)
+    attend(BAD, q=BASE, out=BASE + 1024)                 # 6 rows of 256
+    attend(BAD, q=BASE + 1024, out=BASE)
     attend(dims=(0, 3, 4, 4, 200))
     attend(dims=(2, 0, 4, 4, 200))
 
@@ -133,7 +138,7 @@ def test_score_refusals():
         score(BAD, outs=[BASE + 2 if i == j else BASE for j in range(5)])
     for bits in (0, 16):
         score(UNSUPPORTED, bits=bits)
-    for dims in ((2, 0, 50), (2, 2 ** 24 + 1, 50), (2, 100, 0), (2, 100, 2 ** 31), (2 ** 22, 100, 50), (-1, 100, 50)):
+    for dims in ((2, 0, 50), (2, 2 ** 24, 50), (2, 2 ** 24 + 1, 50), (2, 100, 0), (2, 100, 2 ** 31), (2 ** 22, 100, 50), (-1, 100, 50)):
         score(UNSUPPORTED, dims=dims)
     for top in (65, 101, -1):
         score(UNSUPPORTED, top=top)
