@@ -355,7 +355,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
     static_assert(NB <= 16, "a lane for each group of the wave's blocks");
     static_assert(RT == 4 || NB <= 4, "two planes' sums of a wave's keys in 32 bits");
     constexpr int TU = RT / 4;  // accumulators of a block
-    constexpr int KD = QC == 1 ? (NB < 2 ? NB : RT == 16 || NW >= 8 ? 2 : NB < 4 ? NB : 4) : QC == 2 && NB > 1 && NW <= 8 ? 2 : 1;  // blocks of K in flight, and of V
+    constexpr int KD = QC == 1 && NB <= 8 ? (NB < 2 ? NB : RT == 16 || NW >= 8 ? 2 : NB < 4 ? NB : 4) : QC == 2 && NB > 1 && NW <= 8 ? 2 : 1;  // blocks of K in flight, and of V
     typedef typename std::conditional<HI, int32_t, int64_t>::type Score;
     constexpr Score LOW = HI ? (Score)INT32_MIN : (Score)INT64_MIN;
     extern __shared__ __attribute__((aligned(1024))) int8_t s_mem[];
@@ -1049,11 +1049,17 @@ static PagedPlan paged_plan(const PagedArgs &g) {
     PagedPlan p;
     p.group = g.heads / g.pages.kv_heads;
     const long long rows = (long long)g.t * p.group;
-    const int most = rows > 4 ? 2048 : g.pages.hd > 128 ? 4096 : 8192;  // keys of a tile in one launch
+    p.panels = g.streams * g.pages.kv_heads;
+    // Keys of a tile in one launch, whose dots fit the registers of its waves. It reads K and V and nothing else; several launches
+    // write and read the scores too, but spread a panel over the chip. In us, one launch and several: 768 panels of 8,192 keys 117
+    // and 155, 12 panels 27 and 36; of 16,000 keys 768 panels 238 and 290, 200 panels 71 and 89, 48 panels 50 and 34. 16 rows
+    // (8 query heads of 128 channels, 128 panels of 2,000 keys) 25 and 38.
+    const int most = rows > 4 ? 2048 : g.pages.hd > 128 ? 4096 : g.pages.hd > 64 || p.panels < 128 ? 8192 : 16384;
+    // 64 rows: 16 streams of 64 rows over 4,096 keys 100 us, in tiles of 16 rows 155. 4 rows: a row of 1,000 keys 9.2 us, as one
+    // of 16 rows 12.2 (768 panels 20.5 and 23.8).
     p.rt = rows <= 4 ? 4 : (rows > 16 && g.keys > most ? 64 : 16);
     p.rows = rows < p.rt ? (int)rows : p.rt;
     p.tiles = (int)((rows + p.rt - 1) / p.rt);
-    p.panels = g.streams * g.pages.kv_heads;
     while (1 << p.page_log < g.pages.page) p.page_log++;
     p.span = (g.keys + 63) / 64 * 64;
     if (g.keys > most) {
@@ -1147,7 +1153,9 @@ static hipError_t launch_paged_q(const PagedArgs &g, const PagedPlan &p, void *s
     if (p.span <= 2048) return launch_paged_t<RT, QC, 4, 8, HI>(g, p, stream);
     if constexpr (RT == 4) {
         if (p.span <= 4096) return launch_paged_t<RT, QC, QC == 2 ? 4 : 8, QC == 2 ? 16 : 8, HI>(g, p, stream);
-        if constexpr (QC <= 2) return launch_paged_t<RT, QC, 8, 16, HI>(g, p, stream);
+        if constexpr (QC <= 2)
+            if (p.span <= 8192) return launch_paged_t<RT, QC, 8, 16, HI>(g, p, stream);
+        if constexpr (QC == 1) return launch_paged_t<RT, QC, 16, 16, HI>(g, p, stream);
     }
     return hipErrorInvalidValue;  // (the plan splits longer ones)
 }

@@ -169,6 +169,20 @@ def test_long_caches(gpu, keys, t, heads, kvh):
     check_attend(gpu, 2, t, heads, kvh, 64, 128, keys, [keys, keys // 3], seed=keys)
 
 
+@pytest.mark.parametrize("keys,heads,hd", [(9000, 2, 64), (16384, 6, 64), (16385, 2, 64), (12000, 8, 48)])
+def test_many_long_caches(gpu, keys, heads, hd):
+    """128 panels of a few rows: those of up to 16,384 keys in one launch."""
+    ctx = np.concatenate([[keys, keys - 1, 0, 1, 8192, 8193], np.linspace(3, keys, 58)]).astype(np.uint32)
+    check_attend(gpu, 64, 1, heads, 2, hd, 64, keys, ctx, holes=0.05, seed=keys)
+
+
+@pytest.mark.parametrize("t,heads", [(1, 2), (1, 12), (40, 2)])
+def test_long_caches_with_wide_scores(gpu, t, heads):
+    """A shift below 32: scores of 64 bits."""
+    check_attend(gpu, 2, t, heads, 2, 64, 64, 9000, [9000, 8192], rule=(33_000_000, 20, 1_300_000_000, 56, 24), holes=0.1)
+    check_attend(gpu, 64, 1, 2, 2, 64, 64, 9000, [9000, 8192, 5, 100], rule=(33_000_000, 20, 1_300_000_000, 56, 24))
+
+
 @pytest.mark.parametrize("hd", [128, 256])
 def test_long_caches_of_wide_heads(gpu, hd):
     for t in (1, 20):
