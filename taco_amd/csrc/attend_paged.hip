@@ -192,10 +192,10 @@ __device__ __forceinline__ void paged_v(const PagedArgs &g, const PagedBlocks &b
 #pragma unroll
     for (int t = 0; t < 4; t++) x[t] = paged_load(b.rows(g, g.pages.v, j, t), at);
 }
-// q of a tile's rows from row r0 on as the product's operand: with 16 rows a column is a row; with 4, operand t has row r in column 4 t + r.
+// q of a tile's rows from row r0 on as the product's operand: operand t has row r in column RT t + r.
 template <int RT, int QC>
-__device__ __forceinline__ void paged_q(const PagedArgs &g, const PagedPlan &pl, const PagedTile &T, int r0, int lane, v4i (&q)[RT == 16 ? 1 : 4][QC]) {
-    const int ql = lane & 15, row = r0 + (RT == 16 ? ql : ql & 3), tok = pl.by_group.of(T.row0 + row);
+__device__ __forceinline__ void paged_q(const PagedArgs &g, const PagedPlan &pl, const PagedTile &T, int r0, int lane, v4i (&q)[16 / RT][QC]) {
+    const int ql = lane & 15, row = r0 + ql % RT, tok = pl.by_group.of(T.row0 + row);
     const int head = T.h * pl.group + T.row0 + row - tok * pl.group;
     const v4i zero = v4i{0, 0, 0, 0};
 #pragma unroll
@@ -207,33 +207,35 @@ __device__ __forceinline__ void paged_q(const PagedArgs &g, const PagedPlan &pl,
             q[0][c] = x;
         } else {
 #pragma unroll
-            for (int t = 0; t < 4; t++) q[t][c] = (ql >> 2) == t ? x : zero;
+            for (int t = 0; t < 16 / RT; t++) q[t][c] = ql / RT == t ? x : zero;
         }
     }
 }
 // The dots of a block.
 template <int RT, int QC>
-__device__ __forceinline__ void paged_dots(const v4i (&x)[4][QC], const v4i (&q)[RT == 16 ? 1 : 4][QC], v4i (&D)[RT / 4]) {
+__device__ __forceinline__ void paged_dots(const v4i (&x)[4][QC], const v4i (&q)[16 / RT][QC], v4i (&D)[RT / 4]) {
+    constexpr int G = 16 / RT;  // groups in an accumulator
 #pragma unroll
     for (int u = 0; u < RT / 4; u++) D[u] = v4i{0, 0, 0, 0};
 #pragma unroll
     for (int t = 0; t < 4; t++)
 #pragma unroll
         for (int c = 0; c < QC; c++) {
-            v4i &d = D[RT == 16 ? t : 0];
-            d = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[t][c], q[RT == 16 ? 0 : t][c], d, 0, 0, 0);
+            v4i &d = D[t / G];
+            d = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[t][c], q[t % G][c], d, 0, 0, 0);
         }
 }
 // Of a value that lane 4 j + t holds, that of this lane's group of accumulator u.
 template <int RT>
 __device__ __forceinline__ int paged_of(uint32_t x, int j, int u, int lane) {
-    return RT == 16 ? __builtin_amdgcn_readlane((int)x, 4 * j + u) : __shfl((int)x, 4 * j + ((lane & 15) >> 2), 64);
+    return RT == 16 ? __builtin_amdgcn_readlane((int)x, 4 * j + u) : __shfl((int)x, 4 * j + 16 / RT * u + (lane & 15) / RT, 64);
 }
 
 // The digits of w = floor(E 2^P / S) for E = e vs, exactly (softmax_p_of, which holds for E < 2^53 with w <= 2^30), with
 // 0x80808080 inside the rounding constant: the low word of the sum is w + 0x80808080, whose bytes xor 0x80 are balanced
 // digits. From the entries D[u][e]: D[k] word t the digit k of group t's keys (16 rows); D[0] word t digit l % 4 of row
-// l / 4 % 4 of group t's keys (4 rows: the lanes transpose through 1 KiB of LDS).
+// l / 4 % 4 of group t's keys (4 rows), D[k] word t digit 2 k + l % 2 of row l / 2 % 8 (8 rows): the lanes transpose through
+// 256 bytes of LDS a row.
 struct PagedWeight {
     double R, sp;  // rows that are not there and rows without weight: w = 0 (R = 0)
     __device__ __forceinline__ PagedWeight(uint64_t sum, int P, bool live)
@@ -263,14 +265,17 @@ __device__ __forceinline__ void paged_digits(const PagedWeight &wt, uint32_t vs,
 #pragma unroll
             for (int t = 0; t < 4; t++) D[k][t] = (int32_t)(o[t][k] ^ 0x80808080u);
     } else {
-        int *to = (int *)mem + 64 * (ql & 3) + 4 * qg + (ql >> 2);  // [row][digit][l / 16][group]
+        int *to = (int *)mem + 64 * (ql % RT) + 4 * qg + ql / RT;  // [row][digit][l / 16][group]
 #pragma unroll
-        for (int k = 0; k < 4; k++) to[16 * k] = (int)(o[0][k] ^ 0x80808080u);
-        D[0] = *(const v4i *)((const int *)mem + 16 * ql + 4 * qg);
+        for (int u = 0; u < TU; u++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) to[16 * k + 16 / RT * u] = (int)(o[u][k] ^ 0x80808080u);
+#pragma unroll
+        for (int k = 0; k < TU; k++) D[k] = *(const v4i *)((const int *)mem + 64 * (ql / (4 / TU)) + 16 * (4 / TU * k + ql % (4 / TU)) + 4 * qg);
     }
 }
 // acc += V^T digits over a block, 64 channels of V through 4 KiB of LDS: channels 16 i + 4 (l / 16) + e of digit k of row l % 16
-// in acc[k][i][e] (16 rows), of digit l % 4 of row l / 4 % 4 in acc[0][i][e] (4 rows).
+// in acc[k][i][e] (16 rows), of the digit and row of D[k] as above (4 and 8).
 // `then` runs when x has left the registers.
 template <int RT, typename F>
 __device__ __forceinline__ void paged_pv(const v4i (&x)[4], const v4i (&D)[RT / 4], int lane, int8_t *mem, v4i (&acc)[RT / 4][4], F then) {
@@ -309,6 +314,22 @@ __device__ __forceinline__ void paged_add(const v4i (&acc)[RT / 4][4], int live,
                 }
                 atomicAdd(to + 16 * i + e, (unsigned long long)x);
             }
+    } else if constexpr (RT == 8) {
+        // lane l % 2 keeps the four planes' sum of channels 32 (l % 2) ..: the pair's lanes exchange halves
+        const bool b = lane & 1;
+        unsigned long long *to = (unsigned long long *)s_acc + (ql >> 1) * PG_ACC + 32 * (lane & 1) + 4 * qg;
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                int64_t z[2];
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const int32_t keep = b ? acc[k][i + 2][e] : acc[k][i][e], got = dpp_mov<0xB1>(b ? acc[k][i][e] : acc[k][i + 2][e]);
+                    z[k] = b ? (int64_t)keep * 256 + got : (int64_t)got * 256 + keep;
+                }
+                if ((ql >> 1) < live) atomicAdd(to + 16 * i + e, (unsigned long long)(z[1] * 65536 + z[0]));
+            }
     } else {
         // lane l % 4 = i keeps the four planes' sum of channels 16 i ..: the quad's lanes exchange halves twice
         const bool b0 = lane & 1, b1 = lane & 2;
@@ -343,19 +364,20 @@ __device__ __forceinline__ void paged_put(const PagedArgs &g, const PagedPlan &p
     *(uint32_t *)(g.out + (((size_t)s * g.t + tok) * g.heads + head) * g.pages.hd + ch) = packed;
 }
 
-// Tiles of RT rows (16, or 4 where there are no more) of one (stream, cache head): row r is query head r % group of
+// Tiles of RT rows (16, or 4 or 8 where there are no more) of one (stream, cache head): row r is query head r % group of
 // token r / group. Wave w takes the blocks of 64 keys w, w + NW, .. of the range, NB at most, each in four groups of 16
 // keys that lie in one page. K is the first operand of v_mfma_i32_16x16x64_i8, so lane l holds dots of column l % 16
 // with keys 4 (l / 16) + e of a group. With 16 rows a column is a row and D[t] holds group t. With 4 rows column 4 t + r is
 // row r with group t: the products of the four groups add up in one accumulator, each with q in its own columns and
-// zeros in the others, so that no lane idles; the product with V takes the rows' four digit planes as its 16 columns.
+// zeros in the others, so that no lane idles; the product with V takes the rows' four digit planes as its 16 columns. With 8
+// rows two groups share an accumulator and two planes a product.
 // All in one launch, the dots in registers from the one product to the other.
 template <int RT, int QC, int NB, int NW, bool HI>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 || (RT == 4 && NW == 8 && QC <= 2) ? 4 : QC == 1 && RT == 16 ? 3 : 2))) void k_paged_tile(PagedArgs g, PagedPlan pl) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 || (RT <= 8 && NW == 8 && QC <= 2) ? 4 : QC == 1 && RT == 16 ? 3 : 2))) void k_paged_tile(PagedArgs g, PagedPlan pl) {
     static_assert(NB <= 16, "a lane for each group of the wave's blocks");
-    static_assert(RT == 4 || NB <= 4, "two planes' sums of a wave's keys in 32 bits");
+    static_assert(RT < 16 || NB <= 4, "two planes' sums of a wave's keys in 32 bits");
     constexpr int TU = RT / 4;  // accumulators of a block
-    constexpr int KD = QC == 1 && NB <= 8 ? (NB < 2 ? NB : RT == 16 || NW >= 8 ? 2 : NB < 4 ? NB : 4) : QC == 2 && NB > 1 && NW <= 8 ? 2 : 1;  // blocks of K in flight, and of V
+    constexpr int KD = QC == 1 && NB <= 8 ? (NB < 2 ? NB : RT >= 8 || NW >= 8 ? 2 : NB < 4 ? NB : 4) : QC == 2 && NB > 1 && NW <= 8 ? 2 : 1;  // blocks of K in flight, and of V
     typedef typename std::conditional<HI, int32_t, int64_t>::type Score;
     constexpr Score LOW = HI ? (Score)INT32_MIN : (Score)INT64_MIN;
     extern __shared__ __attribute__((aligned(1024))) int8_t s_mem[];
@@ -371,8 +393,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
     const int k1 = T.keys;
     const uint32_t last = (uint32_t)g.exp_len - 1;
 
-    // LDS: the table (of 16 rows), which the sums of the outputs take over, each wave's V, what the waves exchange
-    const bool in_lds = RT == 16 && g.table_lds;
+    // LDS: the table (of more than 4 rows), which the sums of the outputs take over, each wave's V, what the waves exchange
+    const bool in_lds = RT >= 8 && g.table_lds;
     constexpr int ACC_BYTES = (8 * QC * RT * PG_ACC + 1023) / 1024 * 1024;
     const int table_bytes = in_lds ? 1024 * ((g.exp_len + 255) / 256) : 0;
     const int top = table_bytes > ACC_BYTES ? table_bytes : ACC_BYTES;
@@ -388,8 +410,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
     }
     B.until(g, pl, T.h, k1, lane);
     auto mine = [&](int j) { return B.key_of(j) < k1; };  // uniform
-    const int row = RT == 16 ? ql : ql & 3, near = row < T.live ? row : T.live - 1;  // rows that are not there: as the last one
-    v4i D[NB][TU], vr[KD][4], qf[RT == 16 ? 1 : 4][QC];
+    const int row = ql % RT, near = row < T.live ? row : T.live - 1;  // rows that are not there: as the last one
+    v4i D[NB][TU], vr[KD][4], qf[16 / RT][QC];
     // all loads without a branch around them, so that the waits count them exactly
     v4i kr[KD][4][QC];
 #pragma unroll
@@ -417,7 +439,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
     auto all = [&](int j) { return B.key_of(j) + 64 <= most && ((B.there >> (4 * j)) & 15) == 15; };  // uniform
     const int sees = T.before + pl.by_group.of(T.row0 + near) + 1, lim = sees < k1 ? sees : k1;
     auto seen = [&](int j, int u) {  // how many of the lane's four keys
-        const int t = RT == 16 ? u : ql >> 2;
+        const int t = 16 / RT * u + ql / RT;
         return B.has(j, t) ? lim - (B.key_of(j) + 16 * t + 4 * qg) : 0;
     };
     const PagedRule<HI> rule(g);
@@ -442,7 +464,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
         }
     }
 #pragma unroll
-    for (int o = RT == 16 ? 16 : 4; o < 64; o <<= 1) {  // the lanes of the row
+    for (int o = RT; o < 64; o <<= 1) {  // the lanes of the row
         const Score x = __shfl_xor(mx, o, 64);
         mx = x > mx ? x : mx;
     }
@@ -493,7 +515,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
             sum += (uint64_t)((uint32_t)D[j][u][0] + (uint32_t)D[j][u][1]) + ((uint32_t)D[j][u][2] + (uint32_t)D[j][u][3]);
     }
 #pragma unroll
-    for (int o = RT == 16 ? 16 : 4; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+    for (int o = RT; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
     if (lane < RT) s_sum[w * RT + lane] = sum;
     lds_barrier();
     sum = 0;
@@ -556,7 +578,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QC == 4 ? 2
     const int row = RT == 16 ? ql : ql & 3, near = row < T.live ? row : T.live - 1;
     const PagedScratch S = paged_scratch(scratch, pl, g.pages.hd);
     constexpr int KD = QC == 1 ? 3 : 2;  // blocks of K in flight, with the one at work
-    v4i x[KD][4][QC], qf[RT == 16 ? 1 : 4][QC];
+    v4i x[KD][4][QC], qf[16 / RT][QC];
 #pragma unroll
     for (int j = 0; j + 1 < KD; j++) paged_k<QC>(g, B, j, lane, x[j]);
     paged_q<RT, QC>(g, pl, T, 0, lane, qf);
@@ -1054,10 +1076,10 @@ static PagedPlan paged_plan(const PagedArgs &g) {
     // write and read the scores too, but spread a panel over the chip. In us, one launch and several: 768 panels of 8,192 keys 117
     // and 155, 12 panels 27 and 36; of 16,000 keys 768 panels 238 and 290, 200 panels 71 and 89, 48 panels 50 and 34. 16 rows
     // (8 query heads of 128 channels, 128 panels of 2,000 keys) 25 and 38.
-    const int most = rows > 4 ? 2048 : g.pages.hd > 128 ? 4096 : g.pages.hd > 64 || p.panels < 128 ? 8192 : 16384;
+    const int most = rows > 8 || (rows > 4 && g.pages.hd > 128) ? 2048 : rows > 4 ? 4096 : g.pages.hd > 128 ? 4096 : g.pages.hd > 64 || p.panels < 128 ? 8192 : 16384;
     // 64 rows: 16 streams of 64 rows over 4,096 keys 100 us, in tiles of 16 rows 155. 4 rows: a row of 1,000 keys 9.2 us, as one
     // of 16 rows 12.2 (768 panels 20.5 and 23.8).
-    p.rt = rows <= 4 ? 4 : (rows > 16 && g.keys > most ? 64 : 16);
+    p.rt = rows <= 4 ? 4 : rows <= 8 && g.keys <= most ? 8 : rows <= 16 || g.keys <= most ? 16 : 64;
     p.rows = rows < p.rt ? (int)rows : p.rt;
     p.tiles = (int)((rows + p.rt - 1) / p.rt);
     while (1 << p.page_log < g.pages.page) p.page_log++;
@@ -1106,7 +1128,7 @@ size_t paged_workspace(const PagedArgs &g) {
 template <int RT, int QC, int NB, int NW, bool HI>
 static hipError_t launch_paged_t(const PagedArgs &g, const PagedPlan &p, hipStream_t stream) {
     const int acc = (8 * QC * RT * PG_ACC + 1023) / 1024 * 1024;
-    const int table = RT == 16 && g.table_lds ? 1024 * ((g.exp_len + 255) / 256) : 0;
+    const int table = RT >= 8 && g.table_lds ? 1024 * ((g.exp_len + 255) / 256) : 0;
     const size_t lds = (size_t)(table > acc ? table : acc) + 4096 * NW + 16 * NW * RT;
     const hipError_t e = allow_dynamic_lds((const void *)k_paged_tile<RT, QC, NB, NW, HI>, lds);
     if (e != hipSuccess) return e;
@@ -1116,7 +1138,7 @@ static hipError_t launch_paged_t(const PagedArgs &g, const PagedPlan &p, hipStre
 
 template <int RT, int QC, bool HI>
 static hipError_t launch_paged_q(const PagedArgs &g, const PagedPlan &p, void *scratch, hipStream_t stream) {
-    if (p.split) {
+    if constexpr (RT != 8) if (p.split) {
         hipError_t e;
         const unsigned grid = (unsigned)((p.panels + 7) / 8 * 8) * p.tiles * p.ng;
         const size_t table = g.table_lds ? (size_t)1024 * ((g.exp_len + 255) / 256) : 0;
@@ -1146,11 +1168,12 @@ static hipError_t launch_paged_q(const PagedArgs &g, const PagedPlan &p, void *s
     // 37.9 us, in one of 16 waves 46.0; 4,096 keys 62.8 and 70.2, and with 128 channels 166 and 141, where eight blocks spill).
     if (p.span <= 256) return launch_paged_t<RT, QC, 1, 4, HI>(g, p, stream);
     if (p.span <= 1024) {
-        if constexpr (RT == 4)
+        if constexpr (RT <= 8)
             if (p.panels <= 256) return launch_paged_t<RT, QC, 1, 16, HI>(g, p, stream);
         return launch_paged_t<RT, QC, 4, 4, HI>(g, p, stream);
     }
     if (p.span <= 2048) return launch_paged_t<RT, QC, 4, 8, HI>(g, p, stream);
+    if constexpr (RT == 8 && QC <= 2) return launch_paged_t<RT, QC, 4, 16, HI>(g, p, stream);
     if constexpr (RT == 4) {
         if (p.span <= 4096) return launch_paged_t<RT, QC, QC == 2 ? 4 : 8, QC == 2 ? 16 : 8, HI>(g, p, stream);
         if constexpr (QC <= 2)
@@ -1172,7 +1195,7 @@ hipError_t launch_paged(const PagedArgs &args, void *workspace, hipStream_t stre
     PagedArgs g = args;
     g.table_lds = g.exp_len <= PG_TABLE && (uintptr_t)g.exp_table % 16 == 0;
     const PagedPlan p = paged_plan(g);
-    return p.rt == 4 ? launch_paged_r<4>(g, p, workspace, stream) : launch_paged_r<16>(g, p, workspace, stream);
+    return p.rt == 4 ? launch_paged_r<4>(g, p, workspace, stream) : p.rt == 8 ? launch_paged_r<8>(g, p, workspace, stream) : launch_paged_r<16>(g, p, workspace, stream);
 }
 
 }  // namespace hs

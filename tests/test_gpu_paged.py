@@ -183,6 +183,16 @@ def test_long_caches_with_wide_scores(gpu, t, heads):
     check_attend(gpu, 64, 1, 2, 2, 64, 64, 9000, [9000, 8192, 5, 100], rule=(33_000_000, 20, 1_300_000_000, 56, 24))
 
 
+@pytest.mark.parametrize("hd", [64, 112, 256])
+@pytest.mark.parametrize("keys", [70, 1000, 2049, 4096, 4097])
+def test_five_to_eight_rows(gpu, hd, keys):
+    """Two groups of keys share an accumulator."""
+    check_attend(gpu, 3, 1, 16, 2, hd, 64, keys, [keys, keys // 2, 3], holes=0.1, seed=keys)
+    check_attend(gpu, 3, 5, 2, 2, hd, 16, keys, [keys, keys - 3, 3], [5, 4, 5], seed=hd)
+    check_attend(gpu, 2, 3, 4, 2, hd, 32, keys, [keys, 2], rule=(33_000_000, 20, 1_300_000_000, 56, 24), exp=np.resize(TABLE, 20_000))
+    check_attend(gpu, 2, 7, 2, 2, hd, 32, keys, [keys, 7], [7, 0])
+
+
 @pytest.mark.parametrize("hd", [128, 256])
 def test_long_caches_of_wide_heads(gpu, hd):
     for t in (1, 20):

@@ -75,7 +75,8 @@ class Step:
 
 # one launch of 4 and of 16 rows, launches that keep the scores (8 rows; 1 row past 8,192 keys), three walks
 SHAPES = [(2, 1, 3, 3, 64, 16, 20, 300), (2, 7, 4, 2, 64, 32, 16, 300), (2, 1, 16, 2, 128, 64, 40, 2200),
-          (1, 1, 2, 2, 64, 128, 66, 8300), (2, 20, 3, 3, 64, 64, 44, 2500)]
+          (1, 1, 2, 2, 64, 128, 66, 8300), (2, 20, 3, 3, 64, 64, 44, 2500),
+          (2, 1, 16, 2, 128, 64, 70, 4200)]
 
 
 @pytest.mark.parametrize("shape", SHAPES)
@@ -162,7 +163,7 @@ def test_streams_that_share_pages(gpu):
 def test_workspaces(gpu):
     """One that is too small or not aligned is refused, and so is a captured call without one."""
     rt, hip = runtime(), gpu.hip
-    s, stream = Step(gpu, 9, *SHAPES[2]), Stream(rt)
+    s, stream = Step(gpu, 9, *SHAPES[3]), Stream(rt)
     b, t, heads, width = s.dims
     assert s.need > 0
     call = lambda **kw: hip.attend_paged(gpu.dev, s.cache, s.d["q"], s.d["table"], s.d_counts[0], None,  # noqa: E731
