@@ -371,7 +371,12 @@ __device__ __forceinline__ void paged_put(const PagedArgs &g, const PagedPlan &p
 // row r with group t: the products of the four groups add up in one accumulator, each with q in its own columns and
 // zeros in the others, so that no lane idles; the product with V takes the rows' four digit planes as its 16 columns. With 8
 // rows two groups share an accumulator and two planes a product.
-// All in one launch, the dots in registers from the one product to the other.
+// What bounds it: one row, HBM (768 panels of 64 channels: 512 to 1,024 keys 76 MB in 19.3 us, 4,096 to 8,192 keys 605 MB in 117,
+// 5.2 TB/s). Few panels, what one CU reads, some 30 KB a us (12 panels of 4,096 to 8,192 keys 27 us; 128 of 2,000 to 4,000 keys
+// with 128 channels and 8 rows 42). Many rows, VALU issue: 192 panels of 256 causal rows over 512 to 1,024 keys, 16.5 M instructions, 27 us of 50.
+// All in one launch, the dots in registers from the one product to the other: the rule needs the row's largest score and its sum
+// before a weight, and forming the dots again would read K again. The table goes to LDS for more than 4 rows; for few rows the
+// lookups are fewer than its entries.
 template <int RT, int QC, int NB, int NW, bool HI>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 || (RT <= 8 && NW == 8 && QC <= 2) ? 4 : QC == 1 && RT == 16 ? 3 : 2))) void k_paged_tile(PagedArgs g, PagedPlan pl) {
     static_assert(NB <= 16, "a lane for each group of the wave's blocks");
@@ -557,7 +562,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
 // ---- Ranges that leave their scores in the scratch ------------------------------------------------------
 // Three launches and a join: the scores of every key (K once), their entries and sums, the products with V (V once). Four waves
 // walk a range's blocks, at most 16 each, with the next blocks' loads under way; what a workgroup has to find out first (counts,
-// pages, scales) is spread over up to 4,096 keys.
+// pages, scales) is spread over up to 4,096 keys. For one row the scratch is 8 (i32) of 136 bytes a key; HBM bounds scores and
+// products: 200 panels of 8,192 to 16,384 keys (which one launch takes now), 158 MB each, 35 and 38 us (4.5 and 4.1 TB/s), the
+// entries between them 8.6, the join 5.
 template <int RT, int QC, bool HI>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QC == 4 ? 2 : 4))) void k_paged_scores(PagedArgs g, PagedPlan pl, void *scratch) {
     typedef typename std::conditional<HI, int32_t, int64_t>::type Score;
@@ -728,7 +735,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RT == 16 &&
 // less than keeping 16 scores a key and tile would cost): the largest scores, the sums of the entries, the products with V.
 // In the first two a wave takes blocks of keys with all four tiles, so that the four waves' loads are of different keys; in
 // the third a wave takes a tile over all blocks, since a tile's sums are 64 registers for 64 channels (the waves' loads of
-// the same rows meet in the L1).
+// the same rows meet in the L1). VALU issue bounds them, and few workgroups where there are few panels: 192 panels of 64 rows over
+// 2,048 to 4,096 keys 100 us (38 M scores), 12 panels of 256 rows over 16,000 keys 157.
 template <int QC, bool HI, int PHASE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QC == 4 ? 2 : 3))) void k_paged_scan(PagedArgs g, PagedPlan pl, void *scratch) {
     extern __shared__ __attribute__((aligned(1024))) int32_t s_exp[];  // the table
@@ -1073,7 +1081,8 @@ static PagedPlan paged_plan(const PagedArgs &g) {
     const long long rows = (long long)g.t * p.group;
     p.panels = g.streams * g.pages.kv_heads;
     // Keys of a tile in one launch, whose dots fit the registers of its waves. It reads K and V and nothing else; several launches
-    // write and read the scores too, but spread a panel over the chip. In us, one launch and several: 768 panels of 8,192 keys 117
+    // write and read the scores too, but spread a panel over the chip. In us, one launch and several, with three quarters of the
+    // keys there in the mean: 768 panels of 8,192 keys 117
     // and 155, 12 panels 27 and 36; of 16,000 keys 768 panels 238 and 290, 200 panels 71 and 89, 48 panels 50 and 34. 16 rows
     // (8 query heads of 128 channels, 128 panels of 2,000 keys) 25 and 38.
     const int most = rows > 8 || (rows > 4 && g.pages.hd > 128) ? 2048 : rows > 4 ? 4096 : g.pages.hd > 128 ? 4096 : g.pages.hd > 64 || p.panels < 128 ? 8192 : 16384;
@@ -1162,7 +1171,7 @@ static hipError_t launch_paged_q(const PagedArgs &g, const PagedPlan &p, void *s
         const size_t quads = (size_t)p.panels * p.tiles * p.rows * (g.pages.hd / 4);
         return run(k_paged_out, dim3((unsigned)((quads + 255) / 256)), 0);
     }
-    // Blocks a wave and waves, by the keys a call may read. One row a panel: a workgroup a CU and less takes 16 waves, whose
+    // Blocks a wave and waves, by the keys a call may read (three quarters of them there in the mean of these figures). One row a panel: a workgroup a CU and less takes 16 waves, whose
     // chains are short (12 panels of 1,000 keys 8.6 us, in four waves 9.3); 768 panels one round of three workgroups a CU (18.9
     // us at 1,024 keys); more keys two workgroups of eight waves a CU, one at its loads while the other works (2,048 keys
     // 37.9 us, in one of 16 waves 46.0; 4,096 keys 62.8 and 70.2, and with 128 channels 166 and 141, where eight blocks spill).

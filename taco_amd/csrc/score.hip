@@ -92,7 +92,8 @@ __device__ __forceinline__ void search_top(const ScoreArgs &a, size_t r, int64_t
 }
 
 // A row by itself, any vocabulary and table: the workgroup walks it for the row max, the sum, the entropy and the rank,
-// and for the alternatives.
+// and once for each alternative. The table's entries come from the L2, a symbol at a time: 64 rows of 50,257 symbols, 8 alternatives
+// and 20,000 entries 272 us, where the histogram of shorter tables takes 18.6.
 template <int SRC, int NW>
 __device__ __forceinline__ void score_any_row(const ScoreArgs &a, size_t r, void *slots) {
     const int tid = threadIdx.x, V = a.vocab, NT = 64 * NW;
@@ -139,6 +140,9 @@ __global__ __launch_bounds__(512) void k_score_any(ScoreArgs a) {
 // collected and ranked against each other.
 // G > 0: the row is read once, G groups at most, and its indexes stay in registers, 16 bits each. G = 0, longer rows: read for
 // the max, for the counts, and once each for ties and alternatives.
+// HBM bounds many rows: 4,096 x 50,257 i32 logits, 823 MB in 181 us, 4.6 TB/s, with 53 us of LDS work (counting: over half of it
+// waits for a bank) and 79 of VALU issue beside the loads of the other workgroup of a CU. Few rows are a chain: the loads, the
+// largest, the counts, the sums, the alternatives: one row 17 us, 64 rows 17.6.
 constexpr int SCORE_LIST = 1024;   // symbols collected; where ties make them more, the alternatives are searched one by one
 constexpr int SCORE_BINS = 16384;  // entries of the table at most
 
@@ -552,13 +556,17 @@ static hipError_t launch_score_rows(const ScoreArgs &a, int n_rows, hipStream_t 
 template <int SRC>
 static hipError_t launch_score_src(const ScoreArgs &a, int n_rows, hipStream_t stream) {
     if (a.table_len <= SCORE_BINS) {
+        // As many waves as the row has groups for, in us: 3,001 rows of 299 symbols by one wave 13.6, by eight 63; 512 rows of
+        // 16,000 by eight 19.8, by sixteen 31.8. Rows of 50,257: more rows than CUs share them, one workgroup at its loads while
+        // another counts (4,096 rows: 26 groups of eight waves 181, 13 of sixteen 251; 512 rows 35.9 and 42.4), fewer take a CU
+        // each (64 rows 18.6 and 21); i64 groups are twice the loads, and 26 of them do not fit the registers. The walk takes 451
+        // for the 4,096 rows, and 120 for 512 of i64 (74).
         const int v = a.vocab + 3;  // with the part of 16 bytes before a row
         if (v <= 4 * 64 * 4) return launch_score_rows<SRC, 4, 1>(a, n_rows, stream);
         if (v <= 4 * 512 * 8) return launch_score_rows<SRC, 8, 8>(a, n_rows, stream);
         if constexpr (SRC == SCORE_I64) {
             if (v <= 4 * 1024 * 13) return launch_score_rows<SRC, 13, 16>(a, n_rows, stream);
         } else {
-            // a row a CU: 64 rows 18 us (26 groups of 8 waves 21); more rows share a CU, one at its loads while another counts
             if (n_rows <= 256 && v <= 4 * 1024 * 13) return launch_score_rows<SRC, SRC == SCORE_COMPACT ? 14 : 13, 16>(a, n_rows, stream);
             if (v <= 4 * 512 * 26) return launch_score_rows<SRC, 26, 8>(a, n_rows, stream);
         }
