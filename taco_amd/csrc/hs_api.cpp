@@ -1669,8 +1669,10 @@ extern "C" hs_status hs_batch_run_scored(hs_batch *b, const hs_input *in, const 
     hs::clear_error();
     HS_TRY(check_inputs(b, in, n));
     const Scoring sc{tokens, top, logprob, rank, entropy, top_tokens, top_logprob};
-    HS_TRY(plan_scores(b, tokens, n, sc));
-    return guarded([&] { return run(b, in, n, Out::Scores, nullptr, 0, nullptr, nullptr, &sc); });
+    return guarded([&]() -> hs_status {
+        HS_TRY(plan_scores(b, tokens, n, sc));
+        return run(b, in, n, Out::Scores, nullptr, 0, nullptr, nullptr, &sc);
+    });
 }
 
 extern "C" hs_status hs_batch_run_tree_scored(hs_batch *b, const hs_input *in, const uint32_t *parents,
@@ -1679,8 +1681,10 @@ extern "C" hs_status hs_batch_run_tree_scored(hs_batch *b, const hs_input *in, c
     hs::clear_error();
     HS_TRY(check_inputs(b, in, n));
     const Scoring sc{tokens, top, logprob, rank, entropy, top_tokens, top_logprob};
-    HS_TRY(plan_scores(b, tokens, n, sc));
-    return guarded([&] { return run_tree(b, in, parents, n, Out::Scores, nullptr, 0, nullptr, &sc); });
+    return guarded([&]() -> hs_status {
+        HS_TRY(plan_scores(b, tokens, n, sc));
+        return run_tree(b, in, parents, n, Out::Scores, nullptr, 0, nullptr, &sc);
+    });
 }
 
 static hs_status commit_paths(hs_batch *b, const uint32_t *slots, const uint32_t *lengths, const uint32_t *paths, size_t n) {
@@ -2362,8 +2366,11 @@ extern "C" hs_status hs_op_attend_paged_dev(hs_device *dev, const hs_pages *cach
     if (len == 0 || len > (size_t)INT32_MAX || score_m < 1 || (int64_t)score_m * cache->max_scale > INT32_MAX || softmax_p + bits > 30)
         return hs::fail(HS_UNSUPPORTED, 0, "len >= 1, 1 <= score_m, score_m max_scale < 2^31 and 2^P max_scale <= 2^30");
     if (b == 0 || t == 0) return HS_OK;
-    const size_t far = (size_t)1 << 46;  // (past any allocation)
-    if (overlap(q, b * t > far / q_stride ? far : b * t * q_stride, out, b * t * h * cache->head_dim))
+    // out may lie between two rows of q, or beside them all
+    const size_t far = (size_t)1 << 46, row = h * cache->head_dim, n = b * t * row;  // far: past any allocation
+    const size_t behind = (size_t)((uintptr_t)out - (uintptr_t)q) % q_stride;
+    if (overlap(q, b * t > far / q_stride ? far : (b * t - 1) * q_stride + row, out, n) &&
+        !((uintptr_t)out > (uintptr_t)q && behind >= row && behind + n <= q_stride))
         return hs::fail(HS_INVALID_ARGUMENT, 0, "out must not overlap q");
     g.q = q; g.q_stride = q_stride; g.table = table; g.ctx = ctx; g.rows = rows;
     g.score_m = score_m; g.score_s = score_s; g.out_m = out_m; g.out_s = out_s;

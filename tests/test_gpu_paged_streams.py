@@ -73,7 +73,7 @@ class Step:
             assert np.array_equal(self.gpu.back(d, x), x)
 
 
-# one launch of 4 and of 16 rows, launches that keep the scores (8 rows; 1 row past 8,192 keys), three walks
+# one launch of 4, 16 and 8 rows, launches that keep the scores (1 row past 8,192 keys), three walks, 8 rows past 4,096 keys
 SHAPES = [(2, 1, 3, 3, 64, 16, 20, 300), (2, 7, 4, 2, 64, 32, 16, 300), (2, 1, 16, 2, 128, 64, 40, 2200),
           (1, 1, 2, 2, 64, 128, 66, 8300), (2, 20, 3, 3, 64, 64, 44, 2500),
           (2, 1, 16, 2, 128, 64, 70, 4200)]

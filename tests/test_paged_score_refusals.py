@@ -112,6 +112,12 @@ def test_attend_refusals():
     attend(BAD, workspace=BASE + 16, workspace_bytes=1 << 40)
     attend(BAD, q=BASE, out=BASE + 1024)                 # 6 rows of 256
     attend(BAD, q=BASE + 1024, out=BASE)
+    attend(BAD, dims=(1, 1, 4, 4, 200), q=BASE, q_stride=4096, out=BASE + 240)
+    # beside q, also in the rest of a wider row or between two: refused for its workspace, which is checked after
+    for kw in (dict(dims=(1, 1, 4, 4, 200), q_stride=4096, out=BASE + 256), dict(q_stride=4096, out=BASE + 256),
+               dict(q_stride=2048, out=BASE + 5 * 2048 + 256)):
+        with pytest.raises(hip.HipError, match="workspace"):
+            attend(workspace=BASE + 16, workspace_bytes=1 << 40, **kw)
     attend(dims=(0, 3, 4, 4, 200))
     attend(dims=(2, 0, 4, 4, 200))
 
