@@ -138,8 +138,10 @@ __global__ __launch_bounds__(512) void k_score_any(ScoreArgs a) {
 // its own, so that no symbol needs a test and none of these many collide. The counts give T, the entropy and the token's
 // rank but for ties; one wave walks them for the index up to which the alternatives lie, and the symbols up to there, few, are
 // collected and ranked against each other.
-// G > 0: the row is read once, G groups at most, and its indexes stay in registers, 16 bits each. G = 0, longer rows: read for
-// the max, for the counts, and once each for ties and alternatives.
+// G > 0: the row is read once, G groups at most, and its indexes stay in registers, 16 bits each. G > 26: the logits do not fit
+// there until the largest is known, so 16 bits of each are kept (NARROW); a row whose largest logit lies too far above that
+// of its first groups for those (65,535 less the table and 64) is scored by itself, as by k_score_any. G = 0, longer
+// rows: read for the max, for the counts, and once each for ties and alternatives.
 // HBM bounds many rows: 4,096 x 50,257 i32 logits, 823 MB in 181 us, 4.6 TB/s, with 53 us of LDS work (counting: over half of it
 // waits for a bank) and 79 of VALU issue beside the loads of the other workgroup of a CU. Few rows are a chain: the loads, the
 // largest, the counts, the sums, the alternatives: one row 17 us, 64 rows 17.6.
@@ -148,7 +150,9 @@ constexpr int SCORE_BINS = 16384;  // entries of the table at most
 
 template <int SRC, int G, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) void k_score_rows(ScoreArgs a) {
-    constexpr int NT = 64 * NW, LIST = NW == 1 ? 256 : SCORE_LIST, GS = G ? G : 1;
+    constexpr int NT = 64 * NW, LIST = NW == 1 ? 256 : SCORE_LIST;
+    constexpr bool NARROW = SRC != SCORE_COMPACT && G > 26;  // the logits themselves do not fit the registers: 16 bits of each
+    constexpr int GS = G && !NARROW ? G : 1;
     extern __shared__ uint32_t s_hist[];  // [table_len + 63]
     __shared__ uint64_t slots[NW], s_sum[NW], s_list[LIST], s_best[64];
     __shared__ double s_ent[NW];
@@ -224,6 +228,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
     };
 
     X x[GS][4];
+    X base = LOW;
+    uint32_t d2[2 * (G ? G : 1)];  // G > 0: the indexes, pairs
     Raw raw[SRC == SCORE_COMPACT ? GS : 1];
     int64_t tile[SRC == SCORE_COMPACT ? GS : 1];
     const int64_t *tm = a.tmax + r * a.ntiles;
@@ -237,6 +243,41 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
             }
         }
         start();
+    } else if constexpr (NARROW) {
+        // The largest logit is not known yet, but no smaller than that of the first groups, M0: what lies last + 64 below M0 or
+        // more is past the table, and the others are kept as their difference to that, where 16 bits hold it.
+        constexpr int B = SRC == SCORE_I32 ? 4 : 2;  // groups in flight, besides those at work
+        Raw y[2][B];
+#pragma unroll
+        for (int i = 0; i < B; i++) fetch(i, y[0][i]);
+        __builtin_amdgcn_sched_barrier(0);
+        start();
+        auto keep = [&](int i, const X (&v)[4]) {
+            uint32_t u[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) u[e] = (uint32_t)(v[e] > base ? v[e] : base) - (uint32_t)base;
+            apart |= ((u[0] | u[1]) | (u[2] | u[3])) >> 16;
+            d2[2 * i] = (u[0] & 0xffffu) | u[1] << 16;
+            d2[2 * i + 1] = (u[2] & 0xffffu) | u[3] << 16;
+            // (hidden from the optimizer: it would put this off and keep the logits)
+            asm volatile("" : "+v"(d2[2 * i]), "+v"(d2[2 * i + 1]), "+v"(apart), "+v"(mx));
+        };
+#pragma unroll
+        for (int i0 = 0; i0 < G; i0 += B) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = i0 + B; i < i0 + 2 * B && i < G; i++) fetch(i, y[(i0 / B + 1) & 1][i - i0 - B]);
+            __builtin_amdgcn_sched_barrier(0);
+            X v[B][4];
+#pragma unroll
+            for (int i = i0; i < i0 + B && i < G; i++) values(i, y[(i0 / B) & 1][i - i0], v[i - i0]);
+            if (i0 == 0) {
+                const X M0 = block_join<NW>(mx, slots, Max());
+                base = M0 > (X)(LOW + last + 64) ? (X)(M0 - last - 64) : LOW;
+            }
+#pragma unroll
+            for (int i = i0; i < i0 + B && i < G; i++) keep(i, v[i - i0]);
+        }
     } else if constexpr (G > 0) {
         constexpr int B = SRC == SCORE_I32 ? G : 4;  // groups in flight, besides those at work (i32: all)
         Raw y[2][B];
@@ -277,7 +318,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
         M = SRC == SCORE_I32 ? (int64_t)mx : (int64_t)((uint64_t)(uint32_t)mx + ref);
     }
     // logits that lie further apart; and a table that is not a model's (the entropy below divides by w0): uniform
-    if (w0 == 0 || (SRC == SCORE_I64 && __syncthreads_or(apart != 0))) {
+    if (w0 == 0 || ((SRC == SCORE_I64 || NARROW) && __syncthreads_or(apart != 0))) {
         score_any_row<SRC, NW>(a, r, slots);
         return;
     }
@@ -316,9 +357,32 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
             for (int e = 0; e < 4; e++) d[e] = inside(symbol(i, e)) ? d[e] : cap;
         }
     };
-    uint32_t d2[2 * GS];  // G > 0: the indexes, pairs
     uint32_t places = 0;  // counted
-    if constexpr (G > 0) {
+    if constexpr (NARROW) {
+        const uint32_t most = (uint32_t)mx - (uint32_t)base;
+#pragma unroll
+        for (int i = 0; i < G; i++) {
+            uint32_t d[4] = {cap, cap, cap, cap};
+            if (i < groups) {  // uniform
+                const uint32_t q[2] = {d2[2 * i], d2[2 * i + 1]};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t u = most - (e & 1 ? q[e >> 1] >> 16 : q[e >> 1] & 0xffffu);
+                    d[e] = u < cap ? u : cap;
+                }
+                if (edge(i)) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) d[e] = inside(symbol(i, e)) ? d[e] : cap;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) atomicAdd(&s_hist[d[e]], 1u);
+            }
+            d2[2 * i] = d[0] | d[1] << 16;
+            d2[2 * i + 1] = d[2] | d[3] << 16;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        places = 4 * NT * groups;
+    } else if constexpr (G > 0) {
 #pragma unroll
         for (int i = 0; i < G; i++) {
             uint32_t d[4];
@@ -560,7 +624,8 @@ static hipError_t launch_score_src(const ScoreArgs &a, int n_rows, hipStream_t s
         // 16,000 by eight 19.8, by sixteen 31.8. Rows of 50,257: more rows than CUs share them, one workgroup at its loads while
         // another counts (4,096 rows: 26 groups of eight waves 181, 13 of sixteen 251; 512 rows 35.9 and 42.4), fewer take a CU
         // each (64 rows 18.6 and 21); i64 groups are twice the loads, and 26 of them do not fit the registers. The walk takes 451
-        // for the 4,096 rows, and 120 for 512 of i64 (74).
+        // for the 4,096 rows, and 120 for 512 of i64 (74). Longer rows in 16 bits each, and walked: 512 of 131,072 103 and 163,
+        // 1,024 of 60,000 i64 183 and 264, one of 131,072 27 and 34.
         const int v = a.vocab + 3;  // with the part of 16 bytes before a row
         if (v <= 4 * 64 * 4) return launch_score_rows<SRC, 4, 1>(a, n_rows, stream);
         if (v <= 4 * 512 * 8) return launch_score_rows<SRC, 8, 8>(a, n_rows, stream);
@@ -570,6 +635,8 @@ static hipError_t launch_score_src(const ScoreArgs &a, int n_rows, hipStream_t s
             if (n_rows <= 256 && v <= 4 * 1024 * 13) return launch_score_rows<SRC, SRC == SCORE_COMPACT ? 14 : 13, 16>(a, n_rows, stream);
             if (v <= 4 * 512 * 26) return launch_score_rows<SRC, 26, 8>(a, n_rows, stream);
         }
+        if constexpr (SRC != SCORE_COMPACT)
+            if (v <= 4 * 1024 * 33) return launch_score_rows<SRC, 33, 16>(a, n_rows, stream);
         return launch_score_rows<SRC, 0, 16>(a, n_rows, stream);
     }
     launch_k(k_score_any<SRC>, dim3(n_rows), dim3(512), 0, stream, a);

@@ -79,6 +79,29 @@ def test_ties(gpu):
         check(gpu, logits, WEIGHTS, [0, vocab - 1, 77, vocab - 2, vocab // 2], 64)
 
 
+@pytest.mark.parametrize("dtype", [np.int32, np.int64])
+@pytest.mark.parametrize("vocab,pad", [(53_250, 0), (99_999, 1), (135_165, 2), (135_172, 0)])
+def test_long_rows(gpu, vocab, pad, dtype):
+    """Rows whose symbols are held in 16 bits each, relative to the largest of the first ones: further ones far above it,
+    by as much as that holds and by more, the least numbers there are, and the largest as the last."""
+    r = np.random.default_rng(vocab)
+    low = np.iinfo(np.int32).min
+    logits = normal(r, 9, vocab, np.int64)
+    logits[1, vocab - 1] = 20_000
+    logits[2, 40_000:] += 40_000
+    top = logits[3, :16_384].max()                      # (the first groups are at least these symbols' part)
+    logits[3, 50_000] = top + 65_535 - len(WEIGHTS) - 63
+    logits[4, 50_000:50_010] = 70_000 + np.arange(10)   # past it
+    logits[5] += low + 4000                             # the table reaches below the least number
+    logits[5] = np.maximum(logits[5], low)
+    logits[6] = low
+    logits[6, 52_000] = low + 100
+    logits[7] = r.integers(low, -low, vocab)
+    logits[8, ::3] = low
+    check(gpu, logits.astype(dtype), WEIGHTS, r.integers(0, vocab, 9), 8, pad)
+    check(gpu, logits.astype(dtype), WEIGHTS[:16], None, 1, pad)
+
+
 def test_more_ties_than_a_list(gpu):
     """Thousands of equal symbols at the border of the alternatives, some before them, and past the table's end; the token
     one of them."""
