@@ -1102,12 +1102,12 @@ static PagedPlan paged_plan(const PagedArgs &g) {
             p.span = (int)(((g.keys + ng - 1) / ng + 255) / 256) * 256;
             p.ng = (g.keys + p.span - 1) / p.span;
         };
-        // workgroups in all, of 512, 768, 1,024, 2,048 and 3,072, in us of the scores' launch and the products':
+        // workgroups for each of 256 CUs, of 2, 3, 4, 8 and 12, in us of the scores' launch and the products':
         //   200 panels of one row, 8,192 to 16,384 keys     41 + 41   41 + 41   40 + 41   38 + 38   36 + 39
         //   128 panels of eight rows, 128 channels, 4,000   15 + 17   17 + 23   15 + 22   17 + 30   17 + 30
-        if (p.rt == 4) ranges(1024, 3072);
-        else if (p.rt == 16) ranges(512, 512);
-        else ranges(512, 1024);
+        if (p.rt == 4) ranges(1024, 12 * 256);
+        else if (p.rt == 16) ranges(512, 2 * 256);
+        else ranges(512, 4 * 256);
         p.store = p.rt < 64;
         p.split = 1;
         p.chunks = p.store ? (g.keys + PG_CHUNK - 1) / PG_CHUNK : p.ng;
