@@ -180,13 +180,17 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
         return SRC == SCORE_COMPACT ? 8 * NT * ((i >> 1) + 1) > V : (i == 0 && off > 0) || 4 * NT * (i + 1) > V + off;
     };
     typedef typename std::conditional<SRC == SCORE_I64, v4i[2], typename std::conditional<SRC == SCORE_I32, v4i[1], v2i[1]>::type>::type Raw;
+    // Groups past the row are loaded too (zeros without an access): the place in the lane's offset, which the descriptor's end
+    // bounds. A scalar offset is not part of that check.
+    int place = SRC == SCORE_COMPACT ? 16 * tid : 4 * E * tid;
+    if constexpr (SRC == SCORE_COMPACT) asm volatile("" : "+v"(place));  // (hidden from the optimizer: it would keep all groups' places)
     auto fetch = [&](int i, Raw &y) {
         if constexpr (SRC == SCORE_COMPACT) {
-            y[0] = __builtin_bit_cast(v2i, __builtin_amdgcn_raw_buffer_load_b64(from, 16 * tid + 8 * (i & 1), 16 * NT * (i >> 1), 0));
+            y[0] = __builtin_bit_cast(v2i, __builtin_amdgcn_raw_buffer_load_b64(from, place + 16 * NT * (i >> 1) + 8 * (i & 1), 0, 0));
         } else {
 #pragma unroll
             for (int k = 0; k < E / 4; k++)
-                y[k] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(from, 4 * E * tid + 16 * k, 4 * E * NT * i, 0));
+                y[k] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(from, place + 4 * E * NT * i + 16 * k, 0, 0));
         }
     };
     uint64_t ref = 0;
