@@ -9,6 +9,13 @@ namespace hs {
 
 constexpr int64_t SCORE_LIMIT = (int64_t)1 << 40;  // gpt2/mod.rs:119
 
+// A table that the waves copied to LDS straight is there for the whole workgroup. Such loads are no LDS operations to a barrier, which
+// waits for those alone (lgkmcnt): each wave waits for its own.
+__device__ __forceinline__ void table_there() {
+    wait_vmcnt<0>();
+    __syncthreads();
+}
+
 // ---- wave reductions (wave64) -------------------------------------------------------------
 
 __device__ __forceinline__ int64_t wave_max64(int64_t v) {

@@ -86,7 +86,8 @@ struct PagedRule {
     }
 };
 
-// The table to LDS: whole KiB straight, the rest entry by entry (places past it repeat the last one). The caller waits.
+// The table to LDS: whole KiB straight, the rest entry by entry (places past it repeat the last one). The caller waits: the straight
+// loads are no LDS operations to a barrier, so each wave waits for its own (table_there, or for loads issued after them).
 __device__ __forceinline__ void paged_table(const PagedArgs &g, int32_t *s_exp, int w, int waves, int lane) {
     w = __builtin_amdgcn_readfirstlane(w);
     for (int ch = w; ch < g.exp_len / 256; ch += waves)
@@ -474,8 +475,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 8 
         mx = x > mx ? x : mx;
     }
     if (lane < RT) s_mx[w * RT + lane] = mx == LOW ? INT64_MIN : (int64_t)mx;
-    if (!mine(0)) wait_vmcnt<0>();  // (no K to wait for)
-    lds_barrier();                  // not the fence of __syncthreads, which would wait for V too
+    if (!mine(0)) wait_vmcnt<0>();  // (no K to wait for, whose loads are behind the table's)
+    lds_barrier();                  // (V stays in flight)
     int64_t M = INT64_MIN;
 #pragma unroll
     for (int i = 0; i < NW; i++) M = s_mx[i * RT + row] > M ? s_mx[i * RT + row] : M;
@@ -779,7 +780,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QC == 4 ? 2
         }
     }
     const uint32_t last = (uint32_t)g.exp_len - 1;
-    if constexpr (PHASE == 2) __syncthreads();  // the table
+    if constexpr (PHASE == 2) table_there();
     for (int j = 0; B.key_of(j) < k1; j++) {
         const int key = B.key_of(j);
         const bool pages = ((B.there >> (4 * j)) & 15) == 15;
@@ -893,7 +894,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QC == 1 ? 3
     for (int k = 0; k < 4; k++)
 #pragma unroll
         for (int i = 0; i < 4; i++) acc[k][i] = v4i{0, 0, 0, 0};
-    __syncthreads();  // the table
+    table_there();
     for (int b0 = k0; b0 < k1; b0 += 1024) {  // 16 blocks with one look at the pages
         PagedBlocks B(g, pl, T.s, b0, 64, 16, lane);
         const int e1 = b0 + 1024 < k1 ? b0 + 1024 : k1;
@@ -1013,7 +1014,7 @@ __global__ __launch_bounds__(256) void k_paged_entries(PagedArgs g, PagedPlan pl
         else d = (uint64_t)(M - x[i]) < last ? (uint32_t)(M - x[i]) : last;
         y[i] = (int32_t)(d < last ? d : last);
     }
-    __syncthreads();  // the table
+    table_there();
     if (g.table_lds) {
 #pragma unroll
         for (int i = 0; i < N; i++) y[i] = s_exp[y[i]];

@@ -1,6 +1,7 @@
 """Rules of the kernels' sources whose breach no result shows: read from the files, without a GPU."""
 
 import os
+import re
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "taco_amd", "csrc")
 
@@ -39,3 +40,18 @@ def test_places_past_a_descriptor_lie_in_the_lanes_offset():
             seen += 1
             assert args[2] == "0" or args[2] in kept, (name, args)
     assert seen >= 4
+
+
+def test_tables_are_waited_for():
+    """A kernel that copies its table to LDS straight waits for its own loads right before a barrier; the barrier itself waits
+    for LDS operations, which these loads are not."""
+    there = re.compile(r"\btable_there\(\)|wait_vmcnt<0>\(\);[^\n]*\n\s*(__syncthreads|lds_barrier)\(\)")
+    assert there.search(sources()["attend.h"])
+    kernels = 0
+    for body in re.split(r"\n__global__|\ntemplate <", sources()["attend_paged.hip"]):
+        at = re.search(r"\bpaged_table\((?!const)", body)
+        if at:
+            kernels += 1
+            assert there.search(body, at.end()), body[:200]
+            assert not re.search(r"__syncthreads\(\);  // the table", body), body[:200]
+    assert kernels == 4
