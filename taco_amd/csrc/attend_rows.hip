@@ -468,8 +468,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         s_mm[w * RT_ROWS + ql] = dmax;
         s_mm[(NW + w) * RT_ROWS + ql] = dmin;
     }
-    if (!mine(0)) wait_vmcnt<0>();  // (no K to wait for)
-    lds_barrier();                  // not the fence of __syncthreads, which would wait for V too
+    if (!mine(0)) wait_vmcnt<0>();  // (no K to wait for, whose loads are behind the table's)
+    lds_barrier();                  // (V stays in flight)
 #pragma unroll
     for (int i = 0; i < NW; i++) {
         const int32_t x = s_mm[i * RT_ROWS + ql], y = s_mm[(NW + i) * RT_ROWS + ql];
@@ -671,7 +671,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     if constexpr (PHASE == 2) {
 #pragma unroll
         for (int u = 0; u < WT; u++) index[u] = RowIndex<HI>(a, dmax[u], dmin[u]).c;
-        __syncthreads();  // the table
+        table_there();
     }
     typedef v4i KRows[4][QC];
     int kb = k0 / 64 + w;
@@ -857,7 +857,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QC == 1 ? 3
         }
     }
     const RowIndex<HI> ix(a, dmax, dmin);
-    __syncthreads();  // the table
+    table_there();
     uint64_t sum = 0;
     if constexpr (ALONE) {
         walk([&](int, v4i (&D)[4], bool all, uint32_t ok) {

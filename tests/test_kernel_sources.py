@@ -47,11 +47,12 @@ def test_tables_are_waited_for():
     for LDS operations, which these loads are not."""
     there = re.compile(r"\btable_there\(\)|wait_vmcnt<0>\(\);[^\n]*\n\s*(__syncthreads|lds_barrier)\(\)")
     assert there.search(sources()["attend.h"])
-    kernels = 0
-    for body in re.split(r"\n__global__|\ntemplate <", sources()["attend_paged.hip"]):
-        at = re.search(r"\bpaged_table\((?!const)", body)
-        if at:
-            kernels += 1
-            assert there.search(body, at.end()), body[:200]
-            assert not re.search(r"__syncthreads\(\);  // the table", body), body[:200]
-    assert kernels == 4
+    for name, most in (("attend_paged.hip", 4), ("attend_rows.hip", 3)):
+        kernels = 0
+        for body in re.split(r"\n__global__|\ntemplate <", sources()[name]):
+            at = re.search(r"\b(paged|load)_table\((?!const)", body)
+            if at:
+                kernels += 1
+                assert there.search(body, at.end()), body[:200]
+                assert not re.search(r"__syncthreads\(\);  // the table", body), body[:200]
+        assert kernels == most
