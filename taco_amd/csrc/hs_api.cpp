@@ -2269,9 +2269,11 @@ extern "C" hs_status hs_op_cache_commit_dev(hs_device *dev, int8_t *const *k_cac
 
 namespace {
 
+bool paged_head_dim(size_t hd) { return hd > 0 && hd % 16 == 0 && hd <= 256; }
+
 hs_status pool_args(hs_device *dev, const hs_pages *c, hs::PagePool &p) {
     if (!dev || !c || !c->k || !c->v || !c->k_scale || !c->v_scale) return hs::fail(HS_INVALID_ARGUMENT, 0, "NULL argument");
-    if (c->head_dim == 0 || c->head_dim % 16 != 0 || c->head_dim > 256)
+    if (!paged_head_dim(c->head_dim))
         return hs::fail(HS_UNSUPPORTED, 0, "head_dim must be a multiple of 16 in 16..=256");
     if (c->page < 16 || c->page > 1024 || (c->page & (c->page - 1)))
         return hs::fail(HS_UNSUPPORTED, 0, "a page holds a power of two of tokens, 16..=1024");
@@ -2339,7 +2341,7 @@ extern "C" hs_status hs_op_pages_append_dev(hs_device *dev, const hs_pages *cach
 
 extern "C" size_t hs_op_attend_paged_workspace(size_t b, size_t t, size_t h, size_t kv_heads, size_t hd, size_t keys) {
     hs::PagedArgs g;
-    if (b == 0 || t == 0 || h == 0 || kv_heads == 0 || h % kv_heads || hd == 0 || hd > 256 || keys == 0 ||
+    if (b == 0 || t == 0 || h == 0 || kv_heads == 0 || kv_heads > 65535 || h % kv_heads || !paged_head_dim(hd) || keys == 0 ||
         keys > (size_t)1 << 22 || paged_dims(b, t, h, 1, 16) != HS_OK)
         return 0;  // (the call itself refuses them, or does nothing)
     g.streams = (int)b; g.t = (int)t; g.heads = (int)h; g.keys = (int)keys;

@@ -211,3 +211,12 @@ def test_batch_tokens():
         hip.HipBatch._scored(Batch, 3, [1], 2, call)
     with pytest.raises(hip.Unsupported):
         hip.HipBatch._scored(Batch, 3, [1, 2, 3], -1, call)
+
+
+def test_workspaces_of_other_head_dims():
+    """Head dims that the call refuses need no workspace; 1 to 3 once divided by zero."""
+    for hd in (1, 2, 3, 4, 8, 15, 17, 72, 2 ** 32 + 16):
+        for t, keys in ((1, 100), (1, 20_000), (20, 9000)):
+            assert hip.attend_paged_workspace(1, t, 1, 1, hd, keys) == 0, hd
+    assert hip.attend_paged_workspace(1, 1, 1, 1, 16, 20_000) > 0
+    assert hip.attend_paged_workspace(1, 1, 65536, 65536, 16, 20_000) == 0  # heads of the cache that the call refuses
