@@ -491,8 +491,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
     }
     // T and the entropy from the counts, in one pass: with w0 = table[0], the largest weight there is, the entropy
     // sum (w / T) ln(T / w) = ln(T / w0) + (sum w ln(w0 / w)) / T, two terms that are not negative (log_share takes the first,
-    // exact where T is close to w0). In f32 the logarithms of the second are some 2^-22 off, which the first outweighs: it is
-    // at least the share of all symbols but the largest.
+    // exact where T is close to w0). Symbols of weight w0 add exactly nothing to the second; with them left out its error in
+    // f32, some 2^-21 of their weight for each of the others, is outweighed by the first, at least the share of those others.
     const float w0f = (float)w0;
     uint64_t sum = 0;
     float spread = 0;
@@ -510,7 +510,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
             sum += n[k] * z[k];
             const float y = fmaf((float)(uint32_t)(z[k] >> 32), 0x1p32f, (float)(uint32_t)z[k]);
             const float l = __builtin_amdgcn_logf(w0f * __builtin_amdgcn_rcpf(y));
-            spread += z[k] ? (float)n[k] * y * l : 0.0f;
+            spread += z[k] && z[k] != w0 ? (float)n[k] * y * l : 0.0f;
             ahead += d0 + NT * k < td ? n[k] : 0;
         }
     }
