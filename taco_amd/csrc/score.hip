@@ -491,11 +491,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
     }
     // T and the entropy from the counts, in one pass: with w0 = table[0], the largest weight there is, the entropy
     // sum (w / T) ln(T / w) = ln(T / w0) + (sum w ln(w0 / w)) / T, two terms that are not negative (log_share takes the first,
-    // exact where T is close to w0). Symbols of weight w0 add exactly nothing to the second; with them left out its error in
-    // f32, some 2^-21 of their weight for each of the others, is outweighed by the first, at least the share of those others.
+    // exact where T is close to w0). Symbols of weight w0 add exactly nothing to the second. For each of the others the quotient
+    // and its logarithm in f32 are at most 3.5 2^-23 + 2^-23 ln(w0 / w) off, the product with the weight 2^-22 of itself, and
+    // the sum is in f64: some 2^-21 of the entropy in all, since the first term is at least the share of those others.
     const float w0f = (float)w0;
     uint64_t sum = 0;
-    float spread = 0;
+    double spread = 0;
     for (int d0 = tid; d0 <= last; d0 += 8 * NT) {
         uint32_t n[8];
         uint64_t z[8];
@@ -510,11 +511,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
             sum += n[k] * z[k];
             const float y = fmaf((float)(uint32_t)(z[k] >> 32), 0x1p32f, (float)(uint32_t)z[k]);
             const float l = __builtin_amdgcn_logf(w0f * __builtin_amdgcn_rcpf(y));
-            spread += z[k] && z[k] != w0 ? (float)n[k] * y * l : 0.0f;
+            spread += (double)(z[k] && z[k] != w0 ? (float)n[k] * y * l : 0.0f);
             ahead += d0 + NT * k < td ? n[k] : 0;
         }
     }
-    double h = (double)spread * 0.693147180559945309;
+    double h = spread * 0.693147180559945309;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) h += __shfl_xor(h, o, 64);
     sum = wave_sum_dpp(sum);

@@ -61,3 +61,16 @@ def test_through_a_batch(first, monkeypatch):
         share = w.astype(np.float64) / w.sum()
         want.append((share * np.log1p((w.sum() - w).astype(np.float64) / w.astype(np.float64))).sum())
     ref.close(scored.run_scored(inputs).entropy, np.array(want), 8)
+
+
+@pytest.mark.parametrize("weight", [348_605, 2 ** 20 - 1, 10 ** 6 + 3, 77_777])
+@pytest.mark.parametrize("step,most", [(64, 254), (512, 31), (1024, 15)])
+def test_equal_terms_in_one_lane(gpu, step, most, weight):
+    """Many equal terms whose bins lie a workgroup's lanes apart: a sum in 32 bits would round them all the same way."""
+    table = np.full(16_384, weight, np.uint64)
+    table[0] = 2 ** 40
+    for each, far in ((4, 0), (3, 0), (1, 0), (4, 8000), (4, 40_000)):
+        logits = -np.concatenate([[0], np.repeat(step * np.arange(1, most + 1), each)])
+        logits = np.concatenate([logits, np.full(far, -20_000)])  # longer rows, in the forms of more waves
+        check_entropies(gpu, np.resize(logits, (2, len(logits))).astype(np.int32), table)
+        check_entropies(gpu, np.resize(logits, (2, len(logits))).astype(np.int64), table)
