@@ -363,6 +363,18 @@ class Scores(NamedTuple):
     top_logprob: np.ndarray
 
 
+def _whole(tokens, n: int) -> np.ndarray:
+    """The n tokens of a scored call; None is -1."""
+    t = np.asarray(tokens)
+    if t.dtype.kind == "O":
+        t = np.array([-1 if x is None else x for x in t.tolist()], object)
+    if t.dtype.kind not in "iuO":
+        t = t.astype(np.int64)
+    if len(t) != n:
+        raise LengthMismatch(HS_LENGTH_MISMATCH, 0, f"length mismatch: expected {n}, found {len(t)}")
+    return t
+
+
 class HipBatch:
     """CudaBatch (crates/hardshell-cuda/src/batch.rs:237-476)."""
 
@@ -478,11 +490,7 @@ class HipBatch:
             raise Unsupported(HS_UNSUPPORTED, 0, "top is at most 64, and at most the vocabulary")
         t = None
         if tokens is not None:
-            t = np.asarray(tokens)
-            if t.dtype.kind not in "iuO":
-                t = t.astype(np.int64)
-            if len(t) != n:
-                raise LengthMismatch(HS_LENGTH_MISMATCH, 0, f"length mismatch: expected {n}, found {len(t)}")
+            t = _whole(tokens, n)
             # other numbers that 32 bits do not hold become the vocabulary's size, which is no symbol either
             none = (t == -1) | (t == HS_NO_TOKEN)
             t = np.where(none, HS_NO_TOKEN, np.where((t < 0) | (t > self.vocab), self.vocab, t)).astype(np.uint32)
@@ -493,7 +501,7 @@ class HipBatch:
 
     def run_scored(self, inputs, tokens=None, top: int = 0) -> Scores:
         """Runs the inputs and scores what follows each (hs_batch_run_scored): the log probability and rank of
-        tokens[i] (-1 or HS_NO_TOKEN: none), the entropy, and the first `top` alternatives."""
+        tokens[i] (None, -1 or HS_NO_TOKEN: none), the entropy, and the first `top` alternatives."""
         a = _inputs(inputs)
         return self._scored(len(a), tokens, top, lambda t, *out: lib().hs_batch_run_scored(
             self.h, _ptr(a), t, len(a), top, *out))

@@ -220,3 +220,22 @@ def test_workspaces_of_other_head_dims():
             assert hip.attend_paged_workspace(1, t, 1, 1, hd, keys) == 0, hd
     assert hip.attend_paged_workspace(1, 1, 1, 1, 16, 20_000) > 0
     assert hip.attend_paged_workspace(1, 1, 65536, 65536, 16, 20_000) == 0  # heads of the cache that the call refuses
+
+
+def test_batch_tokens_of_other_kinds():
+    """None is no token, alone among others and for every input."""
+    import numpy as np
+
+    class Batch:
+        vocab = 300
+
+    def words(tokens, n):
+        seen = []
+        hip.HipBatch._scored(Batch, n, tokens, 0, lambda t, *out: seen.extend(C.cast(t, C.POINTER(C.c_uint32))[:n]) or 0)
+        return seen
+
+    none = hip.HS_NO_TOKEN
+    assert words([7, None, 2 ** 40, -3], 4) == [7, none, 300, 300]
+    assert words([None, None], 2) == [none, none]
+    assert words(np.array([200, 1], np.uint8), 2) == [200, 1]
+    assert words(np.array([2 ** 64 - 1, 5], np.uint64), 2) == [300, 5]
