@@ -364,15 +364,20 @@ class Scores(NamedTuple):
 
 
 def _whole(tokens, n: int) -> np.ndarray:
-    """The n tokens of a scored call; None is -1."""
+    """The n tokens of a scored call as whole numbers: None is -1, and what is no whole number is refused."""
     t = np.asarray(tokens)
-    if t.dtype.kind == "O":
-        t = np.array([-1 if x is None else x for x in t.tolist()], object)
-    if t.dtype.kind not in "iuO":
-        t = t.astype(np.int64)
     if len(t) != n:
         raise LengthMismatch(HS_LENGTH_MISMATCH, 0, f"length mismatch: expected {n}, found {len(t)}")
-    return t
+    if t.dtype.kind in "iu":
+        return t
+    given = [-1 if x is None else x for x in t.tolist()]
+    try:
+        whole = [int(x) for x in given]
+    except (TypeError, ValueError, OverflowError):
+        whole = None
+    if whole != given:
+        raise Unsupported(HS_UNSUPPORTED, 0, "a scored token that is no whole number")
+    return np.array(whole, object)
 
 
 class HipBatch:
