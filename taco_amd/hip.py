@@ -366,8 +366,9 @@ class Scores(NamedTuple):
 def _whole(tokens, n: int) -> np.ndarray:
     """The n tokens of a scored call as whole numbers: None is -1, and what is no whole number is refused."""
     t = np.asarray(tokens)
-    if len(t) != n:
-        raise LengthMismatch(HS_LENGTH_MISMATCH, 0, f"length mismatch: expected {n}, found {len(t)}")
+    if t.shape not in ((n,), (n, 1)):
+        raise LengthMismatch(HS_LENGTH_MISMATCH, 0, f"length mismatch: expected {n}, found {' x '.join(map(str, t.shape)) or 'one'}")
+    t = t.reshape(n)
     if t.dtype.kind in "iu":
         return t
     given = [-1 if x is None else x for x in t.tolist()]

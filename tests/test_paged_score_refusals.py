@@ -224,7 +224,7 @@ def test_workspaces_of_other_head_dims():
 
 def test_batch_tokens_of_other_kinds():
     """None is no token, alone among others and for every input; whole numbers of other types are themselves; what is no whole
-    number is refused."""
+    number, and an array of another shape, is refused."""
     import numpy as np
 
     class Batch:
@@ -239,8 +239,11 @@ def test_batch_tokens_of_other_kinds():
     assert words([7, None, 2 ** 40, -3], 4) == [7, none, 300, 300]
     assert words([None, None], 2) == [none, none]
     assert words([3.0, 4.0], 2) == [3, 4] and words([3.0, None], 2) == [3, none]
-    assert words(np.array([200, 1], np.uint8), 2) == [200, 1]
-    assert words(np.array([2 ** 64 - 1, 5], np.uint64), 2) == [300, 5]
+    assert words(np.array([[5], [6]]), 2) == [5, 6] and words(np.array([200, 1], np.uint8), 2) == [200, 1]
+    assert words(np.array([2 ** 64 - 1, 5], np.uint64), 2) == [300, 5] and words([], 0) == []
     for bad in ([5.7, 1], [float("nan"), 1], [float("inf"), 1], [None, 0.5], ["5", "6"], [1j, 2]):
         with pytest.raises(hip.Unsupported):
+            words(bad, 2)
+    for bad in (np.zeros((2, 3), int), np.zeros((1, 2), int), np.zeros((2, 1, 1), int), 5, [1, 2, 3], [None]):
+        with pytest.raises(hip.LengthMismatch):
             words(bad, 2)
