@@ -492,7 +492,7 @@ class HipBatch:
         return out
 
     def _scored(self, n: int, tokens, top: int, call) -> Scores:
-        if not 0 <= top < 2 ** 31:
+        if not 0 <= top <= 64:
             raise Unsupported(HS_UNSUPPORTED, 0, "top is at most 64, and at most the vocabulary")
         t = None
         if tokens is not None:

@@ -247,3 +247,16 @@ def test_batch_tokens_of_other_kinds():
     for bad in (np.zeros((2, 3), int), np.zeros((1, 2), int), np.zeros((2, 1, 1), int), 5, [1, 2, 3], [None]):
         with pytest.raises(hip.LengthMismatch):
             words(bad, 2)
+
+
+def test_batch_alternatives():
+    """More than 64 alternatives are refused before arrays of their size are made."""
+    class Batch:
+        vocab = 2 ** 20
+
+    def call(*args):
+        raise AssertionError("the library is called")
+
+    for top in (65, 2 ** 31 - 1, 2 ** 31, 2 ** 70, -1):
+        with pytest.raises(hip.Unsupported):
+            hip.HipBatch._scored(Batch, 1, None, top, call)
