@@ -1648,6 +1648,20 @@ extern "C" hs_status hs_batch_run_tree_coded(hs_batch *b, const hs_input *in, co
 
 constexpr size_t HS_MAX_TOP = 64;
 
+namespace {
+bool overlap(const void *x, size_t nx, const void *y, size_t ny);
+}
+
+// Whether two results of n rows with `top` alternatives each share memory.
+static bool results_overlap(size_t n, size_t top, const float *logprob, const uint32_t *rank, const float *entropy,
+                            const uint32_t *top_tokens, const float *top_logprob) {
+    const struct { const void *at; size_t words; } r[] = {{logprob, n}, {rank, n}, {entropy, n}, {top_tokens, n * top}, {top_logprob, n * top}};
+    for (int i = 0; i < 5; i++)
+        for (int j = 0; j < i; j++)
+            if (r[i].words && r[j].words && overlap(r[i].at, 4 * r[i].words, r[j].at, 4 * r[j].words)) return true;
+    return false;
+}
+
 // The checks of a scored call's arguments, and its buffers.
 static hs_status plan_scores(hs_batch *b, const uint32_t *tokens, size_t n, const Scoring &sc) {
     const uint32_t V = b->model->host.vocab;
@@ -1655,6 +1669,8 @@ static hs_status plan_scores(hs_batch *b, const uint32_t *tokens, size_t n, cons
     if (!tokens && (sc.logprob || sc.rank)) return hs::fail(HS_INVALID_ARGUMENT, 0, "log probabilities and ranks need tokens");
     for (size_t i = 0; tokens && i < n; i++)
         if (tokens[i] >= V && tokens[i] != HS_NO_TOKEN) return hs::fail(HS_UNSUPPORTED, 0, "a scored token is out of range");
+    if (results_overlap(n, sc.top, sc.logprob, sc.rank, sc.entropy, sc.top_tokens, sc.top_logprob))
+        return hs::fail(HS_INVALID_ARGUMENT, 0, "the results must not overlap");
     if (n == 0 || b->h_scores) return HS_OK;
     HIP_TRY(hipSetDevice(b->model->dev->ordinal));
     const size_t words = b->max_rows * (3 + 2 * HS_MAX_TOP);
@@ -2396,6 +2412,8 @@ extern "C" hs_status hs_op_score_dev(hs_device *dev, const void *logits, uint32_
     if (!aligned(bits / 8, {logits}) || !aligned(8, {table}) || !aligned(4, {tokens, logprob, rank, entropy, top_tokens, top_logprob}))
         return hs::fail(HS_INVALID_ARGUMENT, 0, "logits, tables and results must be aligned to their types");
     if (rows == 0) return HS_OK;
+    if (results_overlap(rows, top, logprob, rank, entropy, top_tokens, top_logprob))
+        return hs::fail(HS_INVALID_ARGUMENT, 0, "the results must not overlap");
     hs::ScoreArgs a;
     a.src = bits == 32 ? hs::SCORE_I32 : hs::SCORE_I64; a.logits = logits; a.ld = ld;
     a.vocab = (int)vocab; a.table = table; a.table_len = (int)len; a.tokens = tokens; a.top = (int)top;

@@ -260,3 +260,21 @@ def test_batch_alternatives():
     for top in (65, 2 ** 31 - 1, 2 ** 31, 2 ** 70, -1):
         with pytest.raises(hip.Unsupported):
             hip.HipBatch._scored(Batch, 1, None, top, call)
+
+
+def test_results_that_overlap():
+    """Results that share memory, also of a few bytes, are refused; side by side, or without alternatives, they are not."""
+    rows, top = 5, 3
+    sizes = [4 * rows] * 3 + [4 * rows * top] * 2
+    at = [BASE + sum(sizes[:i]) for i in range(5)]
+    for i in range(5):
+        for j in range(i):
+            for x, y in ((i, j), (j, i)):
+                outs = [None] * 5
+                outs[x], outs[y] = BASE + 1024, BASE + 1024 + sizes[x] - 4  # y starts on the last word of x
+                score(BAD, dims=(rows, 100, 50), top=top, outs=outs)
+                outs[y] = BASE + 1024
+                score(BAD, dims=(rows, 100, 50), top=top, outs=outs)
+    # a result that lies between others; and one over alternatives of no size, refused for the number of rows only
+    score(BAD, dims=(rows, 100, 50), top=top, outs=at[:4] + [at[4] - 4])
+    score(dims=(0, 100, 50), top=top, outs=(BASE,) * 5)
