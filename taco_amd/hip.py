@@ -646,6 +646,28 @@ def _dptr(x):
     return x.data_ptr()
 
 
+_kinds = {}  # a tensor's type: "i" or "f" for integers or floats, and the bytes of an element
+
+
+def _held(x, kind: str, n: int):
+    """_dptr of a tensor that has to hold `n` elements or more of `kind` ("i4": 32-bit integers). Of an address nothing is known."""
+    if getattr(x, "is_cuda", False) is not True:
+        return _dptr(x)
+    own = _kinds.get(x.dtype) or _kind_of(x)
+    if own != kind or x.numel() < n:
+        raise ValueError(f"a tensor of {x.numel()} {own} where the call reads or writes {n} {kind} "
+                         "(integers or floats, bytes of an element)")
+    if not x.is_contiguous():
+        return _dptr(x)
+    return x.data_ptr()
+
+
+def _kind_of(x) -> str:
+    name = str(x.dtype)
+    own = _kinds[x.dtype] = ("i" if "int" in name else "f" if "float" in name else "?") + str(x.element_size())
+    return own
+
+
 def _dptrs(xs):
     """The layers' device addresses as a host array, from a list of them or from one contiguous tensor
     whose first axis is the layers."""
@@ -763,10 +785,13 @@ class PagedCache(NamedTuple):
     max_scale: int
 
     def _struct(self):
-        k, v, ks, vs, *numbers = self
-        if min(numbers) < 0 or max(numbers) > _U32:
+        k, v, ks, vs, pages, heads, page, hd, most = self
+        if not (0 <= pages <= _U32 and 0 <= heads <= _U32 and 0 <= page <= _U32 and 0 <= hd <= _U32 and 0 <= most <= _U32):
             raise Unsupported(HS_UNSUPPORTED, 0, "a size that 32 bits do not hold")
-        return _Pages(_dptr(k), _dptr(v), _dptr(ks), _dptr(vs), *numbers)
+        n = pages * heads
+        values = n * page * hd
+        return _Pages(_held(k, "i1", values), _held(v, "i1", values), _held(ks, "i4", n), _held(vs, "i4", n),
+                      pages, heads, page, hd, most)
 
 
 def _sizes(*numbers):
@@ -793,9 +818,11 @@ def _rows_of(x, bits: Optional[int], stride: Optional[int], shape):
     head_dim] on the GPU whose heads of a token lie together and whose tokens at one distance, or an address with
     `bits` and `stride` (None: the rows lie together)."""
     b, t, h, hd = shape
-    if not _on_gpu(x):
+    if getattr(x, "is_cuda", False) is not True and not _on_gpu(x):
         return x, bits or 0, h * hd if stride is None else stride
-    st, own = x.stride(), _bits_of(x)
+    st, own = x.stride(), _types.get(x.dtype)
+    if own is None:
+        own = _bits_of(x)
     if x.shape != shape or own == 0 or (bits is not None and bits != own):
         raise ValueError(f"a tensor that does not hold {tuple(shape)} integers of the operator's types")
     step = st[1] if t > 1 else st[0] if b > 1 else h * hd
@@ -809,30 +836,43 @@ def pages_append(dev: HipDevice, cache: PagedCache, k, v, table, ctx, rows, dims
                  bits: Optional[int] = None, stride: Optional[int] = None, stream=None) -> None:
     """Appends rows of keys and values to the streams' pages (hs_op_pages_append_dev): dims = (streams, t, width);
     k and v are tensors [streams, t, kv_heads, head_dim] of int8 or int16, or addresses with `bits` and `stride`."""
-    b, t, width = _sizes(*dims)
+    b, t, width = dims
+    if b < 0 or t < 0 or width < 0:
+        _sizes(b, t, width)
     shape = (b, t, cache.kv_heads, cache.head_dim)
     kp, kb, ks = _rows_of(k, bits, stride, shape)
     vp, vb, vs = _rows_of(v, bits, stride, shape)
     if ks != vs or kb != vb:
         raise ValueError("k and v of different types, or with tokens at different distances")
+    if ks < 0:
+        _sizes(ks)
     if not 0 <= headroom <= _U32:
         raise Unsupported(HS_UNSUPPORTED, 0, "headroom must be in 16..=64 sixteenths")
-    _check(lib().hs_op_pages_append_dev(dev.h, C.byref(cache._struct()), kp, vp, kb, *_sizes(ks), _dptr(table), _dptr(ctx),
-                                        _dptr(rows), b, t, width, headroom, _dptr(ctx_out), stream))
+    _check(lib().hs_op_pages_append_dev(dev.h, C.byref(cache._struct()), kp, vp, kb, ks, _held(table, "i4", b * width),
+                                        _held(ctx, "i4", b), _held(rows, "i4", b), b, t, width, headroom,
+                                        _held(ctx_out, "i4", b), stream))
 
 
 def attend_paged(dev: HipDevice, cache: PagedCache, q, table, ctx, rows, dims, rule: AttentionRule, out,
                  q_stride: Optional[int] = None, workspace=None, workspace_bytes: int = 0, stream=None) -> None:
     """Causal attention over the streams' pages (hs_op_attend_paged_dev): dims = (streams, t, heads, width, keys);
     q is a tensor [streams, t, heads, head_dim] of int8, or an address with `q_stride`; rows may be None (t each)."""
-    b, t, heads, width, keys = _sizes(*dims)
+    b, t, heads, width, keys = dims
+    if b < 0 or t < 0 or heads < 0 or width < 0 or keys < 0:
+        _sizes(*dims)
     qp, bits, step = _rows_of(q, None, q_stride, (b, t, heads, cache.head_dim))
     if bits not in (0, 8):
         raise ValueError("q: [streams, t, heads, head_dim] of int8")
+    if step < 0:
+        _sizes(step)
     m, s, om, os_, exp, length, p = rule
-    _check(lib().hs_op_attend_paged_dev(dev.h, C.byref(cache._struct()), qp, *_sizes(step), _dptr(table), _dptr(ctx),
-                                        _dptr(rows), b, t, heads, width, keys, m, s, om, os_, _dptr(exp), length, p,
-                                        _dptr(out), _dptr(workspace), workspace_bytes, stream))
+    space = _dptr(workspace)
+    if space is not workspace and workspace.numel() * workspace.element_size() < workspace_bytes:
+        raise ValueError("a workspace of fewer bytes than the call says")
+    _check(lib().hs_op_attend_paged_dev(dev.h, C.byref(cache._struct()), qp, step, _held(table, "i4", b * width),
+                                        _held(ctx, "i4", b), _held(rows, "i4", b), b, t, heads, width, keys, m, s, om, os_,
+                                        _held(exp, "i4", length), length, p, _held(out, "i1", b * t * heads * cache.head_dim),
+                                        space, workspace_bytes, stream))
 
 
 def attend_paged_workspace(streams: int, t: int, heads: int, kv_heads: int, head_dim: int, keys: int) -> int:
@@ -844,7 +884,9 @@ def score_tokens(dev: HipDevice, logits, tokens, table, dims, top: int, logprob,
                  bits: Optional[int] = None, stride: Optional[int] = None, stream=None) -> None:
     """The scores of rows of logits on the device (hs_op_score_dev): dims = (rows, vocab, table length); logits is a
     tensor [rows, vocab] of int32 or int64 with its symbols together, or an address with `bits` and `stride`."""
-    rows, vocab, length = _sizes(*dims)
+    rows, vocab, length = dims
+    if rows < 0 or vocab < 0 or length < 0:
+        _sizes(*dims)
     if _on_gpu(logits):
         own, st = _bits_of(logits), logits.stride()
         if logits.shape != (rows, vocab) or own == 0 or (bits is not None and bits != own) or (vocab > 1 and st[1] != 1):
@@ -852,9 +894,11 @@ def score_tokens(dev: HipDevice, logits, tokens, table, dims, top: int, logprob,
         bits, stride, logits = own, st[0] if rows > 1 else vocab, logits.data_ptr()
     elif stride is None:
         stride = vocab
-    _sizes(top, stride)
-    _check(lib().hs_op_score_dev(dev.h, logits, bits or 0, stride, _dptr(tokens), _dptr(table), length, rows, vocab, top,
-                                 _dptr(logprob), _dptr(rank), _dptr(entropy), _dptr(top_tokens), _dptr(top_logprob), stream))
+    if top < 0 or stride < 0:
+        _sizes(top, stride)
+    _check(lib().hs_op_score_dev(dev.h, logits, bits or 0, stride, _held(tokens, "i4", rows), _held(table, "i8", length), length,
+                                 rows, vocab, top, _held(logprob, "f4", rows), _held(rank, "i4", rows), _held(entropy, "f4", rows),
+                                 _held(top_tokens, "i4", rows * top), _held(top_logprob, "f4", rows * top), stream))
 
 
 def kernel_resources(dev: HipDevice):

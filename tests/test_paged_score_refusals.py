@@ -278,3 +278,60 @@ def test_results_that_overlap():
     # a result that lies between others; and one over alternatives of no size, refused for the number of rows only
     score(BAD, dims=(rows, 100, 50), top=top, outs=at[:4] + [at[4] - 4])
     score(dims=(0, 100, 50), top=top, outs=(BASE,) * 5)
+
+
+class OnGpu:
+    """A tensor as if on the GPU, whose address no call uses."""
+    is_cuda = True
+
+    def __init__(self, x):
+        self.x, self.shape, self.dtype = x, x.shape, x.dtype
+
+    def __getattr__(self, name):
+        return getattr(self.x, name)
+
+
+class Library:
+    """Takes every call."""
+
+    def __getattr__(self, name):
+        return lambda *args: 0
+
+
+def test_arrays(monkeypatch):
+    """Tensors that are too short or of another type for what the call reads or writes are refused; longer ones and other
+    types of the same integers are taken."""
+    torch = pytest.importorskip("torch")
+    monkeypatch.setattr(hip, "lib", Library)
+    cache = {"k": (torch.int8, 10 * 2 * 64 * 64), "v": (torch.int8, 10 * 2 * 64 * 64), "k_scale": (torch.int32, 20), "v_scale": (torch.int32, 20)}
+    calls = [
+        (append, {"table": (torch.int32, 8), "ctx": (torch.int32, 2), "rows": (torch.int32, 2), "ctx_out": (torch.int32, 2)}),
+        (attend, {"table": (torch.int32, 8), "ctx": (torch.int32, 2), "rows": (torch.int32, 2), "out": (torch.int8, 6 * 256)}),
+        (score, {"tokens": (torch.int32, 2), "table": (torch.int64, 50)}),
+    ]
+    other = {torch.int8: (torch.int16, torch.float16), torch.int32: (torch.int64, torch.float32, torch.int16), torch.int64: (torch.int32, torch.float64),
+             torch.float32: (torch.float64, torch.int32, torch.bfloat16)}
+    same = {torch.int8: torch.uint8, torch.int32: torch.uint32, torch.int64: torch.uint64, torch.float32: torch.float32}
+
+    def each(give, dtype, n):
+        give(OnGpu(torch.zeros(n, dtype=dtype)))
+        give(OnGpu(torch.zeros(n + 3, dtype=same[dtype])))
+        for bad in [torch.zeros(n - 1, dtype=dtype), torch.zeros(2 * n, dtype=dtype)[::2]] + [torch.zeros(n, dtype=d) for d in other[dtype]]:
+            with pytest.raises(ValueError):
+                give(OnGpu(bad))
+        with pytest.raises(ValueError):
+            give(torch.zeros(n, dtype=dtype))  # in host memory
+
+    for fn, arrays in calls:
+        for name, (dtype, n) in arrays.items():
+            each(lambda x: fn(**{name: x}), dtype, n)
+    for fn in (append, attend):
+        for name, (dtype, n) in cache.items():
+            each(lambda x: fn(cache=CACHE._replace(**{name: x})), dtype, n)
+    each(lambda x: attend(rule=RULE._replace(attn_exp=x)), torch.int32, 100)
+    for i, (dtype, n) in enumerate([(torch.float32, 2), (torch.int32, 2), (torch.float32, 2), (torch.int32, 6), (torch.float32, 6)]):
+        each(lambda x: score(outs=[x if i == j else BASE for j in range(5)]), dtype, n)
+    space = OnGpu(torch.zeros(100, dtype=torch.int32))
+    attend(workspace=space, workspace_bytes=400)
+    with pytest.raises(ValueError):
+        attend(workspace=space, workspace_bytes=401)
