@@ -423,7 +423,8 @@ typedef struct hs_pages {
 /* Appends rows[s] <= t tokens (NULL: t for every stream) to the ctx[s] tokens of each stream: token i
  * of stream s has head h of its key at k[(s t + i) stride + h head_dim], of its value in v alike, i8
  * (bits = 8) or i16 (bits = 16); the rows may be part of a wider row (c_attn's). table [b, width].
- * i8 values are stored as they are with scale 1. Of i16 values the FIRST row of a page sets the page's
+ * i8 values are stored as they are, and the first row of a page gives it scale 1; they and i16 values must not share a
+ * page (behind a first row of i16 they would be read at its scale). Of i16 values the FIRST row of a page sets the page's
  * scale s = clamp(ceil(most headroom / (16 127)), 1, max_scale), most its largest magnitude in the
  * head and headroom in sixteenths (16 ..= 64), and every row x of the page is stored as
  * clamp(floor((2 x + s) / (2 s)), +-127). So the bytes of a token depend on that token and the first
