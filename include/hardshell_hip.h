@@ -438,7 +438,7 @@ hs_status hs_op_pages_append_dev(hs_device *dev, const hs_pages *cache, const vo
                                  uint32_t headroom, uint32_t *ctx_out, void *stream);
 /* Causal attention of the last rows[s] <= t tokens of each stream (NULL: t for every stream; t = 1 is
  * the decode step) over its pages: row i sees the first ctx[s] - rows[s] + 1 + i of the stream's ctx[s]
- * tokens (no more than `keys` of them count). q at [(s t + i) q_stride + h head_dim], out [b, t, h,
+ * tokens. A ctx[s] above `keys`, the most that a stream may hold, counts as `keys` (and the rows as its last). q at [(s t + i) q_stride + h head_dim], out [b, t, h,
  * head_dim]; head j reads head j / (h / kv_heads) of the cache. With ks and vs the scales of a key's page
  *   score = clamp(rescale(q . k, score_m ks, score_s), +-2^40), e = attn_exp[min(M - score, len - 1)],
  *   w = floor(e vs 2^P / S), out = clamp(rescale(sum w v, out_m, out_s), +-127)
