@@ -430,8 +430,8 @@ typedef struct hs_pages {
  * clamp(floor((2 x + s) / (2 s)), +-127). So the bytes of a token depend on that token and the first
  * of its page alone: a stream appended token by token holds what it holds appended at once, and no
  * token changes what an earlier one has read. Tokens past the stream's width * page are dropped. ctx_out[b]
- * (or NULL; not overlapping ctx or rows) receives the new counts. t = 0 does nothing. Two streams must not
- * append to one page in a call. */
+ * (or NULL; not overlapping ctx or rows) receives the new counts. t = 0 does nothing. A page
+ * must not be appended to at two places in a call, by two streams or by one whose table names it twice. */
 hs_status hs_op_pages_append_dev(hs_device *dev, const hs_pages *cache, const void *k, const void *v,
                                  uint32_t bits, size_t stride, const uint32_t *table, const uint32_t *ctx,
                                  const uint32_t *rows, size_t b, size_t t, size_t width,
