@@ -375,6 +375,7 @@ __device__ __forceinline__ void paged_put(const PagedArgs &g, const PagedPlan &p
 // What bounds it: one row, HBM (768 panels of 64 channels: 512 to 1,024 keys 76 MB in 19.3 us, 4,096 to 8,192 keys 605 MB in 117,
 // 5.2 TB/s). Few panels, what one CU reads, some 30 KB a us (12 panels of 4,096 to 8,192 keys 27 us; 128 of 2,000 to 4,000 keys
 // with 128 channels and 8 rows 42). Many rows, VALU issue: 192 panels of 256 causal rows over 512 to 1,024 keys, 16.5 M instructions, 27 us of 50.
+// A few forms spill registers: one row of up to 16,384 keys 4, of 256 channels 8.
 // All in one launch, the dots in registers from the one product to the other: the rule needs the row's largest score and its sum
 // before a weight, and forming the dots again would read K again. The table goes to LDS for more than 4 rows; for few rows the
 // lookups are fewer than its entries.
@@ -738,6 +739,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RT == 16 &&
 // the third a wave takes a tile over all blocks, since a tile's sums are 64 registers for 64 channels (the waves' loads of
 // the same rows meet in the L1). VALU issue bounds them, and few workgroups where there are few panels: 192 panels of 64 rows over
 // 2,048 to 4,096 keys 100 us (38 M scores), 12 panels of 256 rows over 16,000 keys 157.
+// The second walk spills registers past 64 channels: 21 to 128 channels and 47 to 256, with scores of 64 bits 32 and 67.
 template <int QC, bool HI, int PHASE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QC == 4 ? 2 : 3))) void k_paged_scan(PagedArgs g, PagedPlan pl, void *scratch) {
     extern __shared__ __attribute__((aligned(1024))) int32_t s_exp[];  // the table
@@ -1083,9 +1085,9 @@ static PagedPlan paged_plan(const PagedArgs &g) {
     p.panels = g.streams * g.pages.kv_heads;
     // Keys of a tile in one launch, whose dots fit the registers of its waves. It reads K and V and nothing else; several launches
     // write and read the scores too, but spread a panel over the chip. In us, one launch and several, with three quarters of the
-    // keys there in the mean: 768 panels of 8,192 keys 117
-    // and 155, 12 panels 27 and 36; of 16,000 keys 768 panels 238 and 290, 200 panels 71 and 89, 48 panels 50 and 34. 16 rows
-    // (8 query heads of 128 channels, 128 panels of 2,000 keys) 25 and 38.
+    // keys there in the mean: 768 panels of 8,192 keys 117 and 155, 12 panels 27 and 36; of 16,000 keys 768 panels 238 and 290, 200 panels 71 and 89, 156 panels 66 and 77, 132 panels
+    // 62 and 67, 120 panels 60 and 59, 96 panels 59 and 50, 48 panels 50 and 34 (of 9,000 keys the sides meet at some 80 panels).
+    // 16 rows (8 query heads of 128 channels, 128 panels of 2,000 keys) 25 and 38.
     const int most = rows > 8 || (rows > 4 && g.pages.hd > 128) ? 2048 : rows > 4 ? 4096 : g.pages.hd > 128 ? 4096 : g.pages.hd > 64 || p.panels < 128 ? 8192 : 16384;
     // 64 rows: 16 streams of 64 rows over 4,096 keys 100 us, in tiles of 16 rows 155. 4 rows: a row of 1,000 keys 9.2 us, as one
     // of 16 rows 12.2 (768 panels 20.5 and 23.8).
@@ -1103,9 +1105,18 @@ static PagedPlan paged_plan(const PagedArgs &g) {
             p.span = (int)(((g.keys + ng - 1) / ng + 255) / 256) * 256;
             p.ng = (g.keys + p.span - 1) / p.span;
         };
-        // workgroups for each of 256 CUs, of 2, 3, 4, 8 and 12, in us of the scores' launch and the products':
-        //   200 panels of one row, 8,192 to 16,384 keys     41 + 41   41 + 41   40 + 41   38 + 38   36 + 39
-        //   128 panels of eight rows, 128 channels, 4,000   15 + 17   17 + 23   15 + 22   17 + 30   17 + 30
+        // workgroups for each of 256 CUs, in us of whole calls (three quarters of the keys there in the mean):
+        //                                                        1      2      3      4      8     12     16
+        //   one row, 200 panels of up to 32,000 keys                  170    171    171    164    164    161
+        //   one row, 100 panels, 16,000                              58.8   59.2   59.9   57.9   58.1   58.3
+        //   one row, 128 panels of 128 channels, 12,000              85.5   87.5   85.2   84.7   84.6   85.1
+        //   eight rows, 128 panels of 128 channels, 6,000     68.7   67.8   74.0   71.9   76.3
+        //   16 rows, 128 panels, 4,000                        49.9   47.4   49.6   51.3   51.0
+        //   12 rows, 48 panels, 8,000                         42.4   39.7   40.7   41.0   41.0
+        //   64 rows, 192 panels, 4,096                         113    103          99.5    112
+        //   256 rows, 48 panels, 8,000                         195    151           144    161
+        //   256 rows, 12 panels, 16,000                        148    126           156    194
+        // (one stream's 256 rows alone would have two)
         if (p.rt == 4) ranges(1024, 12 * 256);
         else if (p.rt == 16) ranges(512, 2 * 256);
         else ranges(512, 4 * 256);

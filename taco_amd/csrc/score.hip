@@ -140,11 +140,13 @@ __global__ __launch_bounds__(512) void k_score_any(ScoreArgs a) {
 // collected and ranked against each other.
 // G > 0: the row is read once, G groups at most, and its indexes stay in registers, 16 bits each. G > 26: the logits do not fit
 // there until the largest is known, so 16 bits of each are kept (NARROW); a row whose largest logit lies too far above that
-// of its first groups for those (65,535 less the table and 64) is scored by itself, as by k_score_any. G = 0, longer
-// rows: read for the max, for the counts, and once each for ties and alternatives.
-// HBM bounds many rows: 4,096 x 50,257 i32 logits, 823 MB in 181 us, 4.6 TB/s, with 53 us of LDS work (counting: over half of it
-// waits for a bank) and 79 of VALU issue beside the loads of the other workgroup of a CU. Few rows are a chain: the loads, the
-// largest, the counts, the sums, the alternatives: one row 17 us, 64 rows 17.6.
+// of its first groups for those (65,535 less the table and 64) is scored by itself, as by k_score_any: slow (512 rows of 131,072
+// whose first 16,384 symbols lie 100,000 below the others: 0.74 ms with one alternative and 6.8 with 64, others 99 and 109 us).
+// G = 0, longer rows: read for the max, for the counts, and once each for ties and alternatives.
+// HBM bounds many rows: 4,096 x 50,257 i32 logits, 823 MB in 182 us, 4.5 TB/s, with 53 us of LDS work (counting: over half of it
+// waits for a bank) and 83 of VALU issue beside the loads of the other workgroup of a CU. Few rows are a chain: the loads, the
+// largest, the counts, the sums, the alternatives: one row 17 us, 64 rows 17.7.
+// Some forms spill registers: 13 groups of i64 logits 14, those of 16 bits each 25 (i32) and 30, the walk 24 and 42.
 constexpr int SCORE_LIST = 1024;   // symbols collected; where ties make them more, the alternatives are searched one by one
 constexpr int SCORE_BINS = 16384;  // entries of the table at most
 
